@@ -158,6 +158,79 @@ int neko_hip_attention(neko_hip_ctx* ctx, const void* q, int64_t q_stride, const
                        void* out, int64_t out_stride, int64_t T, int n_head, int n_kv, int hd, int64_t pos0, float scale,
                        int dtype);
 
+/* ---------------------------------------------------------------- paged 8-bit KV cache
+ * Many sequences in one cache of fixed-size pages, keys and values in 8 bits. No counterpart in the
+ * reference, which keeps one f16 cache per sequence (cpu_ops.cpp:535-575).
+ *
+ * A page holds page_size tokens (16, 32, 64, 128 or 256) of one sequence, all kv heads: OCP E4M3 codes
+ * [n_pages][n_kv][page_size][hd] for keys and the same for values, and one f32 scale for each page and kv
+ * head, [n_pages][n_kv]; a cached value is code * scale. Scales are powers of two, 2^-64 .. 2^64 (any other
+ * bits are read as the power of two below, clamped). hd is a multiple of 16, 16..256; pages are 16-byte
+ * aligned; the four arrays do not overlap.
+ *
+ * A batch is n_seq sequences whose new rows stand one after another: sequence s has rows row_start[s] ..
+ * row_start[s + 1] - 1 (none: an idle place) and kv_len[s] tokens with them, so its row i stands at position
+ * kv_len[s] - n + i (lengths up to 2^30). Position p is held by page page_table[s * table_stride + p /
+ * page_size]; entries past the length are not read. All three arrays are device memory that the host does
+ * not look at, so one captured graph serves growing lengths. Their values are checked on the device: a page id
+ * outside [0, n_pages), or a position past max_pages, is a token that is not stored and not seen; rows past
+ * row_start[n_seq], or at a negative position (a length below the number of rows), are left alone by the append and
+ * see nothing. Two sequences of a batch may share pages that the batch only reads; pages that it appends to
+ * belong to one sequence, or their contents are unspecified. */
+typedef struct neko_paged_kv {
+    void* k_pages;
+    void* v_pages;
+    float* k_scales;
+    float* v_scales;
+    int64_t n_pages;
+    int page_size;
+    int n_kv;
+    int hd;
+} neko_paged_kv;
+
+typedef struct neko_paged_batch {
+    const int32_t* page_table;
+    int64_t table_stride; /* entries from one sequence's row to the next */
+    int64_t max_pages;    /* entries of a row */
+    const int32_t* row_start; /* [n_seq + 1], non-decreasing */
+    const int32_t* kv_len;    /* [n_seq] */
+    int64_t n_seq;            /* 1 .. 2^24 */
+} neko_paged_batch;
+
+/* neko_hip_qk_norm_rope and the append of what it makes: each row of qkv is [q n_q*hd | k n_kv*hd | v n_kv*hd]; its q
+ * heads are normed (wqk as above; NULL: not), rotated and written to q_out (the q columns of qkv itself: same
+ * pointer and stride; or disjoint); its k heads the same, rounded to the activation type, and with its v heads
+ * rounded to 8 bits into the page of the row's position. qkv's k and v columns are not written.
+ *   rot_dim      the first rot_dim dimensions of each head are rotated, the rest pass (a multiple of 8, up to
+ *                hd; 0: no rotation, cs unused), by cs [n_pos][rot_dim], (cos, sin) pairs as neko_rope_table
+ *                makes them -- tables scaled for long contexts are the caller's.
+ *   interleaved  0: pairs (x_i, x_(i + rot_dim/2)); otherwise pairs (x_2i, x_(2i+1)).
+ * With a rotation, rows at positions from n_pos on are left alone.
+ * A page's scale is the smallest power of two that brings its tokens' largest finite magnitude, per kv head,
+ * to 448 or below. Tokens before the first new one keep the page's scale or, where a new one needs a larger,
+ * are rounded again under that (exact except below the smallest normal code); a page whose first token is
+ * new takes nothing from what it held. Infinities and NaN (and f32 magnitudes past 448 * 2^64) are stored as
+ * NaN. Slots past the last new token are not written. */
+int neko_hip_qk_norm_rope_paged(neko_hip_ctx* ctx, const void* qkv, int64_t row_stride, int64_t rows, int n_q,
+                                const neko_paged_kv* kv, const neko_paged_batch* batch, const float* wqk, const float* cs,
+                                int64_t n_pos, int rot_dim, int interleaved, float eps, void* q_out, int64_t q_out_stride,
+                                int dtype);
+
+/* Causal grouped-query attention of a batch's rows over its pages (which already hold the rows' own tokens):
+ * for the row at position p and query head h < n_head (a multiple of n_kv),
+ *   s_j = b(scale * q . k_j) + slopes[h] * (j - p),   out = sum_j e^(s_j) v_j / sum_j e^(s_j),
+ * over positions j <= p, from p - window + 1 on if window > 0; b(x) = softcap * tanh(x / softcap) if softcap
+ * > 0, else x; slopes f32 [n_head] or NULL. Rows that see nothing give zeros; rows past row_start[n_seq] are
+ * not written. Infinities and NaN in q, and NaN in cached tokens, reach the rows that see them and no others.
+ * q and out rows of n_head*hd (strides in elements); out overlaps neither q nor the cache.
+ * f32 sums; products on the matrix cores, codes exact in f16, f32 q and weights as two f16 each (tested to
+ * 2e-6 (1 + sum w|v| / sum w) of a 64-bit evaluation); f16 calls round as said at the kernels.
+ * Partial results of key splits go to the context's workspace (see neko_hip_matmul): its size goes by rows,
+ * n_seq, heads and head size, not by lengths, so one uncaptured call of these makes every later capture fit. */
+int neko_hip_attention_paged(neko_hip_ctx* ctx, const void* q, int64_t q_stride, int64_t rows, const neko_paged_kv* kv,
+                             const neko_paged_batch* batch, int n_head, float scale, float softcap, int64_t window,
+                             const float* slopes, void* out, int64_t out_stride, int dtype);
+
 /* ---------------------------------------------------------------- residual */
 
 /* Residual add + RMSNorm: x[t] = x[t] + delta[t] (float add, rounded once to the activation type,

@@ -27,6 +27,24 @@ _i32 = ctypes.c_int
 _f32 = ctypes.c_float
 _sz = ctypes.c_size_t
 
+
+class PagedKv(ctypes.Structure):
+    """neko_paged_kv."""
+
+    _fields_ = [("k_pages", _p), ("v_pages", _p), ("k_scales", _p), ("v_scales", _p), ("n_pages", _i64),
+                ("page_size", _i32), ("n_kv", _i32), ("hd", _i32)]
+
+
+class PagedBatch(ctypes.Structure):
+    """neko_paged_batch."""
+
+    _fields_ = [("page_table", _p), ("table_stride", _i64), ("max_pages", _i64), ("row_start", _p), ("kv_len", _p),
+                ("n_seq", _i64)]
+
+
+_kv = ctypes.POINTER(PagedKv)
+_batch = ctypes.POINTER(PagedBatch)
+
 # name -> (restype, argtypes); the order of include/neko_hip.h.
 SIGNATURES = {
     "neko_hip_create": (_i32, [_i32, ctypes.POINTER(_p)]),
@@ -50,6 +68,9 @@ SIGNATURES = {
                                         _i32]),
     "neko_hip_store_kv": (_i32, [_p, _p, _i64, _i64, _i64, _i64, _i64, _i64, _p, _p, _p, _i64, _i32]),
     "neko_hip_attention": (_i32, [_p, _p, _i64, _p, _p, _p, _i64, _i64, _i32, _i32, _i32, _i64, _f32, _i32]),
+    "neko_hip_qk_norm_rope_paged": (_i32, [_p, _p, _i64, _i64, _i32, _kv, _batch, _p, _p, _i64, _i32, _i32, _f32, _p, _i64,
+                                           _i32]),
+    "neko_hip_attention_paged": (_i32, [_p, _p, _i64, _i64, _kv, _batch, _i32, _f32, _f32, _i64, _p, _p, _i64, _i32]),
     "neko_hip_add_rmsnorm": (_i32, [_p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _f32, _i32]),
     "neko_hip_matmul": (_i32, [_p, _p, _i64, _i64, _i64, _p, _i64, _i32, _i64, _p, _p, _i64, _i32, _i32, _i32]),
     "neko_hip_set_matmul_library": (_i32, [_p, _i32]),

@@ -1,0 +1,163 @@
+// Shared by the paged attention kernels: the launch arguments, a workgroup's item, masks and partial results.
+#pragma once
+
+#include "internal.h"
+#include "paged_device.h"
+
+namespace neko_hip {
+
+struct PagedAttnArgs {
+    Paged p;
+    AttnTiling t;
+    const void* q;
+    int64_t qs;
+    void* out;
+    int64_t os;
+    int32_t n_head;
+    int32_t window;  // 0: none
+    float scale;     // of the scores; its sign goes into q
+    float softcap;   // 0: none
+    const float* slopes;
+    float* part;  // [blocks][tile_rows][head size of the kernel] accumulators of split items
+    float* ml;    // [blocks][tile_rows][4]: their maximum, sum, whether any key was seen
+    uint32_t blocks;  // that part and ml hold
+};
+
+constexpr float kAttnLog2e = 1.44269504088896341f;
+constexpr int kPOffset = 15;  // weights go to f16 times 2^kPOffset, the largest power that it holds
+constexpr float kPScale = 1 << kPOffset;
+
+struct AttnItem {
+    int32_t s, tile, split, splits, chunk;
+    uint32_t block;  // index of the (tile, split) among those of a kv head
+};
+
+__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) v += static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(v), m));
+    return v;
+}
+__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {  // inclusive
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t u = static_cast<uint32_t>(__shfl_up(static_cast<int>(v), d));
+        if (lane >= d) v += u;
+    }
+    return v;
+}
+
+// The item of workgroup j of a kv head (by_tile: the tile of merge workgroup j, its first split), by every wave for
+// itself: sequences' tiles and splits are summed 64 at a time. False past the last.
+template <bool BY_TILE>
+__device__ __forceinline__ bool attn_find(const Paged& p, const AttnTiling& t, uint32_t j, AttnItem* it) {
+    const int32_t lane = static_cast<int32_t>(threadIdx.x) & 63;
+    int32_t tiles = 0, units = 0;
+    auto load = [&](int32_t base) {
+        tiles = units = 0;
+        if (base + lane < p.n_seq) {
+            const SeqRows r = paged_seq(p, base + lane);
+            tiles = attn_tiles(t, r);
+            units = attn_units(t, p, r);
+        }
+    };
+    uint64_t work = 0;
+    for (int32_t base = 0; base < p.n_seq; base += 64) {
+        load(base);
+        work += static_cast<uint64_t>(tiles) * static_cast<uint64_t>(units);
+    }
+    work = wave_sum_u64(work) * static_cast<uint64_t>(p.n_kv);
+    const int32_t chunk = attn_chunk(t, work);
+    uint32_t past_tiles = 0, past = 0;
+    for (int32_t base = 0; base < p.n_seq; base += 64) {
+        if (p.n_seq > 64) load(base);
+        const int32_t splits = attn_splits(units, chunk);
+        const uint32_t n = static_cast<uint32_t>(tiles) * static_cast<uint32_t>(splits);
+        const uint32_t sum = wave_scan_u32(n), sum_tiles = BY_TILE ? wave_scan_u32(static_cast<uint32_t>(tiles)) : 0;
+        const uint64_t at = __ballot(BY_TILE ? past_tiles + sum_tiles > j : past + sum > j);
+        if (at) {
+            const int l = __builtin_ctzll(at);
+            const int32_t n_tiles = __builtin_amdgcn_readlane(tiles, l);
+            it->s = base + l;
+            it->chunk = chunk;
+            it->splits = __builtin_amdgcn_readlane(splits, l);
+            const uint32_t first = past + static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum - n), l));
+            if constexpr (BY_TILE) {
+                const uint32_t local = j - past_tiles - static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum_tiles) - tiles, l));
+                it->tile = n_tiles - 1 - static_cast<int32_t>(local);
+                it->split = 0;
+                it->block = first + local * static_cast<uint32_t>(it->splits);
+            } else {  // the last tiles, which see the most keys, first
+                const uint32_t local = j - first;
+                it->tile = n_tiles - 1 - static_cast<int32_t>(local / static_cast<uint32_t>(it->splits));
+                it->split = static_cast<int32_t>(local % static_cast<uint32_t>(it->splits));
+                it->block = j;
+            }
+            return true;
+        }
+        past += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum), 63));
+        if constexpr (BY_TILE) past_tiles += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum_tiles), 63));
+    }
+    return false;
+}
+
+// The keys that a tile's rows see, first and last row: row i sees [lo(i), hi(i)).
+struct TileKeys {
+    int32_t lo_min, lo_max, hi_min, hi_max;
+    int32_t k0, k1;  // this split's, k0 a multiple of 32
+};
+__device__ __forceinline__ int32_t key_lo(int32_t pos, int32_t window) { return window > 0 && pos >= window ? pos - window + 1 : 0; }
+__device__ __forceinline__ TileKeys tile_keys(const PagedAttnArgs& a, const SeqRows& r, const AttnItem& it) {
+    const int32_t n_rows = r.n * a.t.group, row0 = it.tile * a.t.tile_rows;
+    const int32_t row1 = min(row0 + a.t.tile_rows, n_rows) - 1;
+    const int32_t first = r.len - r.n + row0 / a.t.group, last = r.len - r.n + row1 / a.t.group;
+    const int32_t reach = min(r.len, paged_reach(a.p));
+    TileKeys k;
+    k.lo_min = key_lo(first, a.window);
+    k.lo_max = key_lo(last, a.window);
+    k.hi_min = min(first + 1, reach);
+    k.hi_max = min(last + 1, reach);
+    const int64_t per = static_cast<int64_t>(it.chunk) * a.t.unit, from = (k.lo_min & ~31) + it.split * per;
+    const int64_t to = from + per < k.hi_max ? from + per : k.hi_max;
+    k.k0 = static_cast<int32_t>(from < (1 << 30) ? from : 1 << 30);
+    k.k1 = static_cast<int32_t>(to);
+    return k;
+}
+
+// cap * tanh(s / cap) to a few roundings of the value: Lambert's continued fraction for tanh, cut after its fifth
+// term, up to 0.9 (off by 0.9^10 / (945^2 * 11) = 4e-8 there, relative), 1 - 2 / (e^2x + 1) past it. (The latter
+// alone is off by 2^-24 * cap whatever the score: 1.5e-6 of the results of prompts of up to 2048 keys with a cap of 50, 4.1e-7 now.)
+__device__ __forceinline__ float cap_score(float s, float cap, float inv_cap) {
+    const float x = s * inv_cap, x2 = x * x;
+    const float n = __builtin_fmaf(x2, 105.0f + x2, 945.0f), d = __builtin_fmaf(x2, __builtin_fmaf(x2, 15.0f, 420.0f), 945.0f);
+    const float near = s * n * __builtin_amdgcn_rcpf(d);
+    const float far = cap * (1.0f - 2.0f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x * (2.0f * kAttnLog2e)) + 1.0f));
+    return fabsf(x) < 0.9f ? near : far;
+}
+
+__device__ __forceinline__ float swap16_max(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
+}
+__device__ __forceinline__ float swap32_max(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
+}
+__device__ __forceinline__ float swap16_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return __builtin_bit_cast(float, static_cast<uint32_t>(r[0])) + __builtin_bit_cast(float, static_cast<uint32_t>(r[1]));
+}
+__device__ __forceinline__ float swap32_sum(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    return __builtin_bit_cast(float, static_cast<uint32_t>(r[0])) + __builtin_bit_cast(float, static_cast<uint32_t>(r[1]));
+}
+
+// The bytes of x that are NaN codes, as 0x80 each.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// acc / l of a finished row: zeros where it saw nothing, NaN where every score it saw was -inf.
+__device__ __forceinline__ float row_factor(float l, bool seen) {
+    return l == 0.0f ? (seen ? __builtin_nanf("") : 0.0f) : 1.0f / (l * kPScale);
+}
+
+}  // namespace neko_hip

@@ -89,6 +89,19 @@ int launch_store_kv(neko_hip_ctx* ctx, const char* what, const void* qkv, int64_
                     int64_t rows, int64_t width, int64_t pos0, const int32_t* positions, uint16_t* k_cache,
                     uint16_t* v_cache, int64_t cache_rows, int dtype);
 
+// The paged KV cache (paged.h): checks a cache and a batch of `rows` new rows and fills the launch arguments;
+// whether [p, p + bytes) shares a byte with the cache.
+struct Paged;
+int paged_args(neko_hip_ctx* ctx, const char* what, const neko_paged_kv* kv, const neko_paged_batch* batch, int64_t rows,
+               Paged* p);
+bool paged_overlaps(const neko_paged_kv& kv, const void* p, size_t bytes);
+inline size_t paged_code_bytes(const neko_paged_kv& kv) {
+    return static_cast<size_t>(kv.n_pages) * static_cast<size_t>(kv.n_kv) * static_cast<size_t>(kv.page_size) * static_cast<size_t>(kv.hd);
+}
+inline size_t paged_scale_bytes(const neko_paged_kv& kv) {
+    return static_cast<size_t>(kv.n_pages) * static_cast<size_t>(kv.n_kv) * sizeof(float);
+}
+
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 // Byte ranges [a, a + an) and [b, b + bn) share a byte.

@@ -16,10 +16,11 @@ import threading
 import numpy as np
 import torch
 
-from ._lib import DT_F16, DT_F32, FMT_F16, FMT_FP4, FMT_FP8, NEKO_OK, NekoError, lib
+from ._lib import DT_F16, DT_F32, FMT_F16, FMT_FP4, FMT_FP8, NEKO_OK, NekoError, PagedBatch, PagedKv, lib
 
 __all__ = [
     "Context", "context", "layer_norm", "rms_norm", "qk_norm_rope", "qk_norm_rope_kv", "store_kv", "add_rms_norm",
+    "PagedKV", "qk_norm_rope_paged", "attention_paged",
     "silu_mul", "gelu", "gated_rms_norm", "embed", "matmul", "MM_GELU", "MM_ACCUMULATE",
     "prepare", "quantize", "quant_row_bytes", "quantize_rows", "rope_table", "FMT_F16", "FMT_FP8", "FMT_FP4", "NekoError",
 ]
@@ -304,6 +305,109 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_h
     ctx = _ctx_for(q)
     _issue(ctx, lib.neko_hip_attention, ctx.handle, q.data_ptr(), qs, k_cache.data_ptr(), v_cache.data_ptr(),
            out.data_ptr(), out.stride(0), T, int(n_head), int(n_kv), int(hd), int(pos0), float(scale), _dtype_code(q))
+    return out
+
+
+class PagedKV:
+    """A paged 8-bit KV cache (include/neko_hip.h): pages of float8_e4m3fn codes [n_pages, n_kv, page_size, hd] for
+    keys and for values, and float32 power-of-two scales [n_pages, n_kv]; a cached value is code * scale."""
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, k_scales: torch.Tensor, v_scales: torch.Tensor):
+        device = k_pages.device
+        for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
+            _on(t, name, device)
+            if t.dtype != torch.float8_e4m3fn or t.dim() != 4 or not t.is_contiguous() or t.shape != k_pages.shape:
+                raise NekoError(f"{name} must be a contiguous float8_e4m3fn [n_pages, n_kv, page_size, hd] tensor, the same for k and v")
+        for t, name in ((k_scales, "k_scales"), (v_scales, "v_scales")):
+            _on(t, name, device)
+            if t.dtype != torch.float32 or not t.is_contiguous() or t.shape != k_pages.shape[:2]:
+                raise NekoError(f"{name} must be a contiguous float32 [n_pages, n_kv] tensor")
+        self.k_pages, self.v_pages, self.k_scales, self.v_scales = k_pages, v_pages, k_scales, v_scales
+        self.n_pages, self.n_kv, self.page_size, self.hd = k_pages.shape
+        self.device = device
+        self.c = PagedKv(k_pages.data_ptr(), v_pages.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(), self.n_pages,
+                         self.page_size, self.n_kv, self.hd)
+
+    @classmethod
+    def empty(cls, n_pages: int, page_size: int, n_kv: int, hd: int, device="cuda") -> "PagedKV":
+        """A cache that holds nothing yet."""
+        pages = [torch.zeros((n_pages, n_kv, page_size, hd), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+                 for _ in range(2)]
+        return cls(*pages, *(torch.ones((n_pages, n_kv), dtype=torch.float32, device=device) for _ in range(2)))
+
+
+def _paged_batch(page_table: torch.Tensor, row_start: torch.Tensor, kv_len: torch.Tensor, device) -> PagedBatch:
+    for t, name in ((page_table, "page_table"), (row_start, "row_start"), (kv_len, "kv_len")):
+        _on(t, name, device)
+        if t.dtype != torch.int32:
+            raise NekoError(f"{name} must be int32, got {t.dtype}")
+    if page_table.dim() != 2 or page_table.shape[1] == 0 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise NekoError("page_table must be [n_seq, max_pages] with unit stride along rows")
+    n_seq, max_pages = page_table.shape
+    if n_seq == 0 or row_start.shape != (n_seq + 1,) or kv_len.shape != (n_seq,) or not row_start.is_contiguous() or \
+            not kv_len.is_contiguous():
+        raise NekoError(f"row_start and kv_len must be contiguous, of {n_seq + 1} and {n_seq} entries for {n_seq} sequences (at least one)")
+    stride = page_table.stride(0) if n_seq > 1 else max(page_table.stride(0), max_pages)
+    return PagedBatch(page_table.data_ptr(), stride, max_pages, row_start.data_ptr(), kv_len.data_ptr(), n_seq)
+
+
+def qk_norm_rope_paged(qkv: torch.Tensor, n_q: int, cache: PagedKV, page_table: torch.Tensor, row_start: torch.Tensor,
+                       kv_len: torch.Tensor, cs: torch.Tensor | None, eps: float, wqk: torch.Tensor | None = None,
+                       interleaved: bool = False, q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """q / k heads of the batch's new rows normed (wqk) and rotated (cs: float32 [n_pos, rot_dim]; None: not), k and v
+    appended to the sequences' pages in 8 bits; returns the q rows [rows, n_q * hd]. row_start: int32 [n_seq + 1];
+    kv_len: int32 [n_seq], lengths with the new rows; page_table: int32 [n_seq, max_pages]. q_out may be qkv's own q
+    columns. Rows of no sequence, or at positions outside the table, leave their q_out row as it was (zeros in a new one)."""
+    rows, width, stride = _rows(qkv, "qkv")
+    _on(cache.k_pages, "cache", qkv.device)
+    hd, n_kv = cache.hd, cache.n_kv
+    if width < (n_q + 2 * n_kv) * hd:
+        raise NekoError(f"qkv rows hold {width} values, fewer than {n_q + 2 * n_kv} heads x {hd}")
+    batch = _paged_batch(page_table, row_start, kv_len, qkv.device)
+    n_pos = rot = 0
+    if cs is not None:
+        _on(cs, "cs", qkv.device)
+        if cs.dtype != torch.float32 or not cs.is_contiguous() or cs.dim() != 2:
+            raise NekoError("cs must be a contiguous float32 [n_pos, rot_dim] table")
+        n_pos, rot = cs.shape
+    if q_out is None:
+        q_out = torch.zeros((rows, n_q * hd), dtype=qkv.dtype, device=qkv.device)
+    else:
+        q_out = _out_like(qkv, rows, n_q * hd, q_out, "q_out")
+    ctx = _ctx_for(qkv)
+    _issue(ctx, lib.neko_hip_qk_norm_rope_paged, ctx.handle, qkv.data_ptr(), stride if rows > 1 else max(stride, width), rows,
+           int(n_q), ctypes.byref(cache.c), ctypes.byref(batch), _vec(wqk, 2 * hd, "wqk", qkv.device),
+           None if cs is None else cs.data_ptr(), n_pos, rot, 1 if interleaved else 0, float(eps), q_out.data_ptr(),
+           q_out.stride(0) if rows > 1 else max(q_out.stride(0), n_q * hd), _dtype_code(qkv))
+    return q_out
+
+
+def attention_paged(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, row_start: torch.Tensor, kv_len: torch.Tensor,
+                    n_head: int, scale: float | None = None, softcap: float = 0.0, window: int = 0,
+                    slopes: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal grouped-query attention of the batch's rows (as in qk_norm_rope_paged, which has appended them) over their
+    sequences' pages: scores scale * q.k (default 1/sqrt(hd)), capped by softcap * tanh(s / softcap) if softcap > 0,
+    plus slopes[head] * (j - position) if slopes are given, over at most `window` keys if window > 0. Returns
+    [rows, n_head * hd] in q's dtype; rows of no sequence are not written (zeros in a new out)."""
+    rows, width, qs = _rows(q, "q")
+    _on(cache.k_pages, "cache", q.device)
+    hd = cache.hd
+    if n_head <= 0 or n_head % cache.n_kv:
+        raise NekoError("n_head must be a positive multiple of n_kv")
+    if width < n_head * hd:
+        raise NekoError(f"q rows hold {width} values, fewer than {n_head} heads x {hd}")
+    batch = _paged_batch(page_table, row_start, kv_len, q.device)
+    if out is None:
+        out = torch.zeros((rows, n_head * hd), dtype=q.dtype, device=q.device)
+    else:
+        out = _out_like(q, rows, n_head * hd, out, "out")
+    if scale is None:
+        scale = float(np.float32(1.0) / np.sqrt(np.float32(hd)))
+    ctx = _ctx_for(q)
+    _issue(ctx, lib.neko_hip_attention_paged, ctx.handle, q.data_ptr(), qs if rows > 1 else max(qs, width), rows,
+           ctypes.byref(cache.c), ctypes.byref(batch), int(n_head), float(scale), float(softcap), int(window),
+           _vec(slopes, n_head, "slopes", q.device), out.data_ptr(), out.stride(0) if rows > 1 else max(out.stride(0), width),
+           _dtype_code(q))
     return out
 
 
