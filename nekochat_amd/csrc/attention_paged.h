@@ -160,4 +160,9 @@ __device__ __forceinline__ float row_factor(float l, bool seen) {
     return l == 0.0f ? (seen ? __builtin_nanf("") : 0.0f) : 1.0f / (l * kPScale);
 }
 
+// The kernel for many rows per sequence (attention_paged_tile.hip): its tiling, into a.t, and its launch of a.blocks
+// workgroups.
+void attn_paged_tile_form(const neko_hip_ctx* ctx, PagedAttnArgs& a);
+int attn_paged_tile(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a, int dtype);
+
 }  // namespace neko_hip

@@ -25,6 +25,7 @@ namespace {
 constexpr int kWaves = 4;
 constexpr int kTileRows = 16;
 constexpr int kUnit = 32 * kWaves;  // keys of a split: a whole tile for every wave
+constexpr int kFewRows = 32;        // flattened rows up to which a sequence is this kernel's
 
 template <int N>
 struct Words {
@@ -430,36 +431,71 @@ __global__ __launch_bounds__(256) void attn_paged_merge(PagedAttnArgs a) {
     }
 }
 
+// Workgroups and tiles of a launch, from its tiling.
+struct Grid {
+    int64_t blocks, tiles;
+    size_t bytes;  // of partial results
+};
+Grid grid_of(const PagedAttnArgs& a, int dh) {
+    Grid g;
+    g.blocks = attn_blocks_bound(a.t, a.p.rows, a.p.n_seq, a.p.n_kv) * a.p.n_kv;
+    g.tiles = attn_tiles_bound(a.t, a.p.rows, a.p.n_seq) * a.p.n_kv;
+    g.bytes = static_cast<size_t>(g.blocks) * a.t.tile_rows * (dh + 4) * sizeof(float);
+    return g;
+}
+
 template <typename TQ, int DH>
-int launch_rows16(neko_hip_ctx* ctx, const char* what, PagedAttnArgs a) {
-    a.t.tile_rows = kTileRows;
-    a.t.unit = kUnit;
-    a.t.target = 4 * ctx->cu_count;
-    a.t.min_rows = 1;
-    a.t.max_rows = 0x7fffffff;
-    const int64_t blocks = attn_blocks_bound(a.t, a.p.rows, a.p.n_seq, a.p.n_kv) * a.p.n_kv;
-    const int64_t tiles = attn_tiles_bound(a.t, a.p.rows, a.p.n_seq) * a.p.n_kv;
-    NEKO_REQUIRE(ctx, blocks <= 0x7fffffff, "%s: grid too large", what);
-    a.blocks = static_cast<uint32_t>(blocks);
+int launch_dims(neko_hip_ctx* ctx, const char* what, PagedAttnArgs a, int dtype) {
+    // Sequences of up to kFewRows rows on the 16-row kernel, the rest on the tiles. Which a batch has is known on the
+    // device alone, so both are launched, except where no sequence can be the other's: one sequence, or as many rows
+    // as sequences (then any that has more than one is the 16-row kernel's too).
+    const int64_t most = static_cast<int64_t>(a.p.rows) * a.t.group;
+    const bool few = a.p.n_seq > 1 || most <= kFewRows;
+    const bool many = most > kFewRows && a.p.rows > a.p.n_seq;
+    PagedAttnArgs f = a, t = a;
+    f.t.tile_rows = kTileRows;
+    f.t.unit = kUnit;
+    f.t.target = 4 * ctx->cu_count;
+    f.t.min_rows = 1;
+    f.t.max_rows = many ? kFewRows : 0x7fffffff;
+    attn_paged_tile_form(ctx, t);
+    t.t.min_rows = few ? kFewRows + 1 : 1;
+    t.t.max_rows = 0x7fffffff;
+    const Grid fg = few ? grid_of(f, DH) : Grid{}, tg = many ? grid_of(t, DH) : Grid{};
+    NEKO_REQUIRE(ctx, fg.blocks <= 0x7fffffff && tg.blocks <= 0x7fffffff, "%s: grid too large", what);
     void* ws = nullptr;
-    if (int rc = workspace(ctx, static_cast<size_t>(blocks) * kTileRows * (DH + 4) * sizeof(float), &ws)) return rc;
-    a.part = static_cast<float*>(ws);
-    a.ml = a.part + blocks * kTileRows * DH;
+    if (int rc = workspace(ctx, fg.bytes + tg.bytes, &ws)) return rc;
     const bool mods = a.softcap > 0.0f || a.slopes;
-    if (mods) hipLaunchKernelGGL((attn_paged_kernel<TQ, DH, true>), dim3(a.blocks), dim3(256), 0, ctx->stream, a);
-    else hipLaunchKernelGGL((attn_paged_kernel<TQ, DH, false>), dim3(a.blocks), dim3(256), 0, ctx->stream, a);
-    if (int rc = after_launch(ctx, what)) return rc;
-    // Lengths within one unit are never split.
-    if (paged_reach(a.p) <= kUnit) return NEKO_OK;
-    hipLaunchKernelGGL((attn_paged_merge<TQ, DH>), dim3(static_cast<uint32_t>(tiles)), dim3(256), 0, ctx->stream, a);
-    return after_launch(ctx, what);
+    auto place = [](PagedAttnArgs& x, const Grid& g, void* at) {
+        x.blocks = static_cast<uint32_t>(g.blocks);
+        x.part = static_cast<float*>(at);
+        x.ml = x.part + g.blocks * x.t.tile_rows * DH;
+    };
+    auto merge = [&](const PagedAttnArgs& x, const Grid& g) {
+        if (paged_reach(x.p) <= x.t.unit) return NEKO_OK;  // lengths within one unit are never split
+        hipLaunchKernelGGL((attn_paged_merge<TQ, DH>), dim3(static_cast<uint32_t>(g.tiles)), dim3(256), 0, ctx->stream, x);
+        return after_launch(ctx, what);
+    };
+    if (many) {
+        place(t, tg, static_cast<char*>(ws) + fg.bytes);
+        if (int rc = attn_paged_tile(ctx, what, t, dtype)) return rc;
+        if (int rc = merge(t, tg)) return rc;
+    }
+    if (few) {
+        place(f, fg, ws);
+        if (mods) hipLaunchKernelGGL((attn_paged_kernel<TQ, DH, true>), dim3(f.blocks), dim3(256), 0, ctx->stream, f);
+        else hipLaunchKernelGGL((attn_paged_kernel<TQ, DH, false>), dim3(f.blocks), dim3(256), 0, ctx->stream, f);
+        if (int rc = after_launch(ctx, what)) return rc;
+        if (int rc = merge(f, fg)) return rc;
+    }
+    return NEKO_OK;
 }
 
 template <typename TQ>
-int launch_typed(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a) {
-    if (a.p.hd <= 64) return launch_rows16<TQ, 64>(ctx, what, a);
-    if (a.p.hd <= 128) return launch_rows16<TQ, 128>(ctx, what, a);
-    return launch_rows16<TQ, 256>(ctx, what, a);
+int launch_typed(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a, int dtype) {
+    if (a.p.hd <= 64) return launch_dims<TQ, 64>(ctx, what, a, dtype);
+    if (a.p.hd <= 128) return launch_dims<TQ, 128>(ctx, what, a, dtype);
+    return launch_dims<TQ, 256>(ctx, what, a, dtype);
 }
 
 }  // namespace
@@ -503,5 +539,5 @@ extern "C" int neko_hip_attention_paged(neko_hip_ctx* ctx, const void* q, int64_
     a.scale = scale;
     a.softcap = softcap;
     a.slopes = slopes;
-    return dtype == NEKO_DT_F16 ? launch_typed<half_t>(ctx, what, a) : launch_typed<float>(ctx, what, a);
+    return dtype == NEKO_DT_F16 ? launch_typed<half_t>(ctx, what, a, dtype) : launch_typed<float>(ctx, what, a, dtype);
 }

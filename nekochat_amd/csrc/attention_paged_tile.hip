@@ -1,0 +1,468 @@
+// Paged attention for many rows per sequence -- prompts and chunks of them -- on the matrix cores of gfx950.
+//
+// Formulas and scales as in attention_paged.hip. A workgroup's waves hold 32 flattened (token, head) rows each, the
+// columns of v_mfma_f32_32x32x16_f16, and share tiles of keys in LDS, converted to f16 once on the way in: a code is
+// converted once per 128 rows instead of once per wave, and the pipeline needs one barrier a tile (tile t + 1 is
+// written while t is read, and t + 2 is on its way from the pages in registers). S^T = K Q^T leaves a lane with the
+// scores of one row and, by the permutation that the contraction index is free to take, exactly the B operand of
+// O^T = V^T P^T; V^T comes from LDS by transposing reads. Eight consecutive scores of a lane are of one 16-key block,
+// hence of one page: its scales are the same for all lanes.
+//
+// Precision: f16 calls round each weight to f16 (2^-11 of it, the largest term of O being 1; as large as the rounding
+// of the result) and sum the weights before that, in f32: those of a page of small values may carry the sum and be
+// nothing in O. f32 calls split weights and q into two f16 each.
+#include <algorithm>
+#include <atomic>
+
+#include "attention_paged.h"
+
+namespace neko_hip {
+namespace {
+
+typedef short short4v __attribute__((ext_vector_type(4)));
+
+// The slot of 16-byte chunk c of tile row `row` in LDS: the 16 rows of a ds_read_b128 pass at one chunk of K, and
+// the 4 rows x 4 chunks of half a transposing read of V, fall on distinct banks.
+template <int DH>
+__device__ __forceinline__ int k_slot(int row, int c) {
+    return DH >= 128 ? c ^ (row & 15) : c ^ ((row >> 1) & 7);
+}
+template <int DH>
+__device__ __forceinline__ int v_slot(int row, int c) {
+    return DH >= 128 ? c ^ ((row & 3) << 2) : c ^ ((row & 2) << 1);
+}
+
+template <int DH>
+struct TileForm {
+    static constexpr int waves = 4, rows = 32 * waves;
+    static constexpr int keys = DH <= 128 ? 64 : 32;  // (256 dimensions: 32, for LDS)
+    static constexpr int blocks = keys / kBlockKeys;  // pages' parts of a tile
+    static constexpr int units = 2 * blocks / waves;  // (block, K or V) pairs that a wave brings in
+    static constexpr int half_bytes = keys * DH * 2;
+    static constexpr int lds = 4 * half_bytes;         // two buffers of K and V
+    static constexpr int window = 64 / blocks;         // tiles of a page look-up
+    static constexpr int rpi = 64 * 16 / DH;           // rows of a load instruction
+    static constexpr int loads = kBlockKeys / rpi;     // load instructions of a unit
+};
+
+// A block's exponents and whether it has a page, in one scalar.
+__device__ __forceinline__ int pack_block(int ke, int ve, bool ok) { return (ke + 128) | (ve + 128) << 8 | (ok ? 1 << 16 : 0); }
+__device__ __forceinline__ int block_ke(int x) { return (x & 255) - 128; }
+__device__ __forceinline__ int block_ve(int x) { return ((x >> 8) & 255) - 128; }
+
+template <typename TQ, int DH, bool MODS>
+__global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel(PagedAttnArgs a) {
+    typedef TileForm<DH> C;
+    constexpr bool kTwo = sizeof(TQ) == 4;
+    constexpr int NS = DH / 16, ND = DH / 32, KB = C::keys / 32;
+    extern __shared__ __align__(16) uint8_t tile_lds[];
+    __shared__ uint32_t nan_sh[2][C::waves];           // whether a wave took NaN values out of the tile,
+    __shared__ uint32_t nan_bits[2][C::keys][DH / 32];  // and where
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
+    const int l32 = lane & 31, h = lane >> 5;
+    const int kvh = static_cast<int>(blockIdx.x % static_cast<uint32_t>(a.p.n_kv));
+    AttnItem it;
+    if (!attn_find<false>(a.p, a.t, blockIdx.x / static_cast<uint32_t>(a.p.n_kv), &it)) return;
+    const SeqRows r = paged_seq(a.p, it.s);
+    const TileKeys tk = tile_keys(a, r, it);
+    const int hd = a.p.hd;
+    const int32_t reach = min(r.len, paged_reach(a.p));
+
+    // This lane's row, and the keys that this wave's rows see (rows past the last repeat it).
+    const int32_t n_rows = r.n * a.t.group, row0 = it.tile * C::rows + 32 * wave;
+    const int32_t row = min(row0 + l32, n_rows - 1);
+    const int32_t tok = row / a.t.group;
+    const int head = kvh * a.t.group + (row - tok * a.t.group);
+    const int32_t pos = r.len - r.n + tok;
+    const int32_t hi = min(pos + 1, reach), lo = key_lo(pos, a.window);
+    const int32_t w_first = r.len - r.n + min(row0, n_rows - 1) / a.t.group, w_last = r.len - r.n + min(row0 + 31, n_rows - 1) / a.t.group;
+    const int32_t w_lo_min = key_lo(w_first, a.window), w_lo_max = key_lo(w_last, a.window);
+    const int32_t w_hi_min = min(w_first + 1, reach), w_hi_max = min(w_last + 1, reach);
+
+    // q: dimensions 16 s + 8 h .. + 7 of the row as the B operand of step s.
+    half8 qh[NS], ql[kTwo ? NS : 1];
+    float sc = a.scale == 0.0f ? 1.0f : fabsf(a.scale);
+    {
+        const TQ* qr = static_cast<const TQ*>(a.q) + static_cast<int64_t>(r.begin + tok) * a.qs + static_cast<int64_t>(head) * hd;
+        const float sign = a.scale == 0.0f ? 0.0f : a.scale < 0.0f ? -1.0f : 1.0f;
+        float x[NS][8];
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            const int d = 16 * s + 8 * h;
+            TQ v[8];
+            if (d < hd) __builtin_memcpy(v, qr + d, sizeof(v));
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[s][e] = d < hd ? to_f32(v[e]) * sign : 0.0f;
+        }
+        if constexpr (kTwo) {
+            float mx = 0.0f;
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[s][e]));
+            mx = swap32_max(mx);
+            const int ex = mx > 0.0f && mx < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(mx) : 0;
+            const int e1 = ex / 2, e2 = ex - e1;
+            sc = ldexpf(sc, -ex);
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[s][e] = ldexpf(ldexpf(x[s][e], e1), e2);
+        }
+#pragma unroll
+        for (int s = 0; s < NS; s++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                qh[s][e] = static_cast<half_t>(x[s][e]);
+                if constexpr (kTwo) ql[s][e] = static_cast<half_t>(x[s][e] - to_f32(qh[s][e]));
+            }
+    }
+    const float slope = MODS && a.slopes ? a.slopes[head] : 0.0f;
+    const float inv_cap = MODS && a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+
+    // Pages of the next 64 blocks, one to a lane; those after them are asked for half a window ahead.
+    const int nt = tk.k1 > tk.k0 ? (tk.k1 - tk.k0 + C::keys - 1) / C::keys : 0;
+    int32_t page = -1, next_page = -1;
+    int exps = pack_block(0, 0, false);
+    float next_ks = 1.0f, next_vs = 1.0f;
+    auto ask_pages = [&](int tile) {
+        const int32_t at = tk.k0 + C::keys * tile + kBlockKeys * lane;
+        next_page = -1;
+        if (tile < nt && at < tk.k1) next_page = paged_page(a.p, it.s, at);
+    };
+    auto ask_scales = [&]() {
+        const int64_t i = static_cast<int64_t>(next_page < 0 ? 0 : next_page) * a.p.n_kv + kvh;
+        next_ks = a.p.ks[i];
+        next_vs = a.p.vs[i];
+    };
+    auto take_pages = [&]() {
+        page = next_page;
+        exps = page < 0 ? pack_block(0, 0, false) : pack_block(scale_exp(next_ks), scale_exp(next_vs), true);
+    };
+
+    // Units of a tile: block u % blocks, K below u = blocks. Lane (row, 16-byte chunk) of each load.
+    const int lr = lane / (DH / 16), lc = lane % (DH / 16);
+    const int src = lc * 16 < hd ? lc * 16 : 0;  // dimensions past the head's end: any of its own, against zeros in q
+    struct Raw {
+        uint4v x[C::units][C::loads];
+    };
+    Raw raw;
+    int info[C::blocks], info1[C::blocks];  // of the tile in `raw`, of the tile after the one being multiplied
+    auto load = [&](int tile) __attribute__((always_inline)) {
+        const int at = tile % C::window * C::blocks;
+#pragma unroll
+        for (int b = 0; b < C::blocks; b++) info[b] = __builtin_amdgcn_readlane(exps, at + b);
+#pragma unroll
+        for (int i = 0; i < C::units; i++) {
+            const int u = wave * C::units + i, b = u % C::blocks;
+            const int id = __builtin_amdgcn_readlane(page, at + b);
+            const int32_t slot = (tk.k0 + C::keys * tile + kBlockKeys * b) & ((1 << a.p.page_log2) - 1);
+            const uint8_t* from = (u < C::blocks ? a.p.k : a.p.v) +
+                                  (((static_cast<int64_t>(id < 0 ? 0 : id) * a.p.n_kv + kvh) << a.p.page_log2) + slot) * hd;
+#pragma unroll
+            for (int n = 0; n < C::loads; n++) raw.x[i][n] = *reinterpret_cast<const uint4v*>(from + ((n * C::rpi + lr) * hd + src));
+        }
+    };
+    // The tile in `raw` to LDS. A NaN value times a weight of zero is NaN, so in tiles of which some row does not see
+    // all, values that no row sees become zeros (they may be codes of no token), and NaN values are taken out and noted.
+    auto store = [&](int tile, int buf) __attribute__((always_inline)) {
+        const int32_t j0 = tk.k0 + C::keys * tile;
+        const bool differ = j0 < tk.lo_max || j0 + C::keys > tk.hi_min;
+        bool whole = !differ;
+#pragma unroll
+        for (int b = 0; b < C::blocks; b++) whole = whole && (info[b] >> 16);
+        uint32_t bad = 0;
+#pragma unroll
+        for (int i = 0; i < C::units; i++) {
+            const int u = wave * C::units + i, b = u % C::blocks;
+            const bool is_v = u >= C::blocks;
+            uint8_t* to = tile_lds + buf * 2 * C::half_bytes + (is_v ? C::half_bytes : 0);
+#pragma unroll
+            for (int n = 0; n < C::loads; n++) {
+                const int row = b * kBlockKeys + n * C::rpi + lr;
+                uint4v x = raw.x[i][n];
+                if (is_v && !whole) {
+                    const int32_t j = j0 + row;
+                    if (!(info[b] >> 16) || j < tk.lo_min || j >= tk.hi_max) x = uint4v{0, 0, 0, 0};
+                    uint32_t at = 0;  // a bit for each NaN code
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        const uint32_t nan = nan_codes(x[w]) >> 7;
+                        x[w] &= ~(nan * 0xffu);
+                        at |= ((nan * 0x01020408u) >> 24) << (4 * w);
+                    }
+                    reinterpret_cast<uint16_t*>(nan_bits[buf][row])[lc] = static_cast<uint16_t>(at);
+                    bad |= at;
+                }
+#pragma unroll
+                for (int p = 0; p < 2; p++) {
+                    half8 y;
+#pragma unroll
+                    for (int w = 0; w < 2; w++) {
+                        const half2v y0 = f16_of_fp8<false>(x[2 * p + w]), y1 = f16_of_fp8<true>(x[2 * p + w]);
+                        y[4 * w] = y0[0];
+                        y[4 * w + 1] = y0[1];
+                        y[4 * w + 2] = y1[0];
+                        y[4 * w + 3] = y1[1];
+                    }
+                    const int c = 2 * lc + p;
+                    *reinterpret_cast<half8*>(to + row * DH * 2 + 16 * (is_v ? v_slot<DH>(row, c) : k_slot<DH>(row, c))) = y;
+                }
+            }
+        }
+        if (!whole) {
+            const bool any = __any(bad != 0);
+            if (lane == 0) nan_sh[buf][wave] = any;
+        }
+    };
+
+    float16v o[ND] = {};
+    float m = -__builtin_inff(), l = 0.0f;
+    bool seen = false;
+    const int tq = lane & 15, tkr = tq >> 2;  // transposing reads: this lane's row of four, dimensions 4 (tq & 3)
+    auto v_frag = [&](const uint8_t* vd, int d, int b, int i) __attribute__((always_inline)) {
+        const int ch = 4 * d + 2 * ((lane >> 4) & 1) + ((tq & 3) >> 1);
+        const int row = 32 * b + 16 * i + 4 * h + tkr;
+        const uint8_t* p0 = vd + row * DH * 2 + 16 * v_slot<DH>(row, ch) + 8 * (tq & 1);
+        const short4v a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)p0);
+        const short4v a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(p0 + 8 * DH * 2));
+        return __builtin_bit_cast(half8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    auto step = [&](int tile, int buf, const int (&in)[C::blocks]) __attribute__((always_inline)) {
+        const int32_t j0 = tk.k0 + C::keys * tile;
+        if (j0 >= w_hi_max || j0 + C::keys <= w_lo_min) return;
+        const uint8_t* kd = tile_lds + buf * 2 * C::half_bytes;
+        const uint8_t* vd = kd + C::half_bytes;
+        float16v s[KB] = {};
+#pragma unroll
+        for (int b = 0; b < KB; b++) {
+            const int kr = 32 * b + l32;
+#pragma unroll
+            for (int d = 0; d < NS; d++) {
+                const half8 A = *reinterpret_cast<const half8*>(kd + kr * DH * 2 + 16 * k_slot<DH>(kr, 2 * d + h));
+                if constexpr (kTwo) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(A, ql[d], s[b], 0, 0, 0);
+                s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(A, qh[d], s[b], 0, 0, 0);
+            }
+        }
+        float f[C::blocks];
+        bool ok = true;
+#pragma unroll
+        for (int b = 0; b < C::blocks; b++) {
+            f[b] = sc * exp2i(block_ke(in[b]));
+            if constexpr (!MODS) f[b] *= kAttnLog2e;
+            f[b] = fminf(fmaxf(f[b], 0x1p-120f), 0x1p120f);
+            ok = ok && (in[b] >> 16);
+        }
+        if constexpr (MODS) {
+            const int32_t away = j0 + 4 * h - pos;
+#pragma unroll
+            for (int b = 0; b < KB; b++)
+                unrolled<16>([&](auto ec) {
+                    constexpr int e = decltype(ec)::value;
+                    float x = s[b][e] * f[2 * b + e / 8];
+                    if (a.softcap > 0.0f) x = cap_score(x, a.softcap, inv_cap);
+                    if (a.slopes) x = __builtin_fmaf(slope, static_cast<float>(away + 32 * b + 8 * (e >> 2) + (e & 3)), x);
+                    s[b][e] = x;
+                });
+#pragma unroll
+            for (int b = 0; b < C::blocks; b++) f[b] = kAttnLog2e;
+        }
+        const bool partial = j0 < w_lo_max || j0 + C::keys > w_hi_min || !ok;
+        if (partial) {
+            bool any = false;
+#pragma unroll
+            for (int b = 0; b < KB; b++)
+                unrolled<16>([&](auto ec) {
+                    constexpr int e = decltype(ec)::value;
+                    const int32_t j = j0 + 32 * b + 8 * (e >> 2) + 4 * h + (e & 3);
+                    const bool vis = (in[2 * b + e / 8] >> 16) && j >= lo && j < hi;
+                    if (!vis) s[b][e] = -__builtin_inff();
+                    any = any || vis;
+                });
+            seen = seen || any;
+        } else {
+            seen = true;
+        }
+        float top = -__builtin_inff();
+#pragma unroll
+        for (int b = 0; b < KB; b++)
+            unrolled<2>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                float mx = s[b][8 * i];
+                unrolled<7>([&](auto ec) { mx = fmaxf(mx, s[b][8 * i + 1 + decltype(ec)::value]); });
+                top = fmaxf(top, __builtin_fmaf(mx, f[2 * b + i], static_cast<float>(block_ve(in[2 * b + i]))));
+            });
+        top = ceilf(swap32_max(top));
+        if (__any(top > m)) {
+            const float mn = fmaxf(m, top);
+            const float corr = __builtin_amdgcn_exp2f(m - (mn == -__builtin_inff() ? 0.0f : mn));
+            m = mn;
+            l *= corr;
+#pragma unroll
+            for (int d = 0; d < ND; d++)
+                unrolled<16>([&](auto ec) { o[d][decltype(ec)::value] *= corr; });
+        }
+        const float ms = m == -__builtin_inff() ? 0.0f : m;
+        half8 ph[KB][2], pl[KB][2];
+#pragma unroll
+        for (int b = 0; b < KB; b++)
+            unrolled<2>([&](auto ic) {
+                constexpr int i = decltype(ic)::value;
+                const int ve = block_ve(in[2 * b + i]);
+                float sum = 0.0f;
+                if constexpr (kTwo) {
+                    const float base = static_cast<float>(ve) - ms;
+                    float p[8];
+                    unrolled<8>([&](auto ec) {
+                        constexpr int e = decltype(ec)::value;
+                        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * i + e], f[2 * b + i], base));
+                        const float y = p[e] * kPScale;
+                        ph[b][i][e] = static_cast<half_t>(y);
+                        pl[b][i][e] = static_cast<half_t>(y - to_f32(ph[b][i][e]));
+                    });
+                    sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                } else {
+                    // The offset joins the exponent: its rounding, 2^-21 of the weight, is nothing beside the weight's.
+                    const float base = static_cast<float>(ve + kPOffset) - ms;
+                    unrolled<8>([&](auto ec) {
+                        constexpr int e = decltype(ec)::value;
+                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * i + e], f[2 * b + i], base));
+                        ph[b][i][e] = static_cast<half_t>(p);
+                        sum += p;
+                    });
+                }
+                l = __builtin_fmaf(sum, exp2i(-ve), l);
+            });
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int b = 0; b < KB; b++)
+#pragma unroll
+                for (int i = 0; i < 2; i++) {
+                    const half8 A = v_frag(vd, d, b, i);
+                    if constexpr (kTwo) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(A, pl[b][i], o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(A, ph[b][i], o[d], 0, 0, 0);
+                }
+        // NaN values taken out of the tile, put into the dimensions of the rows that see them.
+        if (j0 < tk.lo_max || j0 + C::keys > tk.hi_min || !ok) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int w = 0; w < C::waves; w++) any |= nan_sh[buf][w];
+            if (__builtin_amdgcn_readfirstlane(any) != 0) {
+#pragma unroll 1
+                for (int k = 0; k < C::keys; k++) {
+                    if (j0 + k < lo || j0 + k >= hi) continue;
+#pragma unroll
+                    for (int d = 0; d < ND; d++) {
+                        const uint32_t bits = nan_bits[buf][k][d] >> (4 * h);
+                        unrolled<16>([&](auto ec) {
+                            constexpr int e = decltype(ec)::value;
+                            if ((bits >> (8 * (e >> 2) + (e & 3))) & 1u) o[d][e] = __builtin_nanf("");
+                        });
+                    }
+                }
+            }
+        }
+    };
+
+    if (nt > 0) {
+        ask_pages(0);
+        ask_scales();
+        take_pages();
+        ask_pages(C::window);
+        load(0);
+        store(0, 0);
+#pragma unroll
+        for (int b = 0; b < C::blocks; b++) info1[b] = info[b];
+        if (nt > 1) load(1);
+        __syncthreads();
+        for (int t = 0; t < nt; t++) {
+            int now[C::blocks];
+#pragma unroll
+            for (int b = 0; b < C::blocks; b++) {
+                now[b] = info1[b];
+                info1[b] = info[b];
+            }
+            if (t + 1 < nt) store(t + 1, (t + 1) & 1);  // that buffer's readers passed the barrier
+            if (t + 2 < nt) {
+                const int at = (t + 2) % C::window;
+                if (at == 0) {
+                    take_pages();
+                    ask_pages(t + 2 + C::window);
+                }
+                if (at == C::window / 2) ask_scales();
+                load(t + 2);
+            }
+            step(t, t & 1, now);
+            __syncthreads();
+        }
+    }
+
+    l = swap32_sum(l);
+    const bool any_seen = swap32_max(seen ? 1.0f : 0.0f) > 0.0f;
+    if (row0 + l32 >= n_rows) return;
+    const float l_by = kTwo ? 1.0f : 1.0f / kPScale;  // f16: the sum is of the weights times 2^kPOffset
+    if (it.splits == 1) {
+        const float by = row_factor(l * l_by, any_seen);
+        TQ* out = static_cast<TQ*>(a.out) + static_cast<int64_t>(r.begin + tok) * a.os + static_cast<int64_t>(head) * hd;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+            unrolled<4>([&](auto gc) {
+                constexpr int g = decltype(gc)::value;
+                const int at = 32 * d + 8 * g + 4 * h;
+                TQ v[4];
+                unrolled<4>([&](auto ec) {
+                    constexpr int e = decltype(ec)::value;
+                    v[e] = from_f32<TQ>(by == 0.0f ? 0.0f : o[d][4 * g + e] * by);
+                });
+                if (at < hd) __builtin_memcpy(out + at, v, sizeof(v));
+            });
+        return;
+    }
+    const uint32_t block = it.block * static_cast<uint32_t>(a.p.n_kv) + kvh;
+    if (block >= a.blocks) return;
+    const int64_t at = static_cast<int64_t>(block) * C::rows + 32 * wave + l32;
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+        unrolled<4>([&](auto gc) {
+            constexpr int g = decltype(gc)::value;
+            *reinterpret_cast<float4v*>(a.part + at * DH + 32 * d + 8 * g + 4 * h) =
+                float4v{o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
+        });
+    if (h == 0) *reinterpret_cast<float4v*>(a.ml + at * 4) = float4v{m, l * l_by, any_seen ? 1.0f : 0.0f, 0.0f};
+}
+
+template <typename TQ, int DH, bool MODS>
+int launch_tiles(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a) {
+    typedef TileForm<DH> C;
+    static std::atomic<uint64_t> allowed{0};
+    const void* kernel = reinterpret_cast<const void*>(&attn_paged_tile_kernel<TQ, DH, MODS>);
+    if (C::lds + 4096 > 64 * 1024)  // (with the kernel's static LDS)
+        if (int rc = allow_lds(ctx, kernel, C::lds, allowed)) return rc;
+    hipLaunchKernelGGL((attn_paged_tile_kernel<TQ, DH, MODS>), dim3(a.blocks), dim3(64 * C::waves), C::lds, ctx->stream, a);
+    return after_launch(ctx, what);
+}
+
+template <typename TQ, bool MODS>
+int launch_dims(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a) {
+    if (a.p.hd <= 64) return launch_tiles<TQ, 64, MODS>(ctx, what, a);
+    if (a.p.hd <= 128) return launch_tiles<TQ, 128, MODS>(ctx, what, a);
+    return launch_tiles<TQ, 256, MODS>(ctx, what, a);
+}
+
+}  // namespace
+
+void attn_paged_tile_form(const neko_hip_ctx* ctx, PagedAttnArgs& a) {
+    a.t.tile_rows = TileForm<128>::rows;
+    a.t.unit = 64;  // a whole number of tiles of either size
+    a.t.target = 2 * ctx->cu_count;
+}
+
+int attn_paged_tile(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a, int dtype) {
+    const bool mods = a.softcap > 0.0f || a.slopes;
+    if (dtype == NEKO_DT_F16) return mods ? launch_dims<half_t, true>(ctx, what, a) : launch_dims<half_t, false>(ctx, what, a);
+    return mods ? launch_dims<float, true>(ctx, what, a) : launch_dims<float, false>(ctx, what, a);
+}
+
+}  // namespace neko_hip
