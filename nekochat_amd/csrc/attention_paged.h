@@ -32,24 +32,23 @@ struct AttnItem {
     uint32_t block;  // index of the (tile, split) among those of a kv head
 };
 
-__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
-#pragma unroll
-    for (int m = 32; m > 0; m >>= 1) v += static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(v), m));
-    return v;
-}
-__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {  // inclusive
-    const int lane = static_cast<int>(threadIdx.x) & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t u = static_cast<uint32_t>(__shfl_up(static_cast<int>(v), d));
-        if (lane >= d) v += u;
-    }
+// Inclusive sum over the lanes below and at each (DPP: shifts within 16 lanes, then the rows' last lanes carried on).
+__device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
+    auto add = [&](auto ctrl, auto rows) {
+        v += static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), decltype(ctrl)::value, decltype(rows)::value, 0xF, false));
+    };
+    add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});  // row_shr 1, 2, 4, 8
+    add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast 15 into rows 1 and 3
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast 31 into rows 2 and 3
     return v;
 }
 
-// The item of workgroup j of a kv head (by_tile: the tile of merge workgroup j, its first split), by every wave for
-// itself: sequences' tiles and splits are summed 64 at a time. False past the last.
-template <bool BY_TILE>
+// The item of workgroup j of a kv head (SPLIT: the j-th tile that has splits, its first one), by every wave for itself:
+// sequences' tiles and splits are summed 64 at a time. False past the last.
+template <bool SPLIT>
 __device__ __forceinline__ bool attn_find(const Paged& p, const AttnTiling& t, uint32_t j, AttnItem* it) {
     const int32_t lane = static_cast<int32_t>(threadIdx.x) & 63;
     int32_t tiles = 0, units = 0;
@@ -61,20 +60,20 @@ __device__ __forceinline__ bool attn_find(const Paged& p, const AttnTiling& t, u
             units = attn_units(t, p, r);
         }
     };
-    uint64_t work = 0;
+    double work = 0.0;  // (whole numbers below 2^53: exact)
     for (int32_t base = 0; base < p.n_seq; base += 64) {
         load(base);
-        work += static_cast<uint64_t>(tiles) * static_cast<uint64_t>(units);
+        work += wave_sum_f64(static_cast<double>(tiles) * static_cast<double>(units));
     }
-    work = wave_sum_u64(work) * static_cast<uint64_t>(p.n_kv);
-    const int32_t chunk = attn_chunk(t, work);
+    const int32_t chunk = attn_chunk(t, static_cast<uint64_t>(work * p.n_kv));
     uint32_t past_tiles = 0, past = 0;
     for (int32_t base = 0; base < p.n_seq; base += 64) {
         if (p.n_seq > 64) load(base);
         const int32_t splits = attn_splits(units, chunk);
         const uint32_t n = static_cast<uint32_t>(tiles) * static_cast<uint32_t>(splits);
-        const uint32_t sum = wave_scan_u32(n), sum_tiles = BY_TILE ? wave_scan_u32(static_cast<uint32_t>(tiles)) : 0;
-        const uint64_t at = __ballot(BY_TILE ? past_tiles + sum_tiles > j : past + sum > j);
+        const uint32_t split_tiles = splits > 1 ? static_cast<uint32_t>(tiles) : 0;
+        const uint32_t sum = wave_scan_u32(n), sum_tiles = SPLIT ? wave_scan_u32(split_tiles) : 0;
+        const uint64_t at = __ballot(SPLIT ? past_tiles + sum_tiles > j : past + sum > j);
         if (at) {
             const int l = __builtin_ctzll(at);
             const int32_t n_tiles = __builtin_amdgcn_readlane(tiles, l);
@@ -82,8 +81,8 @@ __device__ __forceinline__ bool attn_find(const Paged& p, const AttnTiling& t, u
             it->chunk = chunk;
             it->splits = __builtin_amdgcn_readlane(splits, l);
             const uint32_t first = past + static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum - n), l));
-            if constexpr (BY_TILE) {
-                const uint32_t local = j - past_tiles - static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum_tiles) - tiles, l));
+            if constexpr (SPLIT) {
+                const uint32_t local = j - past_tiles - static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum_tiles - split_tiles), l));
                 it->tile = n_tiles - 1 - static_cast<int32_t>(local);
                 it->split = 0;
                 it->block = first + local * static_cast<uint32_t>(it->splits);
@@ -96,7 +95,7 @@ __device__ __forceinline__ bool attn_find(const Paged& p, const AttnTiling& t, u
             return true;
         }
         past += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum), 63));
-        if constexpr (BY_TILE) past_tiles += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum_tiles), 63));
+        if constexpr (SPLIT) past_tiles += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum_tiles), 63));
     }
     return false;
 }

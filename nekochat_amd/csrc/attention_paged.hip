@@ -16,15 +16,15 @@
 // are split into two f16 (24 bits of every weight above 2^-16 of the largest, 2^-39 of it below), f32 q as well, brought
 // to [2^14, 2^15) first; l and O are f32.
 #include <algorithm>
+#include <atomic>
 
 #include "attention_paged.h"
 
 namespace neko_hip {
 namespace {
 
-constexpr int kWaves = 4;
 constexpr int kTileRows = 16;
-constexpr int kUnit = 32 * kWaves;  // keys of a split: a whole tile for every wave
+constexpr int kLeast = 8;           // tiles of 32 keys to a wave below which no keys are split
 constexpr int kFewRows = 32;        // flattened rows up to which a sequence is this kernel's
 
 template <int N>
@@ -37,16 +37,30 @@ template <int DH>
 struct KvTile {
     uint4v k[2][DH / 64];
     Words<DH / 64> v[2][4];
-    int ke[2], ve[2];  // scale exponents of the two 16-key blocks
-    bool ok[2];        // whether they have a page
 };
 
-template <typename TQ, int DH, bool MODS>
-__global__ __launch_bounds__(256) void attn_paged_kernel(PagedAttnArgs a) {
+// Waves per SIMD that the kernel is compiled for.
+template <typename TQ, int DH>
+constexpr int kResident = DH <= 64 ? 4 : DH <= 128 ? (sizeof(TQ) == 2 ? 4 : 3) : 2;
+
+// Four dimensions, from d on, of a finished row.
+template <typename TQ>
+__device__ __forceinline__ void store_row(const PagedAttnArgs& a, const SeqRows& r, int kvh, int32_t row, int d, float4v x, float by) {
+    const int32_t tok = row / a.t.group;
+    const int head = kvh * a.t.group + (row - tok * a.t.group);
+    TQ v[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) v[e] = from_f32<TQ>(by == 0.0f ? 0.0f : x[e] * by);
+    __builtin_memcpy(static_cast<TQ*>(a.out) + static_cast<int64_t>(r.begin + tok) * a.os + static_cast<int64_t>(head) * a.p.hd + d, v, sizeof(v));
+}
+
+template <typename TQ, int DH, int NW, bool MODS>
+__global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kResident<TQ, DH>)) void attn_paged_kernel(PagedAttnArgs a) {
     constexpr bool kTwo = sizeof(TQ) == 4;
     constexpr int NU = DH / 64, NE = DH / 16, VW = DH / 64;
-    __shared__ float m_sh[kWaves][16], l_sh[kWaves][16], seen_sh[kWaves][16];
-    __shared__ float o_sh[kWaves][4][DH <= 128 ? NE : NE / 2][64];
+    constexpr int kRow = DH + 4;  // floats of a row in LDS
+    extern __shared__ __align__(16) float o_sh[];  // [NW][16][kRow]
+    __shared__ float m_sh[NW][16], l_sh[NW][16], seen_sh[NW][16];
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
     const int c = lane & 15, g4 = lane >> 4;
@@ -108,7 +122,7 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(PagedAttnArgs a) {
 
     // This wave's tiles of 32 keys, from key kw on.
     const int nt = tk.k1 > tk.k0 ? (tk.k1 - tk.k0 + 31) / 32 : 0;
-    const int per = (nt + kWaves - 1) / kWaves;
+    const int per = (nt + NW - 1) / NW;
     const int32_t kw = tk.k0 + 32 * per * wave;
     const int n = clamp_i32(nt - per * wave, 0, per);
 
@@ -126,66 +140,67 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(PagedAttnArgs a) {
             ve = scale_exp(a.p.vs[i]);
         }
     };
-    const int dk = g4 * 16, dv = c * VW * 4;
-    auto load = [&](int tile, KvTile<DH>& t) {
+    // Offsets in a block of 16 keys. Dimensions past the head's end read its first ones, against zeros in q.
+    uint32_t koff[NU];
+#pragma unroll
+    for (int u = 0; u < NU; u++) koff[u] = static_cast<uint32_t>(c * hd + (u * 64 + g4 * 16 < hd ? u * 64 + g4 * 16 : 0));
+    const uint32_t voff = static_cast<uint32_t>(4 * g4 * hd + (c * VW * 4 < hd ? c * VW * 4 : 0));
+    auto load = [&](int tile, KvTile<DH>& t) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            const int idx = 2 * (tile & 31) + b;
-            const int id = __builtin_amdgcn_readlane(page, idx);
-            t.ke[b] = __builtin_amdgcn_readlane(ke, idx);
-            t.ve[b] = __builtin_amdgcn_readlane(ve, idx);
-            t.ok[b] = id >= 0;
+            const int id = __builtin_amdgcn_readlane(page, 2 * (tile & 31) + b);
             // A block without a page reads page 0; its keys are masked. Every slot of a page may be read.
             const int32_t slot = (kw + 32 * tile + 16 * b) & ((1 << a.p.page_log2) - 1);
             const int64_t at = ((static_cast<int64_t>(id < 0 ? 0 : id) * a.p.n_kv + kvh) << a.p.page_log2) + slot;
             const uint8_t* kp = a.p.k + at * hd;
             const uint8_t* vp = a.p.v + at * hd;
 #pragma unroll
-            for (int u = 0; u < NU; u++) {
-                // Dimensions past the head's end read its first ones, against zeros in q.
-                const int d = u * 64 + dk;
-                t.k[b][u] = *reinterpret_cast<const uint4v*>(kp + (c * hd + (d < hd ? d : 0)));
-            }
+            for (int u = 0; u < NU; u++) t.k[b][u] = *reinterpret_cast<const uint4v*>(kp + koff[u]);
 #pragma unroll
-            for (int i = 0; i < 4; i++)
-                t.v[b][i] = *reinterpret_cast<const Words<VW>*>(vp + ((4 * g4 + i) * hd + (dv < hd ? dv : 0)));
+            for (int i = 0; i < 4; i++) t.v[b][i] = *reinterpret_cast<const Words<VW>*>(vp + i * hd + voff);
         }
     };
 
     float4v o[NE] = {};
     float m = -__builtin_inff(), l = 0.0f;
     bool seen = false;
-    // O^T += V^T B of one tile.
-    auto product = [&](const Words<VW> (&v)[2][4], half8 bh, half8 bl, bool two, float4v* acc) __attribute__((always_inline)) {
+    // acc += V^T B of one tile, four dimensions of each lane: x, a word of each key's row.
+    auto product = [&](const uint32_t (&x)[2][4], half8 bh, half8 bl, bool two, float4v* acc) __attribute__((always_inline)) {
+        half2v y[4][2][2];  // [dimension][block][key pair]
 #pragma unroll
-        for (int w = 0; w < VW; w++) {
-            half2v x[4][2][2];  // [dimension][block][key pair]
+        for (int b = 0; b < 2; b++) {
+            const uint32_t t0 = __builtin_amdgcn_perm(x[b][1], x[b][0], 0x05010400u);
+            const uint32_t t1 = __builtin_amdgcn_perm(x[b][3], x[b][2], 0x05010400u);
+            const uint32_t t2 = __builtin_amdgcn_perm(x[b][1], x[b][0], 0x07030602u);
+            const uint32_t t3 = __builtin_amdgcn_perm(x[b][3], x[b][2], 0x07030602u);
+            y[0][b][0] = f16_of_fp8<false>(t0);
+            y[0][b][1] = f16_of_fp8<false>(t1);
+            y[1][b][0] = f16_of_fp8<true>(t0);
+            y[1][b][1] = f16_of_fp8<true>(t1);
+            y[2][b][0] = f16_of_fp8<false>(t2);
+            y[2][b][1] = f16_of_fp8<false>(t3);
+            y[3][b][0] = f16_of_fp8<true>(t2);
+            y[3][b][1] = f16_of_fp8<true>(t3);
+        }
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
-                const uint32_t t0 = __builtin_amdgcn_perm(v[b][1].w[w], v[b][0].w[w], 0x05010400u);
-                const uint32_t t1 = __builtin_amdgcn_perm(v[b][3].w[w], v[b][2].w[w], 0x05010400u);
-                const uint32_t t2 = __builtin_amdgcn_perm(v[b][1].w[w], v[b][0].w[w], 0x07030602u);
-                const uint32_t t3 = __builtin_amdgcn_perm(v[b][3].w[w], v[b][2].w[w], 0x07030602u);
-                x[0][b][0] = f16_of_fp8<false>(t0);
-                x[0][b][1] = f16_of_fp8<false>(t1);
-                x[1][b][0] = f16_of_fp8<true>(t0);
-                x[1][b][1] = f16_of_fp8<true>(t1);
-                x[2][b][0] = f16_of_fp8<false>(t2);
-                x[2][b][1] = f16_of_fp8<false>(t3);
-                x[3][b][0] = f16_of_fp8<true>(t2);
-                x[3][b][1] = f16_of_fp8<true>(t3);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const half8 A = {x[e][0][0][0], x[e][0][0][1], x[e][0][1][0], x[e][0][1][1],
-                                 x[e][1][0][0], x[e][1][0][1], x[e][1][1][0], x[e][1][1][1]};
-                if (two) acc[4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bl, acc[4 * w + e], 0, 0, 0);
-                acc[4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bh, acc[4 * w + e], 0, 0, 0);
-            }
+        for (int e = 0; e < 4; e++) {
+            const half8 A = {y[e][0][0][0], y[e][0][0][1], y[e][0][1][0], y[e][0][1][1],
+                             y[e][1][0][0], y[e][1][0][1], y[e][1][1][0], y[e][1][1][1]};
+            if (two) acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bl, acc[e], 0, 0, 0);
+            acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bh, acc[e], 0, 0, 0);
         }
     };
     auto step = [&](int tile, KvTile<DH>& t) __attribute__((always_inline)) {
         const int32_t j0 = kw + 32 * tile;
+        int ke2[2], ve2[2];
+        bool ok[2];
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int idx = 2 * (tile & 31) + b;
+            ke2[b] = __builtin_amdgcn_readlane(ke, idx);
+            ve2[b] = __builtin_amdgcn_readlane(ve, idx);
+            ok[b] = __builtin_amdgcn_readlane(page, idx) >= 0;
+        }
         float4v s[2] = {};
 #pragma unroll
         for (int b = 0; b < 2; b++)
@@ -208,7 +223,7 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(PagedAttnArgs a) {
         float f[2];  // score -> exponent of 2
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            f[b] = sc * exp2i(t.ke[b]);
+            f[b] = sc * exp2i(ke2[b]);
             if constexpr (!MODS) f[b] *= kAttnLog2e;
             f[b] = fminf(fmaxf(f[b], 0x1p-120f), 0x1p120f);  // (never 0 or infinite: masked scores are -inf)
         }
@@ -226,7 +241,7 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(PagedAttnArgs a) {
             }
         }
         // Keys that some row of the tile does not see.
-        const bool partial = j0 < tk.lo_max || j0 + 32 > tk.hi_min || !t.ok[0] || !t.ok[1];
+        const bool partial = j0 < tk.lo_max || j0 + 32 > tk.hi_min || !ok[0] || !ok[1];
         uint32_t visible = 0xff;
         if (partial) {
 #pragma unroll
@@ -234,13 +249,13 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(PagedAttnArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int32_t j = j0 + 16 * b + 4 * g4 + i;
-                    const bool vis = t.ok[b] && j >= lo && j < hi;
+                    const bool vis = ok[b] && j >= lo && j < hi;
                     if (!vis) {
                         s[b][i] = -__builtin_inff();
                         visible &= ~(1u << (4 * b + i));
                     }
                     // What no row sees may be anything, codes of no token included.
-                    if (!(t.ok[b] && j >= tk.lo_min && j < tk.hi_max)) t.v[b][i] = Words<VW>{};
+                    if (!(ok[b] && j >= tk.lo_min && j < tk.hi_max)) t.v[b][i] = Words<VW>{};
                 }
         }
         seen = seen || visible != 0;
@@ -248,7 +263,7 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(PagedAttnArgs a) {
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             const float mx = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3]));
-            top = fmaxf(top, __builtin_fmaf(mx, f[b], static_cast<float>(t.ve[b])));
+            top = fmaxf(top, __builtin_fmaf(mx, f[b], static_cast<float>(ve2[b])));
         }
         top = ceilf(swap32_max(swap16_max(top)));
         if (__any(top > m)) {
@@ -265,7 +280,7 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(PagedAttnArgs a) {
         half8 ph, pl;
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            const float base = static_cast<float>(t.ve[b]) - ms;
+            const float base = static_cast<float>(ve2[b]) - ms;
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -275,10 +290,11 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(PagedAttnArgs a) {
                 ph[4 * b + i] = static_cast<half_t>(y);
                 pl[4 * b + i] = static_cast<half_t>(y - to_f32(ph[4 * b + i]));
             }
-            l = __builtin_fmaf(sum, exp2i(-t.ve[b]), l);
+            l = __builtin_fmaf(sum, exp2i(-ve2[b]), l);
         }
-        // A NaN code times a weight of zero is NaN, so where rows see different keys NaN codes are taken out and
-        // put into the dimensions of the rows that do see them.
+        // A NaN code times a weight of zero is NaN, so where rows see different keys NaN codes are taken out, and put
+        // into the dimensions of the rows that do see them.
+        bool mend = false;
         if (partial && (tk.hi_min != tk.hi_max || tk.lo_min != tk.lo_max)) {
             uint32_t any = 0;
 #pragma unroll
@@ -287,51 +303,47 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(PagedAttnArgs a) {
                 for (int i = 0; i < 4; i++)
 #pragma unroll
                     for (int w = 0; w < VW; w++) any |= nan_codes(t.v[b][i].w[w]);
-            if (__any(any != 0)) {
-                Words<VW> bad[2][4];
+            mend = __any(any != 0);
+        }
+#pragma unroll
+        for (int w = 0; w < VW; w++) {
+            uint32_t x[2][4];
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) x[b][i] = t.v[b][i].w[w];
+            if (mend) {
+                uint32_t bad[2][4];
                 half8 sees;
 #pragma unroll
                 for (int b = 0; b < 2; b++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         sees[4 * b + i] = static_cast<half_t>((visible >> (4 * b + i)) & 1u ? 1.0f : 0.0f);
-#pragma unroll
-                        for (int w = 0; w < VW; w++) {
-                            const uint32_t x = nan_codes(t.v[b][i].w[w]) >> 7;
-                            bad[b][i].w[w] = x * 0x38u;  // the code of 1
-                            t.v[b][i].w[w] &= ~(x * 0xffu);
-                        }
+                        const uint32_t nan = nan_codes(x[b][i]) >> 7;
+                        bad[b][i] = nan * 0x38u;  // the code of 1
+                        x[b][i] &= ~(nan * 0xffu);
                     }
-                float4v count[NE] = {};
+                float4v count[4] = {};
                 product(bad, sees, sees, false, count);
 #pragma unroll
-                for (int e = 0; e < NE; e++)
+                for (int e = 0; e < 4; e++)
 #pragma unroll
                     for (int i = 0; i < 4; i++)
-                        if (count[e][i] > 0.0f) o[e][i] = __builtin_nanf("");
+                        if (count[e][i] > 0.0f) o[4 * w + e][i] = __builtin_nanf("");
             }
+            product(x, ph, pl, true, o + 4 * w);
         }
-        product(t.v, ph, pl, true, o);
     };
 
-    if (n > 0) {
-        KvTile<DH> t0, t1;
-        look_up(0);
-        load(0, t0);
-        for (int i = 0; i < n; i += 2) {
-            // (32 tiles to a look-up, an even number, so only even tiles begin one)
-            if (i + 1 < n) load(i + 1, t1);
-            step(i, t0);
-            if (i + 2 < n) {
-                if (((i + 2) & 31) == 0) look_up(i + 2);
-                load(i + 2, t0);
-            }
-            if (i + 1 < n) step(i + 1, t1);
-        }
+    for (int i = 0; i < n; i++) {
+        if ((i & 31) == 0) look_up(i);
+        KvTile<DH> t;
+        load(i, t);
+        step(i, t);
     }
 
-    // The waves' results meet: every wave puts its own in LDS and joins a quarter of the dimensions, those of
-    // accumulator element `wave`.
+    // The waves' results meet in LDS.
     l = swap32_sum(swap16_sum(l));
     const float any_seen = swap32_max(swap16_max(seen ? 1.0f : 0.0f));
     if (g4 == 0) {
@@ -339,109 +351,123 @@ __global__ __launch_bounds__(256) void attn_paged_kernel(PagedAttnArgs a) {
         l_sh[wave][c] = l;
         seen_sh[wave][c] = any_seen;
     }
-    constexpr int NH = DH <= 128 ? NE : NE / 2;  // dimensions' blocks in LDS at once
-    float res[NE];
-    float f[kWaves], mm = -__builtin_inff(), ll = 0.0f, ss = 0.0f;
-#pragma unroll
-    for (int half = 0; half < NE / NH; half++) {
-        if (half) __syncthreads();
+    const int rows_here = min(kTileRows, n_rows - it.tile * kTileRows);
+    if (c < rows_here) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int e = 0; e < NH; e++) o_sh[wave][i][e][lane] = o[half * NH + e][i];
-        __syncthreads();
-        if (half == 0) {
-#pragma unroll
-            for (int w = 0; w < kWaves; w++) mm = fmaxf(mm, m_sh[w][c]);
-            const float ms = mm == -__builtin_inff() ? 0.0f : mm;
-#pragma unroll
-            for (int w = 0; w < kWaves; w++) {
-                f[w] = __builtin_amdgcn_exp2f(m_sh[w][c] - ms);
-                ll = __builtin_fmaf(l_sh[w][c], f[w], ll);
-                ss = fmaxf(ss, seen_sh[w][c]);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < NH; e++) {
-            float x = 0.0f;
-#pragma unroll
-            for (int w = 0; w < kWaves; w++) x = __builtin_fmaf(o_sh[w][wave][e][lane], f[w], x);
-            res[half * NH + e] = x;
-        }
+            for (int e = 0; e < NE; e += 4)
+                *reinterpret_cast<float4v*>(o_sh + (wave * kTileRows + c) * kRow + (4 * g4 + i) * NE + e) =
+                    float4v{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
     }
-    if (it.tile * kTileRows + c >= n_rows) return;
-    const int d = (4 * g4 + wave) * NE;  // this lane's dimensions: row 4 g4 + wave of every block e
-    if (it.splits == 1) {
-        const float by = row_factor(ll, ss > 0.0f);
-        if (d < hd) {
-            TQ* out = static_cast<TQ*>(a.out) + static_cast<int64_t>(r.begin + tok) * a.os + static_cast<int64_t>(head) * hd + d;
-            TQ v[NE];
-#pragma unroll
-            for (int e = 0; e < NE; e++) v[e] = from_f32<TQ>(by == 0.0f ? 0.0f : res[e] * by);
-            __builtin_memcpy(out, v, sizeof(v));
-        }
-        return;
-    }
+    __syncthreads();
+    constexpr int LPR = DH / 4;  // threads to a row, four dimensions each
     const uint32_t block = it.block * static_cast<uint32_t>(a.p.n_kv) + kvh;
-    if (block >= a.blocks) return;
-    const int64_t at = static_cast<int64_t>(block) * kTileRows + c;
+    for (int i = static_cast<int>(threadIdx.x) / LPR; i < rows_here; i += 64 * NW / LPR) {
+        const int d = static_cast<int>(threadIdx.x) % LPR * 4;
+        float mm = -__builtin_inff(), ll = 0.0f, ss = 0.0f;
 #pragma unroll
-    for (int e = 0; e < NE; e += 4) *reinterpret_cast<float4v*>(a.part + at * DH + d + e) = float4v{res[e], res[e + 1], res[e + 2], res[e + 3]};
-    if (g4 == 0 && wave == 0) *reinterpret_cast<float4v*>(a.ml + at * 4) = float4v{mm, ll, ss, 0.0f};
+        for (int w = 0; w < NW; w++) mm = fmaxf(mm, m_sh[w][i]);
+        const float ms = mm == -__builtin_inff() ? 0.0f : mm;
+        float4v x = {};
+#pragma unroll 4
+        for (int w = 0; w < NW; w++) {
+            const float f = __builtin_amdgcn_exp2f(m_sh[w][i] - ms);
+            const float4v y = *reinterpret_cast<const float4v*>(o_sh + (w * kTileRows + i) * kRow + d);
+            ll = __builtin_fmaf(l_sh[w][i], f, ll);
+            ss = fmaxf(ss, seen_sh[w][i]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf(y[e], f, x[e]);
+        }
+        if (it.splits > 1) {
+            if (block >= a.blocks) return;
+            const int64_t at = static_cast<int64_t>(block) * kTileRows + i;
+            *reinterpret_cast<float4v*>(a.part + at * DH + d) = x;
+            if (d == 0) *reinterpret_cast<float4v*>(a.ml + at * 4) = float4v{mm, ll, ss, 0.0f};
+        } else if (d < hd) {
+            store_row<TQ>(a, r, kvh, it.tile * kTileRows + i, d, x, row_factor(ll, ss > 0.0f));
+        }
+    }
 }
 
-// Joins the splits of one tile: DH / 4 lanes to a row, four dimensions each.
+// Joins the splits of one tile, eight rows of 128 dimensions to a workgroup: DH / 4 lanes to a row, four dimensions
+// each, the partial results of eight splits asked for at once.
 template <typename TQ, int DH>
 __global__ __launch_bounds__(256) void attn_paged_merge(PagedAttnArgs a) {
+    constexpr int LPR = DH / 4, RPB = 256 / LPR, AHEAD = 8;
     const int kvh = static_cast<int>(blockIdx.x % static_cast<uint32_t>(a.p.n_kv));
     AttnItem it;
     if (!attn_find<true>(a.p, a.t, blockIdx.x / static_cast<uint32_t>(a.p.n_kv), &it)) return;
-    if (it.splits == 1) return;
     const SeqRows r = paged_seq(a.p, it.s);
-    const int32_t n_rows = r.n * a.t.group;
-    constexpr int LPR = DH / 4, RPP = 256 / LPR;
     const int d = static_cast<int>(threadIdx.x) % LPR * 4;
-    const uint32_t n_kv = static_cast<uint32_t>(a.p.n_kv), block0 = it.block * n_kv + kvh;
-    if (static_cast<uint64_t>(it.block) * n_kv + static_cast<uint64_t>(it.splits) * n_kv > a.blocks) return;
-    for (int i = static_cast<int>(threadIdx.x) / LPR; i < a.t.tile_rows; i += RPP) {
-        const int32_t row = it.tile * a.t.tile_rows + i;
-        if (row >= n_rows) return;
-        const int64_t first = static_cast<int64_t>(block0) * a.t.tile_rows + i, step = static_cast<int64_t>(n_kv) * a.t.tile_rows;
-        float m = -__builtin_inff(), ss = 0.0f, l = 0.0f;
-        for (int k = 0; k < it.splits; k++) m = fmaxf(m, a.ml[(first + k * step) * 4]);
-        const float ms = m == -__builtin_inff() ? 0.0f : m;
-        float4v x = {};
-        for (int k = 0; k < it.splits; k++) {
-            const float4v s = *reinterpret_cast<const float4v*>(a.ml + (first + k * step) * 4);
-            const float4v p = *reinterpret_cast<const float4v*>(a.part + (first + k * step) * DH + d);
-            const float f = __builtin_amdgcn_exp2f(s[0] - ms);
-            l = __builtin_fmaf(s[1], f, l);
-            ss = fmaxf(ss, s[2]);
+    const int i = static_cast<int>(blockIdx.y) * RPB + static_cast<int>(threadIdx.x) / LPR;
+    const int32_t row = it.tile * a.t.tile_rows + i;
+    const uint32_t n_kv = static_cast<uint32_t>(a.p.n_kv);
+    if (i >= a.t.tile_rows || row >= r.n * a.t.group) return;
+    if ((static_cast<uint64_t>(it.block) + static_cast<uint64_t>(it.splits)) * n_kv > a.blocks) return;
+    const int64_t first = static_cast<int64_t>(it.block * n_kv + kvh) * a.t.tile_rows + i, step = static_cast<int64_t>(n_kv) * a.t.tile_rows;
+    float m = -__builtin_inff(), l = 0.0f, ss = 0.0f;
+    float4v x = {};
+    for (int k0 = 0; k0 < it.splits; k0 += AHEAD) {
+        float4v s[AHEAD], p[AHEAD];
 #pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf(p[e], f, x[e]);
+        for (int k = 0; k < AHEAD; k++) {
+            const int64_t at = first + min(k0 + k, it.splits - 1) * step;
+            s[k] = *reinterpret_cast<const float4v*>(a.ml + at * 4);
+            p[k] = *reinterpret_cast<const float4v*>(a.part + at * DH + d);
         }
-        if (d >= a.p.hd) continue;
-        const float by = row_factor(l, ss > 0.0f);
-        const int32_t tok = row / a.t.group;
-        const int head = kvh * a.t.group + (row - tok * a.t.group);
-        TQ v[4];
+        float mn = m;
 #pragma unroll
-        for (int e = 0; e < 4; e++) v[e] = from_f32<TQ>(by == 0.0f ? 0.0f : x[e] * by);
-        __builtin_memcpy(static_cast<TQ*>(a.out) + static_cast<int64_t>(r.begin + tok) * a.os + static_cast<int64_t>(head) * a.p.hd + d, v, sizeof(v));
+        for (int k = 0; k < AHEAD; k++) mn = fmaxf(mn, s[k][0]);
+        const float ms = mn == -__builtin_inff() ? 0.0f : mn, corr = __builtin_amdgcn_exp2f(m - ms);
+        m = mn;
+        l *= corr;
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] *= corr;
+#pragma unroll
+        for (int k = 0; k < AHEAD; k++) {
+            if (k0 + k < it.splits) {
+                const float f = __builtin_amdgcn_exp2f(s[k][0] - ms);
+                l = __builtin_fmaf(s[k][1], f, l);
+                ss = fmaxf(ss, s[k][2]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf(p[k][e], f, x[e]);
+            }
+        }
     }
+    if (d < a.p.hd) store_row<TQ>(a, r, kvh, row, d, x, row_factor(l, ss > 0.0f));
 }
 
-// Workgroups and tiles of a launch, from its tiling.
+// Workgroups of a launch and the bytes of its partial results, from its tiling.
 struct Grid {
-    int64_t blocks, tiles;
-    size_t bytes;  // of partial results
+    int64_t blocks;
+    size_t bytes;
 };
 Grid grid_of(const PagedAttnArgs& a, int dh) {
     Grid g;
     g.blocks = attn_blocks_bound(a.t, a.p.rows, a.p.n_seq, a.p.n_kv) * a.p.n_kv;
-    g.tiles = attn_tiles_bound(a.t, a.p.rows, a.p.n_seq) * a.p.n_kv;
-    g.bytes = static_cast<size_t>(g.blocks) * a.t.tile_rows * (dh + 4) * sizeof(float);
+    g.bytes = attn_may_split(a.t, a.p) ? static_cast<size_t>(g.blocks) * a.t.tile_rows * (dh + 4) * sizeof(float) : 0;
     return g;
+}
+
+// The tiling of the 16-row kernel with `waves` waves to a workgroup, 16 of which a CU holds: as many workgroups as
+// are resident at once, tiles that are not split included.
+void few_form(const neko_hip_ctx* ctx, PagedAttnArgs& a, int waves) {
+    a.t.tile_rows = kTileRows;
+    a.t.unit = 32 * waves;
+    a.t.least = kLeast;
+    const int64_t room = 16LL * ctx->cu_count / waves, items = attn_tiles_bound(a.t, a.p.rows, a.p.n_seq) * a.p.n_kv;
+    a.t.target = static_cast<int32_t>(std::max<int64_t>(room - items, room / 2));
+}
+
+template <typename TQ, int DH, int NW, bool MODS>
+int launch_few(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a) {
+    static std::atomic<uint64_t> allowed{0};
+    constexpr size_t lds = NW * kTileRows * (DH + 4) * sizeof(float);
+    if (lds + 4096 > 64 * 1024)
+        if (int rc = allow_lds(ctx, reinterpret_cast<const void*>(&attn_paged_kernel<TQ, DH, NW, MODS>), lds, allowed)) return rc;
+    hipLaunchKernelGGL((attn_paged_kernel<TQ, DH, NW, MODS>), dim3(a.blocks), dim3(64 * NW), lds, ctx->stream, a);
+    return after_launch(ctx, what);
 }
 
 template <typename TQ, int DH>
@@ -452,10 +478,13 @@ int launch_dims(neko_hip_ctx* ctx, const char* what, PagedAttnArgs a, int dtype)
     const int64_t most = static_cast<int64_t>(a.p.rows) * a.t.group;
     const bool few = a.p.n_seq > 1 || most <= kFewRows;
     const bool many = most > kFewRows && a.p.rows > a.p.n_seq;
+    constexpr int kMostWaves = DH <= 128 && sizeof(TQ) == 2 ? 16 : 8;
     PagedAttnArgs f = a, t = a;
+    // Few items: many waves to each, whose results meet in LDS.
     f.t.tile_rows = kTileRows;
-    f.t.unit = kUnit;
-    f.t.target = 4 * ctx->cu_count;
+    const int64_t items = attn_tiles_bound(f.t, a.p.rows, a.p.n_seq) * a.p.n_kv;
+    const bool wide = items <= ctx->cu_count;
+    few_form(ctx, f, wide ? kMostWaves : 4);
     f.t.min_rows = 1;
     f.t.max_rows = many ? kFewRows : 0x7fffffff;
     attn_paged_tile_form(ctx, t);
@@ -464,29 +493,33 @@ int launch_dims(neko_hip_ctx* ctx, const char* what, PagedAttnArgs a, int dtype)
     const Grid fg = few ? grid_of(f, DH) : Grid{}, tg = many ? grid_of(t, DH) : Grid{};
     NEKO_REQUIRE(ctx, fg.blocks <= 0x7fffffff && tg.blocks <= 0x7fffffff, "%s: grid too large", what);
     void* ws = nullptr;
-    if (int rc = workspace(ctx, fg.bytes + tg.bytes, &ws)) return rc;
+    if (fg.bytes + tg.bytes)
+        if (int rc = workspace(ctx, fg.bytes + tg.bytes, &ws)) return rc;
     const bool mods = a.softcap > 0.0f || a.slopes;
     auto place = [](PagedAttnArgs& x, const Grid& g, void* at) {
         x.blocks = static_cast<uint32_t>(g.blocks);
         x.part = static_cast<float*>(at);
         x.ml = x.part + g.blocks * x.t.tile_rows * DH;
     };
-    auto merge = [&](const PagedAttnArgs& x, const Grid& g) {
-        if (paged_reach(x.p) <= x.t.unit) return NEKO_OK;  // lengths within one unit are never split
-        hipLaunchKernelGGL((attn_paged_merge<TQ, DH>), dim3(static_cast<uint32_t>(g.tiles)), dim3(256), 0, ctx->stream, x);
+    auto merge = [&](const PagedAttnArgs& x) {
+        if (!attn_may_split(x.t, x.p)) return NEKO_OK;
+        const int64_t tiles = attn_split_tiles_bound(x.t, x.p.rows, x.p.n_seq, x.p.n_kv) * x.p.n_kv;
+        const dim3 grid(static_cast<uint32_t>(tiles), static_cast<uint32_t>((x.t.tile_rows * DH + 1023) / 1024));
+        hipLaunchKernelGGL((attn_paged_merge<TQ, DH>), grid, dim3(256), 0, ctx->stream, x);
         return after_launch(ctx, what);
     };
     if (many) {
         place(t, tg, static_cast<char*>(ws) + fg.bytes);
         if (int rc = attn_paged_tile(ctx, what, t, dtype)) return rc;
-        if (int rc = merge(t, tg)) return rc;
+        if (int rc = merge(t)) return rc;
     }
     if (few) {
         place(f, fg, ws);
-        if (mods) hipLaunchKernelGGL((attn_paged_kernel<TQ, DH, true>), dim3(f.blocks), dim3(256), 0, ctx->stream, f);
-        else hipLaunchKernelGGL((attn_paged_kernel<TQ, DH, false>), dim3(f.blocks), dim3(256), 0, ctx->stream, f);
-        if (int rc = after_launch(ctx, what)) return rc;
-        if (int rc = merge(f, fg)) return rc;
+        int rc;
+        if (wide) rc = mods ? launch_few<TQ, DH, kMostWaves, true>(ctx, what, f) : launch_few<TQ, DH, kMostWaves, false>(ctx, what, f);
+        else rc = mods ? launch_few<TQ, DH, 4, true>(ctx, what, f) : launch_few<TQ, DH, 4, false>(ctx, what, f);
+        if (rc) return rc;
+        if (int rc2 = merge(f)) return rc2;
     }
     return NEKO_OK;
 }

@@ -457,6 +457,7 @@ void attn_paged_tile_form(const neko_hip_ctx* ctx, PagedAttnArgs& a) {
     a.t.tile_rows = TileForm<128>::rows;
     a.t.unit = 64;  // a whole number of tiles of either size
     a.t.target = 2 * ctx->cu_count;
+    a.t.least = 1;
 }
 
 int attn_paged_tile(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a, int dtype) {

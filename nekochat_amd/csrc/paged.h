@@ -131,6 +131,7 @@ struct AttnTiling {
     int32_t tile_rows;  // flattened (token, head) rows of a tile
     int32_t unit;       // keys that a split is a multiple of
     int32_t target;     // workgroups wanted
+    int32_t least;      // units of a split, at least
     int64_t window;     // 0: none
     // Sequences with min_rows <= flattened rows <= max_rows are this launch's.
     int32_t min_rows, max_rows;
@@ -154,19 +155,32 @@ NEKO_HD int32_t attn_units(const AttnTiling& t, const Paged& p, const SeqRows& r
 // Units per split, from the launch's work: the sum over sequences and kv heads of tiles * units.
 NEKO_HD int32_t attn_chunk(const AttnTiling& t, uint64_t work) {
     const uint64_t c = (work + static_cast<uint64_t>(t.target) - 1) / static_cast<uint64_t>(t.target);
-    return c < 1 ? 1 : c > (1u << 30) ? 1 << 30 : static_cast<int32_t>(c);
+    return c < static_cast<uint64_t>(t.least) ? t.least : c > (1u << 30) ? 1 << 30 : static_cast<int32_t>(c);
 }
 
 NEKO_HD int32_t attn_splits(int32_t units, int32_t chunk) { return units <= chunk ? 1 : (units + chunk - 1) / chunk; }
 
 // Workgroups per kv head that the splits above can come to: sum of tiles * splits <= work / (n_kv * chunk) +
-// sum of tiles, and the tiles number at most rows * group / tile_rows + n_seq.
+// sum of tiles, and the tiles number at most rows * group / tile_rows + n_seq. Tiles that are split have more than
+// chunk units each, so they number at most work / (n_kv * chunk) <= target / n_kv.
 NEKO_HD int64_t attn_tiles_bound(const AttnTiling& t, int64_t rows, int64_t n_seq) {
     const int64_t tiles = rows * t.group / t.tile_rows + (rows < n_seq ? rows : n_seq);
     return tiles < rows * t.group ? tiles : rows * t.group;
 }
 NEKO_HD int64_t attn_blocks_bound(const AttnTiling& t, int64_t rows, int64_t n_seq, int n_kv) {
     return attn_tiles_bound(t, rows, n_seq) + (t.target + n_kv - 1) / n_kv;
+}
+
+NEKO_HD int64_t attn_split_tiles_bound(const AttnTiling& t, int64_t rows, int64_t n_seq, int n_kv) {
+    const int64_t tiles = attn_tiles_bound(t, rows, n_seq), most = (t.target + n_kv - 1) / n_kv;
+    return tiles < most ? tiles : most;
+}
+// Whether any tile can be split. One sequence: its tiles are known, and with as many as wanted chunk >= units.
+NEKO_HD bool attn_may_split(const AttnTiling& t, const Paged& p) {
+    if (paged_reach(p) <= static_cast<int64_t>(t.least) * t.unit) return false;
+    if (p.n_seq > 1) return true;
+    const int64_t tiles = (static_cast<int64_t>(p.rows) * t.group + t.tile_rows - 1) / t.tile_rows;
+    return tiles * p.n_kv < t.target;
 }
 
 }  // namespace neko_hip

@@ -70,19 +70,22 @@ void check_blocks(const Batch* b, const AttnTiling* t, int64_t* out) {
         work += static_cast<uint64_t>(attn_tiles(*t, r)) * static_cast<uint64_t>(attn_units(*t, p, r));
     }
     const int32_t chunk = attn_chunk(*t, work * static_cast<uint64_t>(p.n_kv));
-    int64_t tiles = 0, blocks = 0, uncovered = 0;
+    int64_t tiles = 0, blocks = 0, uncovered = 0, split = 0;
     for (int32_t s = 0; s < p.n_seq; s++) {
         const SeqRows r = paged_seq(p, s);
         const int64_t n = attn_tiles(*t, r), units = attn_units(*t, p, r), splits = attn_splits(static_cast<int32_t>(units), chunk);
         tiles += n;
         blocks += n * splits;
         if (n && splits * chunk < units) uncovered++;
+        if (splits > 1) split += n;
     }
     out[0] = tiles;
     out[1] = blocks;
     out[2] = attn_tiles_bound(*t, p.rows, p.n_seq);
     out[3] = attn_blocks_bound(*t, p.rows, p.n_seq, p.n_kv);
     out[4] = uncovered;
+    out[5] = split;
+    out[6] = attn_may_split(*t, p) ? attn_split_tiles_bound(*t, p.rows, p.n_seq, p.n_kv) : 0;
 }
 
 }  // extern "C"

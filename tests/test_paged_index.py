@@ -20,7 +20,7 @@ class Batch(ctypes.Structure):
 
 class Tiling(ctypes.Structure):
     _fields_ = [("group", ctypes.c_int32), ("tile_rows", ctypes.c_int32), ("unit", ctypes.c_int32),
-                ("target", ctypes.c_int32), ("window", ctypes.c_int64), ("min_rows", ctypes.c_int32),
+                ("target", ctypes.c_int32), ("least", ctypes.c_int32), ("window", ctypes.c_int64), ("min_rows", ctypes.c_int32),
                 ("max_rows", ctypes.c_int32)]
 
 
@@ -117,11 +117,11 @@ def test_attention_blocks_stay_within_the_grid(lib, seed):
     group = int(rng.choice([1, 2, 3, 4, 8, 16, 40]))
     few = int(rng.choice([0, 16, 32]))
     t = Tiling(group, int(rng.choice([16, 64, 128, 256])), int(rng.choice([64, 128])), int(rng.choice([1, 7, 256, 1024])),
-               int(rng.choice([0, 1, 40, 1000])), *((1, 2**31 - 1) if not few else (few + 1, 2**31 - 1) if rng.random() < 0.5 else (1, few)))
-    out = (ctypes.c_int64 * 5)()
+               int(rng.choice([1, 8])), int(rng.choice([0, 1, 40, 1000])), *((1, 2**31 - 1) if not few else (few + 1, 2**31 - 1) if rng.random() < 0.5 else (1, few)))
+    out = (ctypes.c_int64 * 7)()
     lib.check_blocks(ctypes.byref(b), ctypes.byref(t), out)
-    tiles, blocks, tiles_bound, blocks_bound, uncovered = out
-    assert tiles <= tiles_bound and blocks <= blocks_bound and uncovered == 0
+    tiles, blocks, tiles_bound, blocks_bound, uncovered, split, split_bound = out
+    assert tiles <= tiles_bound and blocks <= blocks_bound and uncovered == 0 and split <= split_bound
 
 
 def test_scale_exponents(lib):
