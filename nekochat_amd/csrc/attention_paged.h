@@ -14,7 +14,8 @@ struct PagedAttnArgs {
     void* out;
     int64_t os;
     int32_t n_head;
-    int32_t window;  // 0: none
+    FastDiv by_group;  // flattened row -> token
+    FastDiv by_kv;     // workgroup -> (item, kv head)
     float scale;     // of the scores; its sign goes into q
     float softcap;   // 0: none
     const float* slopes;
@@ -51,13 +52,14 @@ __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
 template <bool SPLIT>
 __device__ __forceinline__ bool attn_find(const Paged& p, const AttnTiling& t, uint32_t j, AttnItem* it) {
     const int32_t lane = static_cast<int32_t>(threadIdx.x) & 63;
+    const int32_t reach = paged_reach(p);
     int32_t tiles = 0, units = 0;
     auto load = [&](int32_t base) {
         tiles = units = 0;
         if (base + lane < p.n_seq) {
             const SeqRows r = paged_seq(p, base + lane);
             tiles = attn_tiles(t, r);
-            units = attn_units(t, p, r);
+            units = attn_units(t, reach, r);
         }
     };
     double work = 0.0;  // (whole numbers below 2^53: exact)
@@ -65,7 +67,7 @@ __device__ __forceinline__ bool attn_find(const Paged& p, const AttnTiling& t, u
         load(base);
         work += wave_sum_f64(static_cast<double>(tiles) * static_cast<double>(units));
     }
-    const int32_t chunk = attn_chunk(t, static_cast<uint64_t>(work * p.n_kv));
+    const int32_t chunk = attn_chunk(t, work * p.n_kv);
     uint32_t past_tiles = 0, past = 0;
     for (int32_t base = 0; base < p.n_seq; base += 64) {
         if (p.n_seq > 64) load(base);
@@ -88,8 +90,9 @@ __device__ __forceinline__ bool attn_find(const Paged& p, const AttnTiling& t, u
                 it->block = first + local * static_cast<uint32_t>(it->splits);
             } else {  // the last tiles, which see the most keys, first
                 const uint32_t local = j - first;
-                it->tile = n_tiles - 1 - static_cast<int32_t>(local / static_cast<uint32_t>(it->splits));
-                it->split = static_cast<int32_t>(local % static_cast<uint32_t>(it->splits));
+                const uint32_t up = it->splits == 1 ? local : local / static_cast<uint32_t>(it->splits);
+                it->tile = n_tiles - 1 - static_cast<int32_t>(up);
+                it->split = static_cast<int32_t>(local - up * static_cast<uint32_t>(it->splits));
                 it->block = j;
             }
             return true;
@@ -107,19 +110,23 @@ struct TileKeys {
 };
 __device__ __forceinline__ int32_t key_lo(int32_t pos, int32_t window) { return window > 0 && pos >= window ? pos - window + 1 : 0; }
 __device__ __forceinline__ TileKeys tile_keys(const PagedAttnArgs& a, const SeqRows& r, const AttnItem& it) {
-    const int32_t n_rows = r.n * a.t.group, row0 = it.tile * a.t.tile_rows;
-    const int32_t row1 = min(row0 + a.t.tile_rows, n_rows) - 1;
-    const int32_t first = r.len - r.n + row0 / a.t.group, last = r.len - r.n + row1 / a.t.group;
+    const int32_t n_rows = r.n * a.t.group, row0 = it.tile << a.t.tile_log2;
+    const int32_t row1 = min(row0 + (1 << a.t.tile_log2), n_rows) - 1;
+    const int32_t first = r.len - r.n + static_cast<int32_t>(fast_div(static_cast<uint32_t>(row0), a.by_group));
+    const int32_t last = r.len - r.n + static_cast<int32_t>(fast_div(static_cast<uint32_t>(row1), a.by_group));
     const int32_t reach = min(r.len, paged_reach(a.p));
     TileKeys k;
-    k.lo_min = key_lo(first, a.window);
-    k.lo_max = key_lo(last, a.window);
+    k.lo_min = key_lo(first, a.t.window);
+    k.lo_max = key_lo(last, a.t.window);
     k.hi_min = min(first + 1, reach);
     k.hi_max = min(last + 1, reach);
-    const int64_t per = static_cast<int64_t>(it.chunk) * a.t.unit, from = (k.lo_min & ~31) + it.split * per;
-    const int64_t to = from + per < k.hi_max ? from + per : k.hi_max;
-    k.k0 = static_cast<int32_t>(from < (1 << 30) ? from : 1 << 30);
-    k.k1 = static_cast<int32_t>(to);
+    k.k0 = k.lo_min & ~31;
+    k.k1 = k.hi_max;
+    if (it.splits > 1) {
+        const int64_t per = static_cast<int64_t>(it.chunk) << a.t.unit_log2, from = k.k0 + it.split * per;
+        k.k0 = static_cast<int32_t>(from < (1 << 30) ? from : 1 << 30);
+        if (from + per < k.k1) k.k1 = static_cast<int32_t>(from + per);
+    }
     return k;
 }
 
@@ -149,6 +156,14 @@ __device__ __forceinline__ float swap16_sum(float v) {
 __device__ __forceinline__ float swap32_sum(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
     return __builtin_bit_cast(float, static_cast<uint32_t>(r[0])) + __builtin_bit_cast(float, static_cast<uint32_t>(r[1]));
+}
+
+// Workgroup -> item number and kv head: the kv head fastest, so that with eight of them each XCD reads one head's part
+// of the pages.
+__device__ __forceinline__ uint32_t item_of(const PagedAttnArgs& a, int* kvh) {
+    const uint32_t j = fast_div(blockIdx.x, a.by_kv);
+    *kvh = static_cast<int>(blockIdx.x - j * a.by_kv.d);
+    return j;
 }
 
 // The bytes of x that are NaN codes, as 0x80 each.

@@ -26,6 +26,7 @@ namespace {
 constexpr int kTileRows = 16;
 constexpr int kLeast = 8;           // tiles of 32 keys to a wave below which no keys are split
 constexpr int kFewRows = 32;        // flattened rows up to which a sequence is this kernel's
+constexpr int kSpareRows = 256;     // flattened rows past one token to a sequence that still make a decoding batch
 
 template <int N>
 struct Words {
@@ -46,7 +47,7 @@ constexpr int kResident = DH <= 64 ? 4 : DH <= 128 ? (sizeof(TQ) == 2 ? 4 : 3) :
 // Four dimensions, from d on, of a finished row.
 template <typename TQ>
 __device__ __forceinline__ void store_row(const PagedAttnArgs& a, const SeqRows& r, int kvh, int32_t row, int d, float4v x, float by) {
-    const int32_t tok = row / a.t.group;
+    const int32_t tok = static_cast<int32_t>(fast_div(static_cast<uint32_t>(row), a.by_group));
     const int head = kvh * a.t.group + (row - tok * a.t.group);
     TQ v[4];
 #pragma unroll
@@ -61,61 +62,72 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
     constexpr int kRow = DH + 4;  // floats of a row in LDS
     extern __shared__ __align__(16) float o_sh[];  // [NW][16][kRow]
     __shared__ float m_sh[NW][16], l_sh[NW][16], seen_sh[NW][16];
+    __shared__ half8 q_sh[kTwo ? 2 : 1][2 * NU][64];
+    __shared__ float sc_sh[16];
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
     const int c = lane & 15, g4 = lane >> 4;
-    const int kvh = static_cast<int>(blockIdx.x % static_cast<uint32_t>(a.p.n_kv));
+    int kvh;
+    const uint32_t item = item_of(a, &kvh);
     AttnItem it;
-    if (!attn_find<false>(a.p, a.t, blockIdx.x / static_cast<uint32_t>(a.p.n_kv), &it)) return;
+    if (!attn_find<false>(a.p, a.t, item, &it)) return;
     const SeqRows r = paged_seq(a.p, it.s);
     const TileKeys tk = tile_keys(a, r, it);
     const int hd = a.p.hd;
 
     // This lane's row (rows past the last repeat it and are not written).
     const int32_t n_rows = r.n * a.t.group;
-    const int32_t row = min(it.tile * kTileRows + c, n_rows - 1);
-    const int32_t tok = row / a.t.group;
+    const int32_t row = min((it.tile << 4) + c, n_rows - 1);
+    const int32_t tok = static_cast<int32_t>(fast_div(static_cast<uint32_t>(row), a.by_group));
     const int head = kvh * a.t.group + (row - tok * a.t.group);
     const int32_t pos = r.len - r.n + tok;
-    const int32_t hi = min(pos + 1, min(r.len, paged_reach(a.p))), lo = key_lo(pos, a.window);
+    const int32_t hi = min(pos + 1, min(r.len, paged_reach(a.p))), lo = key_lo(pos, a.t.window);
 
-    half8 qh[2 * NU], ql[kTwo ? 2 * NU : 1];
-    // Of the scores, in natural units; a scale of 0 weights all alike.
-    float sc = a.scale == 0.0f ? 1.0f : fabsf(a.scale);
-    {
+    // q as the B operands of the first product, the same for all waves, by the last of them: in LDS, where each
+    // wave's registers have room for other things (128 of them at four waves per SIMD). f32 rows are brought to
+    // [2^14, 2^15) and split; sc_sh then undoes that. A scale's sign goes into q; a scale of 0 weights all alike.
+    if (wave == NW - 1) {
         const TQ* qr = static_cast<const TQ*>(a.q) + static_cast<int64_t>(r.begin + tok) * a.qs + static_cast<int64_t>(head) * hd;
         const float sign = a.scale == 0.0f ? 0.0f : a.scale < 0.0f ? -1.0f : 1.0f;
-        float x[NU][16];
+        TQ x[2 * NU][8];
 #pragma unroll
-        for (int u = 0; u < NU; u++) {
-            const int d = u * 64 + g4 * 16;
-            TQ v[16];
-            if (d < hd) __builtin_memcpy(v, qr + d, sizeof(v));
+        for (int u = 0; u < 2 * NU; u++) {
+            const int d = u / 2 * 64 + g4 * 16 + u % 2 * 8;
 #pragma unroll
-            for (int e = 0; e < 16; e++) x[u][e] = d < hd ? to_f32(v[e]) * sign : 0.0f;
+            for (int e = 0; e < 8; e++) x[u][e] = static_cast<TQ>(0.0f);
+            if (d < hd) __builtin_memcpy(x[u], qr + d, sizeof(x[u]));
         }
         if constexpr (kTwo) {
             float mx = 0.0f;
 #pragma unroll
-            for (int u = 0; u < NU; u++)
+            for (int u = 0; u < 2 * NU; u++)
 #pragma unroll
-                for (int e = 0; e < 16; e++) mx = fmaxf(mx, fabsf(x[u][e]));
+                for (int e = 0; e < 8; e++) mx = fmaxf(mx, fabsf(x[u][e]));
             mx = swap32_max(swap16_max(mx));
             const int ex = mx > 0.0f && mx < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(mx) : 0;
             const int e1 = ex / 2, e2 = ex - e1;  // two factors of which each is a normal float
-            sc = ldexpf(sc, -ex);
+            sc_sh[c] = ldexpf(a.scale == 0.0f ? 1.0f : fabsf(a.scale), -ex);
 #pragma unroll
-            for (int u = 0; u < NU; u++)
+            for (int u = 0; u < 2 * NU; u++) {
+                half8 y, z;
 #pragma unroll
-                for (int e = 0; e < 16; e++) x[u][e] = ldexpf(ldexpf(x[u][e], e1), e2);
-        }
-#pragma unroll
-        for (int u = 0; u < NU; u++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                qh[2 * u + e / 8][e % 8] = static_cast<half_t>(x[u][e]);
-                if constexpr (kTwo) ql[2 * u + e / 8][e % 8] = static_cast<half_t>(x[u][e] - to_f32(qh[2 * u + e / 8][e % 8]));
+                for (int e = 0; e < 8; e++) {
+                    const float v = ldexpf(ldexpf(x[u][e], e1), e2) * sign;
+                    y[e] = static_cast<half_t>(v);
+                    z[e] = static_cast<half_t>(v - to_f32(y[e]));
+                }
+                q_sh[0][u][lane] = y;
+                q_sh[1][u][lane] = z;
             }
+        } else {
+#pragma unroll
+            for (int u = 0; u < 2 * NU; u++) {
+                half8 y;
+                __builtin_memcpy(&y, x[u], sizeof(y));
+                if (sign != 1.0f) y *= static_cast<half_t>(sign);
+                q_sh[0][u][lane] = y;
+            }
+        }
     }
     const float slope = MODS && a.slopes ? a.slopes[head] : 0.0f;
     const float inv_cap = MODS && a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
@@ -133,7 +145,7 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
         const int32_t at = kw + 32 * tile + 16 * lane;
         page = -1;
         ke = ve = 0;
-        if (at < tk.k1) page = paged_page(a.p, it.s, at);
+        if (lane < 2 * (n - tile) && at < tk.k1) page = paged_page(a.p, it.s, at);
         if (page >= 0) {
             const int64_t i = static_cast<int64_t>(page) * a.p.n_kv + kvh;
             ke = scale_exp(a.p.ks[i]);
@@ -145,15 +157,17 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
 #pragma unroll
     for (int u = 0; u < NU; u++) koff[u] = static_cast<uint32_t>(c * hd + (u * 64 + g4 * 16 < hd ? u * 64 + g4 * 16 : 0));
     const uint32_t voff = static_cast<uint32_t>(4 * g4 * hd + (c * VW * 4 < hd ? c * VW * 4 : 0));
+    const uint8_t* k_head = a.p.k + kvh * a.p.head_bytes;
+    const uint8_t* v_head = a.p.v + kvh * a.p.head_bytes;
     auto load = [&](int tile, KvTile<DH>& t) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             const int id = __builtin_amdgcn_readlane(page, 2 * (tile & 31) + b);
             // A block without a page reads page 0; its keys are masked. Every slot of a page may be read.
             const int32_t slot = (kw + 32 * tile + 16 * b) & ((1 << a.p.page_log2) - 1);
-            const int64_t at = ((static_cast<int64_t>(id < 0 ? 0 : id) * a.p.n_kv + kvh) << a.p.page_log2) + slot;
-            const uint8_t* kp = a.p.k + at * hd;
-            const uint8_t* vp = a.p.v + at * hd;
+            const uint64_t at = static_cast<uint64_t>(static_cast<uint32_t>(id < 0 ? 0 : id)) * a.p.page_bytes + static_cast<uint32_t>(slot * hd);
+            const uint8_t* kp = k_head + at;
+            const uint8_t* vp = v_head + at;
 #pragma unroll
             for (int u = 0; u < NU; u++) t.k[b][u] = *reinterpret_cast<const uint4v*>(kp + koff[u]);
 #pragma unroll
@@ -165,7 +179,7 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
     float m = -__builtin_inff(), l = 0.0f;
     bool seen = false;
     // acc += V^T B of one tile, four dimensions of each lane: x, a word of each key's row.
-    auto product = [&](const uint32_t (&x)[2][4], half8 bh, half8 bl, bool two, float4v* acc) __attribute__((always_inline)) {
+    auto product = [&](const uint32_t (&x)[2][4], half8 bh, half8 bl, float4v* acc) __attribute__((always_inline)) {
         half2v y[4][2][2];  // [dimension][block][key pair]
 #pragma unroll
         for (int b = 0; b < 2; b++) {
@@ -186,7 +200,7 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
         for (int e = 0; e < 4; e++) {
             const half8 A = {y[e][0][0][0], y[e][0][0][1], y[e][0][1][0], y[e][0][1][1],
                              y[e][1][0][0], y[e][1][0][1], y[e][1][1][0], y[e][1][1][1]};
-            if (two) acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bl, acc[e], 0, 0, 0);
+            acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bl, acc[e], 0, 0, 0);
             acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bh, acc[e], 0, 0, 0);
         }
     };
@@ -217,9 +231,10 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
                         A[4 * w + 2] = x1[0];
                         A[4 * w + 3] = x1[1];
                     }
-                    if constexpr (kTwo) s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, ql[2 * u + h], s[b], 0, 0, 0);
-                    s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, qh[2 * u + h], s[b], 0, 0, 0);
+                    if constexpr (kTwo) s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, q_sh[1][2 * u + h][lane], s[b], 0, 0, 0);
+                    s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, q_sh[0][2 * u + h][lane], s[b], 0, 0, 0);
                 }
+        const float sc = kTwo ? sc_sh[c] : a.scale == 0.0f ? 1.0f : fabsf(a.scale);
         float f[2];  // score -> exponent of 2
 #pragma unroll
         for (int b = 0; b < 2; b++) {
@@ -242,23 +257,22 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
         }
         // Keys that some row of the tile does not see.
         const bool partial = j0 < tk.lo_max || j0 + 32 > tk.hi_min || !ok[0] || !ok[1];
-        uint32_t visible = 0xff;
+        bool any_visible = true;
         if (partial) {
+            any_visible = false;
 #pragma unroll
             for (int b = 0; b < 2; b++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int32_t j = j0 + 16 * b + 4 * g4 + i;
                     const bool vis = ok[b] && j >= lo && j < hi;
-                    if (!vis) {
-                        s[b][i] = -__builtin_inff();
-                        visible &= ~(1u << (4 * b + i));
-                    }
+                    if (!vis) s[b][i] = -__builtin_inff();
+                    any_visible = any_visible || vis;
                     // What no row sees may be anything, codes of no token included.
                     if (!(ok[b] && j >= tk.lo_min && j < tk.hi_max)) t.v[b][i] = Words<VW>{};
                 }
         }
-        seen = seen || visible != 0;
+        seen = seen || any_visible;
         float top = -__builtin_inff();
 #pragma unroll
         for (int b = 0; b < 2; b++) {
@@ -292,8 +306,10 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
             }
             l = __builtin_fmaf(sum, exp2i(-ve2[b]), l);
         }
-        // A NaN code times a weight of zero is NaN, so where rows see different keys NaN codes are taken out, and put
-        // into the dimensions of the rows that do see them.
+        // A NaN code times a weight of zero is NaN, so where rows see different keys NaN codes are taken out, noted by
+        // key and lane in this wave's part of the LDS that is free until the end, and put into the dimensions of the
+        // rows that do see them.
+        uint16_t* nan_at = reinterpret_cast<uint16_t*>(o_sh + wave * kTileRows * kRow);  // [32 keys][16]
         bool mend = false;
         if (partial && (tk.hi_min != tk.hi_max || tk.lo_min != tk.lo_max)) {
             uint32_t any = 0;
@@ -304,6 +320,22 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
 #pragma unroll
                     for (int w = 0; w < VW; w++) any |= nan_codes(t.v[b][i].w[w]);
             mend = __any(any != 0);
+            if (mend) {
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        uint32_t at = 0;
+#pragma unroll
+                        for (int w = 0; w < VW; w++) {
+                            const uint32_t nan = nan_codes(t.v[b][i].w[w]) >> 7;
+                            t.v[b][i].w[w] &= ~(nan * 0xffu);
+                            at |= ((nan * 0x01020408u) >> 24) << (4 * w);
+                        }
+                        nan_at[(16 * b + 4 * g4 + i) * 16 + c] = static_cast<uint16_t>(at);
+                    }
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            }
         }
 #pragma unroll
         for (int w = 0; w < VW; w++) {
@@ -312,35 +344,35 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
             for (int b = 0; b < 2; b++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[b][i] = t.v[b][i].w[w];
-            if (mend) {
-                uint32_t bad[2][4];
-                half8 sees;
+            product(x, ph, pl, o + 4 * w);
+        }
+        if (mend) {
+#pragma unroll 1
+            for (int k = 0; k < 32; k++) {
+                if (j0 + k < lo || j0 + k >= hi) continue;  // (a block without a page has no NaN left)
 #pragma unroll
-                for (int b = 0; b < 2; b++)
+                for (int i = 0; i < 4; i++) {
+                    const uint32_t at = nan_at[k * 16 + 4 * g4 + i];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        sees[4 * b + i] = static_cast<half_t>((visible >> (4 * b + i)) & 1u ? 1.0f : 0.0f);
-                        const uint32_t nan = nan_codes(x[b][i]) >> 7;
-                        bad[b][i] = nan * 0x38u;  // the code of 1
-                        x[b][i] &= ~(nan * 0xffu);
-                    }
-                float4v count[4] = {};
-                product(bad, sees, sees, false, count);
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (count[e][i] > 0.0f) o[4 * w + e][i] = __builtin_nanf("");
+                    for (int e = 0; e < NE; e++)
+                        if ((at >> e) & 1u) o[e][i] = __builtin_nanf("");
+                }
             }
-            product(x, ph, pl, true, o + 4 * w);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
     };
 
+    if (n > 0) look_up(0);
+    KvTile<DH> t;
+    if (n > 0) load(0, t);
+    __syncthreads();  // q is there
     for (int i = 0; i < n; i++) {
-        if ((i & 31) == 0) look_up(i);
-        KvTile<DH> t;
-        load(i, t);
+        asm volatile("" ::: "memory");  // (q is read again for each tile)
         step(i, t);
+        if (i + 1 < n) {
+            if (((i + 1) & 31) == 0) look_up(i + 1);
+            load(i + 1, t);
+        }
     }
 
     // The waves' results meet in LDS.
@@ -351,7 +383,7 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
         l_sh[wave][c] = l;
         seen_sh[wave][c] = any_seen;
     }
-    const int rows_here = min(kTileRows, n_rows - it.tile * kTileRows);
+    const int rows_here = min(kTileRows, n_rows - (it.tile << 4));
     if (c < rows_here) {
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -385,7 +417,7 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
             *reinterpret_cast<float4v*>(a.part + at * DH + d) = x;
             if (d == 0) *reinterpret_cast<float4v*>(a.ml + at * 4) = float4v{mm, ll, ss, 0.0f};
         } else if (d < hd) {
-            store_row<TQ>(a, r, kvh, it.tile * kTileRows + i, d, x, row_factor(ll, ss > 0.0f));
+            store_row<TQ>(a, r, kvh, (it.tile << 4) + i, d, x, row_factor(ll, ss > 0.0f));
         }
     }
 }
@@ -395,17 +427,18 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
 template <typename TQ, int DH>
 __global__ __launch_bounds__(256) void attn_paged_merge(PagedAttnArgs a) {
     constexpr int LPR = DH / 4, RPB = 256 / LPR, AHEAD = 8;
-    const int kvh = static_cast<int>(blockIdx.x % static_cast<uint32_t>(a.p.n_kv));
+    int kvh;
+    const uint32_t item = item_of(a, &kvh);
     AttnItem it;
-    if (!attn_find<true>(a.p, a.t, blockIdx.x / static_cast<uint32_t>(a.p.n_kv), &it)) return;
+    if (!attn_find<true>(a.p, a.t, item, &it)) return;
     const SeqRows r = paged_seq(a.p, it.s);
     const int d = static_cast<int>(threadIdx.x) % LPR * 4;
     const int i = static_cast<int>(blockIdx.y) * RPB + static_cast<int>(threadIdx.x) / LPR;
-    const int32_t row = it.tile * a.t.tile_rows + i;
+    const int32_t row = (it.tile << a.t.tile_log2) + i;
     const uint32_t n_kv = static_cast<uint32_t>(a.p.n_kv);
-    if (i >= a.t.tile_rows || row >= r.n * a.t.group) return;
+    if (row >= r.n * a.t.group) return;
     if ((static_cast<uint64_t>(it.block) + static_cast<uint64_t>(it.splits)) * n_kv > a.blocks) return;
-    const int64_t first = static_cast<int64_t>(it.block * n_kv + kvh) * a.t.tile_rows + i, step = static_cast<int64_t>(n_kv) * a.t.tile_rows;
+    const int64_t first = (static_cast<int64_t>(it.block * n_kv + kvh) << a.t.tile_log2) + i, step = static_cast<int64_t>(n_kv) << a.t.tile_log2;
     float m = -__builtin_inff(), l = 0.0f, ss = 0.0f;
     float4v x = {};
     for (int k0 = 0; k0 < it.splits; k0 += AHEAD) {
@@ -446,18 +479,19 @@ struct Grid {
 Grid grid_of(const PagedAttnArgs& a, int dh) {
     Grid g;
     g.blocks = attn_blocks_bound(a.t, a.p.rows, a.p.n_seq, a.p.n_kv) * a.p.n_kv;
-    g.bytes = attn_may_split(a.t, a.p) ? static_cast<size_t>(g.blocks) * a.t.tile_rows * (dh + 4) * sizeof(float) : 0;
+    g.bytes = attn_may_split(a.t, a.p) ? (static_cast<size_t>(g.blocks) << a.t.tile_log2) * (dh + 4) * sizeof(float) : 0;
     return g;
 }
 
 // The tiling of the 16-row kernel with `waves` waves to a workgroup, 16 of which a CU holds: as many workgroups as
 // are resident at once, tiles that are not split included.
 void few_form(const neko_hip_ctx* ctx, PagedAttnArgs& a, int waves) {
-    a.t.tile_rows = kTileRows;
-    a.t.unit = 32 * waves;
+    a.t.tile_log2 = 4;
+    a.t.unit_log2 = 5 + __builtin_ctz(static_cast<unsigned>(waves));
     a.t.least = kLeast;
     const int64_t room = 16LL * ctx->cu_count / waves, items = attn_tiles_bound(a.t, a.p.rows, a.p.n_seq) * a.p.n_kv;
     a.t.target = static_cast<int32_t>(std::max<int64_t>(room - items, room / 2));
+    attn_set(a.t);
 }
 
 template <typename TQ, int DH, int NW, bool MODS>
@@ -473,15 +507,15 @@ int launch_few(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a) {
 template <typename TQ, int DH>
 int launch_dims(neko_hip_ctx* ctx, const char* what, PagedAttnArgs a, int dtype) {
     // Sequences of up to kFewRows rows on the 16-row kernel, the rest on the tiles. Which a batch has is known on the
-    // device alone, so both are launched, except where no sequence can be the other's: one sequence, or as many rows
-    // as sequences (then any that has more than one is the 16-row kernel's too).
+    // device alone, so both are launched, except where there is one sequence, or no more rows than a padded decoding
+    // batch has: then the 16-row kernel takes whatever there is.
     const int64_t most = static_cast<int64_t>(a.p.rows) * a.t.group;
-    const bool few = a.p.n_seq > 1 || most <= kFewRows;
-    const bool many = most > kFewRows && a.p.rows > a.p.n_seq;
+    const bool many = a.p.n_seq == 1 ? most > kFewRows : most > static_cast<int64_t>(a.p.n_seq) * a.t.group + kSpareRows;
+    const bool few = a.p.n_seq > 1 || !many;
     constexpr int kMostWaves = DH <= 128 && sizeof(TQ) == 2 ? 16 : 8;
     PagedAttnArgs f = a, t = a;
     // Few items: many waves to each, whose results meet in LDS.
-    f.t.tile_rows = kTileRows;
+    f.t.tile_log2 = 4;
     const int64_t items = attn_tiles_bound(f.t, a.p.rows, a.p.n_seq) * a.p.n_kv;
     const bool wide = items <= ctx->cu_count;
     few_form(ctx, f, wide ? kMostWaves : 4);
@@ -499,12 +533,12 @@ int launch_dims(neko_hip_ctx* ctx, const char* what, PagedAttnArgs a, int dtype)
     auto place = [](PagedAttnArgs& x, const Grid& g, void* at) {
         x.blocks = static_cast<uint32_t>(g.blocks);
         x.part = static_cast<float*>(at);
-        x.ml = x.part + g.blocks * x.t.tile_rows * DH;
+        x.ml = x.part + (g.blocks << x.t.tile_log2) * DH;
     };
     auto merge = [&](const PagedAttnArgs& x) {
         if (!attn_may_split(x.t, x.p)) return NEKO_OK;
         const int64_t tiles = attn_split_tiles_bound(x.t, x.p.rows, x.p.n_seq, x.p.n_kv) * x.p.n_kv;
-        const dim3 grid(static_cast<uint32_t>(tiles), static_cast<uint32_t>((x.t.tile_rows * DH + 1023) / 1024));
+        const dim3 grid(static_cast<uint32_t>(tiles), static_cast<uint32_t>((DH << x.t.tile_log2) / 1024));
         hipLaunchKernelGGL((attn_paged_merge<TQ, DH>), grid, dim3(256), 0, ctx->stream, x);
         return after_launch(ctx, what);
     };
@@ -567,8 +601,9 @@ extern "C" int neko_hip_attention_paged(neko_hip_ctx* ctx, const void* q, int64_
     a.os = out_stride;
     a.n_head = n_head;
     a.t.group = n_head / kv->n_kv;
-    a.window = window < (1 << 30) ? static_cast<int32_t>(window) : 0;
-    a.t.window = a.window;
+    a.t.window = window < (1 << 30) ? static_cast<int32_t>(window) : 0;
+    a.by_group = make_fast_div(static_cast<uint32_t>(a.t.group));
+    a.by_kv = make_fast_div(static_cast<uint32_t>(kv->n_kv));
     a.scale = scale;
     a.softcap = softcap;
     a.slopes = slopes;

@@ -61,9 +61,10 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
     const int l32 = lane & 31, h = lane >> 5;
-    const int kvh = static_cast<int>(blockIdx.x % static_cast<uint32_t>(a.p.n_kv));
+    int kvh;
+    const uint32_t item = item_of(a, &kvh);
     AttnItem it;
-    if (!attn_find<false>(a.p, a.t, blockIdx.x / static_cast<uint32_t>(a.p.n_kv), &it)) return;
+    if (!attn_find<false>(a.p, a.t, item, &it)) return;
     const SeqRows r = paged_seq(a.p, it.s);
     const TileKeys tk = tile_keys(a, r, it);
     const int hd = a.p.hd;
@@ -72,12 +73,13 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     // This lane's row, and the keys that this wave's rows see (rows past the last repeat it).
     const int32_t n_rows = r.n * a.t.group, row0 = it.tile * C::rows + 32 * wave;
     const int32_t row = min(row0 + l32, n_rows - 1);
-    const int32_t tok = row / a.t.group;
+    const int32_t tok = static_cast<int32_t>(fast_div(static_cast<uint32_t>(row), a.by_group));
     const int head = kvh * a.t.group + (row - tok * a.t.group);
     const int32_t pos = r.len - r.n + tok;
-    const int32_t hi = min(pos + 1, reach), lo = key_lo(pos, a.window);
-    const int32_t w_first = r.len - r.n + min(row0, n_rows - 1) / a.t.group, w_last = r.len - r.n + min(row0 + 31, n_rows - 1) / a.t.group;
-    const int32_t w_lo_min = key_lo(w_first, a.window), w_lo_max = key_lo(w_last, a.window);
+    const int32_t hi = min(pos + 1, reach), lo = key_lo(pos, a.t.window);
+    const int32_t w_first = r.len - r.n + static_cast<int32_t>(fast_div(static_cast<uint32_t>(min(row0, n_rows - 1)), a.by_group));
+    const int32_t w_last = r.len - r.n + static_cast<int32_t>(fast_div(static_cast<uint32_t>(min(row0 + 31, n_rows - 1)), a.by_group));
+    const int32_t w_lo_min = key_lo(w_first, a.t.window), w_lo_max = key_lo(w_last, a.t.window);
     const int32_t w_hi_min = min(w_first + 1, reach), w_hi_max = min(w_last + 1, reach);
 
     // q: dimensions 16 s + 8 h .. + 7 of the row as the B operand of step s.
@@ -149,6 +151,8 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     };
     Raw raw;
     int info[C::blocks], info1[C::blocks];  // of the tile in `raw`, of the tile after the one being multiplied
+    const uint8_t* k_head = a.p.k + kvh * a.p.head_bytes;
+    const uint8_t* v_head = a.p.v + kvh * a.p.head_bytes;
     auto load = [&](int tile) __attribute__((always_inline)) {
         const int at = tile % C::window * C::blocks;
 #pragma unroll
@@ -158,8 +162,8 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
             const int u = wave * C::units + i, b = u % C::blocks;
             const int id = __builtin_amdgcn_readlane(page, at + b);
             const int32_t slot = (tk.k0 + C::keys * tile + kBlockKeys * b) & ((1 << a.p.page_log2) - 1);
-            const uint8_t* from = (u < C::blocks ? a.p.k : a.p.v) +
-                                  (((static_cast<int64_t>(id < 0 ? 0 : id) * a.p.n_kv + kvh) << a.p.page_log2) + slot) * hd;
+            const uint8_t* from = (u < C::blocks ? k_head : v_head) + static_cast<uint64_t>(static_cast<uint32_t>(id < 0 ? 0 : id)) * a.p.page_bytes +
+                                  static_cast<uint32_t>(slot * hd);
 #pragma unroll
             for (int n = 0; n < C::loads; n++) raw.x[i][n] = *reinterpret_cast<const uint4v*>(from + ((n * C::rpi + lr) * hd + src));
         }
@@ -454,10 +458,11 @@ int launch_dims(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a) {
 }  // namespace
 
 void attn_paged_tile_form(const neko_hip_ctx* ctx, PagedAttnArgs& a) {
-    a.t.tile_rows = TileForm<128>::rows;
-    a.t.unit = 64;  // a whole number of tiles of either size
+    a.t.tile_log2 = 7;  // TileForm::rows
+    a.t.unit_log2 = 6;  // a whole number of tiles of either size
     a.t.target = 2 * ctx->cu_count;
     a.t.least = 1;
+    attn_set(a.t);
 }
 
 int attn_paged_tile(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a, int dtype) {

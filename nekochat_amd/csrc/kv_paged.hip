@@ -166,8 +166,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, const Segment& 
     }
     const int need = need_exp(top);
     const int e = need > had ? need : had;
-    uint8_t* page = (is_k ? a.p.k : a.p.v) +
-                    ((static_cast<int64_t>(seg.page) * a.p.n_kv + g) << a.p.page_log2) * static_cast<int64_t>(hd);
+    uint8_t* page = (is_k ? a.p.k : a.p.v) + static_cast<uint64_t>(seg.page) * a.p.page_bytes + g * a.p.head_bytes;
     if (seg.a > 0 && e > had) {  // the tokens that were there, under the new scale
         const float down = exp2i(had - e < -126 ? -126 : had - e);
 #pragma unroll 1
@@ -331,7 +330,7 @@ int paged_args(neko_hip_ctx* ctx, const char* what, const neko_paged_kv* kv, con
                  kv->hd);
     NEKO_REQUIRE(ctx, kv->page_size >= 16 && kv->page_size <= 256 && (kv->page_size & (kv->page_size - 1)) == 0,
                  "%s: page size %d (a power of two, 16..256)", what, kv->page_size);
-    NEKO_REQUIRE(ctx, kv->n_kv > 0 && kv->n_kv <= 4096, "%s: n_kv=%d (1..4096)", what, kv->n_kv);
+    NEKO_REQUIRE(ctx, kv->n_kv > 0 && kv->n_kv <= 4095, "%s: n_kv=%d (1..4095)", what, kv->n_kv);
     NEKO_REQUIRE(ctx, kv->n_pages > 0 && kv->n_pages <= 0x7fffffff, "%s: n_pages=%lld", what, (long long)kv->n_pages);
     NEKO_REQUIRE(ctx, aligned(kv->k_pages, 16) && aligned(kv->v_pages, 16) && aligned(kv->k_scales, 4) && aligned(kv->v_scales, 4),
                  "%s: pages must be 16-byte aligned, scales 4-byte", what);
@@ -361,6 +360,8 @@ int paged_args(neko_hip_ctx* ctx, const char* what, const neko_paged_kv* kv, con
     p->page_log2 = __builtin_ctz(static_cast<unsigned>(kv->page_size));
     p->n_kv = kv->n_kv;
     p->hd = kv->hd;
+    p->head_bytes = static_cast<uint32_t>(kv->page_size * kv->hd);
+    p->page_bytes = p->head_bytes * static_cast<uint32_t>(kv->n_kv);
     return NEKO_OK;
 }
 

@@ -36,6 +36,8 @@ struct Paged {
     int32_t page_log2;
     int32_t n_kv;
     int32_t hd;
+    uint32_t head_bytes;  // of one kv head's tokens of a page: page * hd
+    uint32_t page_bytes;  // n_kv * head_bytes (paged_args: below 2^28)
 };
 
 struct SeqRows {
@@ -127,44 +129,63 @@ NEKO_HD Segment paged_segment(const Paged& p, int32_t s, int32_t i, int32_t limi
 // into tiles of `tile_rows`; a tile's keys into splits of `chunk` keys, so that the launch has about `target`
 // workgroups whatever the lengths are, which only the device knows.
 struct AttnTiling {
-    int32_t group;      // query heads per kv head
-    int32_t tile_rows;  // flattened (token, head) rows of a tile
-    int32_t unit;       // keys that a split is a multiple of
-    int32_t target;     // workgroups wanted
-    int32_t least;      // units of a split, at least
-    int64_t window;     // 0: none
+    int32_t group;       // query heads per kv head
+    int32_t tile_log2;   // flattened (token, head) rows of a tile
+    int32_t unit_log2;   // keys that a split is a multiple of
+    int32_t target;      // workgroups wanted
+    int32_t least;       // units of a split, at least
+    int32_t window;      // 0: none
+    int32_t span;        // with a window: the keys that a tile spans at most (attn_set)
+    double per_target;   // 1 / target (attn_set)
     // Sequences with min_rows <= flattened rows <= max_rows are this launch's.
     int32_t min_rows, max_rows;
 };
 
+// The derived fields. A tile spans its first token's window and its further tokens, from a multiple of 32.
+NEKO_HD void attn_set(AttnTiling& t) {
+    const int64_t span = static_cast<int64_t>(t.window) + ((1 << t.tile_log2) / t.group + 2) + 32;
+    t.span = span < (1 << 30) ? static_cast<int32_t>(span) : 1 << 30;
+    t.per_target = 1.0 / t.target;
+}
+
 NEKO_HD int32_t attn_tiles(const AttnTiling& t, const SeqRows& r) {
-    const int64_t rows = static_cast<int64_t>(r.n) * t.group;
+    const int32_t rows = r.n * t.group;  // rows * n_head <= 2^30
     if (rows < t.min_rows || rows > t.max_rows) return 0;
-    return static_cast<int32_t>((rows + t.tile_rows - 1) / t.tile_rows);
+    return (rows + (1 << t.tile_log2) - 1) >> t.tile_log2;
 }
 
-// Units of keys that a tile of this sequence spans at most: all of them, or the window and the tokens of the
-// tile past its first, from a multiple of 32.
-NEKO_HD int32_t attn_units(const AttnTiling& t, const Paged& p, const SeqRows& r) {
-    int64_t keys = r.len < paged_reach(p) ? r.len : paged_reach(p);
-    const int64_t most = t.window + (t.tile_rows / t.group + 2) + 32;
-    if (t.window > 0 && most < keys) keys = most;
-    return static_cast<int32_t>((keys + t.unit - 1) / t.unit);
+// Units of keys that a tile of this sequence spans at most: all of them, or the window's.
+NEKO_HD int32_t attn_units(const AttnTiling& t, int32_t reach, const SeqRows& r) {
+    int32_t keys = r.len < reach ? r.len : reach;
+    if (t.window > 0 && t.span < keys) keys = t.span;
+    return (keys + (1 << t.unit_log2) - 1) >> t.unit_log2;
 }
 
-// Units per split, from the launch's work: the sum over sequences and kv heads of tiles * units.
-NEKO_HD int32_t attn_chunk(const AttnTiling& t, uint64_t work) {
-    const uint64_t c = (work + static_cast<uint64_t>(t.target) - 1) / static_cast<uint64_t>(t.target);
-    return c < static_cast<uint64_t>(t.least) ? t.least : c > (1u << 30) ? 1 << 30 : static_cast<int32_t>(c);
+// Units per split, from the launch's work, the sum over sequences and kv heads of tiles * units (a whole number below
+// 2^53): at least work / target.
+NEKO_HD int32_t attn_chunk(const AttnTiling& t, double work) {
+    const double c = work * t.per_target;
+    const int32_t n = (c < 1e9 ? static_cast<int32_t>(c) : 1000000000) + 1;
+    return n < t.least ? t.least : n;
 }
 
-NEKO_HD int32_t attn_splits(int32_t units, int32_t chunk) { return units <= chunk ? 1 : (units + chunk - 1) / chunk; }
+// ceil(units / chunk) without an integer division: the quotient by a reciprocal is off by one at most for the fewer
+// than 2^20 splits that there are, and put right.
+NEKO_HD int32_t attn_splits(int32_t units, int32_t chunk) {
+    if (units <= chunk) return 1;
+    int32_t q = static_cast<int32_t>(static_cast<float>(units) * (1.0f / static_cast<float>(chunk)));
+    const int32_t left = units - q * chunk;
+    if (left > 0) q++;
+    if (left > chunk) q++;
+    if (left <= -chunk) q--;
+    return q;
+}
 
 // Workgroups per kv head that the splits above can come to: sum of tiles * splits <= work / (n_kv * chunk) +
 // sum of tiles, and the tiles number at most rows * group / tile_rows + n_seq. Tiles that are split have more than
 // chunk units each, so they number at most work / (n_kv * chunk) <= target / n_kv.
 NEKO_HD int64_t attn_tiles_bound(const AttnTiling& t, int64_t rows, int64_t n_seq) {
-    const int64_t tiles = rows * t.group / t.tile_rows + (rows < n_seq ? rows : n_seq);
+    const int64_t tiles = ((rows * t.group) >> t.tile_log2) + (rows < n_seq ? rows : n_seq);
     return tiles < rows * t.group ? tiles : rows * t.group;
 }
 NEKO_HD int64_t attn_blocks_bound(const AttnTiling& t, int64_t rows, int64_t n_seq, int n_kv) {
@@ -177,9 +198,9 @@ NEKO_HD int64_t attn_split_tiles_bound(const AttnTiling& t, int64_t rows, int64_
 }
 // Whether any tile can be split. One sequence: its tiles are known, and with as many as wanted chunk >= units.
 NEKO_HD bool attn_may_split(const AttnTiling& t, const Paged& p) {
-    if (paged_reach(p) <= static_cast<int64_t>(t.least) * t.unit) return false;
+    if (paged_reach(p) <= static_cast<int64_t>(t.least) << t.unit_log2) return false;
     if (p.n_seq > 1) return true;
-    const int64_t tiles = (static_cast<int64_t>(p.rows) * t.group + t.tile_rows - 1) / t.tile_rows;
+    const int64_t tiles = (static_cast<int64_t>(p.rows) * t.group + (1 << t.tile_log2) - 1) >> t.tile_log2;
     return tiles * p.n_kv < t.target;
 }
 

@@ -62,18 +62,21 @@ int64_t check_segments(const Batch* b, int32_t limit, int32_t* out, int64_t room
 }
 
 // The attention launch's workgroups per kv head and the bounds that the host sizes the grid and workspace by.
-void check_blocks(const Batch* b, const AttnTiling* t, int64_t* out) {
+void check_blocks(const Batch* b, const AttnTiling* given, int64_t* out) {
     const Paged p = paged(b);
-    uint64_t work = 0;
+    AttnTiling t = *given;
+    attn_set(t);
+    const int32_t reach = paged_reach(p);
+    double work = 0;
     for (int32_t s = 0; s < p.n_seq; s++) {
         const SeqRows r = paged_seq(p, s);
-        work += static_cast<uint64_t>(attn_tiles(*t, r)) * static_cast<uint64_t>(attn_units(*t, p, r));
+        work += static_cast<double>(attn_tiles(t, r)) * attn_units(t, reach, r);
     }
-    const int32_t chunk = attn_chunk(*t, work * static_cast<uint64_t>(p.n_kv));
+    const int32_t chunk = attn_chunk(t, work * p.n_kv);
     int64_t tiles = 0, blocks = 0, uncovered = 0, split = 0;
     for (int32_t s = 0; s < p.n_seq; s++) {
         const SeqRows r = paged_seq(p, s);
-        const int64_t n = attn_tiles(*t, r), units = attn_units(*t, p, r), splits = attn_splits(static_cast<int32_t>(units), chunk);
+        const int64_t n = attn_tiles(t, r), units = attn_units(t, reach, r), splits = attn_splits(static_cast<int32_t>(units), chunk);
         tiles += n;
         blocks += n * splits;
         if (n && splits * chunk < units) uncovered++;
@@ -81,11 +84,13 @@ void check_blocks(const Batch* b, const AttnTiling* t, int64_t* out) {
     }
     out[0] = tiles;
     out[1] = blocks;
-    out[2] = attn_tiles_bound(*t, p.rows, p.n_seq);
-    out[3] = attn_blocks_bound(*t, p.rows, p.n_seq, p.n_kv);
+    out[2] = attn_tiles_bound(t, p.rows, p.n_seq);
+    out[3] = attn_blocks_bound(t, p.rows, p.n_seq, p.n_kv);
     out[4] = uncovered;
     out[5] = split;
-    out[6] = attn_may_split(*t, p) ? attn_split_tiles_bound(*t, p.rows, p.n_seq, p.n_kv) : 0;
+    out[6] = attn_may_split(t, p) ? attn_split_tiles_bound(t, p.rows, p.n_seq, p.n_kv) : 0;
 }
+
+int check_splits(int32_t units, int32_t chunk) { return attn_splits(units, chunk); }
 
 }  // extern "C"

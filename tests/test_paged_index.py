@@ -19,9 +19,9 @@ class Batch(ctypes.Structure):
 
 
 class Tiling(ctypes.Structure):
-    _fields_ = [("group", ctypes.c_int32), ("tile_rows", ctypes.c_int32), ("unit", ctypes.c_int32),
-                ("target", ctypes.c_int32), ("least", ctypes.c_int32), ("window", ctypes.c_int64), ("min_rows", ctypes.c_int32),
-                ("max_rows", ctypes.c_int32)]
+    _fields_ = [("group", ctypes.c_int32), ("tile_log2", ctypes.c_int32), ("unit_log2", ctypes.c_int32),
+                ("target", ctypes.c_int32), ("least", ctypes.c_int32), ("window", ctypes.c_int32), ("span", ctypes.c_int32),
+                ("per_target", ctypes.c_double), ("min_rows", ctypes.c_int32), ("max_rows", ctypes.c_int32)]
 
 
 @pytest.fixture(scope="module")
@@ -116,12 +116,24 @@ def test_attention_blocks_stay_within_the_grid(lib, seed):
     b = _batch(rng, wild=False)
     group = int(rng.choice([1, 2, 3, 4, 8, 16, 40]))
     few = int(rng.choice([0, 16, 32]))
-    t = Tiling(group, int(rng.choice([16, 64, 128, 256])), int(rng.choice([64, 128])), int(rng.choice([1, 7, 256, 1024])),
-               int(rng.choice([1, 8])), int(rng.choice([0, 1, 40, 1000])), *((1, 2**31 - 1) if not few else (few + 1, 2**31 - 1) if rng.random() < 0.5 else (1, few)))
+    few = (few + 1, 2**31 - 1) if few and rng.random() < 0.5 else (1, few or 2**31 - 1)
+    t = Tiling(group, int(rng.choice([4, 6, 7, 8])), int(rng.choice([6, 7, 9])), int(rng.choice([1, 7, 256, 1024])),
+               int(rng.choice([1, 8])), int(rng.choice([0, 1, 40, 1000])), 0, 0.0, *few)
     out = (ctypes.c_int64 * 7)()
     lib.check_blocks(ctypes.byref(b), ctypes.byref(t), out)
     tiles, blocks, tiles_bound, blocks_bound, uncovered, split, split_bound = out
     assert tiles <= tiles_bound and blocks <= blocks_bound and uncovered == 0 and split <= split_bound
+
+
+def test_splits_are_the_ceiling(lib):
+    rng = np.random.default_rng(2)
+    for _ in range(20000):
+        chunk = int(np.exp(rng.uniform(0, 14)))
+        units = int(rng.integers(0, min(2**25, chunk * 4000)))
+        if rng.random() < 0.5:
+            units = units // chunk * chunk + int(rng.integers(-1, 2))
+        units = max(units, 0)
+        assert lib.check_splits(units, chunk) == max(1, -(-units // chunk)), (units, chunk)
 
 
 def test_scale_exponents(lib):
