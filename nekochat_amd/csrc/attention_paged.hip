@@ -42,7 +42,7 @@ struct KvTile {
 
 // Waves per SIMD that the kernel is compiled for.
 template <typename TQ, int DH>
-constexpr int kResident = DH <= 64 ? 4 : DH <= 128 ? (sizeof(TQ) == 2 ? 4 : 3) : 2;
+constexpr int kResident = DH <= 64 ? 4 : DH <= 128 ? 3 : 1;
 
 // Four dimensions, from d on, of a finished row.
 template <typename TQ>
@@ -69,10 +69,34 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
     const int c = lane & 15, g4 = lane >> 4;
     int kvh;
     const uint32_t item = item_of(a, &kvh);
+    // The item, by one wave for all: the search is issue-bound, and waves of a SIMD would do it in turn.
+    __shared__ int32_t item_sh[16];
+    if (wave == 0) {
+        AttnItem f;
+        const bool found = attn_find<false>(a.p, a.t, item, &f);
+        if (found) {
+            const SeqRows r = paged_seq(a.p, f.s);
+            const TileKeys k = tile_keys(a, r, f);
+            if (lane == 0) {
+                const int32_t x[14] = {f.s,      f.tile,   f.splits, static_cast<int32_t>(f.block), r.begin, r.n, r.len, k.lo_min,
+                                       k.lo_max, k.hi_min, k.hi_max, k.k0, k.k1, 1};
+#pragma unroll
+                for (int i = 0; i < 14; i++) item_sh[i] = x[i];
+            }
+        } else if (lane == 0) {
+            item_sh[13] = 0;
+        }
+    }
+    __syncthreads();
+    auto shared_at = [&](int i) { return __builtin_amdgcn_readfirstlane(item_sh[i]); };
+    if (!shared_at(13)) return;
     AttnItem it;
-    if (!attn_find<false>(a.p, a.t, item, &it)) return;
-    const SeqRows r = paged_seq(a.p, it.s);
-    const TileKeys tk = tile_keys(a, r, it);
+    it.s = shared_at(0);
+    it.tile = shared_at(1);
+    it.splits = shared_at(2);
+    it.block = static_cast<uint32_t>(shared_at(3));
+    const SeqRows r = {shared_at(4), shared_at(5), shared_at(6)};
+    const TileKeys tk = {shared_at(7), shared_at(8), shared_at(9), shared_at(10), shared_at(11), shared_at(12)};
     const int hd = a.p.hd;
 
     // This lane's row (rows past the last repeat it and are not written).
@@ -83,10 +107,10 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
     const int32_t pos = r.len - r.n + tok;
     const int32_t hi = min(pos + 1, min(r.len, paged_reach(a.p))), lo = key_lo(pos, a.t.window);
 
-    // q as the B operands of the first product, the same for all waves, by the last of them: in LDS, where each
+    // q as the B operands of the first product, the same for all waves, by one of them: in LDS, where each
     // wave's registers have room for other things (128 of them at four waves per SIMD). f32 rows are brought to
     // [2^14, 2^15) and split; sc_sh then undoes that. A scale's sign goes into q; a scale of 0 weights all alike.
-    if (wave == NW - 1) {
+    if (wave == 1) {
         const TQ* qr = static_cast<const TQ*>(a.q) + static_cast<int64_t>(r.begin + tok) * a.qs + static_cast<int64_t>(head) * hd;
         const float sign = a.scale == 0.0f ? 0.0f : a.scale < 0.0f ? -1.0f : 1.0f;
         TQ x[2 * NU][8];
@@ -204,16 +228,16 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
             acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bh, acc[e], 0, 0, 0);
         }
     };
-    auto step = [&](int tile, KvTile<DH>& t) __attribute__((always_inline)) {
+    auto step = [&](int tile, KvTile<DH>& t, int32_t pages, int kes, int ves) __attribute__((always_inline)) {
         const int32_t j0 = kw + 32 * tile;
         int ke2[2], ve2[2];
         bool ok[2];
 #pragma unroll
         for (int b = 0; b < 2; b++) {
             const int idx = 2 * (tile & 31) + b;
-            ke2[b] = __builtin_amdgcn_readlane(ke, idx);
-            ve2[b] = __builtin_amdgcn_readlane(ve, idx);
-            ok[b] = __builtin_amdgcn_readlane(page, idx) >= 0;
+            ke2[b] = __builtin_amdgcn_readlane(kes, idx);
+            ve2[b] = __builtin_amdgcn_readlane(ves, idx);
+            ok[b] = __builtin_amdgcn_readlane(pages, idx) >= 0;
         }
         float4v s[2] = {};
 #pragma unroll
@@ -363,16 +387,19 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
     };
 
     if (n > 0) look_up(0);
-    KvTile<DH> t;
+    KvTile<DH> t, next;
     if (n > 0) load(0, t);
     __syncthreads();  // q is there
     for (int i = 0; i < n; i++) {
         asm volatile("" ::: "memory");  // (q is read again for each tile)
-        step(i, t);
+        const int32_t page_now = page;
+        const int ke_now = ke, ve_now = ve;
         if (i + 1 < n) {
             if (((i + 1) & 31) == 0) look_up(i + 1);
-            load(i + 1, t);
+            load(i + 1, next);
         }
+        step(i, t, page_now, ke_now, ve_now);
+        t = next;
     }
 
     // The waves' results meet in LDS.
@@ -483,13 +510,13 @@ Grid grid_of(const PagedAttnArgs& a, int dh) {
     return g;
 }
 
-// The tiling of the 16-row kernel with `waves` waves to a workgroup, 16 of which a CU holds: as many workgroups as
-// are resident at once, tiles that are not split included.
-void few_form(const neko_hip_ctx* ctx, PagedAttnArgs& a, int waves) {
+// The tiling of the 16-row kernel with `waves` waves to a workgroup, `resident` workgroups to a CU: as many as are
+// resident at once, tiles that are not split included.
+void few_form(const neko_hip_ctx* ctx, PagedAttnArgs& a, int waves, int resident) {
     a.t.tile_log2 = 4;
     a.t.unit_log2 = 5 + __builtin_ctz(static_cast<unsigned>(waves));
-    a.t.least = kLeast;
-    const int64_t room = 16LL * ctx->cu_count / waves, items = attn_tiles_bound(a.t, a.p.rows, a.p.n_seq) * a.p.n_kv;
+    a.t.least = paged_reach(a.p) <= (kLeast << a.t.unit_log2) ? kLeast : 2;
+    const int64_t room = static_cast<int64_t>(resident) * ctx->cu_count, items = attn_tiles_bound(a.t, a.p.rows, a.p.n_seq) * a.p.n_kv;
     a.t.target = static_cast<int32_t>(std::max<int64_t>(room - items, room / 2));
     attn_set(a.t);
 }
@@ -512,13 +539,13 @@ int launch_dims(neko_hip_ctx* ctx, const char* what, PagedAttnArgs a, int dtype)
     const int64_t most = static_cast<int64_t>(a.p.rows) * a.t.group;
     const bool many = a.p.n_seq == 1 ? most > kFewRows : most > static_cast<int64_t>(a.p.n_seq) * a.t.group + kSpareRows;
     const bool few = a.p.n_seq > 1 || !many;
-    constexpr int kMostWaves = DH <= 128 && sizeof(TQ) == 2 ? 16 : 8;
+    constexpr int kMostWaves = DH <= 128 ? 8 : 4;
     PagedAttnArgs f = a, t = a;
     // Few items: many waves to each, whose results meet in LDS.
     f.t.tile_log2 = 4;
     const int64_t items = attn_tiles_bound(f.t, a.p.rows, a.p.n_seq) * a.p.n_kv;
     const bool wide = items <= ctx->cu_count;
-    few_form(ctx, f, wide ? kMostWaves : 4);
+    few_form(ctx, f, wide ? kMostWaves : 4, wide ? kResident<TQ, DH> * 4 / kMostWaves : kResident<TQ, DH>);
     f.t.min_rows = 1;
     f.t.max_rows = many ? kFewRows : 0x7fffffff;
     attn_paged_tile_form(ctx, t);
