@@ -29,7 +29,8 @@ constexpr int kPOffset = 15;  // weights go to f16 times 2^kPOffset, the largest
 constexpr float kPScale = 1 << kPOffset;
 
 struct AttnItem {
-    int32_t s, tile, split, splits, chunk;
+    int32_t s, tile, split, splits;
+    int32_t chunk;  // units of a split
     uint32_t block;  // index of the (tile, split) among those of a kv head
 };
 
@@ -63,11 +64,13 @@ __device__ __forceinline__ bool attn_find(const Paged& p, const AttnTiling& t, u
         }
     };
     double work = 0.0;  // (whole numbers below 2^53: exact)
+    uint32_t all = 0;
     for (int32_t base = 0; base < p.n_seq; base += 64) {
         load(base);
         work += wave_sum_f64(static_cast<double>(tiles) * static_cast<double>(units));
+        all += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_scan_u32(static_cast<uint32_t>(tiles))), 63));
     }
-    const int32_t chunk = attn_chunk(t, work * p.n_kv);
+    const int32_t chunk = attn_chunk(t, work * p.n_kv, static_cast<int64_t>(all) * p.n_kv);
     uint32_t past_tiles = 0, past = 0;
     for (int32_t base = 0; base < p.n_seq; base += 64) {
         if (p.n_seq > 64) load(base);
@@ -80,8 +83,8 @@ __device__ __forceinline__ bool attn_find(const Paged& p, const AttnTiling& t, u
             const int l = __builtin_ctzll(at);
             const int32_t n_tiles = __builtin_amdgcn_readlane(tiles, l);
             it->s = base + l;
-            it->chunk = chunk;
             it->splits = __builtin_amdgcn_readlane(splits, l);
+            it->chunk = attn_splits(__builtin_amdgcn_readlane(units, l), it->splits);  // even ones
             const uint32_t first = past + static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum - n), l));
             if constexpr (SPLIT) {
                 const uint32_t local = j - past_tiles - static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum_tiles - split_tiles), l));

@@ -24,7 +24,7 @@ namespace neko_hip {
 namespace {
 
 constexpr int kTileRows = 16;
-constexpr int kLeast = 8;           // tiles of 32 keys to a wave below which no keys are split
+constexpr int kLeast = 8;           // tiles of 32 keys to a wave up to which a cache's keys are never split
 constexpr int kFewRows = 32;        // flattened rows up to which a sequence is this kernel's
 constexpr int kSpareRows = 256;     // flattened rows past one token to a sequence that still make a decoding batch
 
@@ -268,32 +268,44 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
         }
         if constexpr (MODS) {
 #pragma unroll
-            for (int b = 0; b < 2; b++) {
+            for (int b = 0; b < 2; b++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    float x = s[b][i] * f[b];
-                    if (a.softcap > 0.0f) x = cap_score(x, a.softcap, inv_cap);
-                    if (a.slopes) x = __builtin_fmaf(slope, static_cast<float>(j0 + 16 * b + 4 * g4 + i - pos), x);
-                    s[b][i] = x;
-                }
-                f[b] = kAttnLog2e;
+                for (int i = 0; i < 4; i++) s[b][i] *= f[b];
+            if (a.softcap > 0.0f) {
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) s[b][i] = cap_score(s[b][i], a.softcap, inv_cap);
             }
+            if (a.slopes) {
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        s[b][i] = __builtin_fmaf(slope, static_cast<float>(j0 + 16 * b + 4 * g4 + i - pos), s[b][i]);
+            }
+            f[0] = f[1] = kAttnLog2e;
         }
         // Keys that some row of the tile does not see.
         const bool partial = j0 < tk.lo_max || j0 + 32 > tk.hi_min || !ok[0] || !ok[1];
         bool any_visible = true;
         if (partial) {
             any_visible = false;
+            // Visible: lo <= j < hi, as one unsigned comparison; no key of a block without a page. Likewise what any row sees.
+            const uint32_t many = hi > lo ? static_cast<uint32_t>(hi - lo) : 0u;
+            const uint32_t many_any = tk.hi_max > tk.lo_min ? static_cast<uint32_t>(tk.hi_max - tk.lo_min) : 0u;
 #pragma unroll
             for (int b = 0; b < 2; b++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int32_t j = j0 + 16 * b + 4 * g4 + i;
-                    const bool vis = ok[b] && j >= lo && j < hi;
-                    if (!vis) s[b][i] = -__builtin_inff();
-                    any_visible = any_visible || vis;
+                    const bool vis = static_cast<uint32_t>(j - lo) < (ok[b] ? many : 0u);
+                    s[b][i] = vis ? s[b][i] : -__builtin_inff();
+                    any_visible |= vis;
                     // What no row sees may be anything, codes of no token included.
-                    if (!(ok[b] && j >= tk.lo_min && j < tk.hi_max)) t.v[b][i] = Words<VW>{};
+                    const bool held = static_cast<uint32_t>(j - tk.lo_min) < (ok[b] ? many_any : 0u);
+#pragma unroll
+                    for (int w = 0; w < VW; w++) t.v[b][i].w[w] = held ? t.v[b][i].w[w] : 0u;
                 }
         }
         seen = seen || any_visible;
@@ -510,14 +522,12 @@ Grid grid_of(const PagedAttnArgs& a, int dh) {
     return g;
 }
 
-// The tiling of the 16-row kernel with `waves` waves to a workgroup, `resident` workgroups to a CU: as many as are
-// resident at once, tiles that are not split included.
+// The tiling of the 16-row kernel with `waves` waves to a workgroup, `resident` workgroups to a CU.
 void few_form(const neko_hip_ctx* ctx, PagedAttnArgs& a, int waves, int resident) {
     a.t.tile_log2 = 4;
     a.t.unit_log2 = 5 + __builtin_ctz(static_cast<unsigned>(waves));
-    a.t.least = paged_reach(a.p) <= (kLeast << a.t.unit_log2) ? kLeast : 2;
-    const int64_t room = static_cast<int64_t>(resident) * ctx->cu_count, items = attn_tiles_bound(a.t, a.p.rows, a.p.n_seq) * a.p.n_kv;
-    a.t.target = static_cast<int32_t>(std::max<int64_t>(room - items, room / 2));
+    a.t.least = paged_reach(a.p) <= (kLeast << a.t.unit_log2) ? kLeast : kLeast / 2;
+    a.t.target = resident * ctx->cu_count;
     attn_set(a.t);
 }
 

@@ -259,30 +259,46 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
             ok = ok && (in[b] >> 16);
         }
         if constexpr (MODS) {
-            const int32_t away = j0 + 4 * h - pos;
 #pragma unroll
             for (int b = 0; b < KB; b++)
                 unrolled<16>([&](auto ec) {
                     constexpr int e = decltype(ec)::value;
-                    float x = s[b][e] * f[2 * b + e / 8];
-                    if (a.softcap > 0.0f) x = cap_score(x, a.softcap, inv_cap);
-                    if (a.slopes) x = __builtin_fmaf(slope, static_cast<float>(away + 32 * b + 8 * (e >> 2) + (e & 3)), x);
-                    s[b][e] = x;
+                    s[b][e] *= f[2 * b + e / 8];
                 });
+            if (a.softcap > 0.0f) {
+#pragma unroll
+                for (int b = 0; b < KB; b++)
+                    unrolled<16>([&](auto ec) { s[b][decltype(ec)::value] = cap_score(s[b][decltype(ec)::value], a.softcap, inv_cap); });
+            }
+            if (a.slopes) {
+                const int32_t away = j0 + 4 * h - pos;
+#pragma unroll
+                for (int b = 0; b < KB; b++)
+                    unrolled<16>([&](auto ec) {
+                        constexpr int e = decltype(ec)::value;
+                        s[b][e] = __builtin_fmaf(slope, static_cast<float>(away + 32 * b + 8 * (e >> 2) + (e & 3)), s[b][e]);
+                    });
+            }
 #pragma unroll
             for (int b = 0; b < C::blocks; b++) f[b] = kAttnLog2e;
         }
         const bool partial = j0 < w_lo_max || j0 + C::keys > w_hi_min || !ok;
         if (partial) {
+            // Visible: lo <= j < hi, as one unsigned comparison of the distance from the first key seen; no key of a block
+            // without a page.
+            const uint32_t first = static_cast<uint32_t>(j0 + 4 * h - lo), many = hi > lo ? static_cast<uint32_t>(hi - lo) : 0u;
             bool any = false;
 #pragma unroll
             for (int b = 0; b < KB; b++)
-                unrolled<16>([&](auto ec) {
-                    constexpr int e = decltype(ec)::value;
-                    const int32_t j = j0 + 32 * b + 8 * (e >> 2) + 4 * h + (e & 3);
-                    const bool vis = (in[2 * b + e / 8] >> 16) && j >= lo && j < hi;
-                    if (!vis) s[b][e] = -__builtin_inff();
-                    any = any || vis;
+                unrolled<2>([&](auto ic) {
+                    constexpr int i = decltype(ic)::value;
+                    const uint32_t most = (in[2 * b + i] >> 16) ? many : 0u;
+                    unrolled<8>([&](auto ec) {
+                        constexpr int e = 8 * i + decltype(ec)::value;
+                        const bool vis = first + static_cast<uint32_t>(32 * b + 8 * (e >> 2) + (e & 3)) < most;
+                        s[b][e] = vis ? s[b][e] : -__builtin_inff();
+                        any |= vis;
+                    });
                 });
             seen = seen || any;
         } else {

@@ -132,11 +132,10 @@ struct AttnTiling {
     int32_t group;       // query heads per kv head
     int32_t tile_log2;   // flattened (token, head) rows of a tile
     int32_t unit_log2;   // keys that a split is a multiple of
-    int32_t target;      // workgroups wanted
+    int32_t target;      // workgroups that are resident at once
     int32_t least;       // units of a split, at least
     int32_t window;      // 0: none
     int32_t span;        // with a window: the keys that a tile spans at most (attn_set)
-    double per_target;   // 1 / target (attn_set)
     // Sequences with min_rows <= flattened rows <= max_rows are this launch's.
     int32_t min_rows, max_rows;
 };
@@ -145,7 +144,6 @@ struct AttnTiling {
 NEKO_HD void attn_set(AttnTiling& t) {
     const int64_t span = static_cast<int64_t>(t.window) + ((1 << t.tile_log2) / t.group + 2) + 32;
     t.span = span < (1 << 30) ? static_cast<int32_t>(span) : 1 << 30;
-    t.per_target = 1.0 / t.target;
 }
 
 NEKO_HD int32_t attn_tiles(const AttnTiling& t, const SeqRows& r) {
@@ -161,11 +159,16 @@ NEKO_HD int32_t attn_units(const AttnTiling& t, int32_t reach, const SeqRows& r)
     return (keys + (1 << t.unit_log2) - 1) >> t.unit_log2;
 }
 
-// Units per split, from the launch's work, the sum over sequences and kv heads of tiles * units (a whole number below
-// 2^53): at least work / target.
-NEKO_HD int32_t attn_chunk(const AttnTiling& t, double work) {
-    const double c = work * t.per_target;
-    const int32_t n = (c < 1e9 ? static_cast<int32_t>(c) : 1000000000) + 1;
+// Units per split, at most, from the launch's tiles and its work, the sum over its tiles of their units (whole
+// numbers, both over all kv heads): as many workgroups as are resident at once, or, where the tiles alone are half of
+// those, half, so that only what is longer than average is split. (f32's rounding may leave a chunk short of work /
+// wanted by 2^-22 of it: the one workgroup more in attn_blocks_bound.) Measured with 509 rows over 8190 keys (128
+// tiles, 512 resident): four splits 129 us, three (what is free beside one for each tile) 153; 344 tiles of ten
+// units: 112 split in two, 93 whole.
+NEKO_HD int32_t attn_chunk(const AttnTiling& t, double work, int64_t tiles) {
+    const int32_t wanted = 2 * tiles >= t.target ? (t.target + 1) / 2 : t.target;
+    const float c = static_cast<float>(work) / static_cast<float>(wanted);
+    const int32_t n = (c < 1e9f ? static_cast<int32_t>(c) : 1000000000) + 1;
     return n < t.least ? t.least : n;
 }
 
@@ -189,11 +192,11 @@ NEKO_HD int64_t attn_tiles_bound(const AttnTiling& t, int64_t rows, int64_t n_se
     return tiles < rows * t.group ? tiles : rows * t.group;
 }
 NEKO_HD int64_t attn_blocks_bound(const AttnTiling& t, int64_t rows, int64_t n_seq, int n_kv) {
-    return attn_tiles_bound(t, rows, n_seq) + (t.target + n_kv - 1) / n_kv;
+    return attn_tiles_bound(t, rows, n_seq) + (t.target + n_kv - 1) / n_kv + 1;
 }
 
 NEKO_HD int64_t attn_split_tiles_bound(const AttnTiling& t, int64_t rows, int64_t n_seq, int n_kv) {
-    const int64_t tiles = attn_tiles_bound(t, rows, n_seq), most = (t.target + n_kv - 1) / n_kv;
+    const int64_t tiles = attn_tiles_bound(t, rows, n_seq), most = (t.target + n_kv - 1) / n_kv + 1;
     return tiles < most ? tiles : most;
 }
 // Whether any tile can be split. One sequence: its tiles are known, and with as many as wanted chunk >= units.

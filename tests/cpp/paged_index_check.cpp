@@ -68,11 +68,13 @@ void check_blocks(const Batch* b, const AttnTiling* given, int64_t* out) {
     attn_set(t);
     const int32_t reach = paged_reach(p);
     double work = 0;
+    int64_t all = 0;
     for (int32_t s = 0; s < p.n_seq; s++) {
         const SeqRows r = paged_seq(p, s);
         work += static_cast<double>(attn_tiles(t, r)) * attn_units(t, reach, r);
+        all += attn_tiles(t, r);
     }
-    const int32_t chunk = attn_chunk(t, work * p.n_kv);
+    const int32_t chunk = attn_chunk(t, work * p.n_kv, all * p.n_kv);
     int64_t tiles = 0, blocks = 0, uncovered = 0, split = 0;
     for (int32_t s = 0; s < p.n_seq; s++) {
         const SeqRows r = paged_seq(p, s);

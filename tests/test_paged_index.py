@@ -21,7 +21,7 @@ class Batch(ctypes.Structure):
 class Tiling(ctypes.Structure):
     _fields_ = [("group", ctypes.c_int32), ("tile_log2", ctypes.c_int32), ("unit_log2", ctypes.c_int32),
                 ("target", ctypes.c_int32), ("least", ctypes.c_int32), ("window", ctypes.c_int32), ("span", ctypes.c_int32),
-                ("per_target", ctypes.c_double), ("min_rows", ctypes.c_int32), ("max_rows", ctypes.c_int32)]
+                ("min_rows", ctypes.c_int32), ("max_rows", ctypes.c_int32)]
 
 
 @pytest.fixture(scope="module")
@@ -118,7 +118,7 @@ def test_attention_blocks_stay_within_the_grid(lib, seed):
     few = int(rng.choice([0, 16, 32]))
     few = (few + 1, 2**31 - 1) if few and rng.random() < 0.5 else (1, few or 2**31 - 1)
     t = Tiling(group, int(rng.choice([4, 6, 7, 8])), int(rng.choice([6, 7, 9])), int(rng.choice([1, 7, 256, 1024])),
-               int(rng.choice([1, 8])), int(rng.choice([0, 1, 40, 1000])), 0, 0.0, *few)
+               int(rng.choice([1, 8])), int(rng.choice([0, 1, 40, 1000])), 0, *few)
     out = (ctypes.c_int64 * 7)()
     lib.check_blocks(ctypes.byref(b), ctypes.byref(t), out)
     tiles, blocks, tiles_bound, blocks_bound, uncovered, split, split_bound = out
