@@ -37,7 +37,7 @@ struct TileForm {
     static constexpr int waves = 4, rows = 32 * waves;
     static constexpr int keys = DH <= 128 ? 64 : 32;  // (256 dimensions: 32, for LDS)
     static constexpr int blocks = keys / kBlockKeys;  // pages' parts of a tile
-    static constexpr int units = 2 * blocks / waves;  // (block, K or V) pairs that a wave brings in
+    static constexpr int units = blocks / 2;          // blocks that a wave brings in, of K or V
     static constexpr int half_bytes = keys * DH * 2;
     static constexpr int lds = 4 * half_bytes;         // two buffers of K and V
     static constexpr int window = 64 / blocks;         // tiles of a page look-up
@@ -123,102 +123,123 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     const float slope = MODS && a.slopes ? a.slopes[head] : 0.0f;
     const float inv_cap = MODS && a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
 
-    // Pages of the next 64 blocks, one to a lane; those after them are asked for half a window ahead.
+    // Waves 0 and 1 bring in K, 2 and 3 V: half of a tile's blocks each.
+    const bool is_v = wave >= C::waves / 2;
+    const int block0 = (wave & 1) * C::units;
+    const uint8_t* head_base = (is_v ? a.p.v : a.p.k) + kvh * a.p.head_bytes;
+
+    // The next 64 blocks of 16 keys, one to a lane: where this wave's operand of it stands, and its exponents. Those
+    // after them are asked for half a window ahead.
     const int nt = tk.k1 > tk.k0 ? (tk.k1 - tk.k0 + C::keys - 1) / C::keys : 0;
-    int32_t page = -1, next_page = -1;
-    int exps = pack_block(0, 0, false);
+    uint32_t from_lo = 0, from_hi = 0;
+    int32_t next_page = -1;
+    int exps = pack_block(0, 0, false), next_slot = 0;
     float next_ks = 1.0f, next_vs = 1.0f;
-    auto ask_pages = [&](int tile) {
+    auto ask_pages = [&](int tile) __attribute__((always_inline)) {
         const int32_t at = tk.k0 + C::keys * tile + kBlockKeys * lane;
         next_page = -1;
+        next_slot = at & ((1 << a.p.page_log2) - 1);
         if (tile < nt && at < tk.k1) next_page = paged_page(a.p, it.s, at);
     };
-    auto ask_scales = [&]() {
+    auto ask_scales = [&]() __attribute__((always_inline)) {
         const int64_t i = static_cast<int64_t>(next_page < 0 ? 0 : next_page) * a.p.n_kv + kvh;
         next_ks = a.p.ks[i];
         next_vs = a.p.vs[i];
     };
-    auto take_pages = [&]() {
-        page = next_page;
-        exps = page < 0 ? pack_block(0, 0, false) : pack_block(scale_exp(next_ks), scale_exp(next_vs), true);
+    auto take_pages = [&]() __attribute__((always_inline)) {
+        // (a block without a page reads page 0 and is masked; every slot of a page may be read)
+        const uint64_t at = reinterpret_cast<uint64_t>(head_base) + static_cast<uint64_t>(static_cast<uint32_t>(next_page < 0 ? 0 : next_page)) * a.p.page_bytes +
+                            static_cast<uint32_t>(next_slot * hd);
+        from_lo = static_cast<uint32_t>(at);
+        from_hi = static_cast<uint32_t>(at >> 32);
+        exps = next_page < 0 ? pack_block(0, 0, false) : pack_block(scale_exp(next_ks), scale_exp(next_vs), true);
     };
 
-    // Units of a tile: block u % blocks, K below u = blocks. Lane (row, 16-byte chunk) of each load.
+    // Lane (row, 16-byte chunk) of a load instruction. Dimensions past the head's end: any of its own, against zeros in q.
     const int lr = lane / (DH / 16), lc = lane % (DH / 16);
-    const int src = lc * 16 < hd ? lc * 16 : 0;  // dimensions past the head's end: any of its own, against zeros in q
+    uint32_t src[C::loads];
+#pragma unroll
+    for (int n = 0; n < C::loads; n++) src[n] = static_cast<uint32_t>((n * C::rpi + lr) * hd + (lc * 16 < hd ? lc * 16 : 0));
     struct Raw {
         uint4v x[C::units][C::loads];
     };
     Raw raw;
     int info[C::blocks], info1[C::blocks];  // of the tile in `raw`, of the tile after the one being multiplied
-    const uint8_t* k_head = a.p.k + kvh * a.p.head_bytes;
-    const uint8_t* v_head = a.p.v + kvh * a.p.head_bytes;
     auto load = [&](int tile) __attribute__((always_inline)) {
         const int at = tile % C::window * C::blocks;
 #pragma unroll
         for (int b = 0; b < C::blocks; b++) info[b] = __builtin_amdgcn_readlane(exps, at + b);
 #pragma unroll
         for (int i = 0; i < C::units; i++) {
-            const int u = wave * C::units + i, b = u % C::blocks;
-            const int id = __builtin_amdgcn_readlane(page, at + b);
-            const int32_t slot = (tk.k0 + C::keys * tile + kBlockKeys * b) & ((1 << a.p.page_log2) - 1);
-            const uint8_t* from = (u < C::blocks ? k_head : v_head) + static_cast<uint64_t>(static_cast<uint32_t>(id < 0 ? 0 : id)) * a.p.page_bytes +
-                                  static_cast<uint32_t>(slot * hd);
+            const uint32_t lo32 = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(from_lo), at + block0 + i));
+            const uint32_t hi32 = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(from_hi), at + block0 + i));
+            const uint8_t* from = reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(hi32) << 32 | lo32);
 #pragma unroll
-            for (int n = 0; n < C::loads; n++) raw.x[i][n] = *reinterpret_cast<const uint4v*>(from + ((n * C::rpi + lr) * hd + src));
+            for (int n = 0; n < C::loads; n++) raw.x[i][n] = *reinterpret_cast<const uint4v*>(from + src[n]);
         }
     };
+    // Where this wave's codes go in LDS.
+    uint32_t dst[C::units][C::loads][2];
+#pragma unroll
+    for (int i = 0; i < C::units; i++)
+#pragma unroll
+        for (int n = 0; n < C::loads; n++)
+#pragma unroll
+            for (int p = 0; p < 2; p++) {
+                const int row = (block0 + i) * kBlockKeys + n * C::rpi + lr, c = 2 * lc + p;
+                dst[i][n][p] = static_cast<uint32_t>((is_v ? C::half_bytes : 0) + row * DH * 2 + 16 * (is_v ? v_slot<DH>(row, c) : k_slot<DH>(row, c)));
+            }
     // The tile in `raw` to LDS. A NaN value times a weight of zero is NaN, so in tiles of which some row does not see
     // all, values that no row sees become zeros (they may be codes of no token), and NaN values are taken out and noted.
     auto store = [&](int tile, int buf) __attribute__((always_inline)) {
         const int32_t j0 = tk.k0 + C::keys * tile;
-        const bool differ = j0 < tk.lo_max || j0 + C::keys > tk.hi_min;
-        bool whole = !differ;
+        bool whole = j0 >= tk.lo_max && j0 + C::keys <= tk.hi_min;
 #pragma unroll
         for (int b = 0; b < C::blocks; b++) whole = whole && (info[b] >> 16);
-        uint32_t bad = 0;
+        if (!whole) {
+            bool any = false;
+            if (is_v) {
+                uint32_t bad = 0;
 #pragma unroll
-        for (int i = 0; i < C::units; i++) {
-            const int u = wave * C::units + i, b = u % C::blocks;
-            const bool is_v = u >= C::blocks;
-            uint8_t* to = tile_lds + buf * 2 * C::half_bytes + (is_v ? C::half_bytes : 0);
+                for (int i = 0; i < C::units; i++)
 #pragma unroll
-            for (int n = 0; n < C::loads; n++) {
-                const int row = b * kBlockKeys + n * C::rpi + lr;
-                uint4v x = raw.x[i][n];
-                if (is_v && !whole) {
-                    const int32_t j = j0 + row;
-                    if (!(info[b] >> 16) || j < tk.lo_min || j >= tk.hi_max) x = uint4v{0, 0, 0, 0};
-                    uint32_t at = 0;  // a bit for each NaN code
+                    for (int n = 0; n < C::loads; n++) {
+                        const int row = (block0 + i) * kBlockKeys + n * C::rpi + lr;
+                        const bool held = ((C::units == 2 ? (block0 ? info[C::blocks - 2 + i] : info[i]) : (block0 ? info[1] : info[0])) >> 16) &&
+                                          j0 + row >= tk.lo_min && j0 + row < tk.hi_max;
+                        uint32_t at = 0;  // a bit for each NaN code
 #pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        const uint32_t nan = nan_codes(x[w]) >> 7;
-                        x[w] &= ~(nan * 0xffu);
-                        at |= ((nan * 0x01020408u) >> 24) << (4 * w);
+                        for (int w = 0; w < 4; w++) {
+                            const uint32_t y = held ? raw.x[i][n][w] : 0u, nan = nan_codes(y) >> 7;
+                            raw.x[i][n][w] = y & ~(nan * 0xffu);
+                            at |= ((nan * 0x01020408u) >> 24) << (4 * w);
+                        }
+                        reinterpret_cast<uint16_t*>(nan_bits[buf][row])[lc] = static_cast<uint16_t>(at);
+                        bad |= at;
                     }
-                    reinterpret_cast<uint16_t*>(nan_bits[buf][row])[lc] = static_cast<uint16_t>(at);
-                    bad |= at;
-                }
+                any = __any(bad != 0);
+            }
+            if (lane == 0) nan_sh[buf][wave] = any;
+        }
+        uint8_t* to = tile_lds + buf * 2 * C::half_bytes;
+#pragma unroll
+        for (int i = 0; i < C::units; i++)
+#pragma unroll
+            for (int n = 0; n < C::loads; n++)
 #pragma unroll
                 for (int p = 0; p < 2; p++) {
                     half8 y;
 #pragma unroll
                     for (int w = 0; w < 2; w++) {
-                        const half2v y0 = f16_of_fp8<false>(x[2 * p + w]), y1 = f16_of_fp8<true>(x[2 * p + w]);
+                        const uint32_t x = raw.x[i][n][2 * p + w];
+                        const half2v y0 = f16_of_fp8<false>(x), y1 = f16_of_fp8<true>(x);
                         y[4 * w] = y0[0];
                         y[4 * w + 1] = y0[1];
                         y[4 * w + 2] = y1[0];
                         y[4 * w + 3] = y1[1];
                     }
-                    const int c = 2 * lc + p;
-                    *reinterpret_cast<half8*>(to + row * DH * 2 + 16 * (is_v ? v_slot<DH>(row, c) : k_slot<DH>(row, c))) = y;
+                    *reinterpret_cast<half8*>(to + dst[i][n][p]) = y;
                 }
-            }
-        }
-        if (!whole) {
-            const bool any = __any(bad != 0);
-            if (lane == 0) nan_sh[buf][wave] = any;
-        }
     };
 
     float16v o[ND] = {};
