@@ -45,6 +45,33 @@ struct TileForm {
     static constexpr int loads = kBlockKeys / rpi;     // load instructions of a unit
 };
 
+// The kernel's paged arguments, read again where this stands.
+__device__ __forceinline__ Paged paged_again() {
+    typedef const __attribute__((address_space(4))) PagedAttnArgs* Args;
+    Args p = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    Paged q;
+    q.k = p->p.k;
+    q.v = p->p.v;
+    q.ks = p->p.ks;
+    q.vs = p->p.vs;
+    q.table = p->p.table;
+    q.table_stride = p->p.table_stride;
+    q.n_pages = p->p.n_pages;
+    q.max_pages = p->p.max_pages;
+    q.page_log2 = p->p.page_log2;
+    q.n_kv = p->p.n_kv;
+    q.head_bytes = p->p.head_bytes;
+    q.page_bytes = p->p.page_bytes;
+    return q;
+}
+
+// The largest of three, NaN if one is (v_maximum3_f32; fmaxf first quiets operands that may be signalling NaNs, an
+// instruction each). A row with a NaN score is NaN whatever its maximum.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
+}
+
 // A block's exponents and whether it has a page, in one scalar.
 __device__ __forceinline__ int pack_block(int ke, int ve, bool ok) { return (ke + 128) | (ve + 128) << 8 | (ok ? 1 << 16 : 0); }
 __device__ __forceinline__ int block_ke(int x) { return (x & 255) - 128; }
@@ -126,7 +153,6 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     // Waves 0 and 1 bring in K, 2 and 3 V: half of a tile's blocks each.
     const bool is_v = wave >= C::waves / 2;
     const int block0 = (wave & 1) * C::units;
-    const uint8_t* head_base = (is_v ? a.p.v : a.p.k) + kvh * a.p.head_bytes;
 
     // The next 64 blocks of 16 keys, one to a lane: where this wave's operand of it stands, and its exponents. Those
     // after them are asked for half a window ahead.
@@ -135,20 +161,26 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     int32_t next_page = -1;
     int exps = pack_block(0, 0, false), next_slot = 0;
     float next_ks = 1.0f, next_vs = 1.0f;
+    // (These run once in a window: the arguments are read for them again, rather than kept in scalar registers that the
+    // loop has no room for.)
     auto ask_pages = [&](int tile) __attribute__((always_inline)) {
+        const Paged p = paged_again();
         const int32_t at = tk.k0 + C::keys * tile + kBlockKeys * lane;
         next_page = -1;
-        next_slot = at & ((1 << a.p.page_log2) - 1);
-        if (tile < nt && at < tk.k1) next_page = paged_page(a.p, it.s, at);
+        next_slot = at & ((1 << p.page_log2) - 1);
+        if (tile < nt && at < tk.k1) next_page = paged_page(p, it.s, at);
     };
     auto ask_scales = [&]() __attribute__((always_inline)) {
-        const int64_t i = static_cast<int64_t>(next_page < 0 ? 0 : next_page) * a.p.n_kv + kvh;
-        next_ks = a.p.ks[i];
-        next_vs = a.p.vs[i];
+        const Paged p = paged_again();
+        const int64_t i = static_cast<int64_t>(next_page < 0 ? 0 : next_page) * p.n_kv + kvh;
+        next_ks = p.ks[i];
+        next_vs = p.vs[i];
     };
     auto take_pages = [&]() __attribute__((always_inline)) {
+        const Paged p = paged_again();
+        const uint8_t* head_base = (is_v ? p.v : p.k) + kvh * p.head_bytes;
         // (a block without a page reads page 0 and is masked; every slot of a page may be read)
-        const uint64_t at = reinterpret_cast<uint64_t>(head_base) + static_cast<uint64_t>(static_cast<uint32_t>(next_page < 0 ? 0 : next_page)) * a.p.page_bytes +
+        const uint64_t at = reinterpret_cast<uint64_t>(head_base) + static_cast<uint64_t>(static_cast<uint32_t>(next_page < 0 ? 0 : next_page)) * p.page_bytes +
                             static_cast<uint32_t>(next_slot * hd);
         from_lo = static_cast<uint32_t>(at);
         from_hi = static_cast<uint32_t>(at >> 32);
@@ -259,17 +291,40 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
         if (j0 >= w_hi_max || j0 + C::keys <= w_lo_min) return;
         const uint8_t* kd = tile_lds + buf * 2 * C::half_bytes;
         const uint8_t* vd = kd + C::half_bytes;
-        float16v s[KB] = {};
-#pragma unroll
-        for (int b = 0; b < KB; b++) {
+        // A group's fragments are all asked for before its first product, which then waits for the first of them alone;
+        // left to itself the compiler puts each read just before its use and waits for it there (a tile's 16 products
+        // took 1200 cycles, half of them waits). f32 q leaves registers for one group of 32 keys at a time.
+        float16v s[KB];
+        auto k_frag = [&](int b, int d) __attribute__((always_inline)) {
             const int kr = 32 * b + l32;
+            return *reinterpret_cast<const half8*>(kd + kr * DH * 2 + 16 * k_slot<DH>(kr, 2 * d + h));
+        };
+        constexpr int GB = kTwo || DH > 128 ? 1 : KB;
 #pragma unroll
-            for (int d = 0; d < NS; d++) {
-                const half8 A = *reinterpret_cast<const half8*>(kd + kr * DH * 2 + 16 * k_slot<DH>(kr, 2 * d + h));
-                if constexpr (kTwo) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(A, ql[d], s[b], 0, 0, 0);
-                s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(A, qh[d], s[b], 0, 0, 0);
-            }
+        for (int b0 = 0; b0 < KB; b0 += GB) {
+            half8 A[GB][NS];
+#pragma unroll
+            for (int d = 0; d < NS; d++)
+#pragma unroll
+                for (int b = 0; b < GB; b++) A[b][d] = k_frag(b0 + b, d);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int b = 0; b < GB; b++) s[b0 + b] = float16v{};
+#pragma unroll
+            for (int d = 0; d < NS; d++)
+#pragma unroll
+                for (int b = 0; b < GB; b++) {
+                    if constexpr (kTwo) s[b0 + b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(A[b][d], ql[d], s[b0 + b], 0, 0, 0);
+                    s[b0 + b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(A[b][d], qh[d], s[b0 + b], 0, 0, 0);
+                }
         }
+        // The first values, on their way while the weights are made.
+        half8 V[KB][2];
+#pragma unroll
+        for (int b = 0; b < KB; b++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) V[b][i] = v_frag(vd, 0, b, i);
+        __builtin_amdgcn_sched_barrier(0);
         float f[C::blocks];
         bool ok = true;
 #pragma unroll
@@ -308,20 +363,19 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
             // Visible: lo <= j < hi, as one unsigned comparison of the distance from the first key seen; no key of a block
             // without a page.
             const uint32_t first = static_cast<uint32_t>(j0 + 4 * h - lo), many = hi > lo ? static_cast<uint32_t>(hi - lo) : 0u;
-            bool any = false;
 #pragma unroll
             for (int b = 0; b < KB; b++)
                 unrolled<2>([&](auto ic) {
                     constexpr int i = decltype(ic)::value;
                     const uint32_t most = (in[2 * b + i] >> 16) ? many : 0u;
+                    const int32_t at = j0 + 32 * b + 16 * i;
+                    seen = seen | (most != 0 && max(at, lo) < min(at + 16, hi));
                     unrolled<8>([&](auto ec) {
                         constexpr int e = 8 * i + decltype(ec)::value;
                         const bool vis = first + static_cast<uint32_t>(32 * b + 8 * (e >> 2) + (e & 3)) < most;
                         s[b][e] = vis ? s[b][e] : -__builtin_inff();
-                        any |= vis;
                     });
                 });
-            seen = seen || any;
         } else {
             seen = true;
         }
@@ -330,8 +384,10 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
         for (int b = 0; b < KB; b++)
             unrolled<2>([&](auto ic) {
                 constexpr int i = decltype(ic)::value;
-                float mx = s[b][8 * i];
-                unrolled<7>([&](auto ec) { mx = fmaxf(mx, s[b][8 * i + 1 + decltype(ec)::value]); });
+                float mx = max3(s[b][8 * i], s[b][8 * i + 1], s[b][8 * i + 2]);
+                mx = max3(mx, s[b][8 * i + 3], s[b][8 * i + 4]);
+                mx = max3(mx, s[b][8 * i + 5], s[b][8 * i + 6]);
+                mx = max3(mx, s[b][8 * i + 7], s[b][8 * i + 7]);
                 top = fmaxf(top, __builtin_fmaf(mx, f[2 * b + i], static_cast<float>(block_ve(in[2 * b + i]))));
             });
         top = ceilf(swap32_max(top));
@@ -375,16 +431,31 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
                 }
                 l = __builtin_fmaf(sum, exp2i(-ve), l);
             });
+        asm volatile("" : "+v"(l));  // (the sums here, beside the products, not after the branch below)
 #pragma unroll
-        for (int d = 0; d < ND; d++)
+        for (int d = 0; d < ND; d++) {
+            half8 next[KB][2];
+            if (d + 1 < ND) {
+#pragma unroll
+                for (int b = 0; b < KB; b++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) next[b][i] = v_frag(vd, d + 1, b, i);
+                __builtin_amdgcn_sched_barrier(0);
+            }
 #pragma unroll
             for (int b = 0; b < KB; b++)
 #pragma unroll
                 for (int i = 0; i < 2; i++) {
-                    const half8 A = v_frag(vd, d, b, i);
-                    if constexpr (kTwo) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(A, pl[b][i], o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(A, ph[b][i], o[d], 0, 0, 0);
+                    if constexpr (kTwo) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(V[b][i], pl[b][i], o[d], 0, 0, 0);
+                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(V[b][i], ph[b][i], o[d], 0, 0, 0);
                 }
+            if (d + 1 < ND) {
+#pragma unroll
+                for (int b = 0; b < KB; b++)
+#pragma unroll
+                    for (int i = 0; i < 2; i++) V[b][i] = next[b][i];
+            }
+        }
         // NaN values taken out of the tile, put into the dimensions of the rows that see them.
         if (j0 < tk.lo_max || j0 + C::keys > tk.hi_min || !ok) {
             uint32_t any = 0;
