@@ -32,10 +32,11 @@ __device__ __forceinline__ int v_slot(int row, int c) {
     return DH >= 128 ? c ^ ((row & 3) << 2) : c ^ ((row & 2) << 1);
 }
 
-template <int DH>
+template <typename TQ, int DH>
 struct TileForm {
     static constexpr int waves = 4, rows = 32 * waves;
-    static constexpr int keys = DH <= 128 ? 64 : 32;  // (256 dimensions: 32, for LDS)
+    // (fewer where registers are short: both planes of f32 q, 256 dimensions)
+    static constexpr int keys = DH <= (sizeof(TQ) == 2 ? 128 : 64) ? 64 : 32;
     static constexpr int blocks = keys / kBlockKeys;  // pages' parts of a tile
     static constexpr int units = blocks / 2;          // blocks that a wave brings in, of K or V
     static constexpr int half_bytes = keys * DH * 2;
@@ -79,7 +80,7 @@ __device__ __forceinline__ int block_ve(int x) { return ((x >> 8) & 255) - 128; 
 
 template <typename TQ, int DH, bool MODS>
 __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel(PagedAttnArgs a) {
-    typedef TileForm<DH> C;
+    typedef TileForm<TQ, DH> C;
     constexpr bool kTwo = sizeof(TQ) == 4;
     constexpr int NS = DH / 16, ND = DH / 32, KB = C::keys / 32;
     extern __shared__ __align__(16) uint8_t tile_lds[];
@@ -189,9 +190,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
 
     // Lane (row, 16-byte chunk) of a load instruction. Dimensions past the head's end: any of its own, against zeros in q.
     const int lr = lane / (DH / 16), lc = lane % (DH / 16);
-    uint32_t src[C::loads];
-#pragma unroll
-    for (int n = 0; n < C::loads; n++) src[n] = static_cast<uint32_t>((n * C::rpi + lr) * hd + (lc * 16 < hd ? lc * 16 : 0));
+    const uint32_t src = static_cast<uint32_t>(lr * hd + (lc * 16 < hd ? lc * 16 : 0));
     struct Raw {
         uint4v x[C::units][C::loads];
     };
@@ -207,23 +206,19 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
             const uint32_t hi32 = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(from_hi), at + block0 + i));
             const uint8_t* from = reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(hi32) << 32 | lo32);
 #pragma unroll
-            for (int n = 0; n < C::loads; n++) raw.x[i][n] = *reinterpret_cast<const uint4v*>(from + src[n]);
+            for (int n = 0; n < C::loads; n++) raw.x[i][n] = *reinterpret_cast<const uint4v*>(from + n * C::rpi * hd + src);
         }
     };
-    // Where this wave's codes go in LDS.
-    uint32_t dst[C::units][C::loads][2];
-#pragma unroll
-    for (int i = 0; i < C::units; i++)
-#pragma unroll
-        for (int n = 0; n < C::loads; n++)
-#pragma unroll
-            for (int p = 0; p < 2; p++) {
-                const int row = (block0 + i) * kBlockKeys + n * C::rpi + lr, c = 2 * lc + p;
-                dst[i][n][p] = static_cast<uint32_t>((is_v ? C::half_bytes : 0) + row * DH * 2 + 16 * (is_v ? v_slot<DH>(row, c) : k_slot<DH>(row, c)));
-            }
-    // The tile in `raw` to LDS. A NaN value times a weight of zero is NaN, so in tiles of which some row does not see
-    // all, values that no row sees become zeros (they may be codes of no token), and NaN values are taken out and noted.
-    auto store = [&](int tile, int buf) __attribute__((always_inline)) {
+    // Where this wave's codes go in LDS: piece (i, n, p) at (dst ^ 16 p ^ n dst_n) + rows, as the slots' exclusive-ors allow.
+    uint32_t dst;
+    {
+        const int row = block0 * kBlockKeys + lr, c = 2 * lc;
+        dst = static_cast<uint32_t>((is_v ? C::half_bytes : 0) + row * DH * 2 + 16 * (is_v ? v_slot<DH>(row, c) : k_slot<DH>(row, c)));
+    }
+    const uint32_t dst_n = is_v || DH < 128 ? 0u : static_cast<uint32_t>(C::rpi) * 16u;
+    // The tile in `raw`: a NaN value times a weight of zero is NaN, so in tiles of which some row does not see all, values
+    // that no row sees become zeros (they may be codes of no token), and NaN values are taken out and noted.
+    auto mend = [&](int tile, int buf) __attribute__((always_inline)) {
         const int32_t j0 = tk.k0 + C::keys * tile;
         bool whole = j0 >= tk.lo_max && j0 + C::keys <= tk.hi_min;
 #pragma unroll
@@ -253,77 +248,82 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
             }
             if (lane == 0) nan_sh[buf][wave] = any;
         }
-        uint8_t* to = tile_lds + buf * 2 * C::half_bytes;
+    };
+    // Eight codes of each lane, converted, to LDS: piece k of kPieces.
+    constexpr int kPieces = C::units * C::loads * 2;
+    auto store_piece = [&](int k, int buf) __attribute__((always_inline)) {
+        const int i = k / (2 * C::loads), n = k / 2 % C::loads, p = k % 2;
+        half8 y;
 #pragma unroll
-        for (int i = 0; i < C::units; i++)
+        for (int w = 0; w < 2; w++) {
+            const uint32_t x = raw.x[i][n][2 * p + w];
+            const half2v y0 = f16_of_fp8<false>(x), y1 = f16_of_fp8<true>(x);
+            y[4 * w] = y0[0];
+            y[4 * w + 1] = y0[1];
+            y[4 * w + 2] = y1[0];
+            y[4 * w + 3] = y1[1];
+        }
+        *reinterpret_cast<half8*>(tile_lds + buf * 2 * C::half_bytes + (i * kBlockKeys + n * C::rpi) * DH * 2 + (dst ^ (16u * p) ^ (static_cast<uint32_t>(n) * dst_n))) = y;
+    };
+    auto store = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
-            for (int n = 0; n < C::loads; n++)
-#pragma unroll
-                for (int p = 0; p < 2; p++) {
-                    half8 y;
-#pragma unroll
-                    for (int w = 0; w < 2; w++) {
-                        const uint32_t x = raw.x[i][n][2 * p + w];
-                        const half2v y0 = f16_of_fp8<false>(x), y1 = f16_of_fp8<true>(x);
-                        y[4 * w] = y0[0];
-                        y[4 * w + 1] = y0[1];
-                        y[4 * w + 2] = y1[0];
-                        y[4 * w + 3] = y1[1];
-                    }
-                    *reinterpret_cast<half8*>(to + dst[i][n][p]) = y;
-                }
+        for (int k = 0; k < kPieces; k++) store_piece(k, buf);
     };
 
     float16v o[ND] = {};
     float m = -__builtin_inff(), l = 0.0f;
     bool seen = false;
-    const int tq = lane & 15, tkr = tq >> 2;  // transposing reads: this lane's row of four, dimensions 4 (tq & 3)
-    auto v_frag = [&](const uint8_t* vd, int d, int b, int i) __attribute__((always_inline)) {
-        const int ch = 4 * d + 2 * ((lane >> 4) & 1) + ((tq & 3) >> 1);
-        const int row = 32 * b + 16 * i + 4 * h + tkr;
-        const uint8_t* p0 = vd + row * DH * 2 + 16 * v_slot<DH>(row, ch) + 8 * (tq & 1);
+    // Fragments: K, 8 dimensions of key 32 b + l32 for step d; V, by transposing reads, of eight keys for 32 dimensions.
+    // The slots make their places k_at ^ 32 d and v_at ^ 64 d, one register each instead of one for every d.
+    uint32_t k_lane = static_cast<uint32_t>(l32 * DH * 2 + 16 * k_slot<DH>(l32, h)), v_lane;
+    {
+        const int tq = lane & 15, row = 4 * h + (tq >> 2);
+        v_lane = static_cast<uint32_t>(C::half_bytes + row * DH * 2 + 16 * v_slot<DH>(row, 2 * ((lane >> 4) & 1) + ((tq & 3) >> 1)) + 8 * (tq & 1));
+    }
+    auto k_frag = [&](uint32_t k_at, int b, int d) __attribute__((always_inline)) {
+        return *reinterpret_cast<const half8*>(tile_lds + 32 * b * DH * 2 + (k_at ^ (32u * d)));
+    };
+    auto v_frag = [&](uint32_t v_at, int d, int b, int i) __attribute__((always_inline)) {
+        const uint8_t* p0 = tile_lds + (32 * b + 16 * i) * DH * 2 + (v_at ^ (64u * d));
         const short4v a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)p0);
         const short4v a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(p0 + 8 * DH * 2));
         return __builtin_bit_cast(half8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
     };
     auto step = [&](int tile, int buf, const int (&in)[C::blocks]) __attribute__((always_inline)) {
         const int32_t j0 = tk.k0 + C::keys * tile;
-        if (j0 >= w_hi_max || j0 + C::keys <= w_lo_min) return;
-        const uint8_t* kd = tile_lds + buf * 2 * C::half_bytes;
-        const uint8_t* vd = kd + C::half_bytes;
-        // A group's fragments are all asked for before its first product, which then waits for the first of them alone;
-        // left to itself the compiler puts each read just before its use and waits for it there (a tile's 16 products
-        // took 1200 cycles, half of them waits). f32 q leaves registers for one group of 32 keys at a time.
+        if (j0 >= w_hi_max || j0 + C::keys <= w_lo_min) {  // nothing for this wave's rows
+            store(buf ^ 1);
+            return;
+        }
+        // (opaque, so that the places are made from these for each tile and not kept)
+        uint32_t k_at = k_lane, v_at = v_lane;
+        asm volatile("" : "+v"(k_at), "+v"(v_at));
+        k_at += static_cast<uint32_t>(buf * 2 * C::half_bytes);
+        v_at += static_cast<uint32_t>(buf * 2 * C::half_bytes);
+        // Fragments are asked for eight products ahead (64 dimensions: four); left to itself the compiler puts each
+        // read just before its use and waits for it there (a tile's 16 products took 1200 cycles, half of them waits).
         float16v s[KB];
-        auto k_frag = [&](int b, int d) __attribute__((always_inline)) {
-            const int kr = 32 * b + l32;
-            return *reinterpret_cast<const half8*>(kd + kr * DH * 2 + 16 * k_slot<DH>(kr, 2 * d + h));
-        };
-        constexpr int GB = kTwo || DH > 128 ? 1 : KB;
+        constexpr int kAhead = 8 < NS ? 8 : NS;
+        half8 A[kAhead];
 #pragma unroll
-        for (int b0 = 0; b0 < KB; b0 += GB) {
-            half8 A[GB][NS];
+        for (int d = 0; d < kAhead; d++) A[d] = k_frag(k_at, 0, d);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int d = 0; d < NS; d++)
+        for (int b = 0; b < KB; b++) {
+            s[b] = float16v{};
 #pragma unroll
-                for (int b = 0; b < GB; b++) A[b][d] = k_frag(b0 + b, d);
-            __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int b = 0; b < GB; b++) s[b0 + b] = float16v{};
-#pragma unroll
-            for (int d = 0; d < NS; d++)
-#pragma unroll
-                for (int b = 0; b < GB; b++) {
-                    if constexpr (kTwo) s[b0 + b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(A[b][d], ql[d], s[b0 + b], 0, 0, 0);
-                    s[b0 + b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(A[b][d], qh[d], s[b0 + b], 0, 0, 0);
-                }
+            for (int d = 0; d < NS; d++) {
+                const int u = b * NS + d, a = u % kAhead, next = u + kAhead;
+                if constexpr (kTwo) s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(A[a], ql[d], s[b], 0, 0, 0);
+                s[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(A[a], qh[d], s[b], 0, 0, 0);
+                if (next < KB * NS) A[a] = k_frag(k_at, next / NS, next % NS);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         // The first values, on their way while the weights are made.
-        half8 V[KB][2];
+        half8 V[2];
 #pragma unroll
-        for (int b = 0; b < KB; b++)
-#pragma unroll
-            for (int i = 0; i < 2; i++) V[b][i] = v_frag(vd, 0, b, i);
+        for (int i = 0; i < 2; i++) V[i] = v_frag(v_at, 0, 0, i);
         __builtin_amdgcn_sched_barrier(0);
         float f[C::blocks];
         bool ok = true;
@@ -402,60 +402,57 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
         }
         const float ms = m == -__builtin_inff() ? 0.0f : m;
         half8 ph[KB][2], pl[KB][2];
-#pragma unroll
-        for (int b = 0; b < KB; b++)
-            unrolled<2>([&](auto ic) {
-                constexpr int i = decltype(ic)::value;
+        float sums[KB][2] = {};
+        // Weights of elements e0 .. e0 + n - 1 of group b, their parts for the matrix cores and their sums.
+        auto weights = [&](auto bc, auto e0c, auto nc) __attribute__((always_inline)) {
+            constexpr int b = decltype(bc)::value;
+            unrolled<decltype(nc)::value>([&](auto ec) {
+                constexpr int e = decltype(e0c)::value + decltype(ec)::value, i = e / 8;
                 const int ve = block_ve(in[2 * b + i]);
-                float sum = 0.0f;
                 if constexpr (kTwo) {
-                    const float base = static_cast<float>(ve) - ms;
-                    float p[8];
-                    unrolled<8>([&](auto ec) {
-                        constexpr int e = decltype(ec)::value;
-                        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * i + e], f[2 * b + i], base));
-                        const float y = p[e] * kPScale;
-                        ph[b][i][e] = static_cast<half_t>(y);
-                        pl[b][i][e] = static_cast<half_t>(y - to_f32(ph[b][i][e]));
-                    });
-                    sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], f[2 * b + i], static_cast<float>(ve) - ms));
+                    const float y = p * kPScale;
+                    ph[b][i][e % 8] = static_cast<half_t>(y);
+                    pl[b][i][e % 8] = static_cast<half_t>(y - to_f32(ph[b][i][e % 8]));
+                    sums[b][i] += p;
                 } else {
                     // The offset joins the exponent: its rounding, 2^-21 of the weight, is nothing beside the weight's.
-                    const float base = static_cast<float>(ve + kPOffset) - ms;
-                    unrolled<8>([&](auto ec) {
-                        constexpr int e = decltype(ec)::value;
-                        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][8 * i + e], f[2 * b + i], base));
-                        ph[b][i][e] = static_cast<half_t>(p);
-                        sum += p;
-                    });
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], f[2 * b + i], static_cast<float>(ve + kPOffset) - ms));
+                    ph[b][i][e % 8] = static_cast<half_t>(p);
+                    sums[b][i] += p;
                 }
-                l = __builtin_fmaf(sum, exp2i(-ve), l);
             });
-        asm volatile("" : "+v"(l));  // (the sums here, beside the products, not after the branch below)
+        };
+        // The matrix cores take the first group's weights while the second's are made, and the second's while the next
+        // tile's codes are converted: with each of these by itself, 16 products and 110 vector operations of a tile ran
+        // one after the other (678 us for a prompt of 8192 tokens).
+        weights(std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{}, std::integral_constant<int, 16>{});
+        unrolled<KB * ND>([&](auto uc) {
+            constexpr int u = decltype(uc)::value, b = u / ND, d = u % ND;
+            half8 next[2];
+            if constexpr (u + 1 < KB * ND) {
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
-            half8 next[KB][2];
-            if (d + 1 < ND) {
-#pragma unroll
-                for (int b = 0; b < KB; b++)
-#pragma unroll
-                    for (int i = 0; i < 2; i++) next[b][i] = v_frag(vd, d + 1, b, i);
-                __builtin_amdgcn_sched_barrier(0);
+                for (int i = 0; i < 2; i++) next[i] = v_frag(v_at, (u + 1) % ND, (u + 1) / ND, i);
             }
 #pragma unroll
-            for (int b = 0; b < KB; b++)
-#pragma unroll
-                for (int i = 0; i < 2; i++) {
-                    if constexpr (kTwo) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(V[b][i], pl[b][i], o[d], 0, 0, 0);
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(V[b][i], ph[b][i], o[d], 0, 0, 0);
-                }
-            if (d + 1 < ND) {
-#pragma unroll
-                for (int b = 0; b < KB; b++)
-#pragma unroll
-                    for (int i = 0; i < 2; i++) V[b][i] = next[b][i];
+            for (int i = 0; i < 2; i++) {
+                if constexpr (kTwo) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(V[i], pl[b][i], o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(V[i], ph[b][i], o[d], 0, 0, 0);
             }
-        }
+            if constexpr (b + 1 < KB) {
+                weights(std::integral_constant<int, b + 1>{}, std::integral_constant<int, 16 / ND * d>{}, std::integral_constant<int, 16 / ND>{});
+            } else {
+                constexpr int n = kPieces / ND;
+                unrolled<n>([&](auto kc) { store_piece(n * d + decltype(kc)::value, buf ^ 1); });
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (u + 1 < KB * ND) {
+#pragma unroll
+                for (int i = 0; i < 2; i++) V[i] = next[i];
+            }
+        });
+#pragma unroll
+        for (int b = 0; b < C::blocks; b++) l = __builtin_fmaf(sums[b / 2][b % 2], exp2i(-block_ve(in[b])), l);
         // NaN values taken out of the tile, put into the dimensions of the rows that see them.
         if (j0 < tk.lo_max || j0 + C::keys > tk.hi_min || !ok) {
             uint32_t any = 0;
@@ -484,7 +481,8 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
         take_pages();
         ask_pages(C::window);
         load(0);
-        store(0, 0);
+        mend(0, 0);
+        store(0);
 #pragma unroll
         for (int b = 0; b < C::blocks; b++) info1[b] = info[b];
         if (nt > 1) load(1);
@@ -496,7 +494,9 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
                 now[b] = info1[b];
                 info1[b] = info[b];
             }
-            if (t + 1 < nt) store(t + 1, (t + 1) & 1);  // that buffer's readers passed the barrier
+            const int buf = t & 1;
+            if (t + 1 < nt) mend(t + 1, buf ^ 1);  // that buffer's readers passed the barrier
+            step(t, buf, now);                     // and stores what is in `raw`, tile t + 1 (or nothing more of use)
             if (t + 2 < nt) {
                 const int at = (t + 2) % C::window;
                 if (at == 0) {
@@ -506,7 +506,6 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
                 if (at == C::window / 2) ask_scales();
                 load(t + 2);
             }
-            step(t, t & 1, now);
             __syncthreads();
         }
     }
@@ -547,7 +546,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
 
 template <typename TQ, int DH, bool MODS>
 int launch_tiles(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a) {
-    typedef TileForm<DH> C;
+    typedef TileForm<TQ, DH> C;
     static std::atomic<uint64_t> allowed{0};
     const void* kernel = reinterpret_cast<const void*>(&attn_paged_tile_kernel<TQ, DH, MODS>);
     if (C::lds + 4096 > 64 * 1024)  // (with the kernel's static LDS)
