@@ -156,19 +156,17 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     const int block0 = (wave & 1) * C::units;
 
     // The next 64 blocks of 16 keys, one to a lane: where this wave's operand of it stands, and its exponents. Those
-    // after them are asked for half a window ahead.
+    // after them are asked for half a window ahead. (These run once in a window: the arguments are read for them again,
+    // rather than kept in scalar registers that the loop has no room for.)
     const int nt = tk.k1 > tk.k0 ? (tk.k1 - tk.k0 + C::keys - 1) / C::keys : 0;
     uint32_t from_lo = 0, from_hi = 0;
     int32_t next_page = -1;
-    int exps = pack_block(0, 0, false), next_slot = 0;
+    int exps = pack_block(0, 0, false);
     float next_ks = 1.0f, next_vs = 1.0f;
-    // (These run once in a window: the arguments are read for them again, rather than kept in scalar registers that the
-    // loop has no room for.)
     auto ask_pages = [&](int tile) __attribute__((always_inline)) {
         const Paged p = paged_again();
         const int32_t at = tk.k0 + C::keys * tile + kBlockKeys * lane;
         next_page = -1;
-        next_slot = at & ((1 << p.page_log2) - 1);
         if (tile < nt && at < tk.k1) next_page = paged_page(p, it.s, at);
     };
     auto ask_scales = [&]() __attribute__((always_inline)) {
@@ -177,16 +175,31 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
         next_ks = p.ks[i];
         next_vs = p.vs[i];
     };
-    auto take_pages = [&]() __attribute__((always_inline)) {
+    auto take_pages = [&](int tile) __attribute__((always_inline)) {
         const Paged p = paged_again();
         const uint8_t* head_base = (is_v ? p.v : p.k) + kvh * p.head_bytes;
+        const int32_t slot = (tk.k0 + C::keys * tile + kBlockKeys * lane) & ((1 << p.page_log2) - 1);
         // (a block without a page reads page 0 and is masked; every slot of a page may be read)
         const uint64_t at = reinterpret_cast<uint64_t>(head_base) + static_cast<uint64_t>(static_cast<uint32_t>(next_page < 0 ? 0 : next_page)) * p.page_bytes +
-                            static_cast<uint32_t>(next_slot * hd);
+                            static_cast<uint32_t>(slot * hd);
         from_lo = static_cast<uint32_t>(at);
         from_hi = static_cast<uint32_t>(at >> 32);
         exps = next_page < 0 ? pack_block(0, 0, false) : pack_block(scale_exp(next_ks), scale_exp(next_vs), true);
     };
+    // Of the blocks of the window that is being multiplied: score -> exponent of 2 (with a cap or a bias: -> natural
+    // units; f32: without the row's own factor), the value scale's exponent and its inverse, and which have a page.
+    float now_f = 0.0f, now_ve = 0.0f, now_inv = 0.0f;
+    uint64_t now_ok = 0;
+    auto use_window = [&]() __attribute__((always_inline)) {
+        now_f = exp2i(block_ke(exps)) * (kTwo ? 1.0f : sc) * (MODS ? 1.0f : kAttnLog2e);
+        now_ve = static_cast<float>(block_ve(exps));
+        now_inv = exp2i(-block_ve(exps));
+        now_ok = __ballot((exps >> 16) != 0);
+    };
+    // Tiles of which every row of the workgroup sees every key, as far as the keys have pages.
+    const int inner0 = tk.lo_max > tk.k0 ? (tk.lo_max - tk.k0 + C::keys - 1) / C::keys : 0;
+    const int inner1 = tk.hi_min > tk.k0 ? (tk.hi_min - tk.k0) / C::keys : 0;
+    constexpr uint64_t kTileBits = (1ull << C::blocks) - 1;
 
     // Lane (row, 16-byte chunk) of a load instruction. Dimensions past the head's end: any of its own, against zeros in q.
     const int lr = lane / (DH / 16), lc = lane % (DH / 16);
@@ -195,11 +208,12 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
         uint4v x[C::units][C::loads];
     };
     Raw raw;
-    int info[C::blocks], info1[C::blocks];  // of the tile in `raw`, of the tile after the one being multiplied
+    bool raw_ok = true;  // whether all its blocks have pages
     auto load = [&](int tile) __attribute__((always_inline)) {
         const int at = tile % C::window * C::blocks;
+        raw_ok = true;
 #pragma unroll
-        for (int b = 0; b < C::blocks; b++) info[b] = __builtin_amdgcn_readlane(exps, at + b);
+        for (int b = 0; b < C::blocks; b++) raw_ok = raw_ok && (__builtin_amdgcn_readlane(exps, at + b) >> 16) != 0;
 #pragma unroll
         for (int i = 0; i < C::units; i++) {
             const uint32_t lo32 = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(from_lo), at + block0 + i));
@@ -220,10 +234,8 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     // that no row sees become zeros (they may be codes of no token), and NaN values are taken out and noted.
     auto mend = [&](int tile, int buf) __attribute__((always_inline)) {
         const int32_t j0 = tk.k0 + C::keys * tile;
-        bool whole = j0 >= tk.lo_max && j0 + C::keys <= tk.hi_min;
-#pragma unroll
-        for (int b = 0; b < C::blocks; b++) whole = whole && (info[b] >> 16);
-        if (!whole) {
+        const int at0 = tile % C::window * C::blocks + block0;
+        {
             bool any = false;
             if (is_v) {
                 uint32_t bad = 0;
@@ -232,8 +244,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
 #pragma unroll
                     for (int n = 0; n < C::loads; n++) {
                         const int row = (block0 + i) * kBlockKeys + n * C::rpi + lr;
-                        const bool held = ((C::units == 2 ? (block0 ? info[C::blocks - 2 + i] : info[i]) : (block0 ? info[1] : info[0])) >> 16) &&
-                                          j0 + row >= tk.lo_min && j0 + row < tk.hi_max;
+                        const bool held = (__builtin_amdgcn_readlane(exps, at0 + i) >> 16) != 0 && j0 + row >= tk.lo_min && j0 + row < tk.hi_max;
                         uint32_t at = 0;  // a bit for each NaN code
 #pragma unroll
                         for (int w = 0; w < 4; w++) {
@@ -289,9 +300,11 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
         const short4v a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(p0 + 8 * DH * 2));
         return __builtin_bit_cast(half8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
     };
-    auto step = [&](int tile, int buf, const int (&in)[C::blocks]) __attribute__((always_inline)) {
+    // `whole`: every row of the workgroup sees all of the tile's keys.
+    auto step = [&](int tile, int buf, bool whole) __attribute__((always_inline)) {
         const int32_t j0 = tk.k0 + C::keys * tile;
-        if (j0 >= w_hi_max || j0 + C::keys <= w_lo_min) {  // nothing for this wave's rows
+        const int at = tile % C::window * C::blocks;
+        if (!whole && (j0 >= w_hi_max || j0 + C::keys <= w_lo_min)) {  // nothing for this wave's rows
             store(buf ^ 1);
             return;
         }
@@ -325,14 +338,15 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
 #pragma unroll
         for (int i = 0; i < 2; i++) V[i] = v_frag(v_at, 0, 0, i);
         __builtin_amdgcn_sched_barrier(0);
+        auto lane_of = [&](float v, int b) __attribute__((always_inline)) {
+            return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), at + b));
+        };
         float f[C::blocks];
-        bool ok = true;
 #pragma unroll
         for (int b = 0; b < C::blocks; b++) {
-            f[b] = sc * exp2i(block_ke(in[b]));
-            if constexpr (!MODS) f[b] *= kAttnLog2e;
-            f[b] = fminf(fmaxf(f[b], 0x1p-120f), 0x1p120f);
-            ok = ok && (in[b] >> 16);
+            f[b] = lane_of(now_f, b);
+            if constexpr (kTwo) f[b] *= sc;
+            f[b] = fminf(fmaxf(f[b], 0x1p-120f), 0x1p120f);  // (never 0 or infinite: masked scores are -inf)
         }
         if constexpr (MODS) {
 #pragma unroll
@@ -358,8 +372,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
 #pragma unroll
             for (int b = 0; b < C::blocks; b++) f[b] = kAttnLog2e;
         }
-        const bool partial = j0 < w_lo_max || j0 + C::keys > w_hi_min || !ok;
-        if (partial) {
+        if (!whole && (j0 < w_lo_max || j0 + C::keys > w_hi_min || ((now_ok >> at) & kTileBits) != kTileBits)) {
             // Visible: lo <= j < hi, as one unsigned comparison of the distance from the first key seen; no key of a block
             // without a page.
             const uint32_t first = static_cast<uint32_t>(j0 + 4 * h - lo), many = hi > lo ? static_cast<uint32_t>(hi - lo) : 0u;
@@ -367,9 +380,9 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
             for (int b = 0; b < KB; b++)
                 unrolled<2>([&](auto ic) {
                     constexpr int i = decltype(ic)::value;
-                    const uint32_t most = (in[2 * b + i] >> 16) ? many : 0u;
-                    const int32_t at = j0 + 32 * b + 16 * i;
-                    seen = seen | (most != 0 && max(at, lo) < min(at + 16, hi));
+                    const uint32_t most = (now_ok >> (at + 2 * b + i)) & 1u ? many : 0u;
+                    const int32_t from = j0 + 32 * b + 16 * i;
+                    seen = seen | (most != 0 && max(from, lo) < min(from + 16, hi));
                     unrolled<8>([&](auto ec) {
                         constexpr int e = 8 * i + decltype(ec)::value;
                         const bool vis = first + static_cast<uint32_t>(32 * b + 8 * (e >> 2) + (e & 3)) < most;
@@ -388,7 +401,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
                 mx = max3(mx, s[b][8 * i + 3], s[b][8 * i + 4]);
                 mx = max3(mx, s[b][8 * i + 5], s[b][8 * i + 6]);
                 mx = max3(mx, s[b][8 * i + 7], s[b][8 * i + 7]);
-                top = fmaxf(top, __builtin_fmaf(mx, f[2 * b + i], static_cast<float>(block_ve(in[2 * b + i]))));
+                top = fmaxf(top, __builtin_fmaf(mx, f[2 * b + i], lane_of(now_ve, 2 * b + i)));
             });
         top = ceilf(swap32_max(top));
         if (__any(top > m)) {
@@ -402,22 +415,23 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
         }
         const float ms = m == -__builtin_inff() ? 0.0f : m;
         half8 ph[KB][2], pl[KB][2];
-        float sums[KB][2] = {};
+        float sums[KB][2] = {}, base[C::blocks];
+        // (f16: the offset joins the exponent; its rounding, 2^-21 of the weight, is nothing beside the weight's)
+#pragma unroll
+        for (int b = 0; b < C::blocks; b++) base[b] = lane_of(now_ve, b) - (kTwo ? ms : ms - static_cast<float>(kPOffset));
         // Weights of elements e0 .. e0 + n - 1 of group b, their parts for the matrix cores and their sums.
         auto weights = [&](auto bc, auto e0c, auto nc) __attribute__((always_inline)) {
             constexpr int b = decltype(bc)::value;
             unrolled<decltype(nc)::value>([&](auto ec) {
                 constexpr int e = decltype(e0c)::value + decltype(ec)::value, i = e / 8;
-                const int ve = block_ve(in[2 * b + i]);
                 if constexpr (kTwo) {
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], f[2 * b + i], static_cast<float>(ve) - ms));
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], f[2 * b + i], base[2 * b + i]));
                     const float y = p * kPScale;
                     ph[b][i][e % 8] = static_cast<half_t>(y);
                     pl[b][i][e % 8] = static_cast<half_t>(y - to_f32(ph[b][i][e % 8]));
                     sums[b][i] += p;
                 } else {
-                    // The offset joins the exponent: its rounding, 2^-21 of the weight, is nothing beside the weight's.
-                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], f[2 * b + i], static_cast<float>(ve + kPOffset) - ms));
+                    const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][e], f[2 * b + i], base[2 * b + i]));
                     ph[b][i][e % 8] = static_cast<half_t>(p);
                     sums[b][i] += p;
                 }
@@ -452,9 +466,9 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
             }
         });
 #pragma unroll
-        for (int b = 0; b < C::blocks; b++) l = __builtin_fmaf(sums[b / 2][b % 2], exp2i(-block_ve(in[b])), l);
+        for (int b = 0; b < C::blocks; b++) l = __builtin_fmaf(sums[b / 2][b % 2], lane_of(now_inv, b), l);
         // NaN values taken out of the tile, put into the dimensions of the rows that see them.
-        if (j0 < tk.lo_max || j0 + C::keys > tk.hi_min || !ok) {
+        if (!whole) {
             uint32_t any = 0;
 #pragma unroll
             for (int w = 0; w < C::waves; w++) any |= nan_sh[buf][w];
@@ -476,31 +490,31 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     };
 
     if (nt > 0) {
+        auto inner = [&](int tile) __attribute__((always_inline)) { return tile >= inner0 && tile < inner1; };
         ask_pages(0);
         ask_scales();
-        take_pages();
+        take_pages(0);
         ask_pages(C::window);
         load(0);
-        mend(0, 0);
+        bool whole = inner(0) && raw_ok;  // of the tile that is multiplied next
+        if (!whole) mend(0, 0);
         store(0);
-#pragma unroll
-        for (int b = 0; b < C::blocks; b++) info1[b] = info[b];
+        use_window();
         if (nt > 1) load(1);
         __syncthreads();
         for (int t = 0; t < nt; t++) {
-            int now[C::blocks];
-#pragma unroll
-            for (int b = 0; b < C::blocks; b++) {
-                now[b] = info1[b];
-                info1[b] = info[b];
-            }
             const int buf = t & 1;
-            if (t + 1 < nt) mend(t + 1, buf ^ 1);  // that buffer's readers passed the barrier
-            step(t, buf, now);                     // and stores what is in `raw`, tile t + 1 (or nothing more of use)
+            // Tile t + 1 is in `raw`: mended here, stored in the step (past the last, nothing of use). That buffer's
+            // readers passed the barrier.
+            const bool next_whole = inner(t + 1) && raw_ok;
+            if (!next_whole && t + 1 < nt) mend(t + 1, buf ^ 1);
+            step(t, buf, whole);
+            whole = next_whole;
+            if ((t + 1) % C::window == 0) use_window();
             if (t + 2 < nt) {
                 const int at = (t + 2) % C::window;
                 if (at == 0) {
-                    take_pages();
+                    take_pages(t + 2);
                     ask_pages(t + 2 + C::window);
                 }
                 if (at == C::window / 2) ask_scales();
