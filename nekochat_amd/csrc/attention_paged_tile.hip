@@ -334,9 +334,12 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
             }
         }
         // The first values, on their way while the weights are made.
-        half8 V[2];
+        constexpr int kSteps = KB * ND, kVAhead = kSteps < 3 ? kSteps : 3;
+        half8 V[kVAhead][2];
 #pragma unroll
-        for (int i = 0; i < 2; i++) V[i] = v_frag(v_at, 0, 0, i);
+        for (int u = 0; u < kVAhead - 1; u++)
+#pragma unroll
+            for (int i = 0; i < 2; i++) V[u][i] = v_frag(v_at, u % ND, u / ND, i);
         __builtin_amdgcn_sched_barrier(0);
         auto lane_of = [&](float v, int b) __attribute__((always_inline)) {
             return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), at + b));
@@ -441,17 +444,16 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
         // tile's codes are converted: with each of these by itself, 16 products and 110 vector operations of a tile ran
         // one after the other (678 us for a prompt of 8192 tokens).
         weights(std::integral_constant<int, 0>{}, std::integral_constant<int, 0>{}, std::integral_constant<int, 16>{});
-        unrolled<KB * ND>([&](auto uc) {
-            constexpr int u = decltype(uc)::value, b = u / ND, d = u % ND;
-            half8 next[2];
-            if constexpr (u + 1 < KB * ND) {
+        unrolled<kSteps>([&](auto uc) {
+            constexpr int u = decltype(uc)::value, b = u / ND, d = u % ND, v = u % kVAhead, ahead = u + kVAhead - 1;
+            if constexpr (ahead < kSteps) {
 #pragma unroll
-                for (int i = 0; i < 2; i++) next[i] = v_frag(v_at, (u + 1) % ND, (u + 1) / ND, i);
+                for (int i = 0; i < 2; i++) V[ahead % kVAhead][i] = v_frag(v_at, ahead % ND, ahead / ND, i);
             }
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                if constexpr (kTwo) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(V[i], pl[b][i], o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(V[i], ph[b][i], o[d], 0, 0, 0);
+                if constexpr (kTwo) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(V[v][i], pl[b][i], o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(V[v][i], ph[b][i], o[d], 0, 0, 0);
             }
             if constexpr (b + 1 < KB) {
                 weights(std::integral_constant<int, b + 1>{}, std::integral_constant<int, 16 / ND * d>{}, std::integral_constant<int, 16 / ND>{});
@@ -459,11 +461,12 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
                 constexpr int n = kPieces / ND;
                 unrolled<n>([&](auto kc) { store_piece(n * d + decltype(kc)::value, buf ^ 1); });
             }
-            __builtin_amdgcn_sched_barrier(0);
-            if constexpr (u + 1 < KB * ND) {
+            // (the sums here, not after the branch below, where the matrix cores have nothing to do)
+            if constexpr (d == ND - 1 && b + 1 == KB) {
 #pragma unroll
-                for (int i = 0; i < 2; i++) V[i] = next[i];
+                for (int x = 0; x < KB; x++) asm volatile("" : "+v"(sums[x][0]), "+v"(sums[x][1]));
             }
+            __builtin_amdgcn_sched_barrier(0);
         });
 #pragma unroll
         for (int b = 0; b < C::blocks; b++) l = __builtin_fmaf(sums[b / 2][b % 2], lane_of(now_inv, b), l);
