@@ -26,6 +26,12 @@ namespace {
 constexpr int kTileRows = 16;
 constexpr int kLeast = 8;           // tiles of 32 keys to a wave up to which a cache's keys are never split
 constexpr int kFewRows = 32;        // flattened rows up to which a sequence is this kernel's
+// Pairs of a query head's row and a key up to which the 16-row kernel alone is faster: it spreads them over more
+// waves and starts sooner, the tiles convert a code once for 128 rows. 76 batches of 64 to 2530 rows, 8 to 32 heads
+// of 64 to 256, on both: f16, from 20 to 35 million neither way by more than 1.35 times, half as long below 2 million
+// (128 rows of 32 heads 7.5 us and 15.9) and 1.6 times as long at 65 (2048 rows 115 and 74); f32 level at 32.
+template <typename TQ>
+constexpr double kFewPairs = sizeof(TQ) == 2 ? 20e6 : 40e6;
 constexpr int kSpareRows = 256;     // flattened rows past one token to a sequence that still make a decoding batch
 
 template <int N>
@@ -544,10 +550,12 @@ int launch_few(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a) {
 template <typename TQ, int DH>
 int launch_dims(neko_hip_ctx* ctx, const char* what, PagedAttnArgs a, int dtype) {
     // Sequences of up to kFewRows rows on the 16-row kernel, the rest on the tiles. Which a batch has is known on the
-    // device alone, so both are launched, except where there is one sequence, or no more rows than a padded decoding
-    // batch has: then the 16-row kernel takes whatever there is.
+    // device alone, so both are launched, except where there is one sequence, where there are no more rows than a
+    // padded decoding batch has, or where all there can be is little: then the 16-row kernel takes whatever there is.
     const int64_t most = static_cast<int64_t>(a.p.rows) * a.t.group;
-    const bool many = a.p.n_seq == 1 ? most > kFewRows : most > static_cast<int64_t>(a.p.n_seq) * a.t.group + kSpareRows;
+    const int64_t reach = paged_reach(a.p), per_row = std::max(reach / 2, reach - a.p.rows / (2 * a.p.n_seq));
+    const double pairs = static_cast<double>(a.p.rows) * a.n_head * static_cast<double>(a.t.window > 0 ? std::min<int64_t>(per_row, a.t.window) : per_row);
+    const bool many = pairs > kFewPairs<TQ> && (a.p.n_seq == 1 ? most > kFewRows : most > static_cast<int64_t>(a.p.n_seq) * a.t.group + kSpareRows);
     const bool few = a.p.n_seq > 1 || !many;
     constexpr int kMostWaves = DH <= 128 ? 8 : 4;
     PagedAttnArgs f = a, t = a;

@@ -313,8 +313,14 @@ def _bar(out, a, s, n_keys, hd, dtype):
     return bar + 2 * U * out.abs()
 
 
-def _check_attention(dev, H, KV, hd, page, dtype, seqs, seed, pad=2, cache=None, scale=None, what="", q=None, batch=None, unaligned=0, **kw):
-    b = batch or P.Batch(seqs, page, seed, pad=pad)
+def _wide(seqs, H, page):
+    """Free places in a row of the page table: with so many the batch could be large, and its longer sequences run on
+    the tiles of 128 rows; without, one of this size runs on the 16-row kernel alone."""
+    return int(60e6) // (sum(n for n, _ in seqs) * H * page) + 1
+
+
+def _check_attention(dev, H, KV, hd, page, dtype, seqs, seed, pad=2, cache=None, scale=None, what="", q=None, batch=None, unaligned=0, wide=False, **kw):
+    b = batch or P.Batch(seqs, page, seed, pad=pad, slack=_wide(seqs, H, page) if wide else 1)
     dt = DT[dtype]
     g = torch.Generator().manual_seed(seed)
     if q is None:
@@ -355,10 +361,10 @@ PROMPT = [(70, 70), (1, 40), (130, 300), (5, 5), (0, 0), (33, 600)]
     (3, 1, 256, 128, "f32"), (5, 1, 80, 16, "f16"), (10, 2, 80, 64, "f32"), (2, 2, 16, 16, "f32"), (20, 1, 128, 256, "f16"),
     (4, 2, 48, 32, "f16"), (2, 1, 144, 32, "f32"), (7, 1, 32, 16, "f16"),
 ])
-@pytest.mark.parametrize("form", ["decode", "prompt"])
+@pytest.mark.parametrize("form", ["decode", "prompt", "wide"])
 def test_attention(dev, H, KV, hd, page, dtype, form):
     _case(f"attention {form} {H}/{KV}/{hd} page {page} {dtype}")
-    _check_attention(dev, H, KV, hd, page, dtype, DECODE if form == "decode" else PROMPT, seed=hd + page, what=form)
+    _check_attention(dev, H, KV, hd, page, dtype, DECODE if form == "decode" else PROMPT, seed=hd + page, what=form, wide=form == "wide")
 
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
@@ -367,6 +373,7 @@ def test_attention_split_keys(dev, seqs, dtype):
     """Few rows over long caches: keys split over workgroups and joined."""
     _case(f"attention, split keys, {seqs} {dtype}")
     _check_attention(dev, 8, 2, 128, 16, dtype, seqs, seed=11, what=str(seqs))
+    _check_attention(dev, 8, 2, 128, 16, dtype, seqs, seed=11, what=str(seqs), wide=True)
 
 
 def test_attention_many_sequences(dev):
@@ -376,7 +383,7 @@ def test_attention_many_sequences(dev):
     _check_attention(dev, 4, 2, 64, 16, "f32", seqs, seed=12)
 
 
-@pytest.mark.parametrize("form", ["decode", "prompt"])
+@pytest.mark.parametrize("form", ["decode", "prompt", "wide"])
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("kw", [dict(softcap=5.0), dict(window=1), dict(window=37), dict(window=10000), dict(slopes=True),
                                 dict(softcap=2.0, window=50, slopes=True)])
@@ -385,7 +392,7 @@ def test_attention_cap_window_slopes(dev, kw, dtype, form):
     H, KV, hd = 6, 2, 64
     if kw.get("slopes"):
         kw = {**kw, "slopes": 2.0 ** -torch.arange(1, H + 1).float()}
-    _check_attention(dev, H, KV, hd, 16, dtype, DECODE if form == "decode" else PROMPT, seed=21, what=form, **kw)
+    _check_attention(dev, H, KV, hd, 16, dtype, DECODE if form == "decode" else PROMPT, seed=21, what=form, wide=form == "wide", **kw)
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.2, 3.0, 1e-20])
@@ -393,15 +400,16 @@ def test_attention_cap_window_slopes(dev, kw, dtype, form):
 def test_attention_scales_of_scores(dev, scale, seqs):
     """A zero scale weights all keys alike, a negative one turns the order, a large one leaves one key."""
     _case(f"attention, scale {scale}")
-    _check_attention(dev, 4, 2, 64, 16, "f32", seqs, seed=31, scale=scale)
-    _check_attention(dev, 4, 2, 128, 16, "f16", seqs, seed=32, scale=scale)
+    for wide in (False, True):
+        _check_attention(dev, 4, 2, 64, 16, "f32", seqs, seed=31, scale=scale, wide=wide)
+        _check_attention(dev, 4, 2, 128, 16, "f16", seqs, seed=32, scale=scale, wide=wide)
 
 
-@pytest.mark.parametrize("seqs", [DECODE, PROMPT])
-def test_attention_pages_of_far_apart_scales(dev, seqs):
+@pytest.mark.parametrize("seqs,wide", [(DECODE, False), (PROMPT, False), (PROMPT, True)])
+def test_attention_pages_of_far_apart_scales(dev, seqs, wide):
     """Value pages whose scales lie 2^50 apart, each row's result as exact as if they did not; keys likewise small."""
     _case("attention, far apart scales")
-    b = P.Batch(seqs, 16, 41)
+    b = P.Batch(seqs, 16, 41, slack=_wide(seqs, 4, 16) if wide else 1)
     cache = P.random_cache(b.n_pages, 2, 16, 64, 42)
     e = torch.from_numpy(np.random.default_rng(1).integers(-25, 26, (b.n_pages, 2)).astype(np.float32))
     cache = (cache[0], cache[1], cache[2] * 2.0 ** -3, cache[3] * torch.exp2(e))
@@ -414,19 +422,20 @@ def test_attention_pages_of_far_apart_scales(dev, seqs):
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_attention_unaligned_rows(dev, dtype):
     _case(f"attention, rows at odd elements, {dtype}")
-    for seqs in (DECODE, PROMPT):
-        _check_attention(dev, 4, 2, 64, 32, dtype, seqs, seed=51, unaligned=6)
+    for seqs, wide in ((DECODE, False), (PROMPT, False), (PROMPT, True)):
+        _check_attention(dev, 4, 2, 64, 32, dtype, seqs, seed=51, unaligned=6, wide=wide)
 
 
+@pytest.mark.parametrize("wide", [False, True])
 @pytest.mark.parametrize("window", [0, 30])
-@pytest.mark.parametrize("hd,dtype", [(64, "f32"), (128, "f16"), (256, "f32"), (80, "f16")])
-def test_attention_nan_where_it_is_seen_only(dev, hd, dtype, window):
+@pytest.mark.parametrize("hd,dtype", [(64, "f32"), (128, "f16"), (128, "f32"), (256, "f32"), (80, "f16")])
+def test_attention_nan_where_it_is_seen_only(dev, hd, dtype, window, wide):
     """NaN in a cached token, key or value, reaches the rows that see it -- a value's only its own dimension -- and no
     others; free slots, pages of others and slots past the length may hold anything."""
     _case(f"attention, NaN tokens, hd {hd} {dtype} window {window}")
     seqs = [(1, 50), (6, 75), (90, 90), (3, 40), (1, 120)]
     page, KV = 16, 2
-    b = P.Batch(seqs, page, 61)
+    b = P.Batch(seqs, page, 61, slack=_wide(seqs, 4, page) if wide else 1)
     cache = P.random_cache(b.n_pages, KV, page, hd, 62)
     kb, vb = cache[0].view(torch.uint8), cache[1].view(torch.uint8)
     for pg in b.free:
@@ -456,8 +465,8 @@ def test_attention_nan_where_it_is_seen_only(dev, hd, dtype, window):
 def test_attention_not_finite_queries(dev, dtype):
     """NaN and infinities in q reach their own head's row alone."""
     _case(f"attention, q not finite, {dtype}")
-    for seqs in ([(1, 60), (5, 40)], [(80, 80)]):
-        b = P.Batch(seqs, 16, 71)
+    for seqs, wide in (([(1, 60), (5, 40)], False), ([(80, 80)], False), ([(80, 80)], True)):
+        b = P.Batch(seqs, 16, 71, slack=_wide(seqs, 4, 16) if wide else 1)
         H, hd = 4, 64
         q = torch.randn((b.rows, H * hd), generator=torch.Generator().manual_seed(1)).to(DT[dtype])
         q[1, 3] = float("nan")
@@ -471,9 +480,9 @@ def test_attention_bad_pages_and_empty_rows(dev):
     """Pages outside the cache hold nothing; rows that see nothing -- all pages bad, a negative position -- give zeros."""
     _case("attention, bad pages, empty rows")
     H, KV, hd, page = 4, 2, 64, 16
-    for n in (1, 40):
+    for n, wide in ((1, False), (40, False), (40, True)):
         seqs = [(n, 60), (n, 50), (1, 20), (2, 20)]
-        b = P.Batch(seqs, page, 81)
+        b = P.Batch(seqs, page, 81, slack=_wide(seqs, H, page) if wide else 1)
         b.table[0, 1] = b.n_pages + 5
         b.table[1, :] = -1
         b.table[2, 1] = -2**31
@@ -540,7 +549,7 @@ def _serve(dev, cache, batch_of, qkv_of, steps, H, KV, hd, cs, wqk):
 
 def test_serving_run(dev):
     """Two prompts in chunks and three decode steps, append and attention in turn; every step against 64 bits on the
-    cache as it stands, and the last near attention over the f16 cache of the unquantised path."""
+    cache as it stands, and near attention over the f16 cache of the unquantised path."""
     _case("a serving run")
     H, KV, hd, page = 8, 2, 128, 16
     g = torch.Generator().manual_seed(1)
