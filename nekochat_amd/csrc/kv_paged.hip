@@ -12,7 +12,7 @@
 //
 // A wave takes 16 tokens of one page, one kv head and one of k and v, all in registers between the maximum and the
 // codes: one pass over the data. Larger pages take several waves, whose maxima meet in LDS. The q heads are waves of
-// the same launch, four rows (128 dimensions) by eight heads each, so the angles are loaded once per row. Lanes: head
+// the same launch, four rows (128 dimensions) by four heads each, so the angles are loaded once per row. Lanes: head
 // size / 8 lanes to a row, each with two quads that rotate into each other, so the rotation needs no exchange.
 #include <algorithm>
 
@@ -22,7 +22,9 @@
 namespace neko_hip {
 namespace {
 
-constexpr int kHeadsPerWave = 8;  // q heads of a wave
+// q heads of a wave: their values in flight set the kernel's registers (8: 98 and five waves per SIMD, a prefill of
+// 8192 rows 51.9 us and 64 decoded tokens 7.1; 4: 45.2 and 5.5; 2: 50.1 and 5.9).
+constexpr int kHeadsPerWave = 4;
 constexpr int kWaveTokens = 16;   // tokens of a page that one wave holds
 
 struct AppendArgs {
@@ -38,9 +40,10 @@ struct AppendArgs {
     int32_t inter;
     int32_t n_q;
     float eps;
-    uint32_t kv_blocks;    // workgroups of the pages' part
+    uint32_t kv_ratio;     // 2^32 times the share of workgroups that are the pages', rounded up
+    uint32_t kv_parts;     // (segment, k or v, kv head) parts of those
     uint32_t by_row;       // segments are looked for at each row instead of in the slots
-    uint32_t q_row_tiles;  // waves along the rows of the q part
+    uint32_t q_groups;     // waves along the heads of the q part
     uint32_t q_waves;
 };
 
@@ -75,7 +78,9 @@ __device__ __forceinline__ void store_quad(T* p, const float* x) {
     T v[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) v[i] = from_f32<T>(x[i]);
-    __builtin_memcpy(p, v, sizeof(v));
+    // Past the caches: a prefill's q is larger than they are (8192 rows 54.3 -> 52.2 us).
+    typedef T Q __attribute__((ext_vector_type(4), aligned(sizeof(T))));
+    __builtin_nontemporal_store(Q{v[0], v[1], v[2], v[3]}, reinterpret_cast<Q*>(p));
 }
 
 // The head's norm over its LPR lanes; lanes past the head's end hold zeros.
@@ -199,14 +204,15 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, const Segment& 
     if (w == 0 && lane == 0) *scale = exp2i(e);
 }
 
-// The q heads [h0, h0 + 8) of rows r0 .. r0 + 64 / LPR - 1.
+// The q heads [h0, h0 + kHeadsPerWave) of rows r0 .. r0 + 64 / LPR - 1.
 template <typename T, int LPR>
 __device__ __forceinline__ void append_q(const AppendArgs& a, uint32_t wave) {
     constexpr int RPL = 64 / LPR;
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int sub = lane % LPR, hd = a.p.hd;
-    const int32_t r0 = static_cast<int32_t>(wave % a.q_row_tiles) * RPL;
-    const int h0 = static_cast<int>(wave / a.q_row_tiles) * kHeadsPerWave;
+    const uint32_t tile = wave / a.q_groups;  // (the groups of a row's heads by waves that run together)
+    const int32_t r0 = static_cast<int32_t>(tile) * RPL;
+    const int h0 = static_cast<int>(wave - tile * a.q_groups) * kHeadsPerWave;
     const int32_t row = r0 + lane / LPR;
     const bool in_head = 8 * sub < hd;
     const bool inter = a.inter != 0;
@@ -247,20 +253,30 @@ __device__ __forceinline__ void append_q(const AppendArgs& a, uint32_t wave) {
     }
 }
 
+// NW waves to a page's part; a workgroup has four such parts where they are one wave each.
+template <int NW>
+constexpr int kParts = NW == 1 ? 4 : 1;
+
 template <typename T, int LPR, int NW>
-__global__ __launch_bounds__(64 * NW) void append_kernel(AppendArgs a) {
+__global__ __launch_bounds__(64 * NW * kParts<NW>) void append_kernel(AppendArgs a) {
     __shared__ uint32_t sh[NW];
-    const int w = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
-    if (blockIdx.x >= a.kv_blocks) {
-        const uint32_t wave = (blockIdx.x - a.kv_blocks) * NW + w;
-        if (wave < a.q_waves) append_q<T, LPR>(a, wave);
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), w = wave % NW;
+    // Workgroups of the pages and of q in turn, in the ratio of their numbers (umulhi(b, ratio) of the first b are the
+    // pages'): one after the other they took 20 and 36 us of a prefill of 8192 rows, one short of memory requests, the
+    // other short of nothing else.
+    const uint32_t kv_block = __umulhi(blockIdx.x, a.kv_ratio);
+    if (__umulhi(blockIdx.x + 1, a.kv_ratio) == kv_block) {
+        const uint32_t q_wave = (blockIdx.x - kv_block) * (NW * kParts<NW>) + wave;
+        if (q_wave < a.q_waves) append_q<T, LPR>(a, q_wave);
         return;
     }
     // Kv heads fastest, so that with eight of them an XCD writes the pages' parts that its attention reads.
     const uint32_t units = 2u * a.p.n_kv;
-    const int32_t at = static_cast<int32_t>(blockIdx.x / units);
-    const int g = static_cast<int>(blockIdx.x % units) % a.p.n_kv;
-    const bool is_k = static_cast<int>(blockIdx.x % units) < a.p.n_kv;
+    const uint32_t part = kv_block * kParts<NW> + wave / NW;
+    if (part >= a.kv_parts) return;
+    const int32_t at = static_cast<int32_t>(part / units);
+    const int g = static_cast<int>(part % units) % a.p.n_kv;
+    const bool is_k = static_cast<int>(part % units) < a.p.n_kv;
     int32_t s, i;
     if (a.by_row) {
         // A segment begins at a sequence's first row and at the first row of each page.
@@ -282,7 +298,7 @@ __global__ __launch_bounds__(64 * NW) void append_kernel(AppendArgs a) {
 template <typename T, int LPR>
 void launch_pages(neko_hip_ctx* ctx, const AppendArgs& a, uint32_t grid) {
     switch (a.p.page_log2) {
-        case 4: hipLaunchKernelGGL((append_kernel<T, LPR, 1>), dim3(grid), dim3(64), 0, ctx->stream, a); break;
+        case 4: hipLaunchKernelGGL((append_kernel<T, LPR, 1>), dim3(grid), dim3(64 * kParts<1>), 0, ctx->stream, a); break;
         case 5: hipLaunchKernelGGL((append_kernel<T, LPR, 2>), dim3(grid), dim3(128), 0, ctx->stream, a); break;
         case 6: hipLaunchKernelGGL((append_kernel<T, LPR, 4>), dim3(grid), dim3(256), 0, ctx->stream, a); break;
         case 7: hipLaunchKernelGGL((append_kernel<T, LPR, 8>), dim3(grid), dim3(512), 0, ctx->stream, a); break;
@@ -296,13 +312,16 @@ int launch_append(neko_hip_ctx* ctx, const char* what, AppendArgs a, int dtype) 
     // The slots of the segments, or the rows where those are fewer (a decode step).
     const int64_t slots = segment_slots(a.p.rows, a.p.n_seq, a.p.page_log2);
     a.by_row = a.p.rows <= slots;
-    const int64_t kv = std::min<int64_t>(slots, a.p.rows) * 2 * a.p.n_kv;
+    const int64_t parts = std::min<int64_t>(slots, a.p.rows) * 2 * a.p.n_kv;
+    const int per_block = nw == 1 ? kParts<1> : 1;
+    const int64_t kv = (parts + per_block - 1) / per_block;
     const int64_t tiles = (static_cast<int64_t>(a.p.rows) * lpr + 63) / 64;
     const int64_t waves = tiles * ((a.n_q + kHeadsPerWave - 1) / kHeadsPerWave);
-    const int64_t grid = kv + (waves + nw - 1) / nw;
-    NEKO_REQUIRE(ctx, grid <= 0x7fffffff, "%s: grid too large", what);
-    a.kv_blocks = static_cast<uint32_t>(kv);
-    a.q_row_tiles = static_cast<uint32_t>(tiles);
+    const int64_t grid = kv + (waves + nw * per_block - 1) / (nw * per_block);
+    NEKO_REQUIRE(ctx, grid <= 0x7fffffff && parts <= 0x7fffffff, "%s: grid too large", what);
+    a.kv_parts = static_cast<uint32_t>(parts);
+    a.kv_ratio = static_cast<uint32_t>((static_cast<uint64_t>(kv) << 32) / static_cast<uint64_t>(grid) + 1);
+    a.q_groups = static_cast<uint32_t>((a.n_q + kHeadsPerWave - 1) / kHeadsPerWave);
     a.q_waves = static_cast<uint32_t>(waves);
     const uint32_t n = static_cast<uint32_t>(grid);
     auto pick = [&](auto t) {
