@@ -230,8 +230,7 @@ __device__ __forceinline__ void append_q(const AppendArgs& a, uint32_t wave) {
         }
     }
     // The sequence of each row: that of the wave's first, then past the sequences that end before it.
-    int32_t s = wave_last(a.p.n_seq, r0, [&](int32_t i) { return clamp_i32(a.p.row_start[i], 0, a.p.rows); });
-    while (s + 1 < a.p.n_seq && clamp_i32(a.p.row_start[s + 1], 0, a.p.rows) <= row) s++;
+    const int32_t s = paged_seq_from(a.p, wave_last(a.p.n_seq, r0, [&](int32_t i) { return clamp_i32(a.p.row_start[i], 0, a.p.rows); }), row);
     const SeqRows r = paged_seq(a.p, s);
     const int32_t pos = r.len - r.n + (row - r.begin);
     const bool mine = inside && row >= r.begin && row < r.begin + r.n && pos >= 0 && pos < a.n_pos;

@@ -93,6 +93,7 @@ void check_blocks(const Batch* b, const AttnTiling* given, int64_t* out) {
     out[6] = attn_may_split(t, p) ? attn_split_tiles_bound(t, p.rows, p.n_seq, p.n_kv) : 0;
 }
 
+int check_seq_from(const Batch* b, int32_t s, int32_t row) { return paged_seq_from(paged(b), s, row); }
 int check_splits(int32_t units, int32_t chunk) { return attn_splits(units, chunk); }
 
 }  // extern "C"

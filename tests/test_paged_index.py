@@ -125,6 +125,39 @@ def test_attention_blocks_stay_within_the_grid(lib, seed):
     assert tiles <= tiles_bound and blocks <= blocks_bound and uncovered == 0 and split <= split_bound
 
 
+@pytest.mark.parametrize("n_seq", [1, 2, 5, 6, 64, 300])
+@pytest.mark.parametrize("wild", [False, True])
+def test_the_sequence_of_a_row(lib, n_seq, wild):
+    """The last sequence that begins at or before a row, from any that does, over idle places too; some sequence of the
+    batch, from the given one on, whatever the starts are."""
+    rng = np.random.default_rng(n_seq)
+    for _ in range(40):
+        n = rng.choice([0, 0, 0, 1, 4], n_seq)
+        start = np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+        rows = int(start[-1]) + int(rng.integers(1, 9))
+        if wild:
+            start = rng.integers(-5, rows + 5, n_seq + 1).astype(np.int32)
+        length = np.ones(n_seq, np.int32)
+        b = Batch(0, start.ctypes.data, length.ctypes.data, 1, 1, 1, n_seq, rows, 4, 1, 64)
+        for row in range(rows):
+            last = int(np.flatnonzero(start[:n_seq] <= row)[-1]) if (start[:n_seq] <= row).any() else 0
+            for s in {0, int(rng.integers(0, last + 1)), last}:
+                got = lib.check_seq_from(ctypes.byref(b), s, row)
+                assert s <= got < n_seq
+                if not wild:
+                    assert got == last, (s, row)
+
+
+def test_calls_without_a_context_are_refused():
+    from nekochat_amd import _lib
+
+    kv, batch = _lib.PagedKv(), _lib.PagedBatch()
+    L = _lib.lib
+    for pair in ((None, None), (ctypes.byref(kv), ctypes.byref(batch))):
+        assert L.neko_hip_qk_norm_rope_paged(None, None, 0, 1, 1, *pair, None, None, 0, 0, 0, 1e-6, None, 0, 1) == _lib.NEKO_ERR_INVALID
+        assert L.neko_hip_attention_paged(None, None, 0, 1, *pair, 1, 1.0, 0.0, 0, None, None, 0, 1) == _lib.NEKO_ERR_INVALID
+
+
 def test_splits_are_the_ceiling(lib):
     rng = np.random.default_rng(2)
     for _ in range(20000):
