@@ -165,8 +165,8 @@ int neko_hip_attention(neko_hip_ctx* ctx, const void* q, int64_t q_stride, const
  * A page holds page_size tokens (16, 32, 64, 128 or 256) of one sequence, all kv heads: OCP E4M3 codes
  * [n_pages][n_kv][page_size][hd] for keys and the same for values, and one f32 scale for each page and kv
  * head, [n_pages][n_kv]; a cached value is code * scale. Scales are powers of two, 2^-64 .. 2^64 (any other
- * bits are read as the power of two below, clamped). hd is a multiple of 16, 16..256; pages are 16-byte
- * aligned; the four arrays do not overlap.
+ * bits are read as the power of two below, clamped, without a sign). hd is a multiple of 16, 16..256; n_kv up
+ * to 4095; pages are 16-byte aligned; the four arrays do not overlap.
  *
  * A batch is n_seq sequences whose new rows stand one after another: sequence s has rows row_start[s] ..
  * row_start[s + 1] - 1 (none: an idle place) and kv_len[s] tokens with them, so its row i stands at position
@@ -225,8 +225,11 @@ int neko_hip_qk_norm_rope_paged(neko_hip_ctx* ctx, const void* qkv, int64_t row_
  * q and out rows of n_head*hd (strides in elements); out overlaps neither q nor the cache.
  * f32 sums; products on the matrix cores, codes exact in f16, f32 q and weights as two f16 each (tested to
  * 2e-6 (1 + sum w|v| / sum w) of a 64-bit evaluation); f16 calls round as said at the kernels.
+ * The tolerance holds while the value scales of a sequence's pages, per kv head, are within 2^96 of each other (a
+ * page of zeros has 2^-64): a weight is held relative to the largest weight * scale that its row sees.
  * Partial results of key splits go to the context's workspace (see neko_hip_matmul): its size goes by rows,
- * n_seq, heads and head size, not by lengths, so one uncaptured call of these makes every later capture fit. */
+ * n_seq, heads, head size, window and the table's width (max_pages), not by lengths, so one uncaptured call
+ * of these makes every later capture fit. */
 int neko_hip_attention_paged(neko_hip_ctx* ctx, const void* q, int64_t q_stride, int64_t rows, const neko_paged_kv* kv,
                              const neko_paged_batch* batch, int n_head, float scale, float softcap, int64_t window,
                              const float* slopes, void* out, int64_t out_stride, int dtype);

@@ -49,61 +49,93 @@ __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
 }
 
 // The item of workgroup j of a kv head (SPLIT: the j-th tile that has splits, its first one), by every wave for itself:
-// sequences' tiles and splits are summed 64 at a time. False past the last.
-template <bool SPLIT>
-__device__ __forceinline__ bool attn_find(const Paged& p, const AttnTiling& t, uint32_t j, AttnItem* it) {
+// sequences' tiles and splits are summed 64 * K at a time, K of them to a lane. False past the last.
+template <bool SPLIT, int K>
+__device__ __forceinline__ bool attn_find_by(const Paged& p, const AttnTiling& t, uint32_t j, AttnItem* it) {
     const int32_t lane = static_cast<int32_t>(threadIdx.x) & 63;
     const int32_t reach = paged_reach(p);
-    int32_t tiles = 0, units = 0;
+    int32_t tiles[K], units[K];
     auto load = [&](int32_t base) {
-        tiles = units = 0;
-        if (base + lane < p.n_seq) {
-            const SeqRows r = paged_seq(p, base + lane);
-            tiles = attn_tiles(t, r);
-            units = attn_units(t, reach, r);
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            const int32_t s = base + lane * K + k;
+            const SeqRows r = paged_seq(p, s < p.n_seq ? s : p.n_seq - 1);
+            tiles[k] = s < p.n_seq ? attn_tiles(t, r) : 0;
+            units[k] = attn_units(t, reach, r);
         }
     };
-    double work = 0.0;  // (whole numbers below 2^53: exact)
-    uint32_t all = 0;
-    for (int32_t base = 0; base < p.n_seq; base += 64) {
-        load(base);
-        work += wave_sum_f64(static_cast<double>(tiles) * static_cast<double>(units));
-        all += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_scan_u32(static_cast<uint32_t>(tiles))), 63));
+    int32_t chunk = t.least;
+    if (K == 1) load(0);
+    if (reach > static_cast<int64_t>(t.least) << t.unit_log2) {  // (else no tile has more units than the least chunk)
+        double work = 0.0;  // (whole numbers below 2^53: exact)
+        uint32_t all = 0;
+        for (int32_t base = 0; base < p.n_seq; base += 64 * K) {
+            if (K > 1) load(base);
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                work += static_cast<double>(tiles[k]) * static_cast<double>(units[k]);
+                all += static_cast<uint32_t>(tiles[k]);
+            }
+        }
+        work = wave_sum_f64(work);
+        all = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_scan_u32(all)), 63));
+        chunk = attn_chunk(t, work * p.n_kv, static_cast<int64_t>(all) * p.n_kv);
     }
-    const int32_t chunk = attn_chunk(t, work * p.n_kv, static_cast<int64_t>(all) * p.n_kv);
-    uint32_t past_tiles = 0, past = 0;
-    for (int32_t base = 0; base < p.n_seq; base += 64) {
-        if (p.n_seq > 64) load(base);
-        const int32_t splits = attn_splits(units, chunk);
-        const uint32_t n = static_cast<uint32_t>(tiles) * static_cast<uint32_t>(splits);
-        const uint32_t split_tiles = splits > 1 ? static_cast<uint32_t>(tiles) : 0;
+    uint32_t past_tiles = 0, past = 0;  // of the sequences before
+    for (int32_t base = 0; base < p.n_seq; base += 64 * K) {
+        if (K > 1) load(base);
+        int32_t splits[K];
+        uint32_t n = 0, split_tiles = 0;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            splits[k] = attn_splits(units[k], chunk);
+            n += static_cast<uint32_t>(tiles[k]) * static_cast<uint32_t>(splits[k]);
+            split_tiles += splits[k] > 1 ? static_cast<uint32_t>(tiles[k]) : 0;
+        }
         const uint32_t sum = wave_scan_u32(n), sum_tiles = SPLIT ? wave_scan_u32(split_tiles) : 0;
         const uint64_t at = __ballot(SPLIT ? past_tiles + sum_tiles > j : past + sum > j);
         if (at) {
             const int l = __builtin_ctzll(at);
-            const int32_t n_tiles = __builtin_amdgcn_readlane(tiles, l);
-            it->s = base + l;
-            it->splits = __builtin_amdgcn_readlane(splits, l);
-            it->chunk = attn_splits(__builtin_amdgcn_readlane(units, l), it->splits);  // even ones
-            const uint32_t first = past + static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum - n), l));
-            if constexpr (SPLIT) {
-                const uint32_t local = j - past_tiles - static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum_tiles - split_tiles), l));
-                it->tile = n_tiles - 1 - static_cast<int32_t>(local);
-                it->split = 0;
-                it->block = first + local * static_cast<uint32_t>(it->splits);
-            } else {  // the last tiles, which see the most keys, first
-                const uint32_t local = j - first;
-                const uint32_t up = it->splits == 1 ? local : local / static_cast<uint32_t>(it->splits);
-                it->tile = n_tiles - 1 - static_cast<int32_t>(up);
-                it->split = static_cast<int32_t>(local - up * static_cast<uint32_t>(it->splits));
-                it->block = j;
+            past += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum - n), l));
+            if constexpr (SPLIT) past_tiles += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum_tiles - split_tiles), l));
+            bool found = false;
+#pragma unroll
+            for (int k = 0; k < K; k++) {  // the lane's sequence that has it
+                const int32_t n_tiles = __builtin_amdgcn_readlane(tiles[k], l), n_splits = __builtin_amdgcn_readlane(splits[k], l);
+                const uint32_t here = static_cast<uint32_t>(n_tiles) * static_cast<uint32_t>(n_splits);
+                const uint32_t split_here = n_splits > 1 ? static_cast<uint32_t>(n_tiles) : 0;
+                if (!found && (SPLIT ? past_tiles + split_here > j : past + here > j)) {
+                    found = true;
+                    it->s = base + l * K + k;
+                    it->splits = n_splits;
+                    it->chunk = attn_splits(__builtin_amdgcn_readlane(units[k], l), n_splits);  // even ones
+                    if constexpr (SPLIT) {
+                        const uint32_t local = j - past_tiles;
+                        it->tile = n_tiles - 1 - static_cast<int32_t>(local);
+                        it->split = 0;
+                        it->block = past + local * static_cast<uint32_t>(n_splits);
+                    } else {  // the last tiles, which see the most keys, first
+                        const uint32_t local = j - past;
+                        const uint32_t up = n_splits == 1 ? local : local / static_cast<uint32_t>(n_splits);
+                        it->tile = n_tiles - 1 - static_cast<int32_t>(up);
+                        it->split = static_cast<int32_t>(local - up * static_cast<uint32_t>(n_splits));
+                        it->block = j;
+                    }
+                }
+                past += found ? 0 : here;
+                past_tiles += found ? 0 : split_here;
             }
-            return true;
+            return found;
         }
         past += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum), 63));
         if constexpr (SPLIT) past_tiles += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum_tiles), 63));
     }
     return false;
+}
+// One sequence to a lane where that holds the batch, else eight, whose loads wait for each other no more.
+template <bool SPLIT>
+__device__ __forceinline__ bool attn_find(const Paged& p, const AttnTiling& t, uint32_t j, AttnItem* it) {
+    return p.n_seq <= 64 ? attn_find_by<SPLIT, 1>(p, t, j, it) : attn_find_by<SPLIT, 8>(p, t, j, it);
 }
 
 // The keys that a tile's rows see, first and last row: row i sees [lo(i), hi(i)).

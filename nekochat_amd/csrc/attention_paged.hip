@@ -113,8 +113,8 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
     const int32_t pos = r.len - r.n + tok;
     const int32_t hi = min(pos + 1, min(r.len, paged_reach(a.p))), lo = key_lo(pos, a.t.window);
 
-    // q as the B operands of the first product, the same for all waves, by one of them: in LDS, where each
-    // wave's registers have room for other things (128 of them at four waves per SIMD). f32 rows are brought to
+    // q as the B operands of the first product, the same for all waves, by one of them: in LDS, so that each
+    // wave's registers have room for other things (168 of them at three waves per SIMD). f32 rows are brought to
     // [2^14, 2^15) and split; sc_sh then undoes that. A scale's sign goes into q; a scale of 0 weights all alike.
     if (wave == 1) {
         const TQ* qr = static_cast<const TQ*>(a.q) + static_cast<int64_t>(r.begin + tok) * a.qs + static_cast<int64_t>(head) * hd;
@@ -160,7 +160,7 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
         }
     }
     const float slope = MODS && a.slopes ? a.slopes[head] : 0.0f;
-    const float inv_cap = MODS && a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+    const float inv_cap = MODS && a.softcap > 0.0f ? fminf(1.0f / a.softcap, 0x1.fffffep127f) : 0.0f;
 
     // This wave's tiles of 32 keys, from key kw on.
     const int nt = tk.k1 > tk.k0 ? (tk.k1 - tk.k0 + 31) / 32 : 0;

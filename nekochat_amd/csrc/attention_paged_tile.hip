@@ -149,7 +149,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
             }
     }
     const float slope = MODS && a.slopes ? a.slopes[head] : 0.0f;
-    const float inv_cap = MODS && a.softcap > 0.0f ? 1.0f / a.softcap : 0.0f;
+    const float inv_cap = MODS && a.softcap > 0.0f ? fminf(1.0f / a.softcap, 0x1.fffffep127f) : 0.0f;
 
     // Waves 0 and 1 bring in K, 2 and 3 V: half of a tile's blocks each.
     const bool is_v = wave >= C::waves / 2;

@@ -144,6 +144,17 @@ def test_append_many_sequences(dev, n_seq, dtype):
     _check_append(dev, 2, 1, 64, 16, dtype, seqs, 64, False, True, seed=n_seq)
 
 
+@pytest.mark.parametrize("n_seq", [65, 700])
+def test_append_padded_batch(dev, n_seq):
+    """Few sequences among many idle places, the rows padded to the places: searches that skip all of them."""
+    _case(f"append, idle places, {n_seq}")
+    seqs = [(0, 5)] * n_seq
+    seqs[3], seqs[n_seq // 2], seqs[-1] = (1, 20), (2, 33), (1, 1)
+    _check_append(dev, 2, 1, 64, 16, "f16", seqs, 64, False, True, seed=1, pad=n_seq - 4)
+    seqs[-1], seqs[0] = (0, 0), (1, 17)
+    _check_append(dev, 2, 1, 128, 32, "f32", seqs, 64, False, True, seed=2, pad=n_seq - 4)
+
+
 def test_append_long_prompt(dev):
     """Slots of page segments instead of rows: one prompt of many pages beside single tokens."""
     _case("append, a long prompt")
@@ -383,6 +394,35 @@ def test_attention_many_sequences(dev):
     _check_attention(dev, 4, 2, 64, 16, "f32", seqs, seed=12)
 
 
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("n_seq", [64, 65, 513, 1100])
+def test_attention_sequences_past_one_search(dev, n_seq, wide):
+    """Batches that a search passes over in one step and in several, most places idle, some sequences long enough to be
+    split, prompts and a padded end among them."""
+    _case(f"attention, {n_seq} places, wide {wide}")
+    rng = np.random.default_rng(n_seq)
+    seqs = [(int(rng.random() < 0.2), int(rng.integers(1, 40))) for _ in range(n_seq)]
+    for at, s in ((0, (1, 1500)), (9, (0, 0)), (n_seq // 2, (70, 300)), (n_seq // 2 + 1, (2, 900)), (n_seq - 3, (1, 1999)), (n_seq - 1, (0, 3))):
+        seqs[at] = s
+    _check_attention(dev, 4, 2, 64, 16, "f16", seqs, seed=13, pad=n_seq + 150 if wide else 7, wide=wide)
+
+
+def test_attention_smallest_cap(dev):
+    """A cap whose inverse is past the largest number caps every score to next to nothing: all keys alike."""
+    _case("attention, a cap of 1e-39")
+    for seqs, wide in (([(1, 40), (3, 9)], False), ([(70, 90)], True)):
+        H, KV, hd, page = 4, 2, 64, 16
+        b = P.Batch(seqs, page, 3, slack=_wide(seqs, H, page) if wide else 1)
+        cache = P.random_cache(b.n_pages, KV, page, hd, 4)
+        q = torch.randn((b.rows, H * hd), generator=torch.Generator().manual_seed(5))
+        q[0] = 0.0  # and scores of zero stay
+        dc = _cache_on(cache, dev)
+        got = ops.attention_paged(q.to(dev), dc, *b.tensors(dev), H, softcap=1e-39)
+        torch.cuda.synchronize()
+        want, a, s = P.attention(q, cache, b, H, 0.0)
+        assert float(((got.cpu().double() - want).abs() - _bar(want, a, s, 90, hd, "f32")).max()) <= 0
+
+
 @pytest.mark.parametrize("form", ["decode", "prompt", "wide"])
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("kw", [dict(softcap=5.0), dict(window=1), dict(window=37), dict(window=10000), dict(slopes=True),
@@ -620,6 +660,106 @@ def test_captured_decode_follows_growing_lengths(dev):
         ops.attention_paged(q, eager, table, start, first, H)  # the workspace is used in between
     assert torch.equal(cache.k_pages.view(torch.uint8), eager.k_pages.view(torch.uint8))
     assert torch.equal(cache.v_scales, eager.v_scales)
+
+
+def test_captured_prompts_of_two_graphs(dev):
+    """Chunks of prompts captured on the tiles and beside single tokens, in two graphs that share the context's workspace,
+    replayed in turn with lengths and pages that change on the device; eager calls in between."""
+    _case("two captured graphs")
+    H, KV, hd, page = 8, 2, 64, 16
+    g = torch.Generator().manual_seed(18)
+    n_pages, width, chunk = 400, 6000, 130
+    cs = _rope(2000, hd).to(dev)
+    init = P.random_cache(n_pages, KV, page, hd, 19)
+    # Graph 0: one sequence's chunk; graph 1: a chunk between two single tokens and an idle place.
+    new = [[chunk], [1, chunk, 0, 1]]
+    start = [torch.tensor(np.cumsum([0] + n), dtype=torch.int32, device=dev) for n in new]
+    lengths = [[[chunk], [2 * chunk], [900]], [[700, chunk, 0, 33], [701, 1300, 0, 34], [17, 2 * chunk, 5, 1]]]
+
+    def table(i, k):
+        t = torch.full((len(new[i]), width), -1, dtype=torch.int32)
+        order = torch.randperm(n_pages, generator=torch.Generator().manual_seed(10 * i + k))
+        at = 0
+        for s, n in enumerate(lengths[i][k]):
+            used = -(-n // page)
+            t[s, :used] = order[at: at + used].int()
+            at += used
+        return t.to(dev)
+
+    rows = [[torch.randn((sum(n), (H + 2 * KV) * hd), generator=g).half().to(dev) for _ in range(3)] for n in new]
+
+    def step(i, x, cache, t, length, q, out):
+        ops.qk_norm_rope_paged(x, H, cache, t, start[i], length, cs, 1e-6, q_out=q)
+        ops.attention_paged(q, cache, t, start[i], length, H, out=out)
+
+    def buffers(i):
+        return tuple(torch.zeros((sum(new[i]), H * hd), dtype=torch.float16, device=dev) for _ in range(2))
+
+    len_of = lambda i, k: torch.tensor(lengths[i][k], dtype=torch.int32, device=dev)
+    eager, want = _cache_on(init, dev), []
+    for k in range(3):
+        for i in range(2):
+            q, out = buffers(i)
+            step(i, rows[i][k], eager, table(i, k), len_of(i, k), q, out)
+            want.append(out)
+    torch.cuda.synchronize()
+
+    cache = _cache_on(init, dev)
+    held, graphs = [], []
+    for i in range(2):
+        x, t, length = torch.empty_like(rows[i][0]), table(i, 0), len_of(i, 0)
+        q, out = buffers(i)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step(i, x, cache, t, length, q, out)
+        held.append((x, t, length, out))
+        graphs.append(graph)
+    for k in range(3):
+        for i in range(2):
+            x, t, length, out = held[i]
+            x.copy_(rows[i][k])
+            t.copy_(table(i, k))
+            length.copy_(len_of(i, k))
+            graphs[i].replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want[2 * k + i]), f"replay {k} of graph {i}"
+            q, o = buffers(1 - i)
+            ops.attention_paged(q, eager, table(1 - i, k), start[1 - i], len_of(1 - i, k), H, out=o)  # (the workspace, between)
+    assert torch.equal(cache.k_pages.view(torch.uint8), eager.k_pages.view(torch.uint8))
+    assert torch.equal(cache.v_pages.view(torch.uint8), eager.v_pages.view(torch.uint8))
+
+
+def test_two_threads(dev):
+    """A context and a stream for each of two host threads, calls of both at once: split keys in each one's workspace."""
+    _case("two threads")
+    import threading
+
+    H, KV, hd, page = 8, 2, 128, 16
+    cases = []
+    for i, seqs in enumerate(([(1, 5000), (1, 70)], [(2, 3000), (150, 200)])):
+        b = P.Batch(seqs, page, 5 + i)
+        dc, t = _cache_on(P.random_cache(b.n_pages, KV, page, hd, 6 + i), dev), b.tensors(dev)
+        q = torch.randn((b.rows, H * hd), generator=torch.Generator().manual_seed(i)).to(dev)
+        cases.append((q, dc, t, ops.attention_paged(q, dc, *t, H)))
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(case):
+        try:
+            q, dc, t, want = case
+            with torch.cuda.stream(torch.cuda.Stream()):
+                got = [ops.attention_paged(q, dc, *t, H) for _ in range(20)]
+                torch.cuda.current_stream().synchronize()
+            bad.extend(i for i, x in enumerate(got) if not torch.equal(x, want))
+        except Exception as e:  # noqa: BLE001 -- reported below
+            bad.append(e)
+
+    threads = [threading.Thread(target=work, args=(c,)) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad, bad
 
 
 def test_another_stream_and_prepared_calls(dev):
