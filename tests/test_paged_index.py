@@ -4,6 +4,9 @@ backwards or past the rows, lengths short of the rows or past the table -- every
 the cache and the call's rows, and for well-formed batches every new row is covered exactly once."""
 import ctypes
 import os
+import re
+import shutil
+import subprocess
 
 import numpy as np
 import pytest
@@ -156,6 +159,18 @@ def test_calls_without_a_context_are_refused():
     for pair in ((None, None), (ctypes.byref(kv), ctypes.byref(batch))):
         assert L.neko_hip_qk_norm_rope_paged(None, None, 0, 1, 1, *pair, None, None, 0, 0, 0, 1e-6, None, 0, 1) == _lib.NEKO_ERR_INVALID
         assert L.neko_hip_attention_paged(None, None, 0, 1, *pair, 1, 1.0, 0.0, 0, None, None, 0, 1) == _lib.NEKO_ERR_INVALID
+
+
+@pytest.mark.skipif(shutil.which("gcc") is None, reason="needs gcc")
+def test_the_documented_layer_compiles(tmp_path):
+    root = os.path.dirname(HERE)
+    with open(os.path.join(root, "INTEGRATION.md")) as f:
+        block = next(b for b in re.findall(r"```c\n(.*?)```", f.read(), flags=re.S) if "neko_paged_kv" in b)
+    src = tmp_path / "layer.c"
+    src.write_text("#include <stddef.h>\n#include <stdint.h>\n#include \"neko_hip.h\"\n" + block)
+    r = subprocess.run(["gcc", "-std=c11", "-Wall", "-Werror", "-fsyntax-only", "-I", os.path.join(root, "include"), str(src)],
+                       capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
 
 
 def test_splits_are_the_ceiling(lib):
