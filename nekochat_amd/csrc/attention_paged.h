@@ -204,6 +204,13 @@ __device__ __forceinline__ uint32_t item_of(const PagedAttnArgs& a, int* kvh) {
 // The bytes of x that are NaN codes, as 0x80 each.
 __device__ __forceinline__ uint32_t nan_codes(uint32_t x) { return ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
+// x, or NaN where bit `bit` is set: two vector operations and no condition, of which dozens held at once would push the
+// scalar registers of the whole kernel out (108 of them were, in the tiles of 128 dimensions).
+__device__ __forceinline__ float nan_if(float x, uint32_t bits, int bit) {
+    const uint32_t all = static_cast<uint32_t>(static_cast<int32_t>(bits << (31 - bit)) >> 31);
+    return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x) | (all & 0x7fc00000u));
+}
+
 // acc / l of a finished row: zeros where it saw nothing, NaN where every score it saw was -inf.
 __device__ __forceinline__ float row_factor(float l, bool seen) {
     return l == 0.0f ? (seen ? __builtin_nanf("") : 0.0f) : 1.0f / (l * kPScale);

@@ -397,7 +397,7 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
                     const uint32_t at = nan_at[k * 16 + 4 * g4 + i];
 #pragma unroll
                     for (int e = 0; e < NE; e++)
-                        if ((at >> e) & 1u) o[e][i] = __builtin_nanf("");
+                        o[e][i] = nan_if(o[e][i], at, e);
                 }
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");

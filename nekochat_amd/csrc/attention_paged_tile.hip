@@ -20,6 +20,7 @@ namespace neko_hip {
 namespace {
 
 typedef short short4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(1))) uint8_t Global;
 
 // The slot of 16-byte chunk c of tile row `row` in LDS: the 16 rows of a ds_read_b128 pass at one chunk of K, and
 // the 4 rows x 4 chunks of half a transposing read of V, fall on distinct banks.
@@ -218,9 +219,11 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
         for (int i = 0; i < C::units; i++) {
             const uint32_t lo32 = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(from_lo), at + block0 + i));
             const uint32_t hi32 = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(from_hi), at + block0 + i));
-            const uint8_t* from = reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(hi32) << 32 | lo32);
+            // (in global memory: through a flat load the compiler would wait for these with the next read of LDS)
+            const Global* from = reinterpret_cast<const Global*>(static_cast<uint64_t>(hi32) << 32 | lo32);
 #pragma unroll
-            for (int n = 0; n < C::loads; n++) raw.x[i][n] = *reinterpret_cast<const uint4v*>(from + n * C::rpi * hd + src);
+            for (int n = 0; n < C::loads; n++)
+                raw.x[i][n] = *reinterpret_cast<const __attribute__((address_space(1))) uint4v*>(from + (n * C::rpi * hd + src));
         }
     };
     // Where this wave's codes go in LDS: piece (i, n, p) at (dst ^ 16 p ^ n dst_n) + rows, as the slots' exclusive-ors allow.
@@ -484,7 +487,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
                         const uint32_t bits = nan_bits[buf][k][d] >> (4 * h);
                         unrolled<16>([&](auto ec) {
                             constexpr int e = decltype(ec)::value;
-                            if ((bits >> (8 * (e >> 2) + (e & 3))) & 1u) o[d][e] = __builtin_nanf("");
+                            o[d][e] = nan_if(o[d][e], bits, 8 * (e >> 2) + (e & 3));
                         });
                     }
                 }
