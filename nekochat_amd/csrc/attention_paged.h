@@ -176,13 +176,14 @@ __device__ __forceinline__ float cap_score(float s, float cap, float inv_cap) {
     return fabsf(x) < 0.9f ? near : far;
 }
 
+// The larger of a lane's and its partner's, neither NaN (fmaxf quiets both first, an instruction each).
 __device__ __forceinline__ float swap16_max(float v) {
     const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
-    return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
+    return __builtin_elementwise_maximum(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
 }
 __device__ __forceinline__ float swap32_max(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
-    return fmaxf(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
+    return __builtin_elementwise_maximum(__builtin_bit_cast(float, static_cast<uint32_t>(r[0])), __builtin_bit_cast(float, static_cast<uint32_t>(r[1])));
 }
 __device__ __forceinline__ float swap16_sum(float v) {
     const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);

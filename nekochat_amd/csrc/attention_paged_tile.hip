@@ -41,7 +41,8 @@ struct TileForm {
     static constexpr int blocks = keys / kBlockKeys;  // pages' parts of a tile
     static constexpr int units = blocks / 2;          // blocks that a wave brings in, of K or V
     static constexpr int half_bytes = keys * DH * 2;
-    static constexpr int lds = 4 * half_bytes;         // two buffers of K and V
+    static constexpr int tiles = 4 * half_bytes;       // two buffers of K and V, from LDS address 0 on (no additions to fragments' places)
+    static constexpr int lds = tiles + 2 * 4 * (waves + keys * (DH / 32));  // and what is noted of NaN values
     static constexpr int window = 64 / blocks;         // tiles of a page look-up
     static constexpr int rpi = 64 * 16 / DH;           // rows of a load instruction
     static constexpr int loads = kBlockKeys / rpi;     // load instructions of a unit
@@ -74,8 +75,8 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return __builtin_elementwise_maximum(__builtin_elementwise_maximum(a, b), c);
 }
 
-// A block's exponents and whether it has a page, in one scalar.
-__device__ __forceinline__ int pack_block(int ke, int ve, bool ok) { return (ke + 128) | (ve + 128) << 8 | (ok ? 1 << 16 : 0); }
+// A block's exponents in one scalar.
+__device__ __forceinline__ int pack_block(int ke, int ve) { return (ke + 128) | (ve + 128) << 8; }
 __device__ __forceinline__ int block_ke(int x) { return (x & 255) - 128; }
 __device__ __forceinline__ int block_ve(int x) { return ((x >> 8) & 255) - 128; }
 
@@ -85,8 +86,8 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     constexpr bool kTwo = sizeof(TQ) == 4;
     constexpr int NS = DH / 16, ND = DH / 32, KB = C::keys / 32;
     extern __shared__ __align__(16) uint8_t tile_lds[];
-    __shared__ uint32_t nan_sh[2][C::waves];           // whether a wave took NaN values out of the tile,
-    __shared__ uint32_t nan_bits[2][C::keys][DH / 32];  // and where
+    auto nan_sh = reinterpret_cast<uint32_t(*)[C::waves]>(tile_lds + C::tiles);  // whether a wave took NaN values out of the tile,
+    auto nan_bits = reinterpret_cast<uint32_t(*)[C::keys][DH / 32]>(tile_lds + C::tiles + 2 * 4 * C::waves);  // and where
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
     const int l32 = lane & 31, h = lane >> 5;
@@ -162,7 +163,8 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     const int nt = tk.k1 > tk.k0 ? (tk.k1 - tk.k0 + C::keys - 1) / C::keys : 0;
     uint32_t from_lo = 0, from_hi = 0;
     int32_t next_page = -1;
-    int exps = pack_block(0, 0, false);
+    int exps = pack_block(0, 0);
+    uint64_t exps_ok = 0;  // which of them have a page
     float next_ks = 1.0f, next_vs = 1.0f;
     auto ask_pages = [&](int tile) __attribute__((always_inline)) {
         const Paged p = paged_again();
@@ -185,7 +187,8 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
                             static_cast<uint32_t>(slot * hd);
         from_lo = static_cast<uint32_t>(at);
         from_hi = static_cast<uint32_t>(at >> 32);
-        exps = next_page < 0 ? pack_block(0, 0, false) : pack_block(scale_exp(next_ks), scale_exp(next_vs), true);
+        exps = next_page < 0 ? pack_block(0, 0) : pack_block(scale_exp(next_ks), scale_exp(next_vs));
+        exps_ok = __ballot(next_page >= 0);
     };
     // Of the blocks of the window that is being multiplied: score -> exponent of 2 (with a cap or a bias: -> natural
     // units; f32: without the row's own factor), the value scale's exponent and its inverse, and which have a page.
@@ -193,9 +196,10 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     uint64_t now_ok = 0;
     auto use_window = [&]() __attribute__((always_inline)) {
         now_f = exp2i(block_ke(exps)) * (kTwo ? 1.0f : sc) * (MODS ? 1.0f : kAttnLog2e);
+        if constexpr (!kTwo) now_f = fminf(fmaxf(now_f, 0x1p-120f), 0x1p120f);  // (never 0 or infinite: masked scores are -inf)
         now_ve = static_cast<float>(block_ve(exps));
         now_inv = exp2i(-block_ve(exps));
-        now_ok = __ballot((exps >> 16) != 0);
+        now_ok = exps_ok;
     };
     // Tiles of which every row of the workgroup sees every key, as far as the keys have pages.
     const int inner0 = tk.lo_max > tk.k0 ? (tk.lo_max - tk.k0 + C::keys - 1) / C::keys : 0;
@@ -209,12 +213,12 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
         uint4v x[C::units][C::loads];
     };
     Raw raw;
-    bool raw_ok = true;  // whether all its blocks have pages
+    int raw_bad = 0;  // -1: not all its blocks have pages
     auto load = [&](int tile) __attribute__((always_inline)) {
         const int at = tile % C::window * C::blocks;
-        raw_ok = true;
-#pragma unroll
-        for (int b = 0; b < C::blocks; b++) raw_ok = raw_ok && (__builtin_amdgcn_readlane(exps, at + b) >> 16) != 0;
+        uint32_t off = src;  // (opaque: a scalar base and this, not a sum of 64 bits that was widened outside the loop)
+        asm volatile("" : "+v"(off));
+        raw_bad = ((exps_ok >> at) & kTileBits) == kTileBits ? 0 : -1;
 #pragma unroll
         for (int i = 0; i < C::units; i++) {
             const uint32_t lo32 = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(from_lo), at + block0 + i));
@@ -223,7 +227,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
             const Global* from = reinterpret_cast<const Global*>(static_cast<uint64_t>(hi32) << 32 | lo32);
 #pragma unroll
             for (int n = 0; n < C::loads; n++)
-                raw.x[i][n] = *reinterpret_cast<const __attribute__((address_space(1))) uint4v*>(from + (n * C::rpi * hd + src));
+                raw.x[i][n] = *reinterpret_cast<const __attribute__((address_space(1))) uint4v*>(from + (n * C::rpi * hd + off));
         }
     };
     // Where this wave's codes go in LDS: piece (i, n, p) at (dst ^ 16 p ^ n dst_n) + rows, as the slots' exclusive-ors allow.
@@ -247,7 +251,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
 #pragma unroll
                     for (int n = 0; n < C::loads; n++) {
                         const int row = (block0 + i) * kBlockKeys + n * C::rpi + lr;
-                        const bool held = (__builtin_amdgcn_readlane(exps, at0 + i) >> 16) != 0 && j0 + row >= tk.lo_min && j0 + row < tk.hi_max;
+                        const bool held = ((exps_ok >> (at0 + i)) & 1) != 0 && j0 + row >= tk.lo_min && j0 + row < tk.hi_max;
                         uint32_t at = 0;  // a bit for each NaN code
 #pragma unroll
                         for (int w = 0; w < 4; w++) {
@@ -286,7 +290,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
 
     float16v o[ND] = {};
     float m = -__builtin_inff(), l = 0.0f;
-    bool seen = false;
+    int seen = 0;
     // Fragments: K, 8 dimensions of key 32 b + l32 for step d; V, by transposing reads, of eight keys for 32 dimensions.
     // The slots make their places k_at ^ 32 d and v_at ^ 64 d, one register each instead of one for every d.
     uint32_t k_lane = static_cast<uint32_t>(l32 * DH * 2 + 16 * k_slot<DH>(l32, h)), v_lane;
@@ -347,12 +351,12 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
         auto lane_of = [&](float v, int b) __attribute__((always_inline)) {
             return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), at + b));
         };
-        float f[C::blocks];
+        float f[C::blocks], ve[C::blocks];
 #pragma unroll
         for (int b = 0; b < C::blocks; b++) {
             f[b] = lane_of(now_f, b);
-            if constexpr (kTwo) f[b] *= sc;
-            f[b] = fminf(fmaxf(f[b], 0x1p-120f), 0x1p120f);  // (never 0 or infinite: masked scores are -inf)
+            ve[b] = lane_of(now_ve, b);
+            if constexpr (kTwo) f[b] = fminf(fmaxf(f[b] * sc, 0x1p-120f), 0x1p120f);
         }
         if constexpr (MODS) {
 #pragma unroll
@@ -388,7 +392,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
                     constexpr int i = decltype(ic)::value;
                     const uint32_t most = (now_ok >> (at + 2 * b + i)) & 1u ? many : 0u;
                     const int32_t from = j0 + 32 * b + 16 * i;
-                    seen = seen | (most != 0 && max(from, lo) < min(from + 16, hi));
+                    seen |= static_cast<int>(most != 0) & static_cast<int>(max(from, lo) < min(from + 16, hi));
                     unrolled<8>([&](auto ec) {
                         constexpr int e = 8 * i + decltype(ec)::value;
                         const bool vis = first + static_cast<uint32_t>(32 * b + 8 * (e >> 2) + (e & 3)) < most;
@@ -396,7 +400,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
                     });
                 });
         } else {
-            seen = true;
+            seen = 1;
         }
         float top = -__builtin_inff();
 #pragma unroll
@@ -407,7 +411,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
                 mx = max3(mx, s[b][8 * i + 3], s[b][8 * i + 4]);
                 mx = max3(mx, s[b][8 * i + 5], s[b][8 * i + 6]);
                 mx = max3(mx, s[b][8 * i + 7], s[b][8 * i + 7]);
-                top = fmaxf(top, __builtin_fmaf(mx, f[2 * b + i], lane_of(now_ve, 2 * b + i)));
+                top = fmaxf(top, __builtin_fmaf(mx, f[2 * b + i], ve[2 * b + i]));
             });
         top = ceilf(swap32_max(top));
         if (__any(top > m)) {
@@ -424,7 +428,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
         float sums[KB][2] = {}, base[C::blocks];
         // (f16: the offset joins the exponent; its rounding, 2^-21 of the weight, is nothing beside the weight's)
 #pragma unroll
-        for (int b = 0; b < C::blocks; b++) base[b] = lane_of(now_ve, b) - (kTwo ? ms : ms - static_cast<float>(kPOffset));
+        for (int b = 0; b < C::blocks; b++) base[b] = ve[b] - (kTwo ? ms : ms - static_cast<float>(kPOffset));
         // Weights of elements e0 .. e0 + n - 1 of group b, their parts for the matrix cores and their sums.
         auto weights = [&](auto bc, auto e0c, auto nc) __attribute__((always_inline)) {
             constexpr int b = decltype(bc)::value;
@@ -496,14 +500,15 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     };
 
     if (nt > 0) {
-        auto inner = [&](int tile) __attribute__((always_inline)) { return tile >= inner0 && tile < inner1; };
+        // (as signs: conditions would be kept as lane masks) below 0: some row does not see all of the tile.
+        auto outer = [&](int tile) __attribute__((always_inline)) { return (tile - inner0) | (inner1 - 1 - tile); };
         ask_pages(0);
         ask_scales();
         take_pages(0);
         ask_pages(C::window);
         load(0);
-        bool whole = inner(0) && raw_ok;  // of the tile that is multiplied next
-        if (!whole) mend(0, 0);
+        int part = outer(0) | raw_bad;  // of the tile that is multiplied next
+        if (part < 0) mend(0, 0);
         store(0);
         use_window();
         if (nt > 1) load(1);
@@ -512,18 +517,21 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
             const int buf = t & 1;
             // Tile t + 1 is in `raw`: mended here, stored in the step (past the last, nothing of use). That buffer's
             // readers passed the barrier.
-            const bool next_whole = inner(t + 1) && raw_ok;
-            if (!next_whole && t + 1 < nt) mend(t + 1, buf ^ 1);
-            step(t, buf, whole);
-            whole = next_whole;
+            const int next_part = outer(t + 1) | raw_bad;
+            if (next_part < 0 && t + 1 < nt) mend(t + 1, buf ^ 1);
+            step(t, buf, part >= 0);
+            part = next_part;
             if ((t + 1) % C::window == 0) use_window();
             if (t + 2 < nt) {
                 const int at = (t + 2) % C::window;
-                if (at == 0) {
-                    take_pages(t + 2);
-                    ask_pages(t + 2 + C::window);
+                if (at % (C::window / 2) == 0) {
+                    if (at == 0) {
+                        take_pages(t + 2);
+                        ask_pages(t + 2 + C::window);
+                    } else {
+                        ask_scales();
+                    }
                 }
-                if (at == C::window / 2) ask_scales();
                 load(t + 2);
             }
             __syncthreads();
@@ -531,7 +539,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     }
 
     l = swap32_sum(l);
-    const bool any_seen = swap32_max(seen ? 1.0f : 0.0f) > 0.0f;
+    const bool any_seen = swap32_max(seen != 0 ? 1.0f : 0.0f) > 0.0f;
     if (row0 + l32 >= n_rows) return;
     const float l_by = kTwo ? 1.0f : 1.0f / kPScale;  // f16: the sum is of the weights times 2^kPOffset
     if (it.splits == 1) {
@@ -569,7 +577,7 @@ int launch_tiles(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a) {
     typedef TileForm<TQ, DH> C;
     static std::atomic<uint64_t> allowed{0};
     const void* kernel = reinterpret_cast<const void*>(&attn_paged_tile_kernel<TQ, DH, MODS>);
-    if (C::lds + 4096 > 64 * 1024)  // (with the kernel's static LDS)
+    if (C::lds > 64 * 1024)
         if (int rc = allow_lds(ctx, kernel, C::lds, allowed)) return rc;
     hipLaunchKernelGGL((attn_paged_tile_kernel<TQ, DH, MODS>), dim3(a.blocks), dim3(64 * C::waves), C::lds, ctx->stream, a);
     return after_launch(ctx, what);
