@@ -22,6 +22,12 @@ namespace {
 typedef short short4v __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(1))) uint8_t Global;
 
+// LDS by its address: through a pointer every place that is not the array's start plus a constant costs an addition of it.
+template <typename T>
+__device__ __forceinline__ __attribute__((address_space(3))) T* lds_at(uint32_t at) {
+    return (__attribute__((address_space(3))) T*)(uintptr_t)at;
+}
+
 // The slot of 16-byte chunk c of tile row `row` in LDS: the 16 rows of a ds_read_b128 pass at one chunk of K, and
 // the 4 rows x 4 chunks of half a transposing read of V, fall on distinct banks.
 template <int DH>
@@ -41,7 +47,7 @@ struct TileForm {
     static constexpr int blocks = keys / kBlockKeys;  // pages' parts of a tile
     static constexpr int units = blocks / 2;          // blocks that a wave brings in, of K or V
     static constexpr int half_bytes = keys * DH * 2;
-    static constexpr int tiles = 4 * half_bytes;       // two buffers of K and V, from LDS address 0 on (no additions to fragments' places)
+    static constexpr int tiles = 4 * half_bytes;       // two buffers of K and V
     static constexpr int lds = tiles + 2 * 4 * (waves + keys * (DH / 32));  // and what is noted of NaN values
     static constexpr int window = 64 / blocks;         // tiles of a page look-up
     static constexpr int rpi = 64 * 16 / DH;           // rows of a load instruction
@@ -85,7 +91,8 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     typedef TileForm<TQ, DH> C;
     constexpr bool kTwo = sizeof(TQ) == 4;
     constexpr int NS = DH / 16, ND = DH / 32, KB = C::keys / 32;
-    extern __shared__ __align__(16) uint8_t tile_lds[];
+    extern __shared__ __align__(512) uint8_t tile_lds[];  // (places in a row are exclusive-ors of these address bits)
+    const uint32_t lds0 = static_cast<uint32_t>((uintptr_t)(__attribute__((address_space(3))) uint8_t*)tile_lds);
     auto nan_sh = reinterpret_cast<uint32_t(*)[C::waves]>(tile_lds + C::tiles);  // whether a wave took NaN values out of the tile,
     auto nan_bits = reinterpret_cast<uint32_t(*)[C::keys][DH / 32]>(tile_lds + C::tiles + 2 * 4 * C::waves);  // and where
     const int lane = static_cast<int>(threadIdx.x) & 63;
@@ -234,7 +241,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     uint32_t dst;
     {
         const int row = block0 * kBlockKeys + lr, c = 2 * lc;
-        dst = static_cast<uint32_t>((is_v ? C::half_bytes : 0) + row * DH * 2 + 16 * (is_v ? v_slot<DH>(row, c) : k_slot<DH>(row, c)));
+        dst = lds0 + static_cast<uint32_t>((is_v ? C::half_bytes : 0) + row * DH * 2 + 16 * (is_v ? v_slot<DH>(row, c) : k_slot<DH>(row, c)));
     }
     const uint32_t dst_n = is_v || DH < 128 ? 0u : static_cast<uint32_t>(C::rpi) * 16u;
     // The tile in `raw`: a NaN value times a weight of zero is NaN, so in tiles of which some row does not see all, values
@@ -281,7 +288,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
             y[4 * w + 2] = y1[0];
             y[4 * w + 3] = y1[1];
         }
-        *reinterpret_cast<half8*>(tile_lds + buf * 2 * C::half_bytes + (i * kBlockKeys + n * C::rpi) * DH * 2 + (dst ^ (16u * p) ^ (static_cast<uint32_t>(n) * dst_n))) = y;
+        *lds_at<half8>(buf * 2 * C::half_bytes + (i * kBlockKeys + n * C::rpi) * DH * 2 + (dst ^ (16u * p) ^ (static_cast<uint32_t>(n) * dst_n))) = y;
     };
     auto store = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
@@ -293,18 +300,18 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     int seen = 0;
     // Fragments: K, 8 dimensions of key 32 b + l32 for step d; V, by transposing reads, of eight keys for 32 dimensions.
     // The slots make their places k_at ^ 32 d and v_at ^ 64 d, one register each instead of one for every d.
-    uint32_t k_lane = static_cast<uint32_t>(l32 * DH * 2 + 16 * k_slot<DH>(l32, h)), v_lane;
+    uint32_t k_lane = lds0 + static_cast<uint32_t>(l32 * DH * 2 + 16 * k_slot<DH>(l32, h)), v_lane;
     {
         const int tq = lane & 15, row = 4 * h + (tq >> 2);
-        v_lane = static_cast<uint32_t>(C::half_bytes + row * DH * 2 + 16 * v_slot<DH>(row, 2 * ((lane >> 4) & 1) + ((tq & 3) >> 1)) + 8 * (tq & 1));
+        v_lane = lds0 + static_cast<uint32_t>(C::half_bytes + row * DH * 2 + 16 * v_slot<DH>(row, 2 * ((lane >> 4) & 1) + ((tq & 3) >> 1)) + 8 * (tq & 1));
     }
     auto k_frag = [&](uint32_t k_at, int b, int d) __attribute__((always_inline)) {
-        return *reinterpret_cast<const half8*>(tile_lds + 32 * b * DH * 2 + (k_at ^ (32u * d)));
+        return *lds_at<half8>(32 * b * DH * 2 + (k_at ^ (32u * d)));
     };
     auto v_frag = [&](uint32_t v_at, int d, int b, int i) __attribute__((always_inline)) {
-        const uint8_t* p0 = tile_lds + (32 * b + 16 * i) * DH * 2 + (v_at ^ (64u * d));
-        const short4v a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)p0);
-        const short4v a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4v*)(p0 + 8 * DH * 2));
+        const uint32_t p0 = (32 * b + 16 * i) * DH * 2 + (v_at ^ (64u * d));
+        const short4v a0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<short4v>(p0));
+        const short4v a1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16(lds_at<short4v>(p0 + 8 * DH * 2));
         return __builtin_bit_cast(half8, __builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
     };
     // `whole`: every row of the workgroup sees all of the tile's keys.
@@ -398,6 +405,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
                         const bool vis = first + static_cast<uint32_t>(32 * b + 8 * (e >> 2) + (e & 3)) < most;
                         s[b][e] = vis ? s[b][e] : -__builtin_inff();
                     });
+                    __builtin_amdgcn_sched_barrier(0);  // (else all comparisons first, their masks in scalar registers that the loop has use for)
                 });
         } else {
             seen = 1;
