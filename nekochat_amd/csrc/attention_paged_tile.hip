@@ -58,27 +58,6 @@ struct TileForm {
     static constexpr int loads = kBlockKeys / rpi;     // load instructions of a unit
 };
 
-// The kernel's paged arguments, read again where this stands.
-__device__ __forceinline__ Paged paged_again() {
-    typedef const __attribute__((address_space(4))) PagedAttnArgs* Args;
-    Args p = (Args)__builtin_amdgcn_kernarg_segment_ptr();
-    asm volatile("" : "+s"(p));
-    Paged q;
-    q.k = p->p.k;
-    q.v = p->p.v;
-    q.ks = p->p.ks;
-    q.vs = p->p.vs;
-    q.table = p->p.table;
-    q.table_stride = p->p.table_stride;
-    q.n_pages = p->p.n_pages;
-    q.max_pages = p->p.max_pages;
-    q.page_log2 = p->p.page_log2;
-    q.n_kv = p->p.n_kv;
-    q.head_bytes = p->p.head_bytes;
-    q.page_bytes = p->p.page_bytes;
-    return q;
-}
-
 // The largest of three, NaN if one is (v_maximum3_f32; fmaxf first quiets operands that may be signalling NaNs, an
 // instruction each). A row with a NaN score is NaN whatever its maximum.
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -169,8 +148,7 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     const int block0 = (wave & 1) * C::units;
 
     // The next 64 blocks of 16 keys, one to a lane: where this wave's operand of it stands, and its exponents. Those
-    // after them are asked for half a window ahead. (These run once in a window: the arguments are read for them again,
-    // rather than kept in scalar registers that the loop has no room for.)
+    // after them are asked for half a window ahead.
     const int nt = tk.k1 > tk.k0 ? (tk.k1 - tk.k0 + C::keys - 1) / C::keys : 0;
     uint32_t from_lo = 0, from_hi = 0;
     int32_t next_page = -1;
@@ -178,23 +156,20 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
     uint64_t exps_ok = 0;  // which of them have a page
     float next_ks = 1.0f, next_vs = 1.0f;
     auto ask_pages = [&](int tile) __attribute__((always_inline)) {
-        const Paged p = paged_again();
         const int32_t at = tk.k0 + C::keys * tile + kBlockKeys * lane;
         next_page = -1;
-        if (tile < nt && at < tk.k1) next_page = paged_page(p, it.s, at);
+        if (tile < nt && at < tk.k1) next_page = paged_page(a.p, it.s, at);
     };
     auto ask_scales = [&]() __attribute__((always_inline)) {
-        const Paged p = paged_again();
-        const int64_t i = static_cast<int64_t>(next_page < 0 ? 0 : next_page) * p.n_kv + kvh;
-        next_ks = p.ks[i];
-        next_vs = p.vs[i];
+        const int64_t i = static_cast<int64_t>(next_page < 0 ? 0 : next_page) * a.p.n_kv + kvh;
+        next_ks = a.p.ks[i];
+        next_vs = a.p.vs[i];
     };
     auto take_pages = [&](int tile) __attribute__((always_inline)) {
-        const Paged p = paged_again();
-        const uint8_t* head_base = (is_v ? p.v : p.k) + kvh * p.head_bytes;
-        const int32_t slot = (tk.k0 + C::keys * tile + kBlockKeys * lane) & ((1 << p.page_log2) - 1);
+        const uint8_t* head_base = (is_v ? a.p.v : a.p.k) + kvh * a.p.head_bytes;
+        const int32_t slot = (tk.k0 + C::keys * tile + kBlockKeys * lane) & ((1 << a.p.page_log2) - 1);
         // (a block without a page reads page 0 and is masked; every slot of a page may be read)
-        const uint64_t at = reinterpret_cast<uint64_t>(head_base) + static_cast<uint64_t>(static_cast<uint32_t>(next_page < 0 ? 0 : next_page)) * p.page_bytes +
+        const uint64_t at = reinterpret_cast<uint64_t>(head_base) + static_cast<uint64_t>(static_cast<uint32_t>(next_page < 0 ? 0 : next_page)) * a.p.page_bytes +
                             static_cast<uint32_t>(slot * hd);
         from_lo = static_cast<uint32_t>(at);
         from_hi = static_cast<uint32_t>(at >> 32);
