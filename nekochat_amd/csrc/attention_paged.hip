@@ -31,9 +31,10 @@ constexpr int kTileRows = 16;
 constexpr int kLeast = 8;           // tiles of 32 keys to a wave up to which a cache's keys are never split
 constexpr int kFewRows = 32;        // flattened rows up to which a sequence is this kernel's
 // Pairs of a query head's row and a key up to which the 16-row kernel alone is faster: it spreads them over more
-// waves and starts sooner, the tiles convert a code once for 128 rows. 76 batches of 64 to 2530 rows, 8 to 32 heads
-// of 64 to 256, on both: f16, from 20 to 35 million neither way by more than 1.35 times, half as long below 2 million
-// (128 rows of 32 heads 7.5 us and 15.9) and 1.6 times as long at 65 (2048 rows 115 and 74); f32 level at 32.
+// waves and starts sooner, the tiles convert a code once for 128 rows. 68 batches of 64 to 4000 rows, 8 to 32 heads
+// of 64 to 256, each on both. f16: up to 8 million faster, half as long at a quarter of one (128 rows of 32 heads 7.3 us and
+// 15.2), from 8 to 20 neither way by more than 1.3 times, slower past 30, 1.9 times as long at 67 (2048 rows 117 and 63).
+// f32: faster up to 8 and mostly to 30 (1024 rows 45 and 59), level from there to 40, 1.2 times as long at 67.
 template <typename TQ>
 constexpr double kFewPairs = sizeof(TQ) == 2 ? 20e6 : 40e6;
 constexpr int kSpareRows = 256;     // flattened rows past one token to a sequence that still make a decoding batch
