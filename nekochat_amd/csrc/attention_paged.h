@@ -64,10 +64,9 @@ __device__ __forceinline__ bool attn_find_by(const Paged& p, const AttnTiling& t
             units[k] = attn_units(t, reach, r);
         }
     };
-    int32_t chunk = t.least;
     if (K == 1) load(0);
-    if (reach > static_cast<int64_t>(t.least) << t.unit_log2) {  // (else no tile has more units than the least chunk)
-        double work = 0.0;  // (whole numbers below 2^53: exact)
+    const int32_t chunk = attn_plan(t, p, [&](double& work, int64_t& n) {
+        work = 0.0;  // (whole numbers below 2^53: exact)
         uint32_t all = 0;
         for (int32_t base = 0; base < p.n_seq; base += 64 * K) {
             if (K > 1) load(base);
@@ -77,10 +76,10 @@ __device__ __forceinline__ bool attn_find_by(const Paged& p, const AttnTiling& t
                 all += static_cast<uint32_t>(tiles[k]);
             }
         }
-        work = wave_sum_f64(work);
         all = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(wave_scan_u32(all)), 63));
-        chunk = attn_chunk(t, work * p.n_kv, static_cast<int64_t>(all) * p.n_kv);
-    }
+        work = wave_sum_f64(work) * p.n_kv;
+        n = static_cast<int64_t>(all) * p.n_kv;
+    });
     uint32_t past_tiles = 0, past = 0;  // of the sequences before
     for (int32_t base = 0; base < p.n_seq; base += 64 * K) {
         if (K > 1) load(base);

@@ -215,12 +215,26 @@ NEKO_HD int64_t attn_split_tiles_bound(const AttnTiling& t, int64_t rows, int64_
     const int64_t tiles = attn_tiles_bound(t, rows, n_seq), most = (t.target + n_kv - 1) / n_kv + 1;
     return tiles < most ? tiles : most;
 }
-// Whether any tile can be split. One sequence: its tiles are known, and with as many as wanted chunk >= units.
+// Whether a launch plans for splits: a workspace for their partial results and the merge. One sequence with as many
+// tiles as wanted would not be split (chunk >= units), unless some of the call's rows are not its own.
 NEKO_HD bool attn_may_split(const AttnTiling& t, const Paged& p) {
     if (paged_reach(p) <= static_cast<int64_t>(t.least) << t.unit_log2) return false;
     if (p.n_seq > 1) return true;
     const int64_t tiles = (static_cast<int64_t>(p.rows) * t.group + (1 << t.tile_log2) - 1) >> t.tile_log2;
     return tiles * p.n_kv < t.target;
+}
+// The chunk of a launch, as the device takes it: more than any tile has where no splits are planned, so that what only
+// the device knows -- rows behind the last sequence, which leave fewer tiles than the call's rows make -- cannot ask for
+// splits that have no place. (Such a call takes no longer than one whose rows are all the sequence's.) `sums`: the work
+// and the tiles of attn_chunk.
+constexpr int32_t kUnsplit = 1 << 30;
+template <typename F>
+NEKO_HD int32_t attn_plan(const AttnTiling& t, const Paged& p, F&& sums) {
+    if (!attn_may_split(t, p)) return kUnsplit;
+    double work;
+    int64_t tiles;
+    sums(work, tiles);
+    return attn_chunk(t, work, tiles);
 }
 
 }  // namespace neko_hip

@@ -93,6 +93,38 @@ void check_blocks(const Batch* b, const AttnTiling* given, int64_t* out) {
     out[6] = attn_may_split(t, p) ? attn_split_tiles_bound(t, p.rows, p.n_seq, p.n_kv) : 0;
 }
 
+// The same of a launch as it is planned: what the device splits beside what the host has made room for: tiles, blocks,
+// tiles that are split, units of keys that no split covers; whether splits are planned, the most blocks and split tiles.
+void check_plan(const Batch* b, const AttnTiling* given, int64_t* out) {
+    const Paged p = paged(b);
+    AttnTiling t = *given;
+    attn_set(t);
+    const int32_t reach = paged_reach(p);
+    const int32_t chunk = attn_plan(t, p, [&](double& work, int64_t& n) {
+        work = 0;
+        n = 0;
+        for (int32_t s = 0; s < p.n_seq; s++) {
+            const SeqRows r = paged_seq(p, s);
+            work += static_cast<double>(attn_tiles(t, r)) * attn_units(t, reach, r);
+            n += attn_tiles(t, r);
+        }
+        work *= p.n_kv;
+        n *= p.n_kv;
+    });
+    for (int i = 0; i < 4; i++) out[i] = 0;
+    for (int32_t s = 0; s < p.n_seq; s++) {
+        const SeqRows r = paged_seq(p, s);
+        const int64_t n = attn_tiles(t, r), units = attn_units(t, reach, r), splits = attn_splits(static_cast<int32_t>(units), chunk);
+        out[0] += n;
+        out[1] += n * splits;
+        if (splits > 1) out[2] += n;
+        if (n && splits * chunk < units) out[3] += units - splits * chunk;
+    }
+    out[4] = attn_may_split(t, p);
+    out[5] = attn_blocks_bound(t, p.rows, p.n_seq, p.n_kv);
+    out[6] = attn_split_tiles_bound(t, p.rows, p.n_seq, p.n_kv);
+}
+
 int check_seq_from(const Batch* b, int32_t s, int32_t row) { return paged_seq_from(paged(b), s, row); }
 int check_splits(int32_t units, int32_t chunk) { return attn_splits(units, chunk); }
 

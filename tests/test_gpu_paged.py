@@ -407,6 +407,19 @@ def test_attention_sequences_past_one_search(dev, n_seq, wide):
     _check_attention(dev, 4, 2, 64, 16, "f16", seqs, seed=13, pad=n_seq + 150 if wide else 7, wide=wide)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("rows,own,length,reach", [
+    (2048, 150, 150, 4000), (2048, 150, 600, 4000), (2048, 1, 1100, 4000), (2048, 500, 500, 4000),  # the tiles
+    (512, 1, 1100, 1104), (512, 33, 1104, 1104),                                                    # the 16-row kernel
+])
+def test_attention_one_sequence_in_a_buffer_of_many_rows(dev, rows, own, length, reach, dtype):
+    """Rows behind the only sequence's, more than it has: the launch is planned by the call's rows."""
+    _case(f"attention, {own} of {rows} rows, length {length}, {dtype}")
+    H, KV, hd, page = 32, 8, 64, 16
+    b = P.Batch([(own, length)], page, 17, pad=rows - own, slack=reach // page - -(-length // page))
+    _check_attention(dev, H, KV, hd, page, dtype, b.seqs, 17, batch=b, what=f"{own} of {rows}")
+
+
 def test_attention_smallest_cap(dev):
     """A cap whose inverse is past the largest number caps every score to next to nothing: all keys alike."""
     _case("attention, a cap of 1e-39")
@@ -727,6 +740,41 @@ def test_captured_prompts_of_two_graphs(dev):
             ops.attention_paged(q, eager, table(1 - i, k), start[1 - i], len_of(1 - i, k), H, out=o)  # (the workspace, between)
     assert torch.equal(cache.k_pages.view(torch.uint8), eager.k_pages.view(torch.uint8))
     assert torch.equal(cache.v_pages.view(torch.uint8), eager.v_pages.view(torch.uint8))
+
+
+def test_one_captured_graph_for_row_ranges_that_shrink(dev):
+    """Graphs captured for a buffer of many rows, replayed as the one sequence of them fills fewer: on the tiles and on the
+    16-row kernel, each replay as the eager call, eager calls in between."""
+    _case("row ranges that shrink")
+    H, KV, hd, page = 32, 8, 64, 16
+    for rows, width, steps in ((2048, 250, [(2048, 2048), (500, 2600), (1, 2601), (64, 4000), (2048, 4000)]),
+                               (512, 69, [(512, 600), (1, 1100), (40, 1104), (512, 1104)])):
+        cache = _cache_on(P.random_cache(width, KV, page, hd, 1), dev)
+        table = torch.randperm(width, generator=torch.Generator().manual_seed(2))[None].int().to(dev)
+        q = torch.randn((rows, H * hd), generator=torch.Generator().manual_seed(3)).half().to(dev)
+        start, length = (torch.zeros(n, dtype=torch.int32, device=dev) for n in (2, 1))
+        call = lambda out: ops.attention_paged(q, cache, table, start, length, H, out=out)
+
+        def set_to(n, total):
+            start.copy_(torch.tensor([0, n], dtype=torch.int32))
+            length.fill_(total)
+
+        want = []
+        for n, total in steps:
+            set_to(n, total)
+            want.append(call(torch.full_like(q, 7.0)))
+            assert bool((want[-1][n:] == 7.0).all()) and bool((want[-1][:n] != 7.0).any(1).all())
+        out = torch.empty_like(q)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call(out)
+        for i in [1, 2, 0, 3, 1]:
+            set_to(*steps[i])
+            out.fill_(7.0)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, want[i]), f"rows {steps[i]} of {rows}"
+            call(torch.empty_like(q))
 
 
 def test_two_threads(dev):

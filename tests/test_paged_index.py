@@ -128,6 +128,57 @@ def test_attention_blocks_stay_within_the_grid(lib, seed):
     assert tiles <= tiles_bound and blocks <= blocks_bound and uncovered == 0 and split <= split_bound
 
 
+def _plan(lib, rows, seqs, log2, max_pages, n_kv, tiling):
+    start = np.cumsum([0] + [n for n, _ in seqs]).astype(np.int32)
+    length = np.array([x for _, x in seqs], np.int32)
+    b = Batch(0, start.ctypes.data, length.ctypes.data, max_pages, 1, max_pages, len(seqs), rows, log2, n_kv, 64)
+    out = (ctypes.c_int64 * 7)()
+    lib.check_plan(ctypes.byref(b), ctypes.byref(tiling), out)
+    return list(out)
+
+
+def _check_plan(lib, *args):
+    tiles, blocks, split, uncovered, planned, blocks_bound, split_bound = _plan(lib, *args)
+    assert uncovered == 0 and blocks <= blocks_bound
+    assert split <= (split_bound if planned else 0), "splits that the launch has no place for"
+    return split, planned
+
+
+@pytest.mark.parametrize("seed", range(400))
+def test_splits_are_those_that_the_launch_planned(lib, seed):
+    """What the device splits has a place in the workspace and a merge, however few of the call's rows are a sequence's:
+    a graph captured for many rows is replayed with few. One sequence alone is the case that the host plans by its rows."""
+    rng = np.random.default_rng(9000 + seed)
+    for _ in range(10):
+        log2, n_kv = int(rng.integers(4, 9)), int(rng.choice([1, 2, 8, 12]))
+        max_pages = int(np.exp(rng.uniform(0, 8)))
+        reach = max_pages << log2
+        n_seq = 1 if rng.random() < 0.6 else int(rng.integers(2, 40))
+        seqs = []
+        for _ in range(n_seq):
+            length = int(rng.integers(0, reach + 1))
+            seqs.append((min(length, int(np.exp(rng.uniform(0, 7))) - 1), length))
+        rows = max(1, int(sum(n for n, _ in seqs) * np.exp(rng.uniform(0, 8)))) + int(rng.integers(0, 9))
+        few = [(1, 2**31 - 1), (33, 2**31 - 1), (1, 32)][int(rng.integers(0, 3))]
+        t = Tiling(int(rng.choice([1, 2, 4, 7, 16])), *[(4, 7), (4, 8), (7, 6)][int(rng.integers(0, 3))],
+                   int(rng.choice([1, 256, 512, 768, 1024])), int(rng.choice([1, 4, 8])), int(rng.choice([0, 0, 40, 1000])), 0, *few)
+        _check_plan(lib, rows, seqs, log2, max_pages, n_kv, t)
+
+
+@pytest.mark.parametrize("tile_log2,unit_log2,target,least,rows,own,length,reach", [
+    (7, 6, 512, 1, 2048, 500, 500, 8192), (7, 6, 512, 1, 2048, 500, 4096, 8192), (7, 6, 512, 1, 4096, 64, 8192, 8192),
+    (7, 6, 512, 1, 8192, 1, 8192, 8192), (4, 7, 768, 4, 512, 1, 1100, 1104), (4, 7, 768, 4, 700, 1, 1040, 1040),
+])
+def test_one_sequence_with_rows_that_are_not_its_own(lib, tile_log2, unit_log2, target, least, rows, own, length, reach):
+    """32 / 8 heads, both kernels' tilings: a chunk's last piece, or one token, in a buffer of many rows."""
+    t = Tiling(4, tile_log2, unit_log2, target, least, 0, 0, 1, 2**31 - 1)
+    split, planned = _check_plan(lib, rows, [(own, length)], 4, reach >> 4, 8, t)
+    assert not planned and split == 0
+    # With the sequence's own rows alone the same tiles are split, and planned for.
+    split, planned = _check_plan(lib, own, [(own, length)], 4, reach >> 4, 8, t)
+    assert planned and split > 0
+
+
 @pytest.mark.parametrize("n_seq", [1, 2, 5, 6, 64, 300])
 @pytest.mark.parametrize("wild", [False, True])
 def test_the_sequence_of_a_row(lib, n_seq, wild):
