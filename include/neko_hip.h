@@ -227,6 +227,9 @@ int neko_hip_qk_norm_rope_paged(neko_hip_ctx* ctx, const void* qkv, int64_t row_
  * 2e-6 (1 + sum w|v| / sum w) of a 64-bit evaluation); f16 calls round as said at the kernels.
  * The tolerance holds while the value scales of a sequence's pages, per kv head, are within 2^96 of each other (a
  * page of zeros has 2^-64): a weight is held relative to the largest weight * scale that its row sees.
+ * Scores are f32: besides its products' roundings s_j is held to 2^-22 |s_j|, and its weight is off by as much. From
+ * 2^22 on that tells close scores apart no more, and equal ones weigh alike only under value scales that are alike.
+ * Any finite scores give a finite row (one key: its value); scores past f32's range are infinities.
  * Partial results of key splits go to the context's workspace (see neko_hip_matmul): its size goes by rows,
  * n_seq, heads, head size, window and the table's width (max_pages), not by lengths, so one uncaptured call
  * of these makes every later capture fit. */

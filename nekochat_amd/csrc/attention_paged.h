@@ -28,6 +28,14 @@ constexpr float kAttnLog2e = 1.44269504088896341f;
 constexpr int kPOffset = 15;  // weights go to f16 times 2^kPOffset, the largest power that it holds
 constexpr float kPScale = 1 << kPOffset;
 
+// A weight's exponent is s * f + ve - m, rounded once, where m is the largest s * f + ve of the row, rounded before that.
+// Past 2^24 the first may pass the second by a whole power of two or more, and the weight what f16 holds. Rows whose m is
+// past this (by less than an eighth below it) take the rounded s * f + ve for both: the largest weight is 1 again.
+constexpr float kFarMax = 0x1p22f;
+__device__ __forceinline__ float exponent_of(float s, float f, float ve, float m) {
+    return fabsf(m) >= kFarMax ? __builtin_fmaf(s, f, ve) - m : __builtin_fmaf(s, f, ve - m);
+}
+
 struct AttnItem {
     int32_t s, tile, split, splits;
     int32_t chunk;  // units of a split

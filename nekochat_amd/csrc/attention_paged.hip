@@ -339,13 +339,22 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
         }
         const float ms = m == -__builtin_inff() ? 0.0f : m;
         half8 ph, pl;
+        float base[2] = {static_cast<float>(ve2[0]) - ms, static_cast<float>(ve2[1]) - ms};
+        if (__any(fabsf(ms) >= kFarMax)) {  // exponents in place of scores
+#pragma unroll
+            for (int b = 0; b < 2; b++) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) s[b][i] = exponent_of(s[b][i], f[b], static_cast<float>(ve2[b]), ms);
+                f[b] = 1.0f;
+                base[b] = 0.0f;
+            }
+        }
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            const float base = static_cast<float>(ve2[b]) - ms;
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], f[b], base));
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], f[b], base[b]));
                 sum += p;
                 const float y = p * kPScale;
                 ph[4 * b + i] = static_cast<half_t>(y);

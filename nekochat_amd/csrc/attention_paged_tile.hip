@@ -69,8 +69,10 @@ __device__ __forceinline__ int pack_block(int ke, int ve) { return (ke + 128) | 
 __device__ __forceinline__ int block_ke(int x) { return (x & 255) - 128; }
 __device__ __forceinline__ int block_ve(int x) { return ((x >> 8) & 255) - 128; }
 
+// (f16 rows of 64 dimensions: three workgroups to a CU, at which four registers are spilled with a cap; 4 prompts of 2048
+// tokens, 12 heads, 151 us, at two 175)
 template <typename TQ, int DH, bool MODS>
-__global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel(PagedAttnArgs a) {
+__global__ __launch_bounds__(256, DH <= 64 && sizeof(TQ) == 2 ? 3 : DH <= 128 ? 2 : 1) void attn_paged_tile_kernel(PagedAttnArgs a) {
     typedef TileForm<TQ, DH> C;
     constexpr bool kTwo = sizeof(TQ) == 4;
     constexpr int NS = DH / 16, ND = DH / 32, KB = C::keys / 32;
@@ -416,6 +418,19 @@ __global__ __launch_bounds__(256, DH <= 128 ? 2 : 1) void attn_paged_tile_kernel
         // (f16: the offset joins the exponent; its rounding, 2^-21 of the weight, is nothing beside the weight's)
 #pragma unroll
         for (int b = 0; b < C::blocks; b++) base[b] = ve[b] - (kTwo ? ms : ms - static_cast<float>(kPOffset));
+        if (__any(fabsf(ms) >= kFarMax)) {  // exponents in place of scores
+#pragma unroll
+            for (int b = 0; b < KB; b++)
+                unrolled<16>([&](auto ec) {
+                    constexpr int e = decltype(ec)::value;
+                    s[b][e] = exponent_of(s[b][e], f[2 * b + e / 8], ve[2 * b + e / 8], ms);
+                });
+#pragma unroll
+            for (int b = 0; b < C::blocks; b++) {
+                f[b] = 1.0f;
+                base[b] = kTwo ? 0.0f : static_cast<float>(kPOffset);
+            }
+        }
         // Weights of elements e0 .. e0 + n - 1 of group b, their parts for the matrix cores and their sums.
         auto weights = [&](auto bc, auto e0c, auto nc) __attribute__((always_inline)) {
             constexpr int b = decltype(bc)::value;

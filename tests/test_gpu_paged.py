@@ -458,6 +458,93 @@ def test_attention_scales_of_scores(dev, scale, seqs):
         _check_attention(dev, 4, 2, 128, 16, "f16", seqs, seed=32, scale=scale, wide=wide)
 
 
+def _check_one_winner(dev, H, KV, hd, dtype, seqs, seed, cache, batch, q, scale, **kw):
+    """Rows whose weights are 1 or nothing (one key seen, or scores further apart than their roundings), up to equal ones:
+    no score's rounding reaches the result, so the bar is _bar's without them."""
+    dc = _cache_on(cache, dev)
+    slopes = kw.get("slopes")
+    got = ops.attention_paged(q.to(dev), dc, *batch.tensors(dev), H, scale=scale,
+                              **{**kw, "slopes": None if slopes is None else slopes.to(dev)})
+    torch.cuda.synchronize()
+    want, a, _ = P.attention(q, cache, batch, H, float(np.float32(scale)), **kw)
+    got = got.cpu().double()
+    assert bool(torch.isfinite(got).all()), "not finite"
+    n = max(n for _, n in seqs)
+    bar = 2 * (8 + n / 32 + 64) * U * a + (H16 * want.abs() + H16 * a + 2.0 ** -25 if dtype == "f16" else 0.0)
+    over = float(((got - want).abs() - bar).max())
+    assert over <= 0, f"off by {over:.3g} past the bar"
+
+
+FORMS = {"decode": (DECODE, False), "prompt": (PROMPT, False), "wide": (PROMPT, True), "split": ([(1, 5000), (2, 40)], False)}
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_one_key_of_any_score(dev, hd, dtype, form):
+    """A row that sees one key gives its value, whatever the score: past 2^24 a score's rounding is a whole exponent."""
+    _case(f"attention {form}, one key, hd {hd} {dtype}")
+    seqs, wide = FORMS[form]
+    H, KV, page = 4, 2, 16
+    b = P.Batch(seqs, page, 23, slack=_wide(seqs, H, page) if wide else 1)
+    cache = P.random_cache(b.n_pages, KV, page, hd, 24)
+    q = torch.randn((b.rows, H * hd), generator=torch.Generator().manual_seed(25)).to(DT[dtype])
+    for scale in (1e5, 1e6, -1e6, 1e7, 1e8, -1e9, 1e12):
+        _check_one_winner(dev, H, KV, hd, dtype, seqs, 23, cache, b, q, scale, window=1)
+    _check_one_winner(dev, H, KV, hd, dtype, seqs, 23, cache, b, q, 1e7, window=1, softcap=1e10, slopes=torch.full((H,), 3.0))
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_scores_far_apart(dev, hd, dtype, form):
+    """Many keys with scores of 1e7 to 1e11 of either sign, at least 1e6 apart or equal: the mean of the largest's values."""
+    _case(f"attention {form}, scores far apart, hd {hd} {dtype}")
+    seqs, wide = FORMS[form]
+    H, KV, page = 4, 2, 16
+    b = P.Batch(seqs, page, 26, slack=_wide(seqs, H, page) if wide else 1)
+    g = torch.Generator().manual_seed(27)
+    cache = list(P.random_cache(b.n_pages, KV, page, hd, 28))
+    keys = torch.zeros(cache[0].shape)
+    keys[..., 0] = 2.0 ** torch.randint(0, 5, keys.shape[:3], generator=g)  # score: q_0 times 1, 2, 4, 8 or 16
+    cache[0], cache[2] = keys.to(P.F8), torch.ones_like(cache[2])
+    cache[3] = torch.full_like(cache[3], 2.0 ** -7)  # (equal scores weigh alike where they are rounded alike)
+    cache = tuple(cache)
+    q = torch.zeros((b.rows, H, hd))
+    q[..., 0] = torch.randint(1000, 2000, (b.rows, H), generator=g).float()
+    q[::3] *= -1.0
+    q = q.reshape(b.rows, -1).to(DT[dtype])
+    for scale in (1e3, 1e4, -1e5, 1e6, 3e6):
+        _check_one_winner(dev, H, KV, hd, dtype, seqs, 26, cache, b, q, scale)
+    _check_one_winner(dev, H, KV, hd, dtype, seqs, 26, cache, b, q, 1e4, softcap=1e9, window=40)
+    # A bias that favours far keys: q of zeros, scores slope * distance.
+    _check_one_winner(dev, H, KV, hd, dtype, seqs, 26, cache, b, torch.zeros_like(q), 1.0, slopes=-torch.tensor([1e6, 3e6, 1e7, 1e8]))
+    _check_one_winner(dev, H, KV, hd, dtype, seqs, 26, cache, b, torch.zeros_like(q), 1.0, slopes=-torch.tensor([1e6, 3e6, 1e7, 1e8]), window=20)
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_attention_rows_beside_large_scores(dev, dtype, form):
+    """Rows of ordinary scores are as exact as ever beside rows of huge ones, which stay within their values."""
+    _case(f"attention {form}, rows beside large scores, {dtype}")
+    seqs, wide = FORMS[form]
+    H, KV, hd, page = 4, 2, 128, 16
+    b = P.Batch(seqs, page, 29, slack=_wide(seqs, H, page) if wide else 1)
+    cache = P.random_cache(b.n_pages, KV, page, hd, 30)
+    q = torch.randn((b.rows, H, hd), generator=torch.Generator().manual_seed(31))
+    big = torch.rand((b.rows, H, 1), generator=torch.Generator().manual_seed(32)) < 0.4
+    q = torch.where(big, q * 1e4, q * 1e-3).reshape(b.rows, -1).to(DT[dtype])
+    dc = _cache_on(cache, dev)
+    got = ops.attention_paged(q.to(dev), dc, *b.tensors(dev), H, scale=1e3)
+    torch.cuda.synchronize()
+    want, a, s = P.attention(q, cache, b, H, 1e3)
+    got, big = got.cpu().double(), big.expand(-1, -1, hd).reshape(b.rows, -1)
+    assert bool(torch.isfinite(got).all())
+    most = float((cache[1].float() * cache[3][..., None, None]).abs().max())
+    over = torch.where(big, got.abs() - 1.01 * most, (got - want).abs() - _bar(want, a, s, max(n for _, n in seqs), hd, dtype))
+    assert float(over.max()) <= 0
+
+
 @pytest.mark.parametrize("seqs,wide", [(DECODE, False), (PROMPT, False), (PROMPT, True)])
 def test_attention_pages_of_far_apart_scales(dev, seqs, wide):
     """Value pages whose scales lie 2^50 apart, each row's result as exact as if they did not; keys likewise small."""
