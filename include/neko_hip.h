@@ -199,7 +199,7 @@ typedef struct neko_paged_batch {
 
 /* neko_hip_qk_norm_rope and the append of what it makes: each row of qkv is [q n_q*hd | k n_kv*hd | v n_kv*hd]; its q
  * heads are normed (wqk as above; NULL: not), rotated and written to q_out (the q columns of qkv itself: same
- * pointer and stride; or disjoint); its k heads the same, rounded to the activation type, and with its v heads
+ * pointer and, past one row, stride; or disjoint); its k heads the same, rounded to the activation type, and with its v heads
  * rounded to 8 bits into the page of the row's position. qkv's k and v columns are not written.
  *   rot_dim      the first rot_dim dimensions of each head are rotated, the rest pass (a multiple of 8, up to
  *                hd; 0: no rotation, cs unused), by cs [n_pos][rot_dim], (cos, sin) pairs as neko_rope_table

@@ -417,7 +417,7 @@ extern "C" int neko_hip_qk_norm_rope_paged(neko_hip_ctx* ctx, const void* qkv, i
     NEKO_REQUIRE(ctx, aligned(qkv, esz) && aligned(q_out, esz), "%s: misaligned rows", what);
     const size_t s_in = rows_span(rows, width, row_stride, esz), s_out = rows_span(rows, q_width, q_out_stride, esz);
     NEKO_REQUIRE(ctx, s_in != 0 && s_out != 0, "%s: rows span more than 2^62 bytes", what);
-    NEKO_REQUIRE(ctx, (q_out == qkv && q_out_stride == row_stride) || !overlaps(q_out, s_out, qkv, s_in),
+    NEKO_REQUIRE(ctx, (q_out == qkv && (rows == 1 || q_out_stride == row_stride)) || !overlaps(q_out, s_out, qkv, s_in),
                  "%s: q_out is the q columns of qkv itself or disjoint from qkv", what);
     NEKO_REQUIRE(ctx, !paged_overlaps(*kv, qkv, s_in) && !paged_overlaps(*kv, q_out, s_out), "%s: the cache may not overlap qkv or q_out",
                  what);

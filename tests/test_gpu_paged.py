@@ -132,6 +132,23 @@ def test_append_unaligned_rows_and_in_place(dev, page):
     _check_append(dev, 4, 2, 128, page, "f16", RAGGED, 128, False, True, seed=7, in_place=True)
 
 
+def test_append_one_row_in_place_at_any_stride(dev):
+    """One row has no stride to speak of: a view of it is its own q columns whatever strides the tensors name."""
+    _case("append, one row in place, odd strides")
+    n_q, n_kv, hd = 4, 2, 64
+    width = (n_q + 2 * n_kv) * hd
+    row = torch.randn(width, generator=torch.Generator().manual_seed(1)).half().to(dev)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)
+    batch = (torch.zeros((1, 1), dtype=torch.int32, device=dev), i32(0, 1), i32(1))
+    cs = _rope(4, hd).to(dev)
+    want = ops.qk_norm_rope_paged(row[None], n_q, ops.PagedKV.empty(1, 16, n_kv, hd, dev), *batch, cs, 1e-6)
+    for stride in (1, 5, width):
+        x = row.clone().as_strided((1, width), (stride, 1))
+        got = ops.qk_norm_rope_paged(x, n_q, ops.PagedKV.empty(1, 16, n_kv, hd, dev), *batch, cs, 1e-6, q_out=x[:, : n_q * hd])
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) and torch.equal(x[:, n_q * hd:], row[None, n_q * hd:])
+
+
 @pytest.mark.parametrize("n_seq,dtype", [(1, "f16"), (70, "f16"), (300, "f32")])
 def test_append_many_sequences(dev, n_seq, dtype):
     """More sequences than one search step holds, idle places in rows, one sequence alone."""
