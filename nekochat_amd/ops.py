@@ -361,6 +361,8 @@ def qk_norm_rope_paged(qkv: torch.Tensor, n_q: int, cache: PagedKV, page_table: 
     rows, width, stride = _rows(qkv, "qkv")
     _on(cache.k_pages, "cache", qkv.device)
     hd, n_kv = cache.hd, cache.n_kv
+    if n_q <= 0:
+        raise NekoError(f"n_q must be positive, got {n_q}")
     if width < (n_q + 2 * n_kv) * hd:
         raise NekoError(f"qkv rows hold {width} values, fewer than {n_q + 2 * n_kv} heads x {hd}")
     batch = _paged_batch(page_table, row_start, kv_len, qkv.device)

@@ -939,6 +939,15 @@ def test_another_stream_and_prepared_calls(dev):
 
 # ------------------------------------------------------------------ refusals
 
+@pytest.mark.parametrize("n_q", [0, -1, -8])
+def test_append_refuses_heads_below_one(dev, n_q):
+    _case(f"refusal of n_q {n_q}")
+    cache, table = ops.PagedKV.empty(1, 16, 2, 64, dev), torch.zeros((1, 1), dtype=torch.int32, device=dev)
+    start, length = torch.tensor([0, 1], dtype=torch.int32, device=dev), torch.ones(1, dtype=torch.int32, device=dev)
+    with pytest.raises(NekoError):
+        ops.qk_norm_rope_paged(torch.zeros((1, 512), device=dev), n_q, cache, table, start, length, None, 1e-6)
+
+
 def test_refusals(dev):
     _case("refusals")
     H, KV, hd, page = 4, 2, 64, 16
