@@ -224,7 +224,9 @@ int neko_hip_qk_norm_rope_paged(neko_hip_ctx* ctx, const void* qkv, int64_t row_
  * not written. Infinities and NaN in q, and NaN in cached tokens, reach the rows that see them and no others.
  * q and out rows of n_head*hd (strides in elements); out overlaps neither q nor the cache.
  * f32 sums; products on the matrix cores, codes exact in f16, f32 q and weights as two f16 each (tested to
- * 2e-6 (1 + sum w|v| / sum w) of a 64-bit evaluation); f16 calls round as said at the kernels.
+ * 2e-6 (1 + sum w|v| / sum w) of a 64-bit evaluation). f16 calls keep 24 bits of each weight where the 16-row kernel runs
+ * (decoding, and prompts as far as rows and the table's reach are small); on the tiles of 128 rows each weight is rounded
+ * to one f16, an error of up to 2^-11 sum w|v| / sum w: the same prompt may take either, by the width of its table.
  * The tolerance holds while the value scales of a sequence's pages, per kv head, are within 2^96 of each other (a
  * page of zeros has 2^-64): a weight is held relative to the largest weight * scale that its row sees.
  * Scores are f32: besides its products' roundings s_j is held to 2^-22 |s_j|, and its weight is off by as much. From

@@ -562,6 +562,22 @@ def test_attention_rows_beside_large_scores(dev, dtype, form):
     assert float(over.max()) <= 0
 
 
+@pytest.mark.parametrize("seqs", [DECODE, PROMPT, [(1, 3), (1, 5), (7, 9)]])
+def test_attention_f16_weights_of_few_rows_are_not_rounded(dev, seqs):
+    """f16 calls on the 16-row kernel keep 24 bits of each weight: f32's bar and the result's own rounding, where values
+    cancel. Weights of one f16 miss it: near-equal scores, so that nothing else is large, and sums near zero beside a."""
+    _case(f"attention, f16 weights, {len(seqs)} sequences")
+    H, KV, hd, page = 8, 2, 64, 16
+    b = P.Batch(seqs, page, 33)
+    cache = P.random_cache(b.n_pages, KV, page, hd, 34)
+    q = torch.randn((b.rows, H * hd), generator=torch.Generator().manual_seed(35)).half()
+    got = ops.attention_paged(q.to(dev), _cache_on(cache, dev), *b.tensors(dev), H, scale=0.02)
+    torch.cuda.synchronize()
+    want, a, s = P.attention(q, cache, b, H, float(np.float32(0.02)))
+    bar = _bar(want, a, s, max(n for _, n in seqs), hd, "f32") + H16 * want.abs() + 2.0 ** -25
+    assert float(((got.cpu().double() - want).abs() - bar).max()) <= 0
+
+
 @pytest.mark.parametrize("seqs,wide", [(DECODE, False), (PROMPT, False), (PROMPT, True)])
 def test_attention_pages_of_far_apart_scales(dev, seqs, wide):
     """Value pages whose scales lie 2^50 apart, each row's result as exact as if they did not; keys likewise small."""
