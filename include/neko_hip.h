@@ -232,9 +232,10 @@ int neko_hip_qk_norm_rope_paged(neko_hip_ctx* ctx, const void* qkv, int64_t row_
  * Scores are f32: besides its products' roundings s_j is held to 2^-22 |s_j|, and its weight is off by as much. From
  * 2^22 on that tells close scores apart no more, and equal ones weigh alike only under value scales that are alike.
  * Any finite scores give a finite row (one key: its value); scores past f32's range are infinities.
- * Partial results of key splits go to the context's workspace (see neko_hip_matmul): its size goes by rows,
- * n_seq, heads, head size, window and the table's width (max_pages), not by lengths, so one uncaptured call
- * of these makes every later capture fit. */
+ * Partial results of key splits go to the context's workspace (see neko_hip_matmul): its size goes by dtype, rows,
+ * n_seq, heads, head size, window and the table's reach (max_pages * page_size), not by lengths, so one uncaptured
+ * call of these makes every later capture fit; with several sequences up to 8 (hd' + 4) bytes for each row and head,
+ * hd' being hd rounded up to 64, 128 or 256. */
 int neko_hip_attention_paged(neko_hip_ctx* ctx, const void* q, int64_t q_stride, int64_t rows, const neko_paged_kv* kv,
                              const neko_paged_batch* batch, int n_head, float scale, float softcap, int64_t window,
                              const float* slopes, void* out, int64_t out_stride, int dtype);

@@ -17,8 +17,8 @@
 // to [2^14, 2^15) first; l and O are f32.
 //
 // What bounds it: with many keys the reading of them, two sequences of 65521 tokens (32 / 8 heads of 128, f16) in 51 us,
-// 5.2 TB/s of codes, and 5 for the merge; with fewer, launches and loads that wait for each other (32 ragged ones of up to
-// 4096 tokens 17.8 us, one of 777 10.9).
+// 5.3 TB/s of codes, and 5 for the merge; with fewer, launches and loads that wait for each other (32 ragged ones of up to
+// 4096 tokens 18.1 us, one of 777 11.0).
 #include <algorithm>
 #include <atomic>
 

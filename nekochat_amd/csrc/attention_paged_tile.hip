@@ -8,7 +8,7 @@
 // O^T = V^T P^T; V^T comes from LDS by transposing reads. Eight consecutive scores of a lane are of one 16-key block,
 // hence of one page: its scales are the same for all lanes.
 //
-// What bounds it: issue. 8192 tokens of 32 / 8 heads of 128 in f16 take 597 us, 921 TFLOP/s, with the matrix units busy
+// What bounds it: issue. 8192 tokens of 32 / 8 heads of 128 in f16 take 605 us, 908 TFLOP/s, with the matrix units busy
 // 43% and the vector units 61% of the cycles; two workgroups to a CU, so that one's vector work runs beside the
 // other's products.
 //
