@@ -240,6 +240,87 @@ int neko_hip_attention_paged(neko_hip_ctx* ctx, const void* q, int64_t q_stride,
                              const neko_paged_batch* batch, int n_head, float scale, float softcap, int64_t window,
                              const float* slopes, void* out, int64_t out_stride, int dtype);
 
+/* ---------------------------------------------------------------- drafted trees
+ * Speculative decoding over the paged cache: a drafter proposes a tree of tokens for each sequence, one call of the
+ * model looks at all of them, and those that it would have sampled itself stay. No counterpart in the reference. A step:
+ * neko_hip_qk_norm_rope_tree_paged and neko_hip_attention_tree_paged in each layer, neko_hip_sample over the rows' logits,
+ * neko_hip_accept_tree, and neko_hip_keep_paged in each layer; the next step's lengths are accept's new_len and its rows.
+ *
+ * A sequence's rows of the batch are its tree: row i < n (n up to 1024) has slot base + i of the sequence, base =
+ * kv_len - n being the tokens before the tree (kv_len counts the whole tree, as in every paged batch), and stands at place
+ * base + depth[i] of the text. Row 0 is the root, the last token that was decided; parents stand before their children.
+ * A row whose depth is outside [0, n) is padding (trees of a fixed size under graph capture): it is not appended, sees
+ * nothing, and is nobody's to see. So is every row of a sequence whose kv_len is below n. */
+
+/* depth and mask of trees given by parents (host memory): row i of a sequence has parents[row] in [0, i), or -1 (a child
+ * of the tokens before the tree, depth 0: the root), or anything else: padding, and all rows below it. mask rows of
+ * `words` words hold a bit for each row of the same tree: the row itself and its ancestors. n_seq sequences of rows
+ * row_start[s] .. row_start[s + 1] - 1, up to 32 * words of them. A drafter that grows its trees on the device needs no
+ * more than mask[child] = mask[parent] | bit of the child. */
+int neko_tree_plan(const int32_t* parents, const int32_t* row_start, int64_t n_seq, int words, int32_t* depth, uint32_t* mask);
+
+/* neko_hip_qk_norm_rope_paged for drafted rows: row i goes to slot base + i and is rotated by the angles of place base +
+ * depth[i]; depth int32 [rows]. Rows that are padding, or at places from n_pos on, are left alone, their slots too; a page
+ * that gets no row keeps its scale. */
+int neko_hip_qk_norm_rope_tree_paged(neko_hip_ctx* ctx, const void* qkv, int64_t row_stride, int64_t rows, int n_q,
+                                     const neko_paged_kv* kv, const neko_paged_batch* batch, const int32_t* depth,
+                                     const float* wqk, const float* cs, int64_t n_pos, int rot_dim, int interleaved,
+                                     float eps, void* q_out, int64_t q_out_stride, int dtype);
+
+typedef struct neko_paged_tree {
+    const int32_t* depth;  /* [rows] */
+    const uint32_t* mask;  /* rows of `words` words (1..32), mask_stride words apart: bit k, row k of the sequence's tree */
+    int64_t mask_stride;
+    int words;
+} neko_paged_tree;
+
+/* neko_hip_attention_paged for drafted rows: a row sees the tokens before its tree and, of the tree, the rows whose bit is
+ * set in its mask (its own too only if it is; bits past the sequence's rows are ignored; those of padding must be clear).
+ * Distances, for the window and the slopes, are between places: base + depth of drafted tokens. Everything else -- types,
+ * precision, infinities and NaN, workspace, capture -- as there. */
+int neko_hip_attention_tree_paged(neko_hip_ctx* ctx, const void* q, int64_t q_stride, int64_t rows, const neko_paged_kv* kv,
+                                  const neko_paged_batch* batch, const neko_paged_tree* tree, int n_head, float scale,
+                                  float softcap, int64_t window, const float* slopes, void* out, int64_t out_stride, int dtype);
+
+/* The path that sampled tokens take through each tree: from the root on, to the first child (the lowest row with that
+ * parent) that holds the token sampled at the row before, while there is one. tokens, sampled, parents int32 [rows], as
+ * in neko_tree_plan (negative samples agree with nothing). Written for each sequence: path int32 [n_seq][max_path], the
+ * rows of the path within the tree, then -1; count, its rows (0 where the sequence has none; at most max_path); next, the
+ * token sampled at its last row (-1 if none); new_len = kv_len - n + count. The outputs overlap nothing. */
+int neko_hip_accept_tree(neko_hip_ctx* ctx, const int32_t* tokens, const int32_t* sampled, const int32_t* parents, int64_t rows,
+                         const int32_t* row_start, const int32_t* kv_len, int64_t n_seq, int32_t* path, int64_t max_path,
+                         int32_t* count, int32_t* next, int32_t* new_len);
+
+/* The cached tokens of a path moved together, so that the sequence goes on behind them: the value in slot base + path[k]
+ * to slot base + k, for k < count (rows path_stride entries apart; batch as of the append, kv_len with the whole tree).
+ * Paths increase (accept_tree's do); entries that do not stand behind their own slot or past the tree are not moved. The
+ * values are stored as neko_hip_qk_norm_rope_paged would store them: a page's scale is the smallest power of two for the
+ * tokens moved into it, at least the one it has where earlier tokens stay before them, which are rounded again where it
+ * grows. Slots past the path may hold anything afterwards. */
+int neko_hip_keep_paged(neko_hip_ctx* ctx, const neko_paged_kv* kv, const neko_paged_batch* batch, const int32_t* path,
+                        int64_t path_stride, int64_t max_path, const int32_t* count);
+
+/* ---------------------------------------------------------------- sampling */
+
+/* A token of each row of logits, from a uniform number of the row's own. No counterpart in the reference. With w_i =
+ * exp((l_i - max l) / temperature) over the vocabulary:
+ *   top_k   the top_k largest logits stay, of equal ones the lower index first;
+ *   top_p   of those, in that order, the shortest prefix whose sum of w is at least top_p times their sum (at least one);
+ *   min_p   of those, the ones with w >= min_p (above 1: 1);
+ * and the token is the first, by index, at which the running sum of w over what stays exceeds u times the whole sum.
+ *   temperature, top_p, min_p f32 [rows], top_k int32 [rows], device memory; each may be NULL: 1, and no such cut. A
+ *             temperature that is not above 0 (NaN included) takes the largest logit, the lowest index of equal ones; a
+ *             top_k not above 0, a top_p from 1 on or NaN and a min_p not above 0 or NaN cut nothing.
+ *   u         f32 [rows] in [0, 1) (brought into it otherwise; NaN: 0).
+ *   tokens    int32 [rows]; -1 where every logit is -inf or NaN. Such logits are never chosen; where the largest is +inf,
+ *             only those that are.
+ * Weights and their sums are held in 64 bits: the token is that of an evaluation in 64 bits unless u * sum or a cut lies
+ * within about 2^-40 of a border; the same inputs give the same token in every batch. rows up to 2^20, vocab up to 2^24.
+ * Partial results go to the context's workspace (see neko_hip_matmul): up to 150 KB for a row, less for each of many. */
+int neko_hip_sample(neko_hip_ctx* ctx, const void* logits, int64_t stride, int64_t rows, int64_t vocab,
+                    const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, const float* u,
+                    int32_t* tokens, int dtype);
+
 /* ---------------------------------------------------------------- residual */
 
 /* Residual add + RMSNorm: x[t] = x[t] + delta[t] (float add, rounded once to the activation type,

@@ -42,8 +42,15 @@ class PagedBatch(ctypes.Structure):
                 ("n_seq", _i64)]
 
 
+class PagedTree(ctypes.Structure):
+    """neko_paged_tree."""
+
+    _fields_ = [("depth", _p), ("mask", _p), ("mask_stride", _i64), ("words", _i32)]
+
+
 _kv = ctypes.POINTER(PagedKv)
 _batch = ctypes.POINTER(PagedBatch)
+_tree = ctypes.POINTER(PagedTree)
 
 # name -> (restype, argtypes); the order of include/neko_hip.h.
 SIGNATURES = {
@@ -71,6 +78,13 @@ SIGNATURES = {
     "neko_hip_qk_norm_rope_paged": (_i32, [_p, _p, _i64, _i64, _i32, _kv, _batch, _p, _p, _i64, _i32, _i32, _f32, _p, _i64,
                                            _i32]),
     "neko_hip_attention_paged": (_i32, [_p, _p, _i64, _i64, _kv, _batch, _i32, _f32, _f32, _i64, _p, _p, _i64, _i32]),
+    "neko_tree_plan": (_i32, [_p, _p, _i64, _i32, _p, _p]),
+    "neko_hip_qk_norm_rope_tree_paged": (_i32, [_p, _p, _i64, _i64, _i32, _kv, _batch, _p, _p, _p, _i64, _i32, _i32, _f32, _p,
+                                                _i64, _i32]),
+    "neko_hip_attention_tree_paged": (_i32, [_p, _p, _i64, _i64, _kv, _batch, _tree, _i32, _f32, _f32, _i64, _p, _p, _i64, _i32]),
+    "neko_hip_accept_tree": (_i32, [_p, _p, _p, _p, _i64, _p, _p, _i64, _p, _i64, _p, _p, _p]),
+    "neko_hip_keep_paged": (_i32, [_p, _kv, _batch, _p, _i64, _i64, _p]),
+    "neko_hip_sample": (_i32, [_p, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _i32]),
     "neko_hip_add_rmsnorm": (_i32, [_p, _p, _i64, _p, _i64, _p, _i64, _p, _i64, _i64, _f32, _i32]),
     "neko_hip_matmul": (_i32, [_p, _p, _i64, _i64, _i64, _p, _i64, _i32, _i64, _p, _p, _i64, _i32, _i32, _i32]),
     "neko_hip_set_matmul_library": (_i32, [_p, _i32]),

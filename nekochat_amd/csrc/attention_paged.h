@@ -19,10 +19,23 @@ struct PagedAttnArgs {
     float scale;     // of the scores; its sign goes into q
     float softcap;   // 0: none
     const float* slopes;
+    // Drafted trees (words 0: none): a row's depth in its tree, and a bit for each row of the tree that it sees.
+    const int32_t* depth;
+    const uint32_t* mask;
+    int64_t mask_stride;
+    int32_t words;
+    int32_t tree_rows;  // of a tree, at most
     float* part;  // [blocks][tile_rows][head size of the kernel] accumulators of split items
     float* ml;    // [blocks][tile_rows][4]: their maximum, sum, whether any key was seen
     uint32_t blocks;  // that part and ml hold
 };
+
+// The tiling's derived fields. A tile of a tree's rows may see all of its tokens besides its window.
+inline void attn_form(PagedAttnArgs& a) {
+    attn_set(a.t);
+    const int64_t span = static_cast<int64_t>(a.t.span) + a.tree_rows;
+    a.t.span = span < (1 << 30) ? static_cast<int32_t>(span) : 1 << 30;
+}
 
 constexpr float kAttnLog2e = 1.44269504088896341f;
 constexpr int kPOffset = 15;  // weights go to f16 times 2^kPOffset, the largest power that it holds
@@ -151,6 +164,16 @@ struct TileKeys {
     int32_t k0, k1;  // this split's, k0 a multiple of 32
 };
 __device__ __forceinline__ int32_t key_lo(int32_t pos, int32_t window) { return window > 0 && pos >= window ? pos - window + 1 : 0; }
+// This split's part of the keys that a tile's rows see.
+__device__ __forceinline__ void split_keys(const PagedAttnArgs& a, const AttnItem& it, TileKeys& k) {
+    k.k0 = k.lo_min & ~31;
+    k.k1 = k.hi_max;
+    if (it.splits > 1) {
+        const int64_t per = static_cast<int64_t>(it.chunk) << a.t.unit_log2, from = k.k0 + it.split * per;
+        k.k0 = static_cast<int32_t>(from < (1 << 30) ? from : 1 << 30);
+        if (from + per < k.k1) k.k1 = static_cast<int32_t>(from + per);
+    }
+}
 __device__ __forceinline__ TileKeys tile_keys(const PagedAttnArgs& a, const SeqRows& r, const AttnItem& it) {
     const int32_t n_rows = r.n * a.t.group, row0 = it.tile << a.t.tile_log2;
     const int32_t row1 = min(row0 + (1 << a.t.tile_log2), n_rows) - 1;
@@ -162,14 +185,59 @@ __device__ __forceinline__ TileKeys tile_keys(const PagedAttnArgs& a, const SeqR
     k.lo_max = key_lo(last, a.t.window);
     k.hi_min = min(first + 1, reach);
     k.hi_max = min(last + 1, reach);
-    k.k0 = k.lo_min & ~31;
-    k.k1 = k.hi_max;
-    if (it.splits > 1) {
-        const int64_t per = static_cast<int64_t>(it.chunk) << a.t.unit_log2, from = k.k0 + it.split * per;
-        k.k0 = static_cast<int32_t>(from < (1 << 30) ? from : 1 << 30);
-        if (from + per < k.k1) k.k1 = static_cast<int32_t>(from + per);
-    }
+    split_keys(a, it, k);
     return k;
+}
+
+// ---- drafted trees. Row i of a sequence's n, at depth d_i, stands at place base + d_i of the text, base = len - n being
+// the tokens before the tree; it sees of those what its window allows and, of the tree, the slots base + k whose bit k is
+// set in its row of the mask (places base + d_k).
+
+// The keys that the tree's rows see: all of them, up to what the mask has bits for.
+__device__ __forceinline__ int32_t tree_reach(const PagedAttnArgs& a, const SeqRows& r) {
+    const int32_t base = r.len - r.n;
+    if (base < 0) return 0;
+    return min(min(r.len, paged_reach(a.p)), base + min(r.n, 32 * a.words));
+}
+__device__ __forceinline__ TileKeys tree_tile_keys(const PagedAttnArgs& a, const SeqRows& r, const AttnItem& it) {
+    const int32_t base = max(r.len - r.n, 0), reach = tree_reach(a, r);
+    TileKeys k;
+    k.lo_min = key_lo(base, a.t.window);
+    k.lo_max = key_lo(base + r.n, a.t.window);
+    k.hi_min = min(base, reach);
+    k.hi_max = reach;
+    split_keys(a, it, k);
+    return k;
+}
+// The depth of a row, -1 where it sees nothing.
+__device__ __forceinline__ int32_t tree_depth(const PagedAttnArgs& a, const SeqRows& r, int32_t tok) {
+    const int32_t d = a.depth[r.begin + tok];
+    return r.len < r.n || d < 0 || d >= r.n ? -1 : d;
+}
+// Which of the keys j0 .. j0 + 31 the row `tok` at depth d sees, a bit each, pages aside. lo, hi: of the keys before the tree.
+__device__ __forceinline__ uint32_t tree_sees(const PagedAttnArgs& a, const SeqRows& r, int32_t tok, int32_t d, int32_t lo, int32_t hi, int32_t j0) {
+    auto below = [](int32_t n) { return n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u; };  // the first n
+    uint32_t sees = below(hi - j0) & ~below(lo - j0);
+    const int32_t base = r.len - r.n, k0 = j0 - base;  // the first key's row of the tree
+    if (k0 > -32 && k0 < 32 * a.words) {
+        const uint32_t* m = a.mask + static_cast<int64_t>(r.begin + tok) * a.mask_stride;
+        const int32_t w = k0 >> 5, by = k0 & 31;
+        const uint32_t m0 = w >= 0 ? m[w] : 0u, m1 = w + 1 < a.words ? m[w + 1] : 0u;
+        uint32_t bits = (m0 >> by | (by ? m1 << (32 - by) : 0u)) & below(tree_reach(a, r) - j0);
+        if (a.t.window > 0 && d >= a.t.window) {  // a window that ends inside the tree
+            for (uint32_t left = bits; left; left &= left - 1) {
+                const int32_t k = __builtin_ctz(left);
+                if (a.depth[r.begin + k0 + k] <= d - a.t.window) bits &= ~(1u << k);
+            }
+        }
+        sees |= bits;
+    }
+    return d < 0 ? 0u : sees;
+}
+// The place in the text of key j, which holds a token.
+__device__ __forceinline__ int32_t tree_key_place(const PagedAttnArgs& a, const SeqRows& r, int32_t j) {
+    const int32_t base = r.len - r.n, k = j - base;
+    return k < 0 || k >= r.n ? j : base + a.depth[r.begin + k];
 }
 
 // cap * tanh(s / cap) to a few roundings of the value: Lambert's continued fraction for tanh, cut after its fifth
@@ -227,6 +295,6 @@ __device__ __forceinline__ float row_factor(float l, bool seen) {
 // The kernel for many rows per sequence (attention_paged_tile.hip): its tiling, into a.t, and its launch of a.blocks
 // workgroups.
 void attn_paged_tile_form(const neko_hip_ctx* ctx, PagedAttnArgs& a);
-int attn_paged_tile(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a, int dtype);
+int attn_paged_tile(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a, int dtype);  // (of drafted trees where a.words > 0)
 
 }  // namespace neko_hip

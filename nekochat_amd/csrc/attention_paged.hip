@@ -66,7 +66,8 @@ __device__ __forceinline__ void store_row(const PagedAttnArgs& a, const SeqRows&
     __builtin_memcpy(static_cast<TQ*>(a.out) + static_cast<int64_t>(r.begin + tok) * a.os + static_cast<int64_t>(head) * a.p.hd + d, v, sizeof(v));
 }
 
-template <typename TQ, int DH, int NW, bool MODS>
+// TREE: rows of drafted trees (attention_paged.h).
+template <typename TQ, int DH, int NW, bool MODS, bool TREE>
 __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kResident<TQ, DH>)) void attn_paged_kernel(PagedAttnArgs a) {
     constexpr bool kTwo = sizeof(TQ) == 4;
     constexpr int NU = DH / 64, NE = DH / 16, VW = DH / 64;
@@ -87,7 +88,7 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
         const bool found = attn_find<false>(a.p, a.t, item, &f);
         if (found) {
             const SeqRows r = paged_seq(a.p, f.s);
-            const TileKeys k = tile_keys(a, r, f);
+            const TileKeys k = TREE ? tree_tile_keys(a, r, f) : tile_keys(a, r, f);
             if (lane == 0) {
                 const int32_t x[14] = {f.s,      f.tile,   f.splits, static_cast<int32_t>(f.block), r.begin, r.n, r.len, k.lo_min,
                                        k.lo_max, k.hi_min, k.hi_max, k.k0, k.k1, 1};
@@ -115,8 +116,9 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
     const int32_t row = min((it.tile << 4) + c, n_rows - 1);
     const int32_t tok = static_cast<int32_t>(fast_div(static_cast<uint32_t>(row), a.by_group));
     const int head = kvh * a.t.group + (row - tok * a.t.group);
-    const int32_t pos = r.len - r.n + tok;
-    const int32_t hi = min(pos + 1, min(r.len, paged_reach(a.p))), lo = key_lo(pos, a.t.window);
+    const int32_t depth = TREE ? tree_depth(a, r, tok) : tok;
+    const int32_t pos = r.len - r.n + depth;
+    const int32_t hi = TREE ? tk.hi_min : min(pos + 1, min(r.len, paged_reach(a.p))), lo = key_lo(pos, a.t.window);
 
     // q as the B operands of the first product, the same for all waves, by one of them: in LDS, so that each
     // wave's registers have room for other things (168 of them at three waves per SIMD). f32 rows are brought to
@@ -289,19 +291,25 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
                     for (int i = 0; i < 4; i++) s[b][i] = cap_score(s[b][i], a.softcap, inv_cap);
             }
             if (a.slopes) {
+                const bool in_tree = TREE && j0 + 32 > tk.hi_min;
 #pragma unroll
                 for (int b = 0; b < 2; b++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        s[b][i] = __builtin_fmaf(slope, static_cast<float>(j0 + 16 * b + 4 * g4 + i - pos), s[b][i]);
+                    for (int i = 0; i < 4; i++) {
+                        int32_t j = j0 + 16 * b + 4 * g4 + i;
+                        if (in_tree) j = tree_key_place(a, r, j);
+                        s[b][i] = __builtin_fmaf(slope, static_cast<float>(j - pos), s[b][i]);
+                    }
             }
             f[0] = f[1] = kAttnLog2e;
         }
         // Keys that some row of the tile does not see.
         const bool partial = j0 < tk.lo_max || j0 + 32 > tk.hi_min || !ok[0] || !ok[1];
         bool any_visible = true;
+        uint32_t sees = 0;  // (TREE) the tile's keys that the row sees
         if (partial) {
             any_visible = false;
+            if constexpr (TREE) sees = tree_sees(a, r, tok, depth, lo, hi, j0) & ((ok[0] ? 0xffffu : 0u) | (ok[1] ? 0xffff0000u : 0u));
             // Visible: lo <= j < hi, as one unsigned comparison; no key of a block without a page. Likewise what any row sees.
             const uint32_t many = hi > lo ? static_cast<uint32_t>(hi - lo) : 0u;
             const uint32_t many_any = tk.hi_max > tk.lo_min ? static_cast<uint32_t>(tk.hi_max - tk.lo_min) : 0u;
@@ -310,7 +318,7 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int32_t j = j0 + 16 * b + 4 * g4 + i;
-                    const bool vis = static_cast<uint32_t>(j - lo) < (ok[b] ? many : 0u);
+                    const bool vis = TREE ? (sees >> (16 * b + 4 * g4 + i) & 1u) != 0 : static_cast<uint32_t>(j - lo) < (ok[b] ? many : 0u);
                     s[b][i] = vis ? s[b][i] : -__builtin_inff();
                     any_visible |= vis;
                     // What no row sees may be anything, codes of no token included.
@@ -367,7 +375,7 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
         // rows that do see them.
         uint16_t* nan_at = reinterpret_cast<uint16_t*>(o_sh + wave * kTileRows * kRow);  // [32 keys][16]
         bool mend = false;
-        if (partial && (tk.hi_min != tk.hi_max || tk.lo_min != tk.lo_max)) {
+        if (partial && (TREE || tk.hi_min != tk.hi_max || tk.lo_min != tk.lo_max)) {
             uint32_t any = 0;
 #pragma unroll
             for (int b = 0; b < 2; b++)
@@ -405,7 +413,7 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
         if (mend) {
 #pragma unroll 1
             for (int k = 0; k < 32; k++) {
-                if (j0 + k < lo || j0 + k >= hi) continue;  // (a block without a page has no NaN left)
+                if (TREE ? (sees >> k & 1u) == 0 : j0 + k < lo || j0 + k >= hi) continue;  // (a block without a page has no NaN left)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const uint32_t at = nan_at[k * 16 + 4 * g4 + i];
@@ -434,6 +442,11 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
         t = next;
     }
 
+    if (TREE && depth < 0) {  // (tiles that all others see whole are not masked for a row that sees nothing)
+        m = -__builtin_inff();
+        l = 0.0f;
+        seen = false;
+    }
     // The waves' results meet in LDS.
     l = swap32_sum(swap16_sum(l));
     const float any_seen = swap32_max(swap16_max(seen ? 1.0f : 0.0f));
@@ -548,16 +561,16 @@ void few_form(const neko_hip_ctx* ctx, PagedAttnArgs& a, int waves, int resident
     a.t.unit_log2 = 5 + __builtin_ctz(static_cast<unsigned>(waves));
     a.t.least = paged_reach(a.p) <= (kLeast << a.t.unit_log2) ? kLeast : kLeast / 2;
     a.t.target = resident * ctx->cu_count;
-    attn_set(a.t);
+    attn_form(a);
 }
 
-template <typename TQ, int DH, int NW, bool MODS>
+template <typename TQ, int DH, int NW, bool MODS, bool TREE>
 int launch_few(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a) {
     static std::atomic<uint64_t> allowed{0};
     constexpr size_t lds = NW * kTileRows * (DH + 4) * sizeof(float);
     if (lds + 4096 > 64 * 1024)
-        if (int rc = allow_lds(ctx, reinterpret_cast<const void*>(&attn_paged_kernel<TQ, DH, NW, MODS>), lds, allowed)) return rc;
-    hipLaunchKernelGGL((attn_paged_kernel<TQ, DH, NW, MODS>), dim3(a.blocks), dim3(64 * NW), lds, ctx->stream, a);
+        if (int rc = allow_lds(ctx, reinterpret_cast<const void*>(&attn_paged_kernel<TQ, DH, NW, MODS, TREE>), lds, allowed)) return rc;
+    hipLaunchKernelGGL((attn_paged_kernel<TQ, DH, NW, MODS, TREE>), dim3(a.blocks), dim3(64 * NW), lds, ctx->stream, a);
     return after_launch(ctx, what);
 }
 
@@ -609,8 +622,12 @@ int launch_dims(neko_hip_ctx* ctx, const char* what, PagedAttnArgs a, int dtype)
     if (few) {
         place(f, fg, ws);
         int rc;
-        if (wide) rc = mods ? launch_few<TQ, DH, kMostWaves, true>(ctx, what, f) : launch_few<TQ, DH, kMostWaves, false>(ctx, what, f);
-        else rc = mods ? launch_few<TQ, DH, 4, true>(ctx, what, f) : launch_few<TQ, DH, 4, false>(ctx, what, f);
+        auto by_form = [&](auto tree) {
+            constexpr bool TREE = decltype(tree)::value;
+            if (wide) return mods ? launch_few<TQ, DH, kMostWaves, true, TREE>(ctx, what, f) : launch_few<TQ, DH, kMostWaves, false, TREE>(ctx, what, f);
+            return mods ? launch_few<TQ, DH, 4, true, TREE>(ctx, what, f) : launch_few<TQ, DH, 4, false, TREE>(ctx, what, f);
+        };
+        rc = a.words > 0 ? by_form(std::true_type{}) : by_form(std::false_type{});
         if (rc) return rc;
         if (int rc2 = merge(f)) return rc2;
     }
@@ -629,12 +646,10 @@ int launch_typed(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a, in
 
 using namespace neko_hip;
 
-extern "C" int neko_hip_attention_paged(neko_hip_ctx* ctx, const void* q, int64_t q_stride, int64_t rows,
-                                        const neko_paged_kv* kv, const neko_paged_batch* batch, int n_head, float scale,
-                                        float softcap, int64_t window, const float* slopes, void* out, int64_t out_stride,
-                                        int dtype) {
-    const char* what = "neko_hip_attention_paged";
-    NEKO_ENTER(ctx);
+// `tree`: null for rows in a line.
+static int attention(neko_hip_ctx* ctx, const char* what, const void* q, int64_t q_stride, int64_t rows, const neko_paged_kv* kv,
+                     const neko_paged_batch* batch, const neko_paged_tree* tree, int n_head, float scale, float softcap,
+                     int64_t window, const float* slopes, void* out, int64_t out_stride, int dtype) {
     NEKO_REQUIRE(ctx, valid_dtype(dtype), "%s: bad dtype %d", what, dtype);
     NEKO_REQUIRE(ctx, rows >= 0, "%s: rows=%lld", what, (long long)rows);
     PagedAttnArgs a{};
@@ -644,6 +659,8 @@ extern "C" int neko_hip_attention_paged(neko_hip_ctx* ctx, const void* q, int64_
     NEKO_REQUIRE(ctx, std::isfinite(scale) && std::isfinite(softcap) && softcap >= 0.0f && window >= 0,
                  "%s: scale=%g softcap=%g window=%lld (finite, the latter two not negative)", what, scale, softcap, (long long)window);
     NEKO_REQUIRE(ctx, rows * n_head <= 0x3fffffff, "%s: too many rows x heads", what);
+    NEKO_REQUIRE(ctx, !tree || (tree->words > 0 && tree->words <= 32 && tree->mask_stride >= tree->words && tree->mask_stride <= (int64_t(1) << 32)),
+                 "%s: masks of %d words (1..32), row stride %lld", what, tree->words, (long long)tree->mask_stride);
     if (rows == 0) return NEKO_OK;
     NEKO_REQUIRE(ctx, q && out, "%s: null pointer", what);
     const int64_t width = static_cast<int64_t>(n_head) * kv->hd;
@@ -654,6 +671,17 @@ extern "C" int neko_hip_attention_paged(neko_hip_ctx* ctx, const void* q, int64_
     const size_t sq = rows_span(rows, width, q_stride, esz), so = rows_span(rows, width, out_stride, esz);
     NEKO_REQUIRE(ctx, sq != 0 && so != 0, "%s: q / out rows span more than 2^62 bytes", what);
     NEKO_REQUIRE(ctx, !overlaps(out, so, q, sq) && !paged_overlaps(*kv, out, so), "%s: out may not overlap q or the cache", what);
+    if (tree) {
+        NEKO_REQUIRE(ctx, tree->depth && tree->mask && aligned(tree->depth, 4) && aligned(tree->mask, 4), "%s: null or misaligned depth or mask", what);
+        const size_t sm = rows_span(rows, tree->words, tree->mask_stride, 4), sd = static_cast<size_t>(rows) * 4;
+        NEKO_REQUIRE(ctx, sm != 0 && !overlaps(out, so, tree->mask, sm) && !overlaps(out, so, tree->depth, sd),
+                     "%s: out may not overlap depth or mask", what);
+        a.depth = tree->depth;
+        a.mask = tree->mask;
+        a.mask_stride = tree->mask_stride;
+        a.words = tree->words;
+        a.tree_rows = static_cast<int32_t>(std::min<int64_t>(rows, 32 * static_cast<int64_t>(tree->words)));
+    }
     a.q = q;
     a.qs = q_stride;
     a.out = out;
@@ -667,4 +695,23 @@ extern "C" int neko_hip_attention_paged(neko_hip_ctx* ctx, const void* q, int64_
     a.softcap = softcap;
     a.slopes = slopes;
     return dtype == NEKO_DT_F16 ? launch_typed<half_t>(ctx, what, a, dtype) : launch_typed<float>(ctx, what, a, dtype);
+}
+
+extern "C" int neko_hip_attention_paged(neko_hip_ctx* ctx, const void* q, int64_t q_stride, int64_t rows,
+                                        const neko_paged_kv* kv, const neko_paged_batch* batch, int n_head, float scale,
+                                        float softcap, int64_t window, const float* slopes, void* out, int64_t out_stride,
+                                        int dtype) {
+    NEKO_ENTER(ctx);
+    return attention(ctx, "neko_hip_attention_paged", q, q_stride, rows, kv, batch, nullptr, n_head, scale, softcap, window, slopes,
+                     out, out_stride, dtype);
+}
+
+extern "C" int neko_hip_attention_tree_paged(neko_hip_ctx* ctx, const void* q, int64_t q_stride, int64_t rows,
+                                             const neko_paged_kv* kv, const neko_paged_batch* batch, const neko_paged_tree* tree,
+                                             int n_head, float scale, float softcap, int64_t window, const float* slopes,
+                                             void* out, int64_t out_stride, int dtype) {
+    const char* what = "neko_hip_attention_tree_paged";
+    NEKO_ENTER(ctx);
+    NEKO_REQUIRE(ctx, tree, "%s: null tree", what);
+    return attention(ctx, what, q, q_stride, rows, kv, batch, tree, n_head, scale, softcap, window, slopes, out, out_stride, dtype);
 }

@@ -71,7 +71,8 @@ __device__ __forceinline__ int block_ve(int x) { return ((x >> 8) & 255) - 128; 
 
 // (f16 rows of 64 dimensions: three workgroups to a CU, at which four registers are spilled with a cap; 4 prompts of 2048
 // tokens, 12 heads, 151 us, at two 175)
-template <typename TQ, int DH, bool MODS>
+// TREE: rows of drafted trees (attention_paged.h).
+template <typename TQ, int DH, bool MODS, bool TREE>
 __global__ __launch_bounds__(256, DH <= 64 && sizeof(TQ) == 2 ? 3 : DH <= 128 ? 2 : 1) void attn_paged_tile_kernel(PagedAttnArgs a) {
     typedef TileForm<TQ, DH> C;
     constexpr bool kTwo = sizeof(TQ) == 4;
@@ -88,7 +89,7 @@ __global__ __launch_bounds__(256, DH <= 64 && sizeof(TQ) == 2 ? 3 : DH <= 128 ? 
     AttnItem it;
     if (!attn_find<false>(a.p, a.t, item, &it)) return;
     const SeqRows r = paged_seq(a.p, it.s);
-    const TileKeys tk = tile_keys(a, r, it);
+    const TileKeys tk = TREE ? tree_tile_keys(a, r, it) : tile_keys(a, r, it);
     const int hd = a.p.hd;
     const int32_t reach = min(r.len, paged_reach(a.p));
 
@@ -97,12 +98,13 @@ __global__ __launch_bounds__(256, DH <= 64 && sizeof(TQ) == 2 ? 3 : DH <= 128 ? 
     const int32_t row = min(row0 + l32, n_rows - 1);
     const int32_t tok = static_cast<int32_t>(fast_div(static_cast<uint32_t>(row), a.by_group));
     const int head = kvh * a.t.group + (row - tok * a.t.group);
-    const int32_t pos = r.len - r.n + tok;
-    const int32_t hi = min(pos + 1, reach), lo = key_lo(pos, a.t.window);
+    const int32_t depth = TREE ? tree_depth(a, r, tok) : tok;
+    const int32_t pos = r.len - r.n + depth;
+    const int32_t hi = TREE ? tk.hi_min : min(pos + 1, reach), lo = key_lo(pos, a.t.window);
     const int32_t w_first = r.len - r.n + static_cast<int32_t>(fast_div(static_cast<uint32_t>(min(row0, n_rows - 1)), a.by_group));
     const int32_t w_last = r.len - r.n + static_cast<int32_t>(fast_div(static_cast<uint32_t>(min(row0 + 31, n_rows - 1)), a.by_group));
-    const int32_t w_lo_min = key_lo(w_first, a.t.window), w_lo_max = key_lo(w_last, a.t.window);
-    const int32_t w_hi_min = min(w_first + 1, reach), w_hi_max = min(w_last + 1, reach);
+    const int32_t w_lo_min = TREE ? tk.lo_min : key_lo(w_first, a.t.window), w_lo_max = TREE ? tk.lo_max : key_lo(w_last, a.t.window);
+    const int32_t w_hi_min = TREE ? tk.hi_min : min(w_first + 1, reach), w_hi_max = TREE ? tk.hi_max : min(w_last + 1, reach);
 
     // q: dimensions 16 s + 8 h .. + 7 of the row as the B operand of step s.
     half8 qh[NS], ql[kTwo ? NS : 1];
@@ -360,11 +362,14 @@ __global__ __launch_bounds__(256, DH <= 64 && sizeof(TQ) == 2 ? 3 : DH <= 128 ? 
             }
             if (a.slopes) {
                 const int32_t away = j0 + 4 * h - pos;
+                const bool in_tree = TREE && j0 + C::keys > tk.hi_min;
 #pragma unroll
                 for (int b = 0; b < KB; b++)
                     unrolled<16>([&](auto ec) {
                         constexpr int e = decltype(ec)::value;
-                        s[b][e] = __builtin_fmaf(slope, static_cast<float>(away + 32 * b + 8 * (e >> 2) + (e & 3)), s[b][e]);
+                        int32_t by = away + 32 * b + 8 * (e >> 2) + (e & 3);
+                        if (in_tree) by = tree_key_place(a, r, by + pos) - pos;
+                        s[b][e] = __builtin_fmaf(slope, static_cast<float>(by), s[b][e]);
                     });
             }
 #pragma unroll
@@ -378,6 +383,17 @@ __global__ __launch_bounds__(256, DH <= 64 && sizeof(TQ) == 2 ? 3 : DH <= 128 ? 
             for (int b = 0; b < KB; b++)
                 unrolled<2>([&](auto ic) {
                     constexpr int i = decltype(ic)::value;
+                    if constexpr (TREE) {
+                        uint32_t sees = tree_sees(a, r, tok, depth, lo, hi, j0 + 32 * b) >> (16 * i) & 0xffffu;
+                        sees = (now_ok >> (at + 2 * b + i)) & 1u ? sees : 0u;
+                        seen |= static_cast<int>(sees != 0);
+                        sees >>= 4 * h;
+                        unrolled<8>([&](auto ec) {
+                            constexpr int e = 8 * i + decltype(ec)::value;
+                            s[b][e] = sees >> (8 * ((e >> 2) & 1) + (e & 3)) & 1u ? s[b][e] : -__builtin_inff();
+                        });
+                        return;
+                    }
                     const uint32_t most = (now_ok >> (at + 2 * b + i)) & 1u ? many : 0u;
                     const int32_t from = j0 + 32 * b + 16 * i;
                     seen |= static_cast<int>(most != 0) & static_cast<int>(max(from, lo) < min(from + 16, hi));
@@ -487,7 +503,7 @@ __global__ __launch_bounds__(256, DH <= 64 && sizeof(TQ) == 2 ? 3 : DH <= 128 ? 
             if (__builtin_amdgcn_readfirstlane(any) != 0) {
 #pragma unroll 1
                 for (int k = 0; k < C::keys; k++) {
-                    if (j0 + k < lo || j0 + k >= hi) continue;
+                    if (TREE ? (tree_sees(a, r, tok, depth, lo, hi, j0 + k) & 1u) == 0 : j0 + k < lo || j0 + k >= hi) continue;
 #pragma unroll
                     for (int d = 0; d < ND; d++) {
                         const uint32_t bits = nan_bits[buf][k][d] >> (4 * h);
@@ -540,6 +556,11 @@ __global__ __launch_bounds__(256, DH <= 64 && sizeof(TQ) == 2 ? 3 : DH <= 128 ? 
         }
     }
 
+    if (TREE && depth < 0) {  // (tiles that all others see whole are not masked for a row that sees nothing)
+        m = -__builtin_inff();
+        l = 0.0f;
+        seen = 0;
+    }
     l = swap32_sum(l);
     const bool any_seen = swap32_max(seen != 0 ? 1.0f : 0.0f) > 0.0f;
     if (row0 + l32 >= n_rows) return;
@@ -574,22 +595,22 @@ __global__ __launch_bounds__(256, DH <= 64 && sizeof(TQ) == 2 ? 3 : DH <= 128 ? 
     if (h == 0) *reinterpret_cast<float4v*>(a.ml + at * 4) = float4v{m, l * l_by, any_seen ? 1.0f : 0.0f, 0.0f};
 }
 
-template <typename TQ, int DH, bool MODS>
+template <typename TQ, int DH, bool MODS, bool TREE>
 int launch_tiles(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a) {
     typedef TileForm<TQ, DH> C;
     static std::atomic<uint64_t> allowed{0};
-    const void* kernel = reinterpret_cast<const void*>(&attn_paged_tile_kernel<TQ, DH, MODS>);
+    const void* kernel = reinterpret_cast<const void*>(&attn_paged_tile_kernel<TQ, DH, MODS, TREE>);
     if (C::lds > 64 * 1024)
         if (int rc = allow_lds(ctx, kernel, C::lds, allowed)) return rc;
-    hipLaunchKernelGGL((attn_paged_tile_kernel<TQ, DH, MODS>), dim3(a.blocks), dim3(64 * C::waves), C::lds, ctx->stream, a);
+    hipLaunchKernelGGL((attn_paged_tile_kernel<TQ, DH, MODS, TREE>), dim3(a.blocks), dim3(64 * C::waves), C::lds, ctx->stream, a);
     return after_launch(ctx, what);
 }
 
-template <typename TQ, bool MODS>
+template <typename TQ, bool MODS, bool TREE>
 int launch_dims(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a) {
-    if (a.p.hd <= 64) return launch_tiles<TQ, 64, MODS>(ctx, what, a);
-    if (a.p.hd <= 128) return launch_tiles<TQ, 128, MODS>(ctx, what, a);
-    return launch_tiles<TQ, 256, MODS>(ctx, what, a);
+    if (a.p.hd <= 64) return launch_tiles<TQ, 64, MODS, TREE>(ctx, what, a);
+    if (a.p.hd <= 128) return launch_tiles<TQ, 128, MODS, TREE>(ctx, what, a);
+    return launch_tiles<TQ, 256, MODS, TREE>(ctx, what, a);
 }
 
 }  // namespace
@@ -599,13 +620,17 @@ void attn_paged_tile_form(const neko_hip_ctx* ctx, PagedAttnArgs& a) {
     a.t.unit_log2 = 6;  // a whole number of tiles of either size
     a.t.target = 2 * ctx->cu_count;
     a.t.least = 1;
-    attn_set(a.t);
+    attn_form(a);
 }
 
 int attn_paged_tile(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a, int dtype) {
     const bool mods = a.softcap > 0.0f || a.slopes;
-    if (dtype == NEKO_DT_F16) return mods ? launch_dims<half_t, true>(ctx, what, a) : launch_dims<half_t, false>(ctx, what, a);
-    return mods ? launch_dims<float, true>(ctx, what, a) : launch_dims<float, false>(ctx, what, a);
+    auto by_form = [&](auto tree) {
+        constexpr bool TREE = decltype(tree)::value;
+        if (dtype == NEKO_DT_F16) return mods ? launch_dims<half_t, true, TREE>(ctx, what, a) : launch_dims<half_t, false, TREE>(ctx, what, a);
+        return mods ? launch_dims<float, true, TREE>(ctx, what, a) : launch_dims<float, false, TREE>(ctx, what, a);
+    };
+    return a.words > 0 ? by_form(std::true_type{}) : by_form(std::false_type{});
 }
 
 }  // namespace neko_hip

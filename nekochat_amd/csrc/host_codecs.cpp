@@ -219,4 +219,29 @@ int neko_rope_table(double theta, int hd, int64_t n_pos, float* cs) {
     return NEKO_OK;
 }
 
+int neko_tree_plan(const int32_t* parents, const int32_t* row_start, int64_t n_seq, int words, int32_t* depth, uint32_t* mask) {
+    if (n_seq < 0 || words <= 0) return NEKO_ERR_INVALID;
+    if (n_seq == 0) return NEKO_OK;
+    if (!row_start || row_start[0] < 0) return NEKO_ERR_INVALID;
+    for (int64_t s = 0; s < n_seq; s++) {
+        const int64_t n = static_cast<int64_t>(row_start[s + 1]) - row_start[s];
+        if (n < 0 || n > 32 * static_cast<int64_t>(words)) return NEKO_ERR_INVALID;
+        if (n > 0 && (!parents || !depth || !mask)) return NEKO_ERR_INVALID;
+    }
+    for (int64_t s = 0; s < n_seq; s++) {
+        const int64_t begin = row_start[s], n = row_start[s + 1] - begin;
+        for (int64_t i = 0; i < n; i++) {
+            const int32_t up = parents[begin + i];
+            uint32_t* row = mask + (begin + i) * words;
+            std::memset(row, 0, sizeof(uint32_t) * static_cast<size_t>(words));
+            int32_t& d = depth[begin + i];
+            d = up == -1 ? 0 : up >= 0 && up < i && depth[begin + up] >= 0 ? depth[begin + up] + 1 : -1;
+            if (d < 0) continue;
+            if (d > 0) std::memcpy(row, mask + (begin + up) * words, sizeof(uint32_t) * static_cast<size_t>(words));
+            row[i / 32] |= uint32_t(1) << (i % 32);
+        }
+    }
+    return NEKO_OK;
+}
+
 }  // extern "C"

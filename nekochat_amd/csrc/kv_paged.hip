@@ -38,6 +38,8 @@ struct AppendArgs {
     const float* wqk;
     const float* cs;
     int32_t n_pos;  // positions from there on are left alone
+    const int32_t* depth;  // drafted trees: row i's place in the text is len - n + depth[i]; null: its position
+    int32_t limit;         // slots from there on are left alone: n_pos, or with a depth none
     int32_t rot;
     int32_t inter;
     int32_t n_q;
@@ -108,9 +110,15 @@ __device__ __forceinline__ void rotate(float* x, const float* cs, bool inter) {
     }
 }
 
+// The place in the text of a row of a drafted tree of sequence r; -1: the row is left alone.
+__device__ __forceinline__ int32_t tree_place(const AppendArgs& a, const SeqRows& r, int32_t row) {
+    const int32_t d = a.depth[row], place = r.len - r.n + d;
+    return r.len < r.n || d < 0 || d >= r.n || place >= a.n_pos ? -1 : place;
+}
+
 // Tokens [a, b) of one page, kv head `g`, of k or v: wave `w` of NW holds slots 16 w .. 16 w + 15.
 template <typename T, int LPR, int NW>
-__device__ __forceinline__ void append_page(const AppendArgs& a, const Segment& seg, int g, bool is_k, int w, uint32_t* sh) {
+__device__ __forceinline__ void append_page(const AppendArgs& a, const SeqRows& r, const Segment& seg, int g, bool is_k, int w, uint32_t* sh) {
     constexpr int RPL = 64 / LPR;                                           // rows of a load
     constexpr int IT = RPL >= kWaveTokens ? 1 : kWaveTokens / RPL;          // loads
     const int lane = static_cast<int>(threadIdx.x) & 63;
@@ -132,6 +140,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, const Segment& 
         const int in_wave = it * RPL + lane / LPR;
         const int slot = w * kWaveTokens + in_wave;
         mine[it] = in_head && in_wave < kWaveTokens && slot >= seg.a && slot < seg.b;
+        if (a.depth) mine[it] = mine[it] && tree_place(a, r, seg.row0 + slot) >= 0;
 #pragma unroll
         for (int i = 0; i < 8; i++) x[it][i] = 0.0f;
         if (mine[it]) {
@@ -148,7 +157,8 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, const Segment& 
             if (d.turns && mine[it]) {
                 float cs[8];
                 const int slot = w * kWaveTokens + it * RPL + lane / LPR;
-                __builtin_memcpy(cs, a.cs + static_cast<int64_t>(seg.pos0 + slot) * a.rot + 8 * sub, 32);
+                const int32_t place = a.depth ? tree_place(a, r, seg.row0 + slot) : seg.pos0 + slot;
+                __builtin_memcpy(cs, a.cs + static_cast<int64_t>(place) * a.rot + 8 * sub, 32);
                 rotate(x[it], cs, inter);
             }
             if constexpr (sizeof(T) == 2) {  // as a row of this type would hold it
@@ -161,6 +171,9 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, const Segment& 
             const uint32_t m = __builtin_bit_cast(uint32_t, x[it][i]) & 0x7fffffffu;
             if (mine[it] && m < 0x7f800000u) top = top > m ? top : m;  // the page's scale is that of its finite values
         }
+        // A page all of whose rows are left alone is told by a maximum of 0; any other is at least 2^-149, which asks for
+        // the same scale.
+        if (a.depth && mine[it]) top = top > 1u ? top : 1u;
     }
     top = wave_max_u32(top);
     float* scale = (is_k ? a.p.ks : a.p.vs) + static_cast<int64_t>(seg.page) * a.p.n_kv + g;
@@ -171,6 +184,7 @@ __device__ __forceinline__ void append_page(const AppendArgs& a, const Segment& 
 #pragma unroll
         for (int i = 0; i < NW; i++) top = top > sh[i] ? top : sh[i];
     }
+    if (a.depth && top == 0) return;
     const int need = need_exp(top);
     const int e = need > had ? need : had;
     uint8_t* page = (is_k ? a.p.k : a.p.v) + static_cast<uint64_t>(seg.page) * a.p.page_bytes + g * a.p.head_bytes;
@@ -234,8 +248,9 @@ __device__ __forceinline__ void append_q(const AppendArgs& a, uint32_t wave) {
     // The sequence of each row: that of the wave's first, then past the sequences that end before it.
     const int32_t s = paged_seq_from(a.p, wave_last(a.p.n_seq, r0, [&](int32_t i) { return clamp_i32(a.p.row_start[i], 0, a.p.rows); }), row);
     const SeqRows r = paged_seq(a.p, s);
-    const int32_t pos = r.len - r.n + (row - r.begin);
-    const bool mine = inside && row >= r.begin && row < r.begin + r.n && pos >= 0 && pos < a.n_pos;
+    const bool of_seq = inside && row >= r.begin && row < r.begin + r.n;
+    const int32_t pos = a.depth ? (of_seq ? tree_place(a, r, row) : -1) : r.len - r.n + (row - r.begin);
+    const bool mine = of_seq && pos >= 0 && pos < a.n_pos;
     float cs[8], wt[8];
     if (mine && d.turns) __builtin_memcpy(cs, a.cs + static_cast<int64_t>(pos) * a.rot + 8 * sub, 32);
     if (a.wqk != nullptr && in_head) {
@@ -291,9 +306,9 @@ __global__ __launch_bounds__(64 * NW * kParts<NW>) void append_kernel(AppendArgs
         s = wave_last(a.p.n_seq, at, [&](int32_t j) { return segment_slot(a.p, j); });
         i = at - segment_slot(a.p, s);
     }
-    const Segment seg = paged_segment(a.p, s, i, a.n_pos);
+    const Segment seg = paged_segment(a.p, s, i, a.limit);
     if (seg.page < 0) return;
-    append_page<T, LPR, NW>(a, seg, g, is_k, w, sh);
+    append_page<T, LPR, NW>(a, paged_seq(a.p, s), seg, g, is_k, w, sh);
 }
 
 template <typename T, int LPR>
@@ -395,11 +410,11 @@ bool paged_overlaps(const neko_paged_kv& kv, const void* p, size_t bytes) {
 
 using namespace neko_hip;
 
-extern "C" int neko_hip_qk_norm_rope_paged(neko_hip_ctx* ctx, const void* qkv, int64_t row_stride, int64_t rows, int n_q,
-                                           const neko_paged_kv* kv, const neko_paged_batch* batch, const float* wqk,
-                                           const float* cs, int64_t n_pos, int rot_dim, int interleaved, float eps,
-                                           void* q_out, int64_t q_out_stride, int dtype) {
-    const char* what = "neko_hip_qk_norm_rope_paged";
+// `tree`: rows at the places of their depths instead of at their positions.
+static int append(neko_hip_ctx* ctx, const char* what, const void* qkv, int64_t row_stride, int64_t rows, int n_q,
+                  const neko_paged_kv* kv, const neko_paged_batch* batch, bool tree, const int32_t* depth, const float* wqk,
+                  const float* cs, int64_t n_pos, int rot_dim, int interleaved, float eps, void* q_out, int64_t q_out_stride,
+                  int dtype) {
     NEKO_ENTER(ctx);
     NEKO_REQUIRE(ctx, valid_dtype(dtype), "%s: bad dtype %d", what, dtype);
     NEKO_REQUIRE(ctx, rows >= 0 && n_q > 0 && n_q <= 65536, "%s: bad shape rows=%lld n_q=%d", what, (long long)rows, n_q);
@@ -409,7 +424,7 @@ extern "C" int neko_hip_qk_norm_rope_paged(neko_hip_ctx* ctx, const void* qkv, i
                  what, rot_dim, kv->hd);
     NEKO_REQUIRE(ctx, rot_dim == 0 || (cs && n_pos >= 0), "%s: a rotation needs a cos/sin table", what);
     if (rows == 0 || (rot_dim > 0 && n_pos == 0)) return NEKO_OK;
-    NEKO_REQUIRE(ctx, qkv && q_out, "%s: null pointer", what);
+    NEKO_REQUIRE(ctx, qkv && q_out && (depth || !tree), "%s: null pointer", what);
     const int64_t q_width = static_cast<int64_t>(n_q) * kv->hd, width = q_width + 2LL * kv->n_kv * kv->hd;
     NEKO_REQUIRE(ctx, row_stride >= width && q_out_stride >= q_width, "%s: row strides (%lld, %lld) below the rows' widths (%lld, %lld)",
                  what, (long long)row_stride, (long long)q_out_stride, (long long)width, (long long)q_width);
@@ -421,6 +436,10 @@ extern "C" int neko_hip_qk_norm_rope_paged(neko_hip_ctx* ctx, const void* qkv, i
                  "%s: q_out is the q columns of qkv itself or disjoint from qkv", what);
     NEKO_REQUIRE(ctx, !paged_overlaps(*kv, qkv, s_in) && !paged_overlaps(*kv, q_out, s_out), "%s: the cache may not overlap qkv or q_out",
                  what);
+    const size_t s_depth = depth ? static_cast<size_t>(rows) * 4 : 0;
+    NEKO_REQUIRE(ctx, aligned(depth, 4) && !overlaps(depth, s_depth, q_out, s_out) && !paged_overlaps(*kv, depth, s_depth),
+                 "%s: depth is misaligned or overlaps q_out or the cache", what);
+    a.depth = depth;
     a.qkv = qkv;
     a.stride = row_stride;
     a.q_out = q_out;
@@ -428,9 +447,26 @@ extern "C" int neko_hip_qk_norm_rope_paged(neko_hip_ctx* ctx, const void* qkv, i
     a.wqk = wqk;
     a.cs = cs;
     a.n_pos = rot_dim > 0 && n_pos < (1 << 30) ? static_cast<int32_t>(n_pos) : 1 << 30;
+    a.limit = depth ? 1 << 30 : a.n_pos;
     a.rot = rot_dim;
     a.inter = interleaved != 0;
     a.n_q = n_q;
     a.eps = eps;
     return launch_append(ctx, what, a, dtype);
+}
+
+extern "C" int neko_hip_qk_norm_rope_paged(neko_hip_ctx* ctx, const void* qkv, int64_t row_stride, int64_t rows, int n_q,
+                                           const neko_paged_kv* kv, const neko_paged_batch* batch, const float* wqk,
+                                           const float* cs, int64_t n_pos, int rot_dim, int interleaved, float eps,
+                                           void* q_out, int64_t q_out_stride, int dtype) {
+    return append(ctx, "neko_hip_qk_norm_rope_paged", qkv, row_stride, rows, n_q, kv, batch, false, nullptr, wqk, cs, n_pos,
+                  rot_dim, interleaved, eps, q_out, q_out_stride, dtype);
+}
+
+extern "C" int neko_hip_qk_norm_rope_tree_paged(neko_hip_ctx* ctx, const void* qkv, int64_t row_stride, int64_t rows, int n_q,
+                                                const neko_paged_kv* kv, const neko_paged_batch* batch, const int32_t* depth,
+                                                const float* wqk, const float* cs, int64_t n_pos, int rot_dim, int interleaved,
+                                                float eps, void* q_out, int64_t q_out_stride, int dtype) {
+    return append(ctx, "neko_hip_qk_norm_rope_tree_paged", qkv, row_stride, rows, n_q, kv, batch, true, depth, wqk, cs, n_pos,
+                  rot_dim, interleaved, eps, q_out, q_out_stride, dtype);
 }

@@ -16,11 +16,12 @@ import threading
 import numpy as np
 import torch
 
-from ._lib import DT_F16, DT_F32, FMT_F16, FMT_FP4, FMT_FP8, NEKO_OK, NekoError, PagedBatch, PagedKv, lib
+from ._lib import DT_F16, DT_F32, FMT_F16, FMT_FP4, FMT_FP8, NEKO_OK, NekoError, PagedBatch, PagedKv, PagedTree, lib
 
 __all__ = [
     "Context", "context", "layer_norm", "rms_norm", "qk_norm_rope", "qk_norm_rope_kv", "store_kv", "add_rms_norm",
     "PagedKV", "qk_norm_rope_paged", "attention_paged",
+    "tree_plan", "qk_norm_rope_tree_paged", "attention_tree_paged", "sample", "accept_tree", "keep_paged",
     "silu_mul", "gelu", "gated_rms_norm", "embed", "matmul", "MM_GELU", "MM_ACCUMULATE",
     "prepare", "quantize", "quant_row_bytes", "quantize_rows", "rope_table", "FMT_F16", "FMT_FP8", "FMT_FP4", "NekoError",
 ]
@@ -358,6 +359,10 @@ def qk_norm_rope_paged(qkv: torch.Tensor, n_q: int, cache: PagedKV, page_table: 
     appended to the sequences' pages in 8 bits; returns the q rows [rows, n_q * hd]. row_start: int32 [n_seq + 1];
     kv_len: int32 [n_seq], lengths with the new rows; page_table: int32 [n_seq, max_pages]. q_out may be qkv's own q
     columns. Rows of no sequence, or at positions outside the table, leave their q_out row as it was (zeros in a new one)."""
+    return _append(lib.neko_hip_qk_norm_rope_paged, qkv, n_q, cache, page_table, row_start, kv_len, (), cs, eps, wqk, interleaved, q_out)
+
+
+def _append(fn, qkv, n_q, cache, page_table, row_start, kv_len, depth, cs, eps, wqk, interleaved, q_out):
     rows, width, stride = _rows(qkv, "qkv")
     _on(cache.k_pages, "cache", qkv.device)
     hd, n_kv = cache.hd, cache.n_kv
@@ -377,8 +382,8 @@ def qk_norm_rope_paged(qkv: torch.Tensor, n_q: int, cache: PagedKV, page_table: 
     else:
         q_out = _out_like(qkv, rows, n_q * hd, q_out, "q_out")
     ctx = _ctx_for(qkv)
-    _issue(ctx, lib.neko_hip_qk_norm_rope_paged, ctx.handle, qkv.data_ptr(), stride if rows > 1 else max(stride, width), rows,
-           int(n_q), ctypes.byref(cache.c), ctypes.byref(batch), _vec(wqk, 2 * hd, "wqk", qkv.device),
+    _issue(ctx, fn, ctx.handle, qkv.data_ptr(), stride if rows > 1 else max(stride, width), rows,
+           int(n_q), ctypes.byref(cache.c), ctypes.byref(batch), *depth, _vec(wqk, 2 * hd, "wqk", qkv.device),
            None if cs is None else cs.data_ptr(), n_pos, rot, 1 if interleaved else 0, float(eps), q_out.data_ptr(),
            q_out.stride(0) if rows > 1 else max(q_out.stride(0), n_q * hd), _dtype_code(qkv))
     return q_out
@@ -391,6 +396,10 @@ def attention_paged(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, r
     sequences' pages: scores scale * q.k (default 1/sqrt(hd)), capped by softcap * tanh(s / softcap) if softcap > 0,
     plus slopes[head] * (j - position) if slopes are given, over at most `window` keys if window > 0. Returns
     [rows, n_head * hd] in q's dtype; rows of no sequence are not written (zeros in a new out)."""
+    return _attend(lib.neko_hip_attention_paged, q, cache, page_table, row_start, kv_len, (), n_head, scale, softcap, window, slopes, out)
+
+
+def _attend(fn, q, cache, page_table, row_start, kv_len, tree, n_head, scale, softcap, window, slopes, out):
     rows, width, qs = _rows(q, "q")
     _on(cache.k_pages, "cache", q.device)
     hd = cache.hd
@@ -406,10 +415,137 @@ def attention_paged(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, r
     if scale is None:
         scale = float(np.float32(1.0) / np.sqrt(np.float32(hd)))
     ctx = _ctx_for(q)
-    _issue(ctx, lib.neko_hip_attention_paged, ctx.handle, q.data_ptr(), qs if rows > 1 else max(qs, width), rows,
-           ctypes.byref(cache.c), ctypes.byref(batch), int(n_head), float(scale), float(softcap), int(window),
+    _issue(ctx, fn, ctx.handle, q.data_ptr(), qs if rows > 1 else max(qs, width), rows,
+           ctypes.byref(cache.c), ctypes.byref(batch), *tree, int(n_head), float(scale), float(softcap), int(window),
            _vec(slopes, n_head, "slopes", q.device), out.data_ptr(), out.stride(0) if rows > 1 else max(out.stride(0), width),
            _dtype_code(q))
+    return out
+
+
+def tree_plan(parents: np.ndarray, row_start: np.ndarray) -> tuple[np.ndarray, np.ndarray]:
+    """(depth int32 [rows], mask int32 [rows, words]) of drafted trees, on the host: parents int32 [rows], each row's parent
+    within its own tree (-1: the root; other values outside [0, its row): padding, with all rows below it), row_start int32
+    [n_seq + 1]. A mask's bits are the row itself and its ancestors. Rows of no sequence are padding."""
+    parents, row_start = np.ascontiguousarray(parents, dtype=np.int32), np.ascontiguousarray(row_start, dtype=np.int32)
+    if parents.ndim != 1 or row_start.ndim != 1 or row_start.size < 2:
+        raise NekoError("parents and row_start must be vectors, row_start of at least 2 entries")
+    n = np.diff(row_start.astype(np.int64))
+    if row_start[0] < 0 or (n < 0).any() or row_start[-1] > parents.size or n.max() > 1024:
+        raise NekoError("row_start must not decrease, within the rows, trees of up to 1024 rows")
+    words = max(1, -(-int(n.max()) // 32))
+    depth, mask = np.full(parents.size, -1, np.int32), np.zeros((parents.size, words), np.int32)
+    rc = lib.neko_tree_plan(parents.ctypes.data_as(ctypes.c_void_p), row_start.ctypes.data_as(ctypes.c_void_p), n.size, words,
+                            depth.ctypes.data_as(ctypes.c_void_p), mask.ctypes.data_as(ctypes.c_void_p))
+    if rc != NEKO_OK:
+        raise NekoError(f"neko_tree_plan failed ({rc})", rc)
+    return depth, mask
+
+
+def _ints(t: torch.Tensor | None, n: int, name: str, device) -> int | None:
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.dim() != 1 or t.numel() != n or t.device != device or not t.is_cuda:
+        raise NekoError(f"{name} must be a contiguous int32 vector of {n} entries on {device}")
+    return t.data_ptr()
+
+
+def _depth(depth: torch.Tensor, rows: int, device) -> int:
+    if depth is None:
+        raise NekoError("depth must be a tensor")
+    return _ints(depth, rows, "depth", device)
+
+
+def qk_norm_rope_tree_paged(qkv: torch.Tensor, n_q: int, cache: PagedKV, page_table: torch.Tensor, row_start: torch.Tensor,
+                            kv_len: torch.Tensor, depth: torch.Tensor, cs: torch.Tensor | None, eps: float,
+                            wqk: torch.Tensor | None = None, interleaved: bool = False,
+                            q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """qk_norm_rope_paged for the rows of drafted trees: row i of a sequence's n goes to slot kv_len - n + i and is rotated
+    by the angles of place kv_len - n + depth (int32 [rows]; outside [0, n): padding, left alone)."""
+    return _append(lib.neko_hip_qk_norm_rope_tree_paged, qkv, n_q, cache, page_table, row_start, kv_len,
+                   (_depth(depth, qkv.shape[0], qkv.device),), cs, eps, wqk, interleaved, q_out)
+
+
+def attention_tree_paged(q: torch.Tensor, cache: PagedKV, page_table: torch.Tensor, row_start: torch.Tensor,
+                         kv_len: torch.Tensor, depth: torch.Tensor, mask: torch.Tensor, n_head: int, scale: float | None = None,
+                         softcap: float = 0.0, window: int = 0, slopes: torch.Tensor | None = None,
+                         out: torch.Tensor | None = None) -> torch.Tensor:
+    """attention_paged for the rows of drafted trees (as in qk_norm_rope_tree_paged, which has appended them): a row sees
+    the tokens before its tree and, of the tree, the rows whose bit is set in its mask (int32 [rows, words], up to 32
+    words; tree_plan); window and slopes go by places (depth, int32 [rows]). Padding rows see nothing and give zeros."""
+    rows = q.shape[0]
+    _on(mask, "mask", q.device)
+    if mask.dtype != torch.int32 or mask.dim() != 2 or mask.shape[0] != rows or not 1 <= mask.shape[1] <= 32 or \
+            (mask.shape[1] > 1 and mask.stride(1) != 1):
+        raise NekoError(f"mask must be int32 [{rows}, 1..32] with unit stride along rows")
+    stride = mask.stride(0) if rows > 1 else max(mask.stride(0), mask.shape[1])
+    tree = PagedTree(_depth(depth, rows, q.device), mask.data_ptr(), stride, mask.shape[1])
+    return _attend(lib.neko_hip_attention_tree_paged, q, cache, page_table, row_start, kv_len, (ctypes.byref(tree),), n_head, scale,
+                   softcap, window, slopes, out)
+
+
+def accept_tree(tokens: torch.Tensor, sampled: torch.Tensor, parents: torch.Tensor, row_start: torch.Tensor, kv_len: torch.Tensor,
+                max_path: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The path that the sampled tokens take through each drafted tree, from its root to a child that holds the token
+    sampled at the row before, as long as there is one (tokens, sampled, parents: int32 [rows]). Returns, int32: path
+    [n_seq, max_path] (rows within the tree, then -1), count [n_seq], the token sampled at the path's last row [n_seq], and
+    the sequences' lengths with the path alone [n_seq]."""
+    device, rows, n_seq = tokens.device, tokens.numel(), kv_len.numel()
+    if n_seq == 0 or max_path <= 0:
+        raise NekoError("accept_tree needs a sequence and max_path above 0")
+    ptrs = [_ints(t, n, name, device) for t, n, name in ((tokens, rows, "tokens"), (sampled, rows, "sampled"), (parents, rows, "parents"),
+                                                         (row_start, n_seq + 1, "row_start"), (kv_len, n_seq, "kv_len"))]
+    path = torch.empty((n_seq, int(max_path)), dtype=torch.int32, device=device)
+    count, after, new_len = (torch.empty((n_seq,), dtype=torch.int32, device=device) for _ in range(3))
+    ctx = _ctx_for(tokens)
+    _issue(ctx, lib.neko_hip_accept_tree, ctx.handle, *ptrs[:3], rows, *ptrs[3:], n_seq, path.data_ptr(), int(max_path),
+           count.data_ptr(), after.data_ptr(), new_len.data_ptr())
+    return path, count, after, new_len
+
+
+def keep_paged(cache: PagedKV, page_table: torch.Tensor, row_start: torch.Tensor, kv_len: torch.Tensor, path: torch.Tensor,
+               count: torch.Tensor) -> None:
+    """The cached tokens of the first `count` rows of each sequence's path (accept_tree) moved together: from slot
+    kv_len - n + path[k] to slot kv_len - n + k, under the scales that the append would give them. kv_len as in the append."""
+    device = cache.device
+    batch = _paged_batch(page_table, row_start, kv_len, device)
+    n_seq = kv_len.numel()
+    _on(path, "path", device)
+    if path.dtype != torch.int32 or path.dim() != 2 or path.shape[0] != n_seq or path.shape[1] == 0 or \
+            (path.shape[1] > 1 and path.stride(1) != 1):
+        raise NekoError(f"path must be int32 [{n_seq}, max_path] with unit stride along rows")
+    stride = path.stride(0) if n_seq > 1 else max(path.stride(0), path.shape[1])
+    ctx = _ctx_for(cache.k_pages)
+    _issue(ctx, lib.neko_hip_keep_paged, ctx.handle, ctypes.byref(cache.c), ctypes.byref(batch), path.data_ptr(), stride,
+           path.shape[1], _ints(count, n_seq, "count", device))
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
+           top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """A token of each row of logits [rows, vocab], int32 [rows], from the uniform numbers u (float32 [rows], in [0, 1)): of
+    the weights exp((l - max) / temperature), the top_k largest, of those the shortest prefix that has top_p of their sum,
+    of those the ones of at least min_p; the first by index whose running sum exceeds u times the whole. temperature, top_p,
+    min_p: float32 [rows], top_k: int32 [rows], or None. A temperature of 0 takes the largest logit; a row of nothing but
+    -inf and NaN gives -1."""
+    rows, vocab, stride = _rows(logits, "logits")
+    if vocab == 0:
+        raise NekoError("logits must have a vocabulary")
+    device = logits.device
+
+    def floats(t, name):
+        if t is None:
+            return None
+        if t.dtype != torch.float32 or not t.is_contiguous() or t.dim() != 1 or t.numel() != rows or t.device != device:
+            raise NekoError(f"{name} must be a contiguous float32 vector of {rows} values on {device}")
+        return t.data_ptr()
+
+    if u is None:
+        raise NekoError("u must be a tensor")
+    if out is None:
+        out = torch.empty((rows,), dtype=torch.int32, device=device)
+    ctx = _ctx_for(logits)
+    _issue(ctx, lib.neko_hip_sample, ctx.handle, logits.data_ptr(), stride if rows > 1 else max(stride, vocab), rows, vocab,
+           floats(temperature, "temperature"), _ints(top_k, rows, "top_k", device), floats(top_p, "top_p"), floats(min_p, "min_p"),
+           floats(u, "u"), _ints(out, rows, "out", device), _dtype_code(logits))
     return out
 
 
