@@ -224,7 +224,7 @@ __device__ __forceinline__ uint32_t tree_sees(const PagedAttnArgs& a, const SeqR
         const int32_t w = k0 >> 5, by = k0 & 31;
         const uint32_t m0 = w >= 0 ? m[w] : 0u, m1 = w + 1 < a.words ? m[w + 1] : 0u;
         uint32_t bits = (m0 >> by | (by ? m1 << (32 - by) : 0u)) & below(tree_reach(a, r) - j0);
-        if (a.t.window > 0 && d >= a.t.window) {  // a window that ends inside the tree
+        if (a.t.window > 0 && d >= a.t.window - 1) {  // a window that ends inside the tree (or at its root)
             for (uint32_t left = bits; left; left &= left - 1) {
                 const int32_t k = __builtin_ctz(left);
                 if (a.depth[r.begin + k0 + k] <= d - a.t.window) bits &= ~(1u << k);

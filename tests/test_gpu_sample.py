@@ -1,0 +1,280 @@
+"""GPU tests of neko_hip_sample against an evaluation in 64 bits (tests/tree_oracle.py).
+
+Tolerance: the tokens are equal. The kernel's weights are e^x in double; its cuts sum them in fixed point of 2^-44, off by
+at most 2^-45 each, its running sum in double. A row that is decided nearer to a border than V * 2^-44 of the sum could
+go either way; the oracle says how near it was, and rows are drawn so that none is (their number is in the assertion).
+"""
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+import tree_oracle as T
+from nekochat_amd import NekoError, ops
+
+pytestmark = pytest.mark.gpu
+
+DT = {"f16": torch.float16, "f32": torch.float32}
+
+
+def _case(msg):
+    print(f"[case] {msg}", flush=True)
+
+
+def _check(dev, x, u, exact_ties=False, at_border=False, **kw):
+    """x: a CPU tensor of logits; kw: per-row settings, as CPU tensors. exact_ties: weights and sums that are whole numbers,
+    whose borders are met exactly; at_border: u may be at one where they are not, and either side of it is right."""
+    got = ops.sample(x.to(dev), u.to(dev), **{k: v.to(dev) for k, v in kw.items()})
+    torch.cuda.synchronize()
+    got = got.cpu().tolist()
+    rows = x.float().double().numpy()
+    for r in range(len(rows)):
+        mine = {k: float(v[r]) if v.dtype != torch.int32 else int(v[r]) for k, v in kw.items()}
+        want, near = T.sample(rows[r], float(u[r]), **mine)
+        if at_border and near <= x.shape[1] * 2.0 ** -44:
+            assert got[r] in [T.sample(rows[r], float(u[r]), shift=by * x.shape[1] * 2.0 ** -44, **mine)[0] for by in (-1, 1)]
+            continue
+        assert exact_ties or near > x.shape[1] * 2.0 ** -44, f"row {r} decided within {near} of a border"
+        assert got[r] == want, f"row {r}: {got[r]}, not {want} ({ {k: v[r].item() for k, v in kw.items()} }, u {float(u[r])})"
+    return got
+
+
+def _settings(rows, vocab, g, mode):
+    f = lambda lo, hi: torch.rand(rows, generator=g) * (hi - lo) + lo  # noqa: E731
+    kw = {"temperature": f(0.3, 1.7)}
+    if mode in ("k", "all"):
+        kw["top_k"] = torch.randint(1, max(2, min(vocab, 300)), (rows,), generator=g, dtype=torch.int32)
+    if mode in ("p", "all"):
+        kw["top_p"] = f(0.05, 0.999)
+    if mode in ("min_p", "all"):
+        kw["min_p"] = f(0.0, 0.3)
+    return kw
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("vocab", [1, 2, 7, 63, 2047, 2049, 50257, 151936])
+@pytest.mark.parametrize("mode", ["none", "k", "p", "min_p", "all"])
+def test_sample(dev, vocab, dtype, mode):
+    _case(f"sample, vocabulary {vocab} {dtype} {mode}")
+    rows = 40 if vocab < 10000 else 6
+    g = torch.Generator().manual_seed(vocab + len(mode))
+    x = (torch.randn((rows, vocab), generator=g) * 3).to(DT[dtype])
+    _check(dev, x, torch.rand(rows, generator=g), **_settings(rows, vocab, g, mode))
+
+
+def test_sample_many_rows(dev):
+    """So many rows that each is one workgroup's."""
+    _case("sample, 1500 rows")
+    g = torch.Generator().manual_seed(3)
+    x = (torch.randn((1500, 5000), generator=g) * 2).half()
+    _check(dev, x, torch.rand(1500, generator=g), **_settings(1500, 5000, g, "all"))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_sample_settings_that_cut_nothing(dev, dtype):
+    """Settings at and past their ends, and not numbers."""
+    _case(f"sample, settings that cut nothing or all, {dtype}")
+    nan, inf = float("nan"), float("inf")
+    k = [0, -5, 1000, 2**31 - 1, 1, 2, 999]
+    p = [1.0, 2.0, nan, inf, 0.0, -1.0, 1e-30]
+    m = [0.0, -1.0, nan, 1.0, 2.0, inf, 1e-30]
+    t = [1.0, 0.0, -2.0, nan, inf, 1e-30, 1e30]
+    g = torch.Generator().manual_seed(2)
+    n = 7
+    base = torch.randn((n, 1000), generator=g).to(DT[dtype])
+    ints = lambda v: torch.tensor(v, dtype=torch.int32)  # noqa: E731
+    u = torch.rand(n, generator=g)
+    _check(dev, base, u, top_k=ints(k))
+    _check(dev, base, u, top_p=torch.tensor(p))
+    _check(dev, base, u, min_p=torch.tensor(m))
+    _check(dev, base, u, temperature=torch.tensor(t))
+    for i in range(n):
+        _check(dev, base, u, top_k=ints(k), top_p=torch.tensor(p[i:] + p[:i]), min_p=torch.tensor(m), temperature=torch.tensor(t[i:] + t[:i]))
+
+
+def test_sample_u_at_its_ends(dev):
+    _case("sample, u at its ends")
+    x = torch.zeros((8, 16))  # sixteen weights of 1: borders at every sixteenth
+    u = torch.tensor([0.0, -0.0, -3.0, float("nan"), 1.0, float("inf"), 1 - 2.0 ** -24, 0.5])
+    got = _check(dev, x, u, exact_ties=True)
+    assert got == [0, 0, 0, 0, 15, 15, 15, 8]
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("vocab", [5, 300, 4097, 30000])
+def test_sample_equal_logits(dev, vocab, dtype):
+    """Nothing but ties: weights of exactly 1, so every cut is at a whole number of tokens, and the lowest indices stay.
+    30000 of them are more than one list holds."""
+    _case(f"sample, {vocab} equal logits {dtype}")
+    k = [1, 2, 3, vocab // 2, vocab - 1, 0]
+    n = len(k)
+    x = torch.full((n, vocab), 2.5).to(DT[dtype])
+    x[:, ::3] = -1.5 if vocab > 10 else 2.5
+    # u a multiple of 2^-10 and sums below 2^15 make every product exact
+    u = torch.tensor([0.0, 0.25, 0.5, 0.75, 0.875, 0.9375])
+    # (with the others kept, weights of e^-4 among those of 1: one in three, so u = 15/16 of 30000 tokens is the border behind
+    # the 28125th in exact arithmetic, 15/16 (20000 + 10000 e^-4) = 18750 + 9375 e^-4, and rounded sums fall to either side)
+    _check(dev, x, u, exact_ties=True, at_border=True, top_k=torch.tensor(k, dtype=torch.int32))
+    zero = torch.zeros((n, vocab)).to(DT[dtype])
+    zero[:, 1::2] = -0.0  # equal to zero
+    _check(dev, zero, u, exact_ties=True, top_k=torch.tensor(k, dtype=torch.int32))
+    _check(dev, zero, u, exact_ties=True, top_p=torch.tensor([0.5, 0.25, 0.125, 0.0625, 0.75, 2.0 ** -20]))
+    _check(dev, zero, u, exact_ties=True, top_k=torch.tensor(k, dtype=torch.int32), top_p=torch.tensor([0.5, 0.25, 0.125, 0.0625, 0.75, 0.875]))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("temperature", [1.0, 1e4])
+def test_sample_crowded_values(dev, dtype, temperature):
+    """More tokens within one bin than are sorted at once: close values, a few of them often, and at a high temperature."""
+    _case(f"sample, crowded values {dtype} at {temperature}")
+    g = torch.Generator().manual_seed(5)
+    rows, vocab = 6, 40000
+    x = (torch.randint(0, 50, (rows, vocab), generator=g) * 2.0 ** -10 + 1.0).to(DT[dtype])
+    x[1::2] = (torch.rand((3, vocab), generator=g) * 0.01 + 3.0).to(DT[dtype])
+    t = torch.full((rows,), temperature)
+    u = torch.rand(rows, generator=g)
+    _check(dev, x, u, temperature=t, top_k=torch.tensor([1, 100, 5000, 20000, 39999, 7], dtype=torch.int32))
+    _check(dev, x, u, temperature=t, top_p=torch.tensor([0.1, 0.3, 0.5, 0.7, 0.9, 0.99]))
+    _check(dev, x, u, temperature=t, top_k=torch.tensor([30000, 100, 5000, 20000, 39999, 7], dtype=torch.int32),
+           top_p=torch.tensor([0.1, 0.3, 0.5, 0.7, 0.9, 0.99]))
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("vocab", [9, 6000])
+def test_sample_masked_and_not_finite(dev, vocab, dtype):
+    """-inf and NaN are never chosen; where the largest is +inf only those that are; nothing to choose from gives -1."""
+    _case(f"sample, masks, infinities and NaN, vocabulary {vocab} {dtype}")
+    g = torch.Generator().manual_seed(6)
+    nan, inf = float("nan"), float("inf")
+    x = torch.randn((8, vocab), generator=g)
+    x[0] = -inf
+    x[1] = nan
+    x[2, : vocab - 1] = -inf
+    x[3, 2:] = nan
+    x[4, 3] = x[4, 5] = inf
+    x[5] = -inf
+    x[5, 1::2] = nan
+    x[6, ::2] = -inf
+    x[7] = -3e38 if dtype == "f32" else -65504.0
+    x[7, 4] = 3e38 if dtype == "f32" else 65504.0
+    x = x.to(DT[dtype])
+    u = torch.rand(8, generator=g)
+    for kw in ({}, {"top_k": torch.full((8,), 3, dtype=torch.int32)}, {"top_p": torch.full((8,), 0.7)}, {"temperature": torch.zeros(8)},
+               {"top_k": torch.full((8,), 4, dtype=torch.int32), "top_p": torch.full((8,), 0.6), "min_p": torch.full((8,), 0.1)},
+               {"temperature": torch.full((8,), inf), "top_p": torch.full((8,), 0.6)}):
+        got = _check(dev, x, u, exact_ties=True, **kw)
+        assert got[0] == got[1] == got[5] == -1 and got[2] == vocab - 1 and got[3] in (0, 1) and got[4] in (3, 5) and got[6] % 2 == 1
+
+
+def test_sample_frequencies(dev):
+    """What comes out over an even grid of u is the weights' distribution: counts within one of their shares."""
+    _case("sample, frequencies")
+    x = torch.tensor([0.0, 1.0, -1.0, 2.0, 0.5])
+    n = 4096
+    got = ops.sample(x.repeat(n, 1).to(dev), ((torch.arange(n) + 0.5) / n).to(dev))
+    torch.cuda.synchronize()
+    counts = torch.bincount(got.cpu().long(), minlength=5).double()
+    assert float((counts - n * torch.softmax(x.double(), 0)).abs().max()) <= 1
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_sample_rows_at_any_element(dev, dtype):
+    """Logits as columns of a wider tensor that begin at odd elements; one row of any stride."""
+    _case(f"sample, rows at odd elements {dtype}")
+    g = torch.Generator().manual_seed(8)
+    wide = torch.randn((9, 3005), generator=g).to(DT[dtype])
+    u, kw = torch.rand(9, generator=g), _settings(9, 3001, g, "all")
+    want = _check(dev, wide[:, 3:3004].contiguous(), u, **kw)
+    on = {k: v.to(dev) for k, v in kw.items()}
+    got = ops.sample(wide.to(dev)[:, 3:3004], u.to(dev), **on)
+    one = ops.sample(wide.to(dev)[4:5, 3:3004], u.to(dev)[4:5], **{k: v[4:5] for k, v in on.items()})
+    torch.cuda.synchronize()
+    assert got.cpu().tolist() == want and one.item() == want[4]
+
+
+def test_sample_same_in_every_batch_and_again(dev):
+    """A row's token does not depend on the rows beside it, nor on when it is drawn."""
+    _case("sample, the same row in several batches")
+    g = torch.Generator().manual_seed(9)
+    x, u = (torch.randn((300, 20000), generator=g) * 2).to(dev), torch.rand(300, generator=g).to(dev)
+    kw = {k: v.to(dev) for k, v in _settings(300, 20000, g, "all").items()}
+    whole = ops.sample(x, u, **kw)
+    again = ops.sample(x, u, **kw)
+    parts = torch.cat([ops.sample(x[a:b], u[a:b], **{k: v[a:b] for k, v in kw.items()}) for a, b in ((0, 1), (1, 8), (8, 300))])
+    torch.cuda.synchronize()
+    assert torch.equal(whole, again) and torch.equal(whole, parts)
+
+
+def test_sample_captured(dev):
+    """A captured graph follows new logits, settings and numbers, beside eager calls of other sizes."""
+    _case("sample, captured")
+    g = torch.Generator().manual_seed(10)
+    x, u = torch.empty((5, 30001), dtype=torch.float16, device=dev), torch.empty(5, device=dev)
+    kw = {k: v.to(dev) for k, v in _settings(5, 30001, g, "all").items()}
+    out = torch.empty(5, dtype=torch.int32, device=dev)
+
+    def fill(i):
+        x.copy_((torch.randn((5, 30001), generator=g) * (1 + i)).half())
+        u.copy_(torch.rand(5, generator=g))
+        for k, v in _settings(5, 30001, g, "all").items():
+            kw[k].copy_(v)
+
+    stream = torch.cuda.Stream(dev)
+    fill(0)
+    with torch.cuda.stream(stream):
+        ops.sample(x, u, out=out, **kw)  # the workspace
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        ops.sample(x, u, out=out, **kw)
+    for i in range(4):
+        fill(i)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = out.clone()
+        want = ops.sample(x, u, **kw)
+        ops.sample(torch.randn((200, 777), device=dev), torch.rand(200, device=dev), top_p=torch.full((200,), 0.5, device=dev))
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+def test_sample_two_threads(dev):
+    _case("sample, two threads")
+    g = torch.Generator().manual_seed(11)
+    jobs = [((torch.randn((20, 9000), generator=g) * 2).to(dev), torch.rand(20, generator=g).to(dev),
+             {k: v.to(dev) for k, v in _settings(20, 9000, g, "all").items()}) for _ in range(2)]
+    want = [ops.sample(x, u, **kw).cpu() for x, u, kw in jobs]
+    got, failed = [None, None], []
+
+    def work(i):
+        try:
+            x, u, kw = jobs[i]
+            with torch.cuda.stream(torch.cuda.Stream(dev)):
+                for _ in range(20):
+                    out = ops.sample(x, u, **kw)
+                got[i] = out.cpu()
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not failed and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_sample_refuses(dev):
+    _case("sample, refusals")
+    x, u = torch.zeros((4, 10), device=dev), torch.zeros(4, device=dev)
+    bad = [
+        lambda: ops.sample(x.double(), u), lambda: ops.sample(x.cpu(), u), lambda: ops.sample(x.t(), u), lambda: ops.sample(x[0], u),
+        lambda: ops.sample(x, u[:3]), lambda: ops.sample(x, u.half()), lambda: ops.sample(x, u.cpu()), lambda: ops.sample(x, None),
+        lambda: ops.sample(x[:, :0], u), lambda: ops.sample(x, u, top_k=u), lambda: ops.sample(x, u, temperature=u[:1]),
+        lambda: ops.sample(x, u, min_p=torch.zeros((4, 1), device=dev)), lambda: ops.sample(x, u, out=torch.zeros(4, device=dev)),
+        lambda: ops.sample(x, u, top_p=torch.zeros(8, device=dev)[::2]),
+        lambda: ops.sample(x, u, out=u.view(torch.int32)), lambda: ops.sample(x, u, out=x.view(torch.int32).reshape(-1)[:4]),
+    ]
+    for f in bad:
+        with pytest.raises(NekoError):
+            f()
+    assert ops.sample(x[:0], u[:0]).shape == (0,)
