@@ -5,17 +5,20 @@
 // running sum of w passes u * (their sum).
 //
 // Numbers. A vocabulary has some 10^5 borders between tokens, and f32 weights, off by 2^-24, would put about one sample in
-// 10^4 on the wrong side of one. Weights are e^x in double; the sums that cut off S1 and S2 are of weights in fixed point
-// (2^-44 of the largest for up to 2^18 tokens), whose order does not matter, so atomics in LDS may take any; the running
-// sum is in double, in an order that the vocabulary alone sets.
+// 10^4 on the wrong side of one. Weights are e^x in double, and exactly 1 for the largest logit, so that rows of equal
+// logits are cut at whole numbers of tokens; running sums are in double, in an order that the vocabulary alone sets. Sums
+// over a histogram's bin are in fixed point (each weight to 2^-30 of itself or better), whose order does not matter, so
+// atomics in LDS may take any.
 //
-// Launches, several workgroups to a row in 1, 2 and 4:
-//   1 the largest logit
-//   2 a histogram of weights and counts over the distance from it, 512 bins of T / 16 (rows with a top-k or top-p)
-//   3 the bin of each cut from that, the few tokens in it sorted: the last logit kept, and of those equal to it the last
-//     index (one workgroup to a row)
-//   4 the kept weights' sums of blocks of 2048 tokens
-//   5 the block, and in it the token
+// Launches, several workgroups ("parts") to a row in the first two:
+//   1 each part's largest logit and, of rows with a top-k or top-p, a histogram of its tokens' number and weight over the
+//     logit, 1024 bins of T / 32 down from its largest's. Bins stand at fixed places of z = 32 l / T, not of the largest,
+//     which no part knows: parts' histograms are shifted and added by whoever reads them. A weight is held relative to its
+//     bin's lower edge, e^(f / 32) with f = z - floor z: a short polynomial and no table, and one atomic for number and sum.
+//   2 every part adds up the row's histogram and finds the bins in which the cuts fall: tokens above those are kept, and
+//     their weights' sums of blocks of 2048 tokens are written; tokens in those bins, some hundreds, are listed
+//   3 one workgroup to a row: the cuts within the list, its kept tokens' weights added to their blocks' sums, and the block
+//     and in it the token that u falls on
 #include <algorithm>
 
 #include "internal.h"
@@ -24,16 +27,34 @@
 namespace neko_hip {
 namespace {
 
-constexpr int kBins = 512;
-constexpr float kBinsPerNat = 16.0f;
-constexpr int kBlockTokens = 2048;  // of a sum in launch 4: 256 threads of 8
-constexpr int kListed = 4096;       // tokens of a bin that launch 3 sorts in LDS
-constexpr uint32_t kMinusInf = 0x007fffffu;  // its key; tokens at or below are left out
+constexpr int kThreads = 1024;
+constexpr int kBins = 1024;  // one to a thread; the last holds whatever is further down
+constexpr double kBinsPerT = 32.0;
+constexpr int kBlockTokens = 2048;               // of a sum: 256 threads of 8
+constexpr int kStepTokens = kThreads * 8;        // four blocks
+constexpr int kMostSteps = 8;                    // of a part: its numbers and weights share 64 bits of a bin
+constexpr int kListed = 4096;                    // tokens in the cuts' bins that are held in LDS
+constexpr int kRanked = 256;                     // of those, what is sorted by ranks
+constexpr int64_t kSlabRows = 1024;              // of a launch: the workspace holds so many
+constexpr uint32_t kMinusInf = 0x007fffffu;      // its key; tokens at or below are left out
 
-struct Cut {
-    uint32_t key;  // kept: keys above, and of those equal the indices up to `last`
-    int32_t last;
+// What launch 1 leaves of a part.
+struct Part {
+    uint64_t best;    // key << 32 | ~index of its largest (greedy rows; the others' has no index)
+    double weight;    // its tokens' weights, relative to the lower edge of its largest's bin
+    uint32_t count;   // its tokens
+    uint32_t unused;
 };
+
+// What launch 2 finds of a row: cuts that fall into bins lo .. hi (top-p) and by_k (top-k: after `need` of its tokens).
+struct Found {
+    int32_t lo, hi, bin_k;
+    uint32_t need;
+    uint32_t listed;            // tokens of those bins
+    uint32_t unused;
+    double below_lo, below_k;   // weights' sums of the bins before lo and bin_k
+    double total;               // of the row
+};  // (weights relative to the row's largest)
 
 struct SampleArgs {
     const void* logits;
@@ -45,31 +66,32 @@ struct SampleArgs {
     const float* u;
     int32_t* out;
     int32_t vocab;
-    int32_t n_max, max_tokens;    // workgroups of a row in launches 1 and 4, and their tokens (whole blocks)
-    int32_t n_hist, hist_tokens;  // of launch 2
-    int32_t n_blocks;             // blocks of a row
-    int32_t fixed;                // fixed-point weights: units of 2^-fixed
-    uint64_t* best;               // [rows][n_max] key << 32 | ~index
-    uint32_t* counts;             // [rows][n_hist][kBins]
-    uint64_t* weights;
-    Cut* cuts;                    // [rows]
-    double* sums;                 // [rows][n_blocks]
+    int32_t parts, part_tokens;  // of a row; whole steps
+    int32_t n_blocks;            // blocks of a row
+    int32_t count_bits;          // the low bits of a bin: its tokens; the others: their weights in units of 2^-fixed
+    int32_t fixed;
+    int32_t narrow;              // fixed-point weights of launch 3, relative to the row's largest: units of 2^-narrow
+    Part* part;                  // [rows][parts]
+    uint64_t* bins;              // [rows][parts][kBins]
+    Found* found;                // [rows]
+    uint32_t* listed;            // [rows] tokens listed so far
+    uint64_t* list;              // [rows][kListed] ~key << 32 | index: ascending is the order of the cuts
+    double* sums;                // [rows][n_blocks]
 };
 
 // What a row asks for, as its numbers are read: a temperature that is not positive is the largest logit's token, a k not
 // positive, a p of 1 or more and a min_p not positive cut off nothing, nor does a NaN.
 struct Row {
     bool greedy, by_k, by_p;
-    float bins;     // per unit of distance
     double inv_t, p, min_p;
     int32_t k;
+    __device__ bool cuts() const { return !greedy && (by_k || by_p); }
 };
 __device__ __forceinline__ Row row_of(const SampleArgs& a, int64_t r) {
     Row w;
     const float t = a.temperature ? a.temperature[r] : 1.0f;
     w.greedy = !(t > 0.0f);
     w.inv_t = 1.0 / static_cast<double>(t);
-    w.bins = kBinsPerNat / t;
     w.k = a.top_k ? a.top_k[r] : 0;
     w.by_k = w.k > 0 && w.k < a.vocab;
     const float p = a.top_p ? a.top_p[r] : 1.0f;
@@ -90,15 +112,30 @@ __device__ __forceinline__ float value_of(uint32_t k) {
     return __builtin_bit_cast(float, k ^ (k & 0x80000000u ? 0x80000000u : 0xffffffffu));
 }
 
-// The bin of a logit below or at the largest: monotone in it, as every rounding here is.
-__device__ __forceinline__ int bin_of(float l, float top, float per) {
-    return l == top ? 0 : static_cast<int>(fminf((top - l) * per, static_cast<float>(kBins - 1)));  // (NaN, an infinite distance at no slope: the last)
+// A logit's place among the bins, monotone in it as every rounding here is, and the number of its bin down from that of
+// place `top`. (An infinite logit stands at 1e300.)
+__device__ __forceinline__ double place_of(float l, double inv_t) { return fmin(static_cast<double>(l) * (kBinsPerT * inv_t), 1e300); }
+__device__ __forceinline__ int bin_at(double place, double top) { return static_cast<int>(fmax(fmin(floor(top) - floor(place), kBins - 1.0), 0.0)); }
+// e^(f / 32) for 0 <= f < 1: the series, cut off by (1/32)^6 / 6! = 1.3e-12 or (LONG) (1/32)^8 / 8! = 2.3e-17.
+template <bool LONG>
+__device__ __forceinline__ double edge_weight(double f) {
+    const double x = f * (1.0 / 32.0);
+    double y = LONG ? __builtin_fma(x, 1.0 / 5040.0, 1.0 / 720.0) : 1.0 / 120.0;
+    if (LONG) y = __builtin_fma(x, y, 1.0 / 120.0);
+    y = __builtin_fma(x, y, 1.0 / 24.0);
+    y = __builtin_fma(x, y, 1.0 / 6.0);
+    y = __builtin_fma(x, y, 0.5);
+    y = __builtin_fma(x, y, 1.0);
+    return __builtin_fma(x, y, 1.0);
 }
 __device__ __forceinline__ double weight_of(float l, float top, double inv_t) {
     const double w = exp((static_cast<double>(l) - static_cast<double>(top)) * inv_t);
-    return l == top ? 1.0 : w == w ? w : 0.0;
+    return l == top ? 1.0 : w == w ? w : 0.0;  // (no number: an infinite distance at an infinite temperature)
 }
-__device__ __forceinline__ uint64_t fixed_of(double w, int bits) { return static_cast<uint64_t>(ldexp(w, bits) + 0.5); }
+// w * units, rounded, below 2^52: the low bits of its sum with 2^52.
+__device__ __forceinline__ uint64_t fixed_of(double w, double units) {
+    return __builtin_bit_cast(uint64_t, __builtin_fma(w, units, 0x1p52)) - __builtin_bit_cast(uint64_t, 0x1p52);
+}
 
 // Logits i .. i + 7 of a row of n, -inf past it. Rows may stand at any element.
 template <typename T>
@@ -126,111 +163,373 @@ __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
 // The largest logit of a row, from launch 1's parts, by every wave for itself: key << 32 | ~index.
 __device__ __forceinline__ uint64_t row_best(const SampleArgs& a, int64_t r) {
     uint64_t b = 0;
-    for (int32_t i = static_cast<int32_t>(threadIdx.x) & 63; i < a.n_max; i += 64) {
-        const uint64_t o = a.best[r * a.n_max + i];
+    for (int32_t i = static_cast<int32_t>(threadIdx.x) & 63; i < a.parts; i += 64) {
+        const uint64_t o = a.part[r * a.parts + i].best;
         b = b > o ? b : o;
     }
     return wave_max_u64(b);
 }
 
-// ------------------------------------------------------------------ 1: the largest
+typedef unsigned long long u64;
+
+// Inclusive sum over the lanes below and at each, within 16 lanes and on (DPP, as wave_scan_u32).
+template <typename V>
+__device__ __forceinline__ V wave_scan(V v) {
+    auto add = [&](auto ctrl, auto rows) {
+        if constexpr (sizeof(V) == 4) {
+            v += __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(ctrl)::value, decltype(rows)::value, 0xF, false));
+        } else {
+            const uint64_t b = __builtin_bit_cast(uint64_t, v);
+            const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(b)), decltype(ctrl)::value, decltype(rows)::value, 0xF, false));
+            const uint32_t hi = static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(static_cast<uint32_t>(b >> 32)), decltype(ctrl)::value, decltype(rows)::value, 0xF, false));
+            v += __builtin_bit_cast(V, static_cast<uint64_t>(hi) << 32 | lo);
+        }
+    };
+    add(std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});  // row_shr 1, 2, 4, 8
+    add(std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});
+    add(std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast 15 into rows 1 and 3
+    add(std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast 31 into rows 2 and 3
+    return v;
+}
+// The sum of the threads' values up to each thread's own. sh: one for each wave.
+template <typename V>
+__device__ __forceinline__ V block_scan(V* sh, V v) {
+    const int lane = static_cast<int>(threadIdx.x) & 63, wave = static_cast<int>(threadIdx.x) >> 6;
+    v = wave_scan(v);
+    __syncthreads();
+    if (lane == 63) sh[wave] = v;
+    __syncthreads();
+    const V before = wave_scan(lane < wave ? sh[lane] : V(0));
+    return __shfl(before, 63) + v;
+}
+
+
+// ------------------------------------------------------------------ 1: parts' largest and histograms
 
 template <typename T>
-__global__ __launch_bounds__(256) void sample_max(SampleArgs a) {
-    __shared__ uint64_t sh[4];
-    const int64_t r = blockIdx.x / static_cast<uint32_t>(a.n_max);
-    const int32_t part = static_cast<int32_t>(blockIdx.x - static_cast<uint32_t>(r) * static_cast<uint32_t>(a.n_max));
+__global__ __launch_bounds__(kThreads) void sample_parts(SampleArgs a) {
+    __shared__ u64 bins[kBins];
+    __shared__ uint32_t sh_top[kThreads / 64];
+    __shared__ uint32_t sh_at;
+    __shared__ double sh_sum[kThreads / 64];
+    __shared__ uint32_t sh_count[kThreads / 64];
+    const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
+    const int64_t r = blockIdx.x / static_cast<uint32_t>(a.parts);
+    const int32_t part = static_cast<int32_t>(blockIdx.x - static_cast<uint32_t>(r) * static_cast<uint32_t>(a.parts));
+    const Row w = row_of(a, r);
     const T* row = static_cast<const T*>(a.logits) + r * a.stride;
-    const int32_t end = static_cast<int32_t>(std::min<int64_t>(a.vocab, static_cast<int64_t>(part + 1) * a.max_tokens));
-    uint32_t top = 0, at = 0;
-    for (int32_t i = part * a.max_tokens + static_cast<int32_t>(threadIdx.x) * 8; i < end; i += kBlockTokens) {
+    const int32_t begin = part * a.part_tokens, end = static_cast<int32_t>(std::min<int64_t>(a.vocab, static_cast<int64_t>(begin) + a.part_tokens));
+    float top = -__builtin_inff();
+    for (int32_t i = begin + tid * 8; i < end; i += kStepTokens) {
+        float x[8];
+        load8(row, i, a.vocab, x);
+#pragma unroll
+        for (int e = 0; e < 8; e++) top = fmaxf(top, x[e]);  // (the other one of a NaN)
+    }
+    bins[tid] = 0;
+    if (tid == 0) sh_at = 0xffffffffu;
+    uint32_t key = wave_max_u32(key_of(top));
+    if (lane == 0) sh_top[tid >> 6] = key;
+    __syncthreads();
+    key = wave_max_u32(sh_top[lane & (kThreads / 64 - 1)]);
+    top = value_of(key);
+    Part* out = a.part + blockIdx.x;
+    if (w.greedy) {
+        // The first that has it.
+        uint32_t at = 0xffffffffu;
+        for (int32_t i = begin + tid * 8; i < end && at == 0xffffffffu; i += kStepTokens) {
+            float x[8];
+            load8(row, i, a.vocab, x);
+#pragma unroll
+            for (int e = 7; e >= 0; e--)
+                if (x[e] == top) at = static_cast<uint32_t>(i + e);
+        }
+        if (at != 0xffffffffu) atomicMin(&sh_at, at);
+        __syncthreads();
+        if (tid == 0) out->best = static_cast<uint64_t>(key) << 32 | (0xffffffffu - sh_at);
+        return;
+    }
+    if (tid == 0) {
+        out->best = static_cast<uint64_t>(key) << 32;
+        if (part == 0) a.listed[r] = 0;
+    }
+    if (!w.cuts() || key <= kMinusInf) return;
+    const double place = place_of(top, w.inv_t), per = kBinsPerT * w.inv_t, first = floor(place), units = ldexp(1.0, a.fixed);
+    const u64 one = 0x4330000000000000ull;  // the bits of 2^52
+    double further = 0.0;  // what the last bin's tokens weigh
+    uint32_t n = 0;
+    for (int32_t i = begin + tid * 8; i < end; i += kStepTokens) {
         float x[8];
         load8(row, i, a.vocab, x);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const uint32_t k = key_of(x[e]);
-            if (k > top) {
-                top = k;
-                at = static_cast<uint32_t>(i + e);
+            if (!(x[e] > -__builtin_inff())) continue;
+            const double z = fmin(static_cast<double>(x[e]) * per, 1e300), g = floor(z);
+            const int b = static_cast<int>(fmin(first - g, kBins - 1.0));
+            const double y = __builtin_fma(edge_weight<false>(z - g), units, 0x1p52);
+            n++;
+            if (b < kBins - 1) {
+                atomicAdd(&bins[b], ((__builtin_bit_cast(u64, y) - one) << a.count_bits) + 1);
+            } else {
+                further += exp((z - first) * (1.0 / kBinsPerT));
             }
         }
     }
-    const uint64_t b = wave_max_u64(static_cast<uint64_t>(top) << 32 | (0xffffffffu - at));
-    if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = b;
     __syncthreads();
-    if (threadIdx.x == 0) a.best[blockIdx.x] = std::max(std::max(sh[0], sh[1]), std::max(sh[2], sh[3]));
-}
-
-// ------------------------------------------------------------------ 2: the histogram
-
-template <typename T>
-__global__ __launch_bounds__(256) void sample_hist(SampleArgs a) {
-    __shared__ uint32_t count[kBins];
-    __shared__ unsigned long long weight[kBins];
-    const int64_t r = blockIdx.x / static_cast<uint32_t>(a.n_hist);
-    const int32_t part = static_cast<int32_t>(blockIdx.x - static_cast<uint32_t>(r) * static_cast<uint32_t>(a.n_hist));
-    const Row w = row_of(a, r);
-    if (w.greedy || !(w.by_k || w.by_p)) return;
-    const float top = value_of(static_cast<uint32_t>(row_best(a, r) >> 32));
-    for (int i = static_cast<int>(threadIdx.x); i < kBins; i += 256) {
-        count[i] = 0;
-        weight[i] = 0;
+    const u64 mine = bins[tid];
+    a.bins[static_cast<int64_t>(blockIdx.x) * kBins + tid] = mine;
+    const double sum = static_cast<double>(mine >> a.count_bits) * ldexp(exp(tid * (-1.0 / kBinsPerT)), -a.fixed) + further;
+    const double sums = wave_sum_f64(sum);
+    const uint32_t counts = wave_scan(n);
+    if (lane == 63) {
+        sh_sum[tid >> 6] = sums;
+        sh_count[tid >> 6] = counts;
     }
     __syncthreads();
-    const T* row = static_cast<const T*>(a.logits) + r * a.stride;
-    const int32_t end = static_cast<int32_t>(std::min<int64_t>(a.vocab, static_cast<int64_t>(part + 1) * a.hist_tokens));
-    for (int32_t i = part * a.hist_tokens + static_cast<int32_t>(threadIdx.x) * 8; i < end; i += kBlockTokens) {
-        float x[8];
-        load8(row, i, a.vocab, x);
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            if (key_of(x[e]) <= kMinusInf) continue;
-            const int b = bin_of(x[e], top, w.bins);
-            atomicAdd(&count[b], 1u);
-            atomicAdd(&weight[b], static_cast<unsigned long long>(fixed_of(weight_of(x[e], top, w.inv_t), a.fixed)));
+    if (tid == 0) {
+        double all = 0.0;
+        uint32_t many = 0;
+        for (int i = 0; i < kThreads / 64; i++) {
+            all += sh_sum[i];
+            many += sh_count[i];
+        }
+        out->count = many;
+        out->weight = all;
+    }
+}
+
+// ------------------------------------------------------------------ the row's histogram
+
+// Thread t's bin of the row, counted down from the largest's: its tokens and their weights, relative to the row's largest.
+// sh_off, sh_n, sh_by: by part, a round of kThreads parts at a time.
+__device__ __forceinline__ void row_bin(const SampleArgs& a, int64_t r, const Row& w, float top, int* sh_off, uint32_t* sh_n, double* sh_by, uint32_t* count,
+                                        double* weight, uint32_t* all, double* total) {
+    const int t = static_cast<int>(threadIdx.x);
+    const double place = place_of(top, w.inv_t);
+    // (weights are sums in units of the largest's own fixed-point weight: equal logits sum up to whole numbers)
+    const double unit = static_cast<double>(fixed_of(edge_weight<false>(place - floor(place)), ldexp(1.0, a.fixed)));
+    uint32_t n = 0, n_all = 0;
+    double s = 0.0, s_all = 0.0;
+    for (int32_t i0 = 0; i0 < a.parts; i0 += kThreads) {
+        const int32_t here = std::min(a.parts - i0, kThreads);
+        __syncthreads();
+        if (t < here) {
+            const Part p = a.part[r * a.parts + i0 + t];
+            const uint32_t key = static_cast<uint32_t>(p.best >> 32);
+            const int off = key <= kMinusInf ? -1 : bin_at(place_of(value_of(key), w.inv_t), place);
+            sh_off[t] = off;
+            sh_by[t] = off < 0 ? 0.0 : p.weight * (off < kBins - 1 ? exp(off * (-1.0 / kBinsPerT)) : exp((floor(place_of(value_of(key), w.inv_t)) - floor(place)) * (1.0 / kBinsPerT)));
+            sh_n[t] = off < 0 ? 0u : p.count;
+        }
+        __syncthreads();
+#pragma unroll 16
+        for (int32_t i = 0; i < here; i++) {
+            const int off = sh_off[i], b = t - off;
+            u64 x = a.bins[(r * a.parts + i0 + i) * kBins + (b < 0 || off < 0 ? 0 : b)];
+            x = off >= 0 && b >= 0 && t < kBins - 1 ? x : 0;
+            n += static_cast<uint32_t>(x & ((u64(1) << a.count_bits) - 1));
+            s += static_cast<double>(x >> a.count_bits);
+            s_all += sh_by[i];
+            n_all += sh_n[i];
         }
     }
-    __syncthreads();
-    for (int i = static_cast<int>(threadIdx.x); i < kBins; i += 256) {
-        a.counts[static_cast<int64_t>(blockIdx.x) * kBins + i] = count[i];
-        a.weights[static_cast<int64_t>(blockIdx.x) * kBins + i] = weight[i];
-    }
+    *count = n;
+    *weight = s * exp(t * (-1.0 / kBinsPerT)) / unit;
+    *all = n_all;
+    *total = ldexp(s_all, a.fixed) / unit;
 }
 
-// ------------------------------------------------------------------ 3: the cuts
+// ------------------------------------------------------------------ 2: kept blocks' sums, and the list
 
-constexpr int kCutThreads = 1024;
+// The smallest logit of the bins up to b, down from place `top`'s: a logit is of those if it is at least that (b = -1: none
+// is). By a wave, 64 keys a step.
+__device__ __forceinline__ float bin_value(int b, double top, double inv_t) {
+    if (b < 0) return __builtin_nanf("");
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t lo = b < kBins - 1 ? kMinusInf + 1 : 0xff800000u, hi = 0xff800000u;  // (of infinity)
+    while (lo < hi) {
+        const uint32_t step = (hi - lo + 63) / 64, k = hi - lo < lane * step ? hi : lo + lane * step;
+        const uint64_t in = __ballot(bin_at(place_of(value_of(k), inv_t), top) <= b);
+        const int l = in ? __builtin_ctzll(in) : 64;
+        const uint32_t next = static_cast<uint32_t>(l) * step;
+        if (l < 64) hi = hi - lo < next ? hi : lo + next;
+        if (l > 0) lo = hi - lo < next - step + 1 ? hi : lo + next - step + 1;
+    }
+    return b < kBins - 1 ? value_of(hi) : -__FLT_MAX__;
+}
 
-struct CutShared {
-    uint64_t list[kListed];  // ~key << 32 | index: ascending is the order of the cuts
-    unsigned long long weight[kBins];
-    uint32_t count[kBins];
-    uint64_t scan[kCutThreads / 64];
-    uint64_t before_weight, taken_weight;
-    uint32_t before_count, n, at;
-    uint32_t key;
-    int32_t last;
-};
-
-__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {
-    const int lane = static_cast<int>(threadIdx.x) & 63;
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sample_sums(SampleArgs a) {
+    __shared__ uint32_t sh_count[kThreads / 64];
+    __shared__ double sh_weight[kThreads / 64];
+    __shared__ Found f_sh;
+    __shared__ int32_t first_sh[3][kThreads / 64], off_sh[kThreads];
+    __shared__ uint32_t n_sh[kThreads];
+    __shared__ double by_sh[kThreads];  // by part; then by bin
+    __shared__ float value_sh[4];
+    const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
+    const int64_t r = blockIdx.x / static_cast<uint32_t>(a.parts);
+    const int32_t part = static_cast<int32_t>(blockIdx.x - static_cast<uint32_t>(r) * static_cast<uint32_t>(a.parts));
+    const Row w = row_of(a, r);
+    if (w.greedy) return;
+    const uint32_t best = static_cast<uint32_t>(row_best(a, r) >> 32);
+    if (best <= kMinusInf) return;
+    const float top = value_of(best);
+    const double place = place_of(top, w.inv_t);
+    int32_t lo = kBins, hi = -1, bin_k = -1;
+    bool lists = false;
+    if (w.cuts()) {
+        uint32_t n, all;
+        double s, total;
+        row_bin(a, r, w, top, off_sh, n_sh, by_sh, &n, &s, &all, &total);
+        // (the last bin: what the others leave)
+        uint32_t counts = block_scan(sh_count, n);
+        double weights = block_scan(sh_weight, s);
+        if (tid == kBins - 1) {
+            n = all - counts;
+            s = total > weights ? total - weights : 0.0;
+            counts = all;
+            weights += s;
+        }
+        const bool by_k = w.by_k && static_cast<uint32_t>(w.k) < all;
+        // The first bins of which something holds, the last where it holds of none.
+        auto note = [&](int which, bool is) {
+            const uint64_t in = __ballot(is);
+            if (lane == 0) first_sh[which][wave] = in ? 64 * wave + __builtin_ctzll(in) : kBins - 1;
+        };
+        auto noted = [&](int which) {
+            int32_t v = kBins - 1;
 #pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-        const uint64_t o = static_cast<uint64_t>(__shfl_up(static_cast<unsigned long long>(v), m));
-        v += lane >= m ? o : 0;
+            for (int i = 0; i < kThreads / 64; i++) v = std::min(v, first_sh[which][i]);
+            return v;
+        };
+        note(0, by_k && counts >= static_cast<uint32_t>(w.k));
+        if (tid == 0) {
+            f_sh.listed = 0;
+            f_sh.need = 0;
+            f_sh.below_k = 0.0;
+        }
+        __syncthreads();
+        bin_k = by_k ? noted(0) : -1;
+        // The sum of what top-k leaves lies between that without its bin and that with it.
+        if (tid == bin_k) {
+            f_sh.below_k = weights - s;
+            f_sh.total = weights;
+            f_sh.need = static_cast<uint32_t>(w.k) - (counts - n);
+        }
+        __syncthreads();
+        if (w.by_p) {
+            // (a little more either way: the list's weights are not rounded as the histogram's)
+            note(1, n && weights >= w.p * (by_k ? f_sh.below_k : total) * (1.0 - 0x1p-28));
+            note(2, n && weights >= w.p * (by_k ? f_sh.total : total) * (1.0 + 0x1p-28));
+            __syncthreads();
+            lo = noted(1);
+            hi = noted(2);
+            if (by_k && hi > bin_k) hi = bin_k;
+            if (lo > hi) lo = hi;
+        } else if (by_k) {
+            lo = hi = bin_k;
+        }
+        lists = lo < kBins;
+        if (lists) {
+            const uint32_t here = wave_scan((tid >= lo && tid <= hi) || tid == bin_k ? n : 0u);
+            if (lane == 63 && here) atomicAdd(&f_sh.listed, here);
+            if (tid == lo) f_sh.below_lo = weights - s;
+            __syncthreads();
+            if (f_sh.listed > kListed) lists = false;
+        }
+        if (part == 0 && tid == 0) {
+            Found f = f_sh;
+            f.lo = lo;
+            f.hi = hi;
+            f.bin_k = bin_k;
+            f.total = total;
+            a.found[r] = f;
+        }
     }
-    return v;
-}
-// The sum of the threads' values up to each thread's own.
-__device__ __forceinline__ uint64_t block_scan(CutShared& sh, uint64_t v) {
-    const int wave = static_cast<int>(threadIdx.x) >> 6;
-    v = wave_scan_u64(v);
+    // Of rows without cuts every token weighs in: e^((z - z of the largest) / 32) by the bin's e^(-b / 32) and the polynomial.
+    const bool whole = lo == kBins;
     __syncthreads();
-    if ((threadIdx.x & 63) == 63) sh.scan[wave] = v;
+    if (whole) by_sh[tid] = exp(tid * (-1.0 / kBinsPerT)) / edge_weight<true>(place - floor(place));
+    // Of the others few do: a comparison of the logits tells which.
+    if (!whole && wave < 4) {
+        const float v = bin_value(wave == 0 ? lo - 1 : wave == 1 ? hi : bin_k > hi ? bin_k - (wave == 2) : -1, place, w.inv_t);
+        if (lane == 0) value_sh[wave] = v;
+    }
+    const double per = kBinsPerT * w.inv_t, first = floor(place);
     __syncthreads();
-    for (int i = 0; i < wave; i++) v += sh.scan[i];
-    return v;
+    const float least_lo = value_sh[0], least_hi = value_sh[1], most_k = value_sh[2], least_k = value_sh[3];
+    const T* row = static_cast<const T*>(a.logits) + r * a.stride;
+    const int32_t begin = part * a.part_tokens, end = static_cast<int32_t>(std::min<int64_t>(a.vocab, static_cast<int64_t>(begin) + a.part_tokens));
+    for (int32_t i0 = begin; i0 < end; i0 += kStepTokens) {
+        const int32_t i = i0 + tid * 8;
+        float x[8];
+        load8(row, std::min(i, a.vocab), a.vocab, x);
+        double sum = 0.0;
+        if (whole) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const double z = fmin(static_cast<double>(x[e]) * per, 1e300), g = floor(z);
+                const int b = static_cast<int>(fmax(fmin(first - g, kBins - 1.0), 0.0));
+                double y = by_sh[b] * edge_weight<true>(z - g);
+                if (b == kBins - 1) y = weight_of(x[e], top, w.inv_t);
+                if (x[e] == top) y = 1.0;
+                sum += x[e] > -__builtin_inff() && y >= w.min_p ? y : 0.0;
+            }
+        } else {
+            uint32_t picked = 0;  // tokens of the list
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                if (x[e] >= least_lo) {
+                    const double y = weight_of(x[e], top, w.inv_t);
+                    sum += y >= w.min_p ? y : 0.0;
+                } else if (x[e] >= least_hi || (x[e] >= least_k && !(x[e] >= most_k))) {
+                    picked |= 1u << e;
+                }
+            }
+            if (lists && __any(picked != 0)) {
+                const uint32_t mine = static_cast<uint32_t>(__popc(picked)), upto = wave_scan(mine);
+                uint32_t from = 0;
+                if (lane == 63) from = atomicAdd(a.listed + r, upto);
+                uint32_t to = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(from), 63)) + upto - mine;
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (picked >> e & 1u) {
+                        if (to < kListed) a.list[r * kListed + to] = static_cast<uint64_t>(~key_of(x[e])) << 32 | static_cast<uint32_t>(i + e);
+                        to++;
+                    }
+            }
+        }
+        sum = wave_sum_f64(sum);
+        __syncthreads();
+        if (lane == 0) sh_weight[wave] = sum;
+        __syncthreads();
+        const int block = i0 / kBlockTokens + tid;
+        if (tid < kStepTokens / kBlockTokens && block < a.n_blocks)
+            a.sums[r * a.n_blocks + block] = (sh_weight[4 * tid] + sh_weight[4 * tid + 1]) + (sh_weight[4 * tid + 2] + sh_weight[4 * tid + 3]);
+    }
 }
+
+// ------------------------------------------------------------------ 3: the cuts, and the token
+
+// The order of the cuts: ascending.
+__device__ __forceinline__ u64 order_of(uint32_t key, int32_t i) { return static_cast<u64>(~key) << 32 | static_cast<uint32_t>(i); }
+__device__ __forceinline__ float ordered_value(u64 x) { return value_of(~static_cast<uint32_t>(x >> 32)); }
+
+struct PickShared {
+    u64 list[kListed];
+    u64 weight[kBins];
+    uint32_t count[kBins];
+    u64 few[kRanked], sorted[kRanked];
+    uint32_t scan[kThreads / 64];
+    double scan_f[kThreads / 64];
+    u64 least, most, cut;
+    double before, taken, left;
+    uint32_t before_n, n, at;
+    int32_t block;
+};
 
 // A cut: after `need` tokens (by_count), or where the weights' sum first reaches `target`.
 struct Goal {
@@ -238,298 +537,183 @@ struct Goal {
     uint32_t need;
     double target;
 };
-__device__ __forceinline__ bool reached(const Goal& g, uint64_t count, uint64_t weight) {
-    return g.by_count ? count >= g.need : static_cast<double>(weight) >= g.target;
-}
 
-// Of n groups in sh.count / sh.weight, in order, the one that reaches the goal, from `count0` tokens and `weight0` before
-// the first (none does: the last that has tokens). Leaves sh.at, and what stands before it.
-__device__ __forceinline__ void find_group(CutShared& sh, const Goal& g, int n, uint32_t count0, uint64_t weight0) {
-    const int i = static_cast<int>(threadIdx.x);
-    const uint64_t c = i < n ? sh.count[i] : 0, w = i < n ? sh.weight[i] : 0;
-    const uint64_t cs = block_scan(sh, c) + count0, ws = block_scan(sh, w) + weight0;
-    if (i == 0) sh.at = 0xffffffffu;
-    __syncthreads();
-    if (i < n && c && reached(g, cs, ws)) atomicMin(&sh.at, static_cast<uint32_t>(i));
-    __syncthreads();
-    if (sh.at == 0xffffffffu) {
-        __syncthreads();
-        if (i < n && c) atomicMin(&sh.at, 0xffffffffu - static_cast<uint32_t>(i) - 1u);
-        __syncthreads();
-        if (i == 0) sh.at = sh.at == 0xffffffffu ? 0u : 0xfffffffeu - sh.at;
-        __syncthreads();
-    }
-    if (static_cast<uint32_t>(i) == sh.at) {
-        sh.before_count = static_cast<uint32_t>(cs - c);
-        sh.before_weight = ws - w;
-    }
-    __syncthreads();
-}
-
-// The goal's last token within bin `bin` of the row, `count` tokens of it, before_* in sh: sh.key, sh.last and the
-// weights' sum with it, sh.taken_weight.
-template <typename T>
-__device__ void cut_bin(const SampleArgs& a, CutShared& sh, const Row& w, const T* row, float top, const Goal& g, int bin, uint32_t count) {
+// Of tokens (each(f) calls f(its place in the order) for every one, at most n of them) the last that the goal takes,
+// before_n tokens of the sum `before` coming before them: its place; the sum with it in sh.taken. More than a few are
+// narrowed first, to one of 1024 equal parts of the order's range and again, by histograms in fixed point.
+template <typename Each>
+__device__ u64 find_cut(PickShared& sh, const Row& w, float top, int fixed, const Goal& g, uint32_t n, uint32_t before_n, double before, Each&& each) {
     const int tid = static_cast<int>(threadIdx.x);
-    uint32_t prefix = 0, mask = 0;
-    auto each = [&](auto&& f) __attribute__((always_inline)) {
-        for (int32_t i = tid * 8; i < a.vocab; i += kCutThreads * 8) {
-            float x[8];
-            load8(row, i, a.vocab, x);
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const uint32_t k = key_of(x[e]);
-                if (k > kMinusInf && bin_of(x[e], top, w.bins) == bin && (k & mask) == prefix) f(k, x[e], i + e);
-            }
-        }
-    };
-    // More of them than are sorted: the keys' bits, eight at a time.
-    for (int shift = 24; count > kListed && shift >= 0; shift -= 8) {
+    const double units = ldexp(1.0, fixed);
+    u64 lo = 0, hi = ~u64(0);
+    if (n > kRanked) {
         __syncthreads();
-        const uint32_t count0 = sh.before_count;
-        const uint64_t weight0 = sh.before_weight;
-        if (tid < 256) {
+        if (tid == 0) {
+            sh.least = ~u64(0);
+            sh.most = 0;
+        }
+        __syncthreads();
+        u64 least = ~u64(0), most = 0;
+        each([&](u64 x) {
+            least = least < x ? least : x;
+            most = most > x ? most : x;
+        });
+        if (least <= most) {
+            atomicMin(&sh.least, least);
+            atomicMax(&sh.most, most);
+        }
+        __syncthreads();
+        lo = sh.least;
+        hi = sh.most;
+        while (n > kRanked && lo < hi) {
+            const int bits = 64 - __clzll(static_cast<long long>(hi - lo)), shift = bits > 10 ? bits - 10 : 0;
+            __syncthreads();
             sh.count[tid] = 0;
             sh.weight[tid] = 0;
-        }
-        __syncthreads();
-        each([&](uint32_t k, float l, int32_t) {
-            const int at = 255 - static_cast<int>((k >> shift) & 255u);  // (the larger ones first)
-            atomicAdd(&sh.count[at], 1u);
-            atomicAdd(&sh.weight[at], static_cast<unsigned long long>(fixed_of(weight_of(l, top, w.inv_t), a.fixed)));
-        });
-        __syncthreads();
-        find_group(sh, g, 256, count0, weight0);
-        count = sh.count[sh.at];
-        prefix |= (255u - sh.at) << shift;
-        mask |= 255u << shift;
-    }
-    const uint32_t count0 = sh.before_count;
-    const uint64_t weight0 = sh.before_weight;
-    __syncthreads();
-    if (count > kListed) {
-        // All are one value, `prefix`: how many of them, then the index of the last.
-        const uint64_t one = fixed_of(weight_of(value_of(prefix), top, w.inv_t), a.fixed);
-        uint32_t take = count;
-        if (g.by_count) {
-            take = g.need - count0;
-        } else if (one) {
-            const double most = ceil((g.target - static_cast<double>(weight0)) / static_cast<double>(one));
-            take = most < static_cast<double>(count) ? static_cast<uint32_t>(most > 1.0 ? most : 1.0) : count;
-            if (take > 1 && reached(g, 0, weight0 + (take - 1) * one)) take--;  // (the quotient's rounding)
-        }
-        uint64_t past = 0;
-        for (int32_t i0 = 0; i0 < a.vocab && past < take; i0 += kCutThreads) {
-            const int32_t i = i0 + tid;
-            const bool is = i < a.vocab && key_of(to_f32(row[i])) == prefix;
-            const uint64_t sum = past + block_scan(sh, is ? 1 : 0);
-            if (is && sum == take) sh.last = i;
-            if (tid == kCutThreads - 1) sh.n = static_cast<uint32_t>(sum);
-            __syncthreads();
-            past = sh.n;
-        }
-        if (tid == 0) {
-            sh.key = prefix;
-            sh.taken_weight = weight0 + take * one;
-        }
-        __syncthreads();
-        return;
-    }
-    // The list, sorted (bitonic, over a power of two), then the first place that reaches the goal.
-    if (tid == 0) sh.n = 0;
-    __syncthreads();
-    each([&](uint32_t k, float, int32_t i) {
-        const uint32_t at = atomicAdd(&sh.n, 1u);
-        if (at < kListed) sh.list[at] = static_cast<uint64_t>(~k) << 32 | static_cast<uint32_t>(i);
-    });
-    __syncthreads();
-    const int n = static_cast<int>(std::min<uint32_t>(std::max<uint32_t>(sh.n, 1u), kListed));
-    int size = 2;
-    while (size < n) size *= 2;
-    for (int i = n + tid; i < size; i += kCutThreads) sh.list[i] = ~uint64_t(0);
-    __syncthreads();
-    for (int run = 2; run <= size; run *= 2)
-        for (int step = run / 2; step > 0; step /= 2) {
-            for (int i = tid; i < size / 2; i += kCutThreads) {
-                const int lo = 2 * i - (i & (step - 1)), hi = lo + step;
-                const uint64_t x = sh.list[lo], y = sh.list[hi];
-                if ((x > y) == ((lo & run) == 0)) {
-                    sh.list[lo] = y;
-                    sh.list[hi] = x;
-                }
+            if (tid == 0) {
+                sh.at = 0xffffffffu;
+                sh.n = 0;
             }
             __syncthreads();
+            each([&](u64 x) {
+                if (x < lo || x > hi) return;
+                const int to = static_cast<int>((x - lo) >> shift);
+                atomicAdd(&sh.count[to], 1u);
+                atomicAdd(&sh.weight[to], static_cast<u64>(fixed_of(weight_of(ordered_value(x), top, w.inv_t), units)));
+            });
+            __syncthreads();
+            const uint32_t c = sh.count[tid];
+            const double s = static_cast<double>(sh.weight[tid]) / units;
+            const uint32_t cs = before_n + block_scan(sh.scan, c);
+            const double ss = before + block_scan(sh.scan_f, s);
+            if (c) {
+                if (g.by_count ? cs >= g.need : ss >= g.target) atomicMin(&sh.at, static_cast<uint32_t>(tid));
+                atomicMax(&sh.n, static_cast<uint32_t>(tid));
+            }
+            __syncthreads();
+            const uint32_t at = sh.at != 0xffffffffu ? sh.at : sh.n;  // (none reaches it: the last)
+            if (static_cast<uint32_t>(tid) == at) {
+                sh.before_n = cs - c;
+                sh.before = ss - s;
+            }
+            __syncthreads();
+            before_n = sh.before_n;
+            before = sh.before;
+            n = sh.count[at];
+            lo += static_cast<u64>(at) << shift;
+            const u64 last = lo + ((u64(1) << shift) - 1);
+            hi = hi < last ? hi : last;
         }
-    constexpr int PER = kListed / kCutThreads;
-    uint64_t mine[PER], sum = 0;
-#pragma unroll
-    for (int e = 0; e < PER; e++) {
-        const int i = tid * PER + e;
-        mine[e] = i < n ? fixed_of(weight_of(value_of(~static_cast<uint32_t>(sh.list[i] >> 32)), top, w.inv_t), a.fixed) : 0;
-        sum += mine[e];
     }
-    uint64_t at = block_scan(sh, sum) - sum + weight0;
-    if (tid == 0) sh.at = static_cast<uint32_t>(n - 1);
+    // Those, sorted by how many are smaller: four threads to each.
     __syncthreads();
-    uint32_t first = 0xffffffffu;
-    uint64_t upto[PER];
-#pragma unroll
-    for (int e = 0; e < PER; e++) {
-        const int i = tid * PER + e;
-        at += mine[e];
-        upto[e] = at;
-        if (i < n && first == 0xffffffffu && reached(g, static_cast<uint64_t>(count0) + static_cast<uint64_t>(i) + 1, at)) first = static_cast<uint32_t>(i);
+    if (tid == 0) {
+        sh.n = 0;
+        sh.at = 0xffffffffu;
     }
-    if (first != 0xffffffffu) atomicMin(&sh.at, first);
+    sh.count[tid] = 0;
     __syncthreads();
-    if (static_cast<int>(sh.at) / PER == tid) {
-        const uint64_t x = sh.list[sh.at];
-        sh.key = ~static_cast<uint32_t>(x >> 32);
-        sh.last = static_cast<int32_t>(static_cast<uint32_t>(x));
-#pragma unroll
-        for (int e = 0; e < PER; e++)
-            if (tid * PER + e == static_cast<int>(sh.at)) sh.taken_weight = upto[e];
+    each([&](u64 x) {
+        if (x < lo || x > hi) return;
+        const uint32_t at = atomicAdd(&sh.n, 1u);
+        if (at < kRanked) sh.few[at] = x;
+    });
+    __syncthreads();
+    const int many = static_cast<int>(std::min<uint32_t>(sh.n, kRanked));
+    {
+        const int e = tid & (kRanked - 1);
+        const u64 x = sh.few[e];
+        uint32_t rank = 0;
+        for (int j = tid / kRanked; j < many; j += kThreads / kRanked) rank += sh.few[j] < x;
+        if (e < many && rank) atomicAdd(&sh.count[e], rank);
     }
     __syncthreads();
+    if (tid < many) sh.sorted[sh.count[tid]] = sh.few[tid];
+    __syncthreads();
+    const double mine = tid < many ? weight_of(ordered_value(sh.sorted[tid]), top, w.inv_t) : 0.0;
+    const double upto = before + block_scan(sh.scan_f, mine);
+    if (tid < many && (tid == many - 1 || (g.by_count ? before_n + static_cast<uint32_t>(tid) + 1 >= g.need : upto >= g.target)))
+        atomicMin(&sh.at, static_cast<uint32_t>(tid));
+    __syncthreads();
+    if (static_cast<uint32_t>(tid) == sh.at) {
+        sh.taken = upto;
+        sh.cut = sh.sorted[tid];
+    }
+    __syncthreads();
+    return sh.cut;
 }
 
 template <typename T>
-__global__ __launch_bounds__(kCutThreads) void sample_cut(SampleArgs a) {
-    __shared__ CutShared sh;
-    const int64_t r = blockIdx.x;
-    const int tid = static_cast<int>(threadIdx.x);
-    const Row w = row_of(a, r);
-    if (w.greedy) return;
-    if (!(w.by_k || w.by_p)) {
-        if (tid == 0) a.cuts[r] = Cut{kMinusInf, -1};
-        return;
-    }
-    const uint64_t best = row_best(a, r);
-    const uint32_t best_key = static_cast<uint32_t>(best >> 32);
-    if (best_key <= kMinusInf) return;  // nothing to choose from
-    const float top = value_of(best_key);
-    const T* row = static_cast<const T*>(a.logits) + r * a.stride;
-    uint32_t count = 0;
-    uint64_t weight = 0;
-    if (tid < kBins) {
-        for (int32_t i = 0; i < a.n_hist; i++) {
-            count += a.counts[(r * a.n_hist + i) * kBins + tid];
-            weight += a.weights[(r * a.n_hist + i) * kBins + tid];
-        }
-    }
-    const uint64_t counts = block_scan(sh, count), weights = block_scan(sh, weight);
-    if (tid == kCutThreads - 1) {
-        sh.before_count = static_cast<uint32_t>(counts);
-        sh.taken_weight = weights;
-    }
-    __syncthreads();
-    const uint32_t all = sh.before_count;
-    uint64_t total = sh.taken_weight;
-    __syncthreads();
-    auto groups = [&]() {
-        if (tid < kBins) {
-            sh.count[tid] = count;
-            sh.weight[tid] = weight;
-        }
-        __syncthreads();
-    };
-    Cut cut = {kMinusInf, -1};
-    if (w.by_k && static_cast<uint32_t>(w.k) < all) {
-        const Goal g = {true, static_cast<uint32_t>(w.k), 0.0};
-        groups();
-        find_group(sh, g, kBins, 0, 0);
-        const int bin = static_cast<int>(sh.at);
-        const uint32_t n = sh.count[bin];
-        cut_bin(a, sh, w, row, top, g, bin, n);
-        cut = Cut{sh.key, sh.last};
-        total = sh.taken_weight;
-        __syncthreads();
-    }
-    if (w.by_p) {
-        const Goal g = {false, 0, w.p * static_cast<double>(total)};
-        if (!(g.target > 0.0)) {  // the first alone
-            cut = Cut{best_key, static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(best))};
-        } else {
-            groups();
-            find_group(sh, g, kBins, 0, 0);
-            const int bin = static_cast<int>(sh.at);
-            const uint32_t n = sh.count[bin];
-            cut_bin(a, sh, w, row, top, g, bin, n);
-            cut = Cut{sh.key, sh.last};
-        }
-    }
-    if (tid == 0) a.cuts[r] = cut;
-}
-
-// ------------------------------------------------------------------ 4 and 5: the kept weights, and the token
-
-// The weight that token i counts with, 0 if it is cut off.
-__device__ __forceinline__ double kept_weight(float l, int32_t i, float top, const Row& w, const Cut& c) {
-    const uint32_t k = key_of(l);
-    if (k <= kMinusInf || k < c.key || (k == c.key && i > c.last)) return 0.0;
-    const double x = weight_of(l, top, w.inv_t);
-    return x >= w.min_p ? x : 0.0;
-}
-
-__device__ __forceinline__ Cut cut_of(const SampleArgs& a, int64_t r, const Row& w) {
-    return w.by_k || w.by_p ? a.cuts[r] : Cut{kMinusInf, -1};
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void sample_sum(SampleArgs a) {
-    __shared__ double sh[4];
-    const int64_t r = blockIdx.x / static_cast<uint32_t>(a.n_max);
-    const int32_t part = static_cast<int32_t>(blockIdx.x - static_cast<uint32_t>(r) * static_cast<uint32_t>(a.n_max));
-    const Row w = row_of(a, r);
-    if (w.greedy) return;
-    const uint32_t best = static_cast<uint32_t>(row_best(a, r) >> 32);
-    if (best <= kMinusInf) return;
-    const float top = value_of(best);
-    const Cut c = cut_of(a, r, w);
-    const T* row = static_cast<const T*>(a.logits) + r * a.stride;
-    const int32_t end = static_cast<int32_t>(std::min<int64_t>(a.vocab, static_cast<int64_t>(part + 1) * a.max_tokens));
-    for (int32_t i0 = part * a.max_tokens; i0 < end; i0 += kBlockTokens) {
-        const int32_t i = i0 + static_cast<int32_t>(threadIdx.x) * 8;
-        double sum = 0.0;
-        if (i < a.vocab) {
-            float x[8];
-            load8(row, i, a.vocab, x);
-#pragma unroll
-            for (int e = 0; e < 8; e++) sum += kept_weight(x[e], i + e, top, w, c);
-        }
-        sum = wave_sum_f64(sum);
-        __syncthreads();
-        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = sum;
-        __syncthreads();
-        if (threadIdx.x == 0) a.sums[r * a.n_blocks + i0 / kBlockTokens] = (sh[0] + sh[1]) + (sh[2] + sh[3]);
-    }
-}
-
-__device__ __forceinline__ double wave_scan_f64(double v) {
-    const int lane = static_cast<int>(threadIdx.x) & 63;
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-        const double o = __shfl_up(v, m);
-        v += lane >= m ? o : 0.0;
-    }
-    return v;
-}
-
-template <typename T>
-__global__ __launch_bounds__(256) void sample_pick(SampleArgs a) {
-    __shared__ double sh[4], left_sh;
-    __shared__ int32_t block_sh;
-    __shared__ uint32_t found;
+__global__ __launch_bounds__(kThreads) void sample_pick(SampleArgs a) {
+    __shared__ PickShared sh;
     const int64_t r = blockIdx.x;
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
     const Row w = row_of(a, r);
     const uint64_t best = row_best(a, r);
-    const uint32_t best_key = static_cast<uint32_t>(best >> 32), best_at = 0xffffffffu - static_cast<uint32_t>(best);
+    const uint32_t best_key = static_cast<uint32_t>(best >> 32);
     if (best_key <= kMinusInf || w.greedy) {
-        if (tid == 0) a.out[r] = best_key <= kMinusInf ? -1 : static_cast<int32_t>(best_at);
+        if (tid == 0) a.out[r] = best_key <= kMinusInf ? -1 : static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(best));
         return;
     }
-    const double* sums = a.sums + r * a.n_blocks;
+    const float top = value_of(best_key);
+    const T* row = static_cast<const T*>(a.logits) + r * a.stride;
+    double* sums = a.sums + r * a.n_blocks;
+    u64 cut = order_of(kMinusInf + 1, 0x7fffffff);  // what stays: tokens up to it
+    if (w.cuts()) {
+        const Found f = a.found[r];
+        if (f.lo < kBins && f.listed > 0) {
+            const double place = place_of(top, w.inv_t);
+            // The tokens of the cuts' bins: from the list, or, where there are more than it holds (logits much alike, high
+            // temperatures), from the row again, by this workgroup alone.
+            const bool crowded = f.listed > kListed;
+            const int n = crowded ? 0 : static_cast<int>(f.listed);
+            for (int i = tid; i < n; i += kThreads) sh.list[i] = a.list[r * kListed + i];
+            __syncthreads();
+            int b0 = f.lo, b1 = f.hi;
+            auto each = [&](auto&& g) __attribute__((always_inline)) {
+                auto one = [&](float l, u64 x) __attribute__((always_inline)) {
+                    const int b = bin_at(place_of(l, w.inv_t), place);
+                    if (b >= b0 && b <= b1 && x <= cut) g(x);
+                };
+                for (int i = tid; i < n; i += kThreads) one(ordered_value(sh.list[i]), sh.list[i]);
+                if (!crowded) return;
+                for (int32_t i = tid * 8; i < a.vocab; i += kStepTokens) {
+                    float x[8];
+                    load8(row, i, a.vocab, x);
+#pragma unroll 1
+                    for (int e = 0; e < 8; e++)
+                        if (x[e] > -__builtin_inff()) one(x[e], order_of(key_of(x[e]), i + e));
+                }
+            };
+            double total = f.total;
+            if (f.bin_k >= 0) {
+                b0 = b1 = f.bin_k;
+                cut = find_cut(sh, w, top, a.narrow, Goal{true, static_cast<uint32_t>(w.k), 0.0}, f.listed, static_cast<uint32_t>(w.k) - f.need, f.below_k, each);
+                total = sh.taken;
+            }
+            if (w.by_p) {
+                b0 = f.lo;
+                b1 = f.hi;
+                cut = find_cut(sh, w, top, a.narrow, Goal{false, 0, w.p * total}, f.listed, 0, f.below_lo, each);
+            }
+            // The kept ones' weights to their blocks' sums: in fixed point, as they come in any order.
+            b0 = f.lo;
+            b1 = kBins - 1;
+            for (int32_t from = 0; from < a.n_blocks; from += kBins) {
+                __syncthreads();
+                sh.weight[tid] = 0;
+                __syncthreads();
+                each([&](u64 x) {
+                    const int b = static_cast<int>(static_cast<uint32_t>(x) / kBlockTokens) - from;
+                    const double y = weight_of(ordered_value(x), top, w.inv_t);
+                    if (b >= 0 && b < kBins && y >= w.min_p) atomicAdd(&sh.weight[b], static_cast<u64>(fixed_of(y, 0x1p44)));
+                });
+                __syncthreads();
+                if (from + tid < a.n_blocks && sh.weight[tid]) sums[from + tid] += static_cast<double>(sh.weight[tid]) * 0x1p-44;
+            }
+            __syncthreads();
+        }
+    }
     if (wave == 0) {
         double total = 0.0;
         for (int32_t b0 = 0; b0 < a.n_blocks; b0 += 64) total += wave_sum_f64(b0 + lane < a.n_blocks ? sums[b0 + lane] : 0.0);
@@ -540,7 +724,7 @@ __global__ __launch_bounds__(256) void sample_pick(SampleArgs a) {
         int32_t block = -1, last = 0;
         for (int32_t b0 = 0; b0 < a.n_blocks && block < 0; b0 += 64) {
             const double x = b0 + lane < a.n_blocks ? sums[b0 + lane] : 0.0;
-            const double upto = past + wave_scan_f64(x);
+            const double upto = past + wave_scan(x);
             const uint64_t over = __ballot(x > 0.0 && upto > target), some = __ballot(x > 0.0);
             if (some) last = b0 + 63 - __builtin_clzll(some);
             if (over) {
@@ -551,65 +735,60 @@ __global__ __launch_bounds__(256) void sample_pick(SampleArgs a) {
             past = readlane_f64(upto, 63);
         }
         if (lane == 0) {
-            block_sh = block < 0 ? last : block;
-            left_sh = block < 0 ? __builtin_inf() : left;
-            found = 0xffffffffu;
+            sh.block = block < 0 ? last : block;
+            sh.left = block < 0 ? __builtin_inf() : left;
+            sh.at = 0xffffffffu;
+            sh.n = 0;
         }
     }
     __syncthreads();
-    const float top = value_of(best_key);
-    const Cut c = cut_of(a, r, w);
-    const T* row = static_cast<const T*>(a.logits) + r * a.stride;
-    const int32_t i = block_sh * kBlockTokens + tid * 8;
-    double y[8], sum = 0.0;
-    float x[8];
-    load8(row, std::min(i, a.vocab), a.vocab, x);
+    // Two tokens to a thread.
+    constexpr int PER = kBlockTokens / kThreads;
+    const int32_t i0 = sh.block * kBlockTokens + tid * PER;
+    double y[PER], sum = 0.0;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        y[e] = i < a.vocab ? kept_weight(x[e], i + e, top, w, c) : 0.0;
+    for (int e = 0; e < PER; e++) {
+        const float l = i0 + e < a.vocab ? to_f32(row[i0 + e]) : -__builtin_inff();
+        y[e] = 0.0;
+        if (l > -__builtin_inff() && order_of(key_of(l), i0 + e) <= cut) y[e] = weight_of(l, top, w.inv_t);
+        if (y[e] < w.min_p) y[e] = 0.0;
         sum += y[e];
     }
-    double at = wave_scan_f64(sum);
-    if (lane == 63) sh[wave] = at;
-    __syncthreads();
-    at -= sum;
-    for (int k = 0; k < wave; k++) at += sh[k];
-    uint32_t last = 0, first = 0xffffffffu;  // (the last one's index and one)
+    double at = block_scan(sh.scan_f, sum) - sum;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
+    for (int e = 0; e < PER; e++) {
         at += y[e];
         if (y[e] > 0.0) {
-            last = static_cast<uint32_t>(i + e) + 1;
-            if (first == 0xffffffffu && at > left_sh) first = static_cast<uint32_t>(i + e);
+            atomicMax(&sh.n, static_cast<uint32_t>(i0 + e));
+            if (at > sh.left) atomicMin(&sh.at, static_cast<uint32_t>(i0 + e));
         }
     }
-    if (first != 0xffffffffu) atomicMin(&found, first);
     __syncthreads();
-    if (found != 0xffffffffu) {
-        if (tid == 0) a.out[r] = static_cast<int32_t>(found);
-        return;
-    }
-    __syncthreads();
-    if (last) atomicMin(&found, 0xffffffffu - last);
-    __syncthreads();
-    if (tid == 0) a.out[r] = found != 0xffffffffu ? static_cast<int32_t>(0xffffffffu - found - 1) : static_cast<int32_t>(best_at);
+    if (tid == 0) a.out[r] = static_cast<int32_t>(sh.at != 0xffffffffu ? sh.at : sh.n);
 }
 
 template <typename T>
-int launch(neko_hip_ctx* ctx, const char* what, const SampleArgs& a, int64_t rows) {
-    const uint32_t parts = static_cast<uint32_t>(rows * a.n_max);
-    hipLaunchKernelGGL((sample_max<T>), dim3(parts), dim3(256), 0, ctx->stream, a);
-    if (int rc = after_launch(ctx, what)) return rc;
-    if (a.top_k || a.top_p) {
-        hipLaunchKernelGGL((sample_hist<T>), dim3(static_cast<uint32_t>(rows * a.n_hist)), dim3(256), 0, ctx->stream, a);
+int launch(neko_hip_ctx* ctx, const char* what, SampleArgs a, int64_t rows) {
+    const SampleArgs all = a;
+    for (int64_t r = 0; r < rows; r += kSlabRows) {
+        const int64_t n = std::min(kSlabRows, rows - r);
+        const uint32_t parts = static_cast<uint32_t>(n * a.parts);
+        auto from = [&](auto* p) { return p ? p + r : p; };
+        a.logits = static_cast<const T*>(all.logits) + r * all.stride;
+        a.temperature = from(all.temperature);
+        a.top_k = from(all.top_k);
+        a.top_p = from(all.top_p);
+        a.min_p = from(all.min_p);
+        a.u = from(all.u);
+        a.out = from(all.out);
+        hipLaunchKernelGGL((sample_parts<T>), dim3(parts), dim3(kThreads), 0, ctx->stream, a);
         if (int rc = after_launch(ctx, what)) return rc;
-        hipLaunchKernelGGL((sample_cut<T>), dim3(static_cast<uint32_t>(rows)), dim3(kCutThreads), 0, ctx->stream, a);
+        hipLaunchKernelGGL((sample_sums<T>), dim3(parts), dim3(kThreads), 0, ctx->stream, a);
+        if (int rc = after_launch(ctx, what)) return rc;
+        hipLaunchKernelGGL((sample_pick<T>), dim3(static_cast<uint32_t>(n)), dim3(kThreads), 0, ctx->stream, a);
         if (int rc = after_launch(ctx, what)) return rc;
     }
-    hipLaunchKernelGGL((sample_sum<T>), dim3(parts), dim3(256), 0, ctx->stream, a);
-    if (int rc = after_launch(ctx, what)) return rc;
-    hipLaunchKernelGGL((sample_pick<T>), dim3(static_cast<uint32_t>(rows)), dim3(256), 0, ctx->stream, a);
-    return after_launch(ctx, what);
+    return NEKO_OK;
 }
 
 }  // namespace
@@ -634,9 +813,9 @@ extern "C" int neko_hip_sample(neko_hip_ctx* ctx, const void* logits, int64_t st
     const size_t span = rows_span(rows, vocab, stride, esz);
     NEKO_REQUIRE(ctx, span != 0, "%s: rows span more than 2^62 bytes", what);
     NEKO_REQUIRE(ctx, !overlaps(tokens, n, logits, span), "%s: tokens may not overlap the logits", what);
-    for (const void* p : {static_cast<const void*>(temperature), static_cast<const void*>(top_k), static_cast<const void*>(top_p),
+    for (const void* q : {static_cast<const void*>(temperature), static_cast<const void*>(top_k), static_cast<const void*>(top_p),
                           static_cast<const void*>(min_p), static_cast<const void*>(u)})
-        NEKO_REQUIRE(ctx, !p || !overlaps(tokens, n, p, n), "%s: tokens may not overlap the settings", what);
+        NEKO_REQUIRE(ctx, !q || !overlaps(tokens, n, q, n), "%s: tokens may not overlap the settings", what);
     SampleArgs a{};
     a.logits = logits;
     a.stride = stride;
@@ -648,32 +827,40 @@ extern "C" int neko_hip_sample(neko_hip_ctx* ctx, const void* logits, int64_t st
     a.out = tokens;
     a.vocab = static_cast<int32_t>(vocab);
     a.n_blocks = static_cast<int32_t>((vocab + kBlockTokens - 1) / kBlockTokens);
-    // About four workgroups to a CU over all rows; a histogram is read again whole, so fewer of those.
-    auto split = [&](int64_t wanted, int32_t* parts, int32_t* tokens_of) {
-        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(a.n_blocks, (wanted + rows - 1) / rows));
-        const int64_t blocks = (a.n_blocks + most - 1) / most;
-        *parts = static_cast<int32_t>((a.n_blocks + blocks - 1) / blocks);
-        *tokens_of = static_cast<int32_t>(blocks * kBlockTokens);
+    // Two workgroups to a CU over all rows, as many as are resident.
+    const int64_t steps = (vocab + kStepTokens - 1) / kStepTokens;
+    const int64_t held = std::min(rows, kSlabRows);
+    const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>(steps, (2LL * ctx->cu_count + held - 1) / held));
+    const int64_t each = std::min<int64_t>(kMostSteps, (steps + wanted - 1) / wanted);
+    a.parts = static_cast<int32_t>((steps + each - 1) / each);
+    a.part_tokens = static_cast<int32_t>(each * kStepTokens);
+    // A bin's number of tokens, up to part_tokens, and above it their weights, each below 1.04 units.
+    auto bits_of = [](int64_t n) {
+        int bits = 0;
+        while ((int64_t(1) << bits) <= n) bits++;
+        return bits;
     };
-    split(4LL * ctx->cu_count, &a.n_max, &a.max_tokens);
-    split(std::min<int64_t>(4LL * ctx->cu_count, 24 * rows), &a.n_hist, &a.hist_tokens);
-    int bits = 0;
-    while ((int64_t(1) << bits) < vocab) bits++;
-    a.fixed = std::min(44, 62 - bits);
-    const size_t best = static_cast<size_t>(rows) * a.n_max * 8, sums = static_cast<size_t>(rows) * a.n_blocks * 8,
-                 hist = static_cast<size_t>(rows) * a.n_hist * kBins, cuts = static_cast<size_t>(rows) * sizeof(Cut);
+    a.count_bits = bits_of(a.part_tokens);
+    a.fixed = std::min(44, 63 - 2 * a.count_bits);
+    a.narrow = std::min(44, 62 - bits_of(vocab));
+    const size_t parts = static_cast<size_t>(held) * a.parts, hist = a.top_k || a.top_p ? parts * kBins : 0;
+    const size_t bytes[] = {parts * sizeof(Part), static_cast<size_t>(held) * a.n_blocks * 8, static_cast<size_t>(held) * sizeof(Found),
+                            hist * 8, hist ? static_cast<size_t>(held) * kListed * 8 : 0, static_cast<size_t>(held) * 4};
+    size_t all = 0;
+    for (size_t b : bytes) all += b;
     void* ws = nullptr;
-    if (int rc = workspace(ctx, best + sums + cuts + hist * 12, &ws)) return rc;
-    char* at = static_cast<char*>(ws);
-    auto take = [&](size_t bytes) {
-        char* p = at;
-        at += bytes;
-        return p;
-    };
-    a.best = reinterpret_cast<uint64_t*>(take(best));
-    a.sums = reinterpret_cast<double*>(take(sums));
-    a.cuts = reinterpret_cast<Cut*>(take(cuts));
-    a.weights = reinterpret_cast<uint64_t*>(take(hist * 8));
-    a.counts = reinterpret_cast<uint32_t*>(take(hist * 4));
+    if (int rc = workspace(ctx, all, &ws)) return rc;
+    void* at[6];
+    char* p = static_cast<char*>(ws);
+    for (int i = 0; i < 6; i++) {
+        at[i] = p;
+        p += bytes[i];
+    }
+    a.part = static_cast<Part*>(at[0]);
+    a.sums = static_cast<double*>(at[1]);
+    a.found = static_cast<Found*>(at[2]);
+    a.bins = static_cast<uint64_t*>(at[3]);
+    a.list = static_cast<uint64_t*>(at[4]);
+    a.listed = static_cast<uint32_t*>(at[5]);
     return dtype == NEKO_DT_F16 ? launch<half_t>(ctx, what, a, rows) : launch<float>(ctx, what, a, rows);
 }

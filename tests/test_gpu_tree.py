@@ -622,7 +622,7 @@ def test_speculative_steps(dev):
         want, a, s = T.attention(q.cpu(), held, t, H, float(np.float32(hd ** -0.5)))
         assert float(((out.cpu().double() - want).abs() - T.bar(want, a, s, max(lens) + 20, hd, "f16"))[: t.rows].max()) <= 0
         for r in range(t.rows):
-            tok, near = T.sample(logits[r].cpu().double().numpy(), float(u[r]), temperature=float(settings["temperature"][r]), top_k=9)
+            tok, near, _ = T.sample(logits[r].cpu().double().numpy(), float(u[r]), temperature=float(settings["temperature"][r]), top_k=9)
             assert sampled[r].item() == tok and near > 1e-9
         roots = []
         for i, (p, n) in enumerate(trees):

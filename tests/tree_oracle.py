@@ -169,18 +169,18 @@ def walk(parents, tokens, sampled, most):
     return path, sampled[path[-1]]
 
 
-def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, shift=0.0):
-    """(token, how near to a border it was decided, relative to the weights' sum) of one row of float64 logits. shift: the
-    place that u times the sum is moved by, relative to the sum."""
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, shift=0.0, shift_p=0.0):
+    """(token, how near to a border it was decided, how near to one top-p cut, relative to the weights' sums) of one row of
+    float64 logits. shift, shift_p: what u and top_p are moved by."""
     x = np.where(np.isnan(logits), -np.inf, logits.astype(np.float64))
     order = np.argsort(-x, kind="stable")
     order = order[x[order] > -np.inf]
     if len(order) == 0:
-        return -1, 1.0
+        return -1, 1.0, 1.0
     top = x[order[0]]
     if not temperature > 0:
-        return int(order[0]), 1.0
-    near = 1.0
+        return int(order[0]), 1.0, 1.0
+    near = near_p = 1.0
 
     def weights(i):
         with np.errstate(invalid="ignore"):
@@ -192,9 +192,9 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, shift=0.0)
     w = weights(order)
     if top_p < 1:
         cum = np.cumsum(w)
-        at = int(np.searchsorted(cum, top_p * w.sum(), side="left")) if top_p > 0 else 0
+        at = min(int(np.searchsorted(cum, (top_p + shift_p) * cum[-1], side="left")), len(cum) - 1) if top_p > 0 else 0
         if top_p > 0:
-            near = min(near, float(np.abs(cum - top_p * w.sum()).min() / w.sum()))
+            near_p = float(np.abs(cum - top_p * cum[-1]).min() / cum[-1])
         order, w = order[: at + 1], w[: at + 1]
     if min_p > 0:
         order = order[w >= min(min_p, 1.0)]
@@ -203,4 +203,4 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, shift=0.0)
     target = max(0.0, (min(max(u, 0.0), 1 - 2.0 ** -24) if u == u else 0.0) + shift) * cum[-1]
     if target > 0:
         near = min(near, float(np.abs(cum - target).min() / cum[-1]))
-    return int(order[min(int(np.searchsorted(cum, target, side="right")), len(order) - 1)]), near
+    return int(order[min(int(np.searchsorted(cum, target, side="right")), len(order) - 1)]), near, near_p
