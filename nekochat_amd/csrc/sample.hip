@@ -10,14 +10,15 @@
 // over a histogram's bin are in fixed point (each weight to 2^-30 of itself or better), whose order does not matter, so
 // atomics in LDS may take any.
 //
-// Launches, several workgroups ("parts") to a row in the first two:
+// Launches, several workgroups ("parts") to a row in 1 and 3:
 //   1 each part's largest logit and, of rows with a top-k or top-p, a histogram of its tokens' number and weight over the
 //     logit, 1024 bins of T / 32 down from its largest's. Bins stand at fixed places of z = 32 l / T, not of the largest,
 //     which no part knows: parts' histograms are shifted and added by whoever reads them. A weight is held relative to its
-//     bin's lower edge, e^(f / 32) with f = z - floor z: a short polynomial and no table, and one atomic for number and sum.
-//   2 every part adds up the row's histogram and finds the bins in which the cuts fall: tokens above those are kept, and
-//     their weights' sums of blocks of 2048 tokens are written; tokens in those bins, some hundreds, are listed
-//   3 one workgroup to a row: the cuts within the list, its kept tokens' weights added to their blocks' sums, and the block
+//     bin's middle, e^(f / 32) with f = z - rint z: a short polynomial and no table, and one atomic for number and sum.
+//   2 one workgroup to a row (with a top-k or top-p): the row's histogram, and the bins in which the cuts fall
+//   3 tokens above those bins are kept, and their weights' sums of blocks of 2048 tokens are written; tokens in them, some
+//     hundreds, are listed
+//   4 one workgroup to a row: the cuts within the list, its kept tokens' weights added to their blocks' sums, and the block
 //     and in it the token that u falls on
 #include <algorithm>
 
@@ -32,8 +33,9 @@ constexpr int kBins = 1024;  // one to a thread; the last holds whatever is furt
 constexpr double kBinsPerT = 32.0;
 constexpr int kBlockTokens = 2048;               // of a sum: 256 threads of 8
 constexpr int kStepTokens = kThreads * 8;        // four blocks
-constexpr int kMostSteps = 8;                    // of a part: its numbers and weights share 64 bits of a bin
+constexpr int kMostSteps = 4;                    // of a part: a thread holds its tokens in registers
 constexpr int kListed = 4096;                    // tokens in the cuts' bins that are held in LDS
+constexpr int kAtOnce = 20;                      // parts' bins that are on their way at once in launch 2
 constexpr int kRanked = 256;                     // of those, what is sorted by ranks
 constexpr int64_t kSlabRows = 1024;              // of a launch: the workspace holds so many
 constexpr uint32_t kMinusInf = 0x007fffffu;      // its key; tokens at or below are left out
@@ -41,7 +43,7 @@ constexpr uint32_t kMinusInf = 0x007fffffu;      // its key; tokens at or below 
 // What launch 1 leaves of a part.
 struct Part {
     uint64_t best;    // key << 32 | ~index of its largest (greedy rows; the others' has no index)
-    double weight;    // its tokens' weights, relative to the lower edge of its largest's bin
+    double weight;    // its tokens' weights, relative to the middle of its largest's bin
     uint32_t count;   // its tokens
     uint32_t unused;
 };
@@ -51,6 +53,9 @@ struct Found {
     int32_t lo, hi, bin_k;
     uint32_t need;
     uint32_t listed;            // tokens of those bins
+    // Logits: at least above_lo, in a bin before lo; at least above_hi, up to hi; at least above_k and not before_k, bin_k's
+    // (where that is past hi). NaN: none.
+    float above_lo, above_hi, above_k, before_k;
     uint32_t unused;
     double below_lo, below_k;   // weights' sums of the bins before lo and bin_k
     double total;               // of the row
@@ -68,9 +73,10 @@ struct SampleArgs {
     int32_t vocab;
     int32_t parts, part_tokens;  // of a row; whole steps
     int32_t n_blocks;            // blocks of a row
+    int32_t groups;              // workgroups of a row in launch 3
     int32_t count_bits;          // the low bits of a bin: its tokens; the others: their weights in units of 2^-fixed
     int32_t fixed;
-    int32_t narrow;              // fixed-point weights of launch 3, relative to the row's largest: units of 2^-narrow
+    int32_t narrow;              // fixed-point weights of launch 4, relative to the row's largest: units of 2^-narrow
     Part* part;                  // [rows][parts]
     uint64_t* bins;              // [rows][parts][kBins]
     Found* found;                // [rows]
@@ -113,20 +119,27 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 }
 
 // A logit's place among the bins, monotone in it as every rounding here is, and the number of its bin down from that of
-// place `top`. (An infinite logit stands at 1e300.)
-__device__ __forceinline__ double place_of(float l, double inv_t) { return fmin(static_cast<double>(l) * (kBinsPerT * inv_t), 1e300); }
-__device__ __forceinline__ int bin_at(double place, double top) { return static_cast<int>(fmax(fmin(floor(top) - floor(place), kBins - 1.0), 0.0)); }
-// e^(f / 32) for 0 <= f < 1: the series, cut off by (1/32)^6 / 6! = 1.3e-12 or (LONG) (1/32)^8 / 8! = 2.3e-17.
+// place `top`. (An infinite logit stands at 1e300; an infinite temperature leaves all finite ones in one bin.)
+__device__ __forceinline__ double bins_per(double inv_t) { return fmax(kBinsPerT * inv_t, 1e-300); }
+__device__ __forceinline__ double place_of(float l, double inv_t) { return fmin(static_cast<double>(l) * bins_per(inv_t), 1e300); }
+__device__ __forceinline__ int bin_at(double place, double top) { return static_cast<int>(fmax(fmin(rint(top) - rint(place), kBins - 1.0), 0.0)); }
+// e^(f / 32) for -1/2 <= f <= 1/2: the series, cut off by (1/64)^5 / 5! = 8e-12 or (LONG) (1/64)^7 / 7! = 5e-17.
 template <bool LONG>
 __device__ __forceinline__ double edge_weight(double f) {
     const double x = f * (1.0 / 32.0);
-    double y = LONG ? __builtin_fma(x, 1.0 / 5040.0, 1.0 / 720.0) : 1.0 / 120.0;
-    if (LONG) y = __builtin_fma(x, y, 1.0 / 120.0);
-    y = __builtin_fma(x, y, 1.0 / 24.0);
+    double y = LONG ? __builtin_fma(x, 1.0 / 720.0, 1.0 / 120.0) : 1.0 / 24.0;
+    if (LONG) y = __builtin_fma(x, y, 1.0 / 24.0);
     y = __builtin_fma(x, y, 1.0 / 6.0);
     y = __builtin_fma(x, y, 0.5);
     y = __builtin_fma(x, y, 1.0);
     return __builtin_fma(x, y, 1.0);
+}
+// The same in fixed point, cut down to units of 2^-fixed and shifted by count_bits, as a bin sums it up: the low bits of
+// its sum with 2^52, whose own high bits come with it.
+constexpr uint64_t kHigh = 0x4330000000000000ull;
+__device__ __forceinline__ uint64_t bin_weight(double f, double units, uint32_t count_mask) {
+    const uint64_t y = __builtin_bit_cast(uint64_t, __builtin_fma(edge_weight<false>(f), units, 0x1p52));
+    return (y & 0xffffffff00000000ull) | (static_cast<uint32_t>(y) & ~count_mask);
 }
 __device__ __forceinline__ double weight_of(float l, float top, double inv_t) {
     const double w = exp((static_cast<double>(l) - static_cast<double>(top)) * inv_t);
@@ -137,18 +150,21 @@ __device__ __forceinline__ uint64_t fixed_of(double w, double units) {
     return __builtin_bit_cast(uint64_t, __builtin_fma(w, units, 0x1p52)) - __builtin_bit_cast(uint64_t, 0x1p52);
 }
 
-// Logits i .. i + 7 of a row of n, -inf past it. Rows may stand at any element.
+// Logits i .. i + 7 of a row, -inf from n on. Rows may stand at any element.
 template <typename T>
-__device__ __forceinline__ void load8(const T* row, int32_t i, int32_t n, float* x) {
+struct Eight {
     T v[8];
+};
+template <typename T>
+__device__ __forceinline__ Eight<T> load8(const T* row, int32_t i, int32_t n) {
+    Eight<T> x;
     if (i + 8 <= n) {
-        __builtin_memcpy(v, row + i, sizeof(v));
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = to_f32(v[e]);
+        __builtin_memcpy(x.v, row + i, sizeof(x.v));
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = i + e < n ? to_f32(row[i + e]) : -__builtin_inff();
+        for (int e = 0; e < 8; e++) x.v[e] = i + e < n ? row[i + e] : static_cast<T>(-__builtin_inff());
     }
+    return x;
 }
 
 __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
@@ -202,14 +218,31 @@ __device__ __forceinline__ V block_scan(V* sh, V v) {
     if (lane == 63) sh[wave] = v;
     __syncthreads();
     const V before = wave_scan(lane < wave ? sh[lane] : V(0));
-    return __shfl(before, 63) + v;
+    if constexpr (sizeof(V) == 8) return readlane_f64(before, 63) + v;
+    else return static_cast<V>(__builtin_amdgcn_readlane(static_cast<int>(before), 63)) + v;
 }
 
 
+// The first (or LAST) thread of which something holds, kThreads (-1) if it holds of none. (Atomics on one address by all
+// threads took 12 us.)
+template <bool LAST>
+__device__ __forceinline__ int block_first(int32_t* sh, bool is) {
+    const int wave = static_cast<int>(threadIdx.x) >> 6;
+    const uint64_t in = __ballot(is);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh[wave] = in ? 64 * wave + (LAST ? 63 - __builtin_clzll(in) : __builtin_ctzll(in)) : LAST ? -1 : kThreads;
+    __syncthreads();
+    int v = sh[0];
+#pragma unroll
+    for (int i = 1; i < kThreads / 64; i++) v = LAST ? std::max(v, sh[i]) : std::min(v, sh[i]);
+    return v;
+}
+
 // ------------------------------------------------------------------ 1: parts' largest and histograms
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_parts(SampleArgs a) {
+// STEPS: of the call's parts.
+template <typename T, int STEPS>
+__global__ __launch_bounds__(kThreads, 8) void sample_parts(SampleArgs a) {
     __shared__ u64 bins[kBins];
     __shared__ uint32_t sh_top[kThreads / 64];
     __shared__ uint32_t sh_at;
@@ -218,16 +251,16 @@ __global__ __launch_bounds__(kThreads) void sample_parts(SampleArgs a) {
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63;
     const int64_t r = blockIdx.x / static_cast<uint32_t>(a.parts);
     const int32_t part = static_cast<int32_t>(blockIdx.x - static_cast<uint32_t>(r) * static_cast<uint32_t>(a.parts));
-    const Row w = row_of(a, r);
-    const T* row = static_cast<const T*>(a.logits) + r * a.stride;
-    const int32_t begin = part * a.part_tokens, end = static_cast<int32_t>(std::min<int64_t>(a.vocab, static_cast<int64_t>(begin) + a.part_tokens));
-    float top = -__builtin_inff();
-    for (int32_t i = begin + tid * 8; i < end; i += kStepTokens) {
-        float x[8];
-        load8(row, i, a.vocab, x);
+    const int32_t begin = part * a.part_tokens + tid * 8;
+    Eight<T> x[STEPS];
 #pragma unroll
-        for (int e = 0; e < 8; e++) top = fmaxf(top, x[e]);  // (the other one of a NaN)
-    }
+    for (int s = 0; s < STEPS; s++) x[s] = load8(static_cast<const T*>(a.logits) + r * a.stride, begin + s * kStepTokens, a.vocab);
+    const Row w = row_of(a, r);
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int s = 0; s < STEPS; s++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) top = fmaxf(top, to_f32(x[s].v[e]));  // (the other one of a NaN)
     bins[tid] = 0;
     if (tid == 0) sh_at = 0xffffffffu;
     uint32_t key = wave_max_u32(key_of(top));
@@ -239,13 +272,11 @@ __global__ __launch_bounds__(kThreads) void sample_parts(SampleArgs a) {
     if (w.greedy) {
         // The first that has it.
         uint32_t at = 0xffffffffu;
-        for (int32_t i = begin + tid * 8; i < end && at == 0xffffffffu; i += kStepTokens) {
-            float x[8];
-            load8(row, i, a.vocab, x);
+#pragma unroll
+        for (int s = STEPS - 1; s >= 0; s--)
 #pragma unroll
             for (int e = 7; e >= 0; e--)
-                if (x[e] == top) at = static_cast<uint32_t>(i + e);
-        }
+                if (to_f32(x[s].v[e]) == top) at = static_cast<uint32_t>(begin + s * kStepTokens + e);
         if (at != 0xffffffffu) atomicMin(&sh_at, at);
         __syncthreads();
         if (tid == 0) out->best = static_cast<uint64_t>(key) << 32 | (0xffffffffu - sh_at);
@@ -256,30 +287,44 @@ __global__ __launch_bounds__(kThreads) void sample_parts(SampleArgs a) {
         if (part == 0) a.listed[r] = 0;
     }
     if (!w.cuts() || key <= kMinusInf) return;
-    const double place = place_of(top, w.inv_t), per = kBinsPerT * w.inv_t, first = floor(place), units = ldexp(1.0, a.fixed);
-    const u64 one = 0x4330000000000000ull;  // the bits of 2^52
+    const double per = bins_per(w.inv_t), first = rint(place_of(top, w.inv_t)), units = ldexp(1.0, a.fixed + a.count_bits);
+    const uint32_t mask = (1u << a.count_bits) - 1;
     double further = 0.0;  // what the last bin's tokens weigh
-    uint32_t n = 0;
-    for (int32_t i = begin + tid * 8; i < end; i += kStepTokens) {
-        float x[8];
-        load8(row, i, a.vocab, x);
+    uint32_t n = 0;        // and how many there are
+#pragma unroll
+    for (int s = 0; s < STEPS; s++) {
+        u64 y[8];
+        int b[8];
+        bool far = false;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            if (!(x[e] > -__builtin_inff())) continue;
-            const double z = fmin(static_cast<double>(x[e]) * per, 1e300), g = floor(z);
-            const int b = static_cast<int>(fmin(first - g, kBins - 1.0));
-            const double y = __builtin_fma(edge_weight<false>(z - g), units, 0x1p52);
-            n++;
-            if (b < kBins - 1) {
-                atomicAdd(&bins[b], ((__builtin_bit_cast(u64, y) - one) << a.count_bits) + 1);
-            } else {
-                further += exp((z - first) * (1.0 / kBinsPerT));
+            const float l = to_f32(x[s].v[e]);
+            const double z = fmin(static_cast<double>(fmaxf(l, -__builtin_inff())) * per, 1e300), g = rint(z);  // (NaN: -inf)
+            b[e] = static_cast<int>(fmin(first - g, kBins - 1.0));
+            y[e] = bin_weight(z - g, units, mask) | 1u;
+            far |= b[e] == kBins - 1 && l > -__builtin_inff();
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (b[e] < kBins - 1) atomicAdd(&bins[b[e]], y[e]);
+        if (__any(far)) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float l = to_f32(x[s].v[e]);
+                if (b[e] == kBins - 1 && l > -__builtin_inff()) {
+                    n++;
+                    further += exp((fmin(static_cast<double>(l) * per, 1e300) - first) * (1.0 / kBinsPerT));
+                }
             }
         }
+        __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
-    const u64 mine = bins[tid];
+    // (without the high bits of each 2^52)
+    u64 mine = bins[tid];
+    mine -= (mine & mask) * kHigh;
     a.bins[static_cast<int64_t>(blockIdx.x) * kBins + tid] = mine;
+    n += static_cast<uint32_t>(mine) & mask;
     const double sum = static_cast<double>(mine >> a.count_bits) * ldexp(exp(tid * (-1.0 / kBinsPerT)), -a.fixed) + further;
     const double sums = wave_sum_f64(sum);
     const uint32_t counts = wave_scan(n);
@@ -300,7 +345,7 @@ __global__ __launch_bounds__(kThreads) void sample_parts(SampleArgs a) {
     }
 }
 
-// ------------------------------------------------------------------ the row's histogram
+// ------------------------------------------------------------------ 2: the cuts' bins
 
 // Thread t's bin of the row, counted down from the largest's: its tokens and their weights, relative to the row's largest.
 // sh_off, sh_n, sh_by: by part, a round of kThreads parts at a time.
@@ -308,40 +353,60 @@ __device__ __forceinline__ void row_bin(const SampleArgs& a, int64_t r, const Ro
                                         double* weight, uint32_t* all, double* total) {
     const int t = static_cast<int>(threadIdx.x);
     const double place = place_of(top, w.inv_t);
-    // (weights are sums in units of the largest's own fixed-point weight: equal logits sum up to whole numbers)
-    const double unit = static_cast<double>(fixed_of(edge_weight<false>(place - floor(place)), ldexp(1.0, a.fixed)));
+    // (in units of the largest's own fixed-point weight)
+    const double unit = static_cast<double>((bin_weight(place - rint(place), ldexp(1.0, a.fixed + a.count_bits), (1u << a.count_bits) - 1) - kHigh) >> a.count_bits);
     uint32_t n = 0, n_all = 0;
-    double s = 0.0, s_all = 0.0;
+    double s = 0.0, s_all = 0.0, edge = 0.0;
+    const uint64_t* bins = a.bins + r * a.parts * kBins;
     for (int32_t i0 = 0; i0 < a.parts; i0 += kThreads) {
         const int32_t here = std::min(a.parts - i0, kThreads);
         __syncthreads();
-        if (t < here) {
-            const Part p = a.part[r * a.parts + i0 + t];
-            const uint32_t key = static_cast<uint32_t>(p.best >> 32);
-            const int off = key <= kMinusInf ? -1 : bin_at(place_of(value_of(key), w.inv_t), place);
-            sh_off[t] = off;
-            sh_by[t] = off < 0 ? 0.0 : p.weight * (off < kBins - 1 ? exp(off * (-1.0 / kBinsPerT)) : exp((floor(place_of(value_of(key), w.inv_t)) - floor(place)) * (1.0 / kBinsPerT)));
-            sh_n[t] = off < 0 ? 0u : p.count;
+        for (int32_t i = t; i < kThreads + kAtOnce; i += kThreads) {  // (past the last: parts that hold nothing)
+            int off = -1;
+            double by = 0.0;
+            uint32_t many = 0;
+            if (i < here) {
+                const Part p = a.part[r * a.parts + i0 + i];
+                const uint32_t key = static_cast<uint32_t>(p.best >> 32);
+                if (key > kMinusInf) {
+                    const double its = place_of(value_of(key), w.inv_t);
+                    off = bin_at(its, place);
+                    by = p.weight * exp((rint(its) - rint(place)) * (1.0 / kBinsPerT));
+                    many = p.count;
+                }
+            }
+            sh_off[i] = off;
+            sh_by[i] = by;
+            sh_n[i] = many;
         }
         __syncthreads();
-#pragma unroll 16
-        for (int32_t i = 0; i < here; i++) {
-            const int off = sh_off[i], b = t - off;
-            u64 x = a.bins[(r * a.parts + i0 + i) * kBins + (b < 0 || off < 0 ? 0 : b)];
-            x = off >= 0 && b >= 0 && t < kBins - 1 ? x : 0;
-            n += static_cast<uint32_t>(x & ((u64(1) << a.count_bits) - 1));
-            s += static_cast<double>(x >> a.count_bits);
-            s_all += sh_by[i];
-            n_all += sh_n[i];
+        for (int32_t i = 0; i < here; i += kAtOnce) {
+            u64 x[kAtOnce];
+#pragma unroll
+            for (int j = 0; j < kAtOnce; j++) {
+                const int off = sh_off[i + j];
+                x[j] = 0;
+                if (off >= 0 && t >= off && t < kBins - 1) {
+                    const uint32_t at = (static_cast<uint32_t>(i0 + i + j) * kBins + static_cast<uint32_t>(t - off)) * 8u;
+                    x[j] = *reinterpret_cast<const u64*>(reinterpret_cast<const char*>(bins) + at);
+                }
+            }
+            if (i0 == 0 && i == 0) edge = exp(t * (-1.0 / kBinsPerT)) / unit;  // (while they are on their way)
+#pragma unroll
+            for (int j = 0; j < kAtOnce; j++) {
+                n += static_cast<uint32_t>(x[j]) & ((1u << a.count_bits) - 1);
+                s += static_cast<double>(x[j] >> a.count_bits);
+                s_all += sh_by[i + j];
+                n_all += sh_n[i + j];
+            }
         }
     }
+    // (the first bin's by a quotient: equal logits sum up to whole numbers)
     *count = n;
-    *weight = s * exp(t * (-1.0 / kBinsPerT)) / unit;
+    *weight = t == 0 ? s / unit : s * edge;
     *all = n_all;
     *total = ldexp(s_all, a.fixed) / unit;
 }
-
-// ------------------------------------------------------------------ 2: kept blocks' sums, and the list
 
 // The smallest logit of the bins up to b, down from place `top`'s: a logit is of those if it is at least that (b = -1: none
 // is). By a wave, 64 keys a step.
@@ -360,159 +425,169 @@ __device__ __forceinline__ float bin_value(int b, double top, double inv_t) {
     return b < kBins - 1 ? value_of(hi) : -__FLT_MAX__;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void sample_sums(SampleArgs a) {
+__global__ __launch_bounds__(kThreads) void sample_find(SampleArgs a) {
     __shared__ uint32_t sh_count[kThreads / 64];
     __shared__ double sh_weight[kThreads / 64];
     __shared__ Found f_sh;
-    __shared__ int32_t first_sh[3][kThreads / 64], off_sh[kThreads];
-    __shared__ uint32_t n_sh[kThreads];
-    __shared__ double by_sh[kThreads];  // by part; then by bin
-    __shared__ float value_sh[4];
+    __shared__ int32_t first_sh[kThreads / 64], off_sh[kThreads + kAtOnce];
+    __shared__ uint32_t n_sh[kThreads + kAtOnce];
+    __shared__ double by_sh[kThreads + kAtOnce];
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
-    const int64_t r = blockIdx.x / static_cast<uint32_t>(a.parts);
-    const int32_t part = static_cast<int32_t>(blockIdx.x - static_cast<uint32_t>(r) * static_cast<uint32_t>(a.parts));
+    const int64_t r = blockIdx.x;
     const Row w = row_of(a, r);
-    if (w.greedy) return;
+    if (!w.cuts()) return;
     const uint32_t best = static_cast<uint32_t>(row_best(a, r) >> 32);
     if (best <= kMinusInf) return;
     const float top = value_of(best);
     const double place = place_of(top, w.inv_t);
     int32_t lo = kBins, hi = -1, bin_k = -1;
-    bool lists = false;
-    if (w.cuts()) {
-        uint32_t n, all;
-        double s, total;
-        row_bin(a, r, w, top, off_sh, n_sh, by_sh, &n, &s, &all, &total);
-        // (the last bin: what the others leave)
-        uint32_t counts = block_scan(sh_count, n);
-        double weights = block_scan(sh_weight, s);
-        if (tid == kBins - 1) {
-            n = all - counts;
-            s = total > weights ? total - weights : 0.0;
-            counts = all;
-            weights += s;
+    uint32_t n, all;
+    double s, total;
+    row_bin(a, r, w, top, off_sh, n_sh, by_sh, &n, &s, &all, &total);
+    // (the last bin: what the others leave)
+    uint32_t counts = block_scan(sh_count, n);
+    double weights = block_scan(sh_weight, s);
+    if (tid == kBins - 1) {
+        n = all - counts;
+        s = total > weights ? total - weights : 0.0;
+        counts = all;
+        weights += s;
+    }
+    const bool by_k = w.by_k && static_cast<uint32_t>(w.k) < all;
+    auto first_bin = [&](bool is) { return std::min(block_first<false>(first_sh, is), kBins - 1); };
+    if (tid == 0) {
+        f_sh.listed = 0;
+        f_sh.need = 0;
+        f_sh.below_k = 0.0;
+    }
+    if (by_k) bin_k = first_bin(counts >= static_cast<uint32_t>(w.k));
+    __syncthreads();
+    // The sum of what top-k leaves lies between that without its bin and that with it.
+    if (tid == bin_k) {
+        f_sh.below_k = weights - s;
+        f_sh.total = weights;
+        f_sh.need = static_cast<uint32_t>(w.k) - (counts - n);
+    }
+    __syncthreads();
+    if (w.by_p) {
+        // (a little more either way: the list's weights are not rounded as the histogram's)
+        lo = first_bin(n && weights >= w.p * (by_k ? f_sh.below_k : total) * (1.0 - 0x1p-28));
+        hi = first_bin(n && weights >= w.p * (by_k ? f_sh.total : total) * (1.0 + 0x1p-28));
+        if (by_k && hi > bin_k) hi = bin_k;
+        if (lo > hi) lo = hi;
+    } else if (by_k) {
+        lo = hi = bin_k;
+    }
+    if (lo < kBins) {
+        const uint32_t here = wave_scan((tid >= lo && tid <= hi) || tid == bin_k ? n : 0u);
+        if (lane == 63 && here) atomicAdd(&f_sh.listed, here);
+        if (tid == lo) f_sh.below_lo = weights - s;
+        if (wave < 4) {
+            const float v = bin_value(wave == 0 ? lo - 1 : wave == 1 ? hi : bin_k > hi ? bin_k - (wave == 3) : -1, place, w.inv_t);
+            if (lane == 0) (wave == 0 ? f_sh.above_lo : wave == 1 ? f_sh.above_hi : wave == 2 ? f_sh.above_k : f_sh.before_k) = v;
         }
-        const bool by_k = w.by_k && static_cast<uint32_t>(w.k) < all;
-        // The first bins of which something holds, the last where it holds of none.
-        auto note = [&](int which, bool is) {
-            const uint64_t in = __ballot(is);
-            if (lane == 0) first_sh[which][wave] = in ? 64 * wave + __builtin_ctzll(in) : kBins - 1;
-        };
-        auto noted = [&](int which) {
-            int32_t v = kBins - 1;
+        __syncthreads();
+    }
+    if (tid == 0) {
+        Found f = f_sh;
+        f.lo = lo;
+        f.hi = hi;
+        f.bin_k = bin_k;
+        f.total = total;
+        a.found[r] = f;
+    }
+}
+
+// ------------------------------------------------------------------ 3: kept blocks' sums, and the list
+
+// STEPS blocks to a workgroup of 256 threads.
+template <typename T, int STEPS>
+__global__ __launch_bounds__(256) void sample_sums(SampleArgs a) {
+    __shared__ double by_sh[64];  // e^(-b / 32) of b = 32 i + j: i's, and j's
+    __shared__ double sh_weight[STEPS][4];
+    const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
+    const int64_t r = blockIdx.x / static_cast<uint32_t>(a.groups);
+    const int32_t group = static_cast<int32_t>(blockIdx.x - static_cast<uint32_t>(r) * static_cast<uint32_t>(a.groups));
+    const int32_t begin = group * STEPS * kBlockTokens + tid * 8;
+    Eight<T> held[STEPS];
 #pragma unroll
-            for (int i = 0; i < kThreads / 64; i++) v = std::min(v, first_sh[which][i]);
-            return v;
-        };
-        note(0, by_k && counts >= static_cast<uint32_t>(w.k));
-        if (tid == 0) {
-            f_sh.listed = 0;
-            f_sh.need = 0;
-            f_sh.below_k = 0.0;
-        }
+    for (int s = 0; s < STEPS; s++) held[s] = load8(static_cast<const T*>(a.logits) + r * a.stride, begin + s * kBlockTokens, a.vocab);
+    const Row w = row_of(a, r);
+    if (w.greedy) return;
+    const uint32_t best = static_cast<uint32_t>(row_best(a, r) >> 32);
+    if (best <= kMinusInf) return;
+    const float top = value_of(best);
+    // Of rows without cuts every token weighs in, of the others few do: a comparison of the logits tells which.
+    Found f;
+    f.lo = kBins;
+    if (w.cuts()) f = a.found[r];
+    const bool whole = f.lo == kBins, lists = !whole && f.listed <= kListed;
+    double sum[STEPS];
+    if (whole) {
+        // e^((z - z of the largest) / 32), by e^(-b / 32) of the bin and the polynomial.
+        const double place = place_of(top, w.inv_t), per = bins_per(w.inv_t), first = rint(place);
+        if (tid < 64) by_sh[tid] = tid < 32 ? exp(-1.0 * tid) / edge_weight<true>(place - first) : exp((tid - 32) * (-1.0 / kBinsPerT));
         __syncthreads();
-        bin_k = by_k ? noted(0) : -1;
-        // The sum of what top-k leaves lies between that without its bin and that with it.
-        if (tid == bin_k) {
-            f_sh.below_k = weights - s;
-            f_sh.total = weights;
-            f_sh.need = static_cast<uint32_t>(w.k) - (counts - n);
-        }
-        __syncthreads();
-        if (w.by_p) {
-            // (a little more either way: the list's weights are not rounded as the histogram's)
-            note(1, n && weights >= w.p * (by_k ? f_sh.below_k : total) * (1.0 - 0x1p-28));
-            note(2, n && weights >= w.p * (by_k ? f_sh.total : total) * (1.0 + 0x1p-28));
-            __syncthreads();
-            lo = noted(1);
-            hi = noted(2);
-            if (by_k && hi > bin_k) hi = bin_k;
-            if (lo > hi) lo = hi;
-        } else if (by_k) {
-            lo = hi = bin_k;
-        }
-        lists = lo < kBins;
-        if (lists) {
-            const uint32_t here = wave_scan((tid >= lo && tid <= hi) || tid == bin_k ? n : 0u);
-            if (lane == 63 && here) atomicAdd(&f_sh.listed, here);
-            if (tid == lo) f_sh.below_lo = weights - s;
-            __syncthreads();
-            if (f_sh.listed > kListed) lists = false;
-        }
-        if (part == 0 && tid == 0) {
-            Found f = f_sh;
-            f.lo = lo;
-            f.hi = hi;
-            f.bin_k = bin_k;
-            f.total = total;
-            a.found[r] = f;
-        }
-    }
-    // Of rows without cuts every token weighs in: e^((z - z of the largest) / 32) by the bin's e^(-b / 32) and the polynomial.
-    const bool whole = lo == kBins;
-    __syncthreads();
-    if (whole) by_sh[tid] = exp(tid * (-1.0 / kBinsPerT)) / edge_weight<true>(place - floor(place));
-    // Of the others few do: a comparison of the logits tells which.
-    if (!whole && wave < 4) {
-        const float v = bin_value(wave == 0 ? lo - 1 : wave == 1 ? hi : bin_k > hi ? bin_k - (wave == 2) : -1, place, w.inv_t);
-        if (lane == 0) value_sh[wave] = v;
-    }
-    const double per = kBinsPerT * w.inv_t, first = floor(place);
-    __syncthreads();
-    const float least_lo = value_sh[0], least_hi = value_sh[1], most_k = value_sh[2], least_k = value_sh[3];
-    const T* row = static_cast<const T*>(a.logits) + r * a.stride;
-    const int32_t begin = part * a.part_tokens, end = static_cast<int32_t>(std::min<int64_t>(a.vocab, static_cast<int64_t>(begin) + a.part_tokens));
-    for (int32_t i0 = begin; i0 < end; i0 += kStepTokens) {
-        const int32_t i = i0 + tid * 8;
-        float x[8];
-        load8(row, std::min(i, a.vocab), a.vocab, x);
-        double sum = 0.0;
-        if (whole) {
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            sum[s] = 0.0;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const double z = fmin(static_cast<double>(x[e]) * per, 1e300), g = floor(z);
-                const int b = static_cast<int>(fmax(fmin(first - g, kBins - 1.0), 0.0));
-                double y = by_sh[b] * edge_weight<true>(z - g);
-                if (b == kBins - 1) y = weight_of(x[e], top, w.inv_t);
-                if (x[e] == top) y = 1.0;
-                sum += x[e] > -__builtin_inff() && y >= w.min_p ? y : 0.0;
+                const float l = fmaxf(to_f32(held[s].v[e]), -__builtin_inff());  // (NaN: -inf)
+                const double z = fmin(static_cast<double>(l) * per, 1e300), g = rint(z);
+                const int b = static_cast<int>(fmin(first - g, kBins - 1.0));
+                double y = by_sh[b >> 5] * by_sh[32 + (b & 31)] * edge_weight<true>(z - g);
+                if (b == kBins - 1) y = l > -__builtin_inff() ? weight_of(l, top, w.inv_t) : 0.0;
+                if (l == top) y = 1.0;
+                sum[s] += y >= w.min_p ? y : 0.0;
             }
-        } else {
-            uint32_t picked = 0;  // tokens of the list
+        }
+    } else {
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            sum[s] = 0.0;
+            uint32_t kept = 0, picked = 0;  // tokens that are surely kept; tokens of the list
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                if (x[e] >= least_lo) {
-                    const double y = weight_of(x[e], top, w.inv_t);
-                    sum += y >= w.min_p ? y : 0.0;
-                } else if (x[e] >= least_hi || (x[e] >= least_k && !(x[e] >= most_k))) {
-                    picked |= 1u << e;
-                }
+                const float l = to_f32(held[s].v[e]);
+                kept |= l >= f.above_lo ? 1u << e : 0u;
+                picked |= l >= f.above_hi || (l >= f.above_k && !(l >= f.before_k)) ? 1u << e : 0u;
+            }
+            picked &= ~kept;
+            auto at = [&](int i) {
+                float l = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) l = i == e ? to_f32(held[s].v[e]) : l;
+                return l;
+            };
+            // One of each lane's at a time: a wave has few of them, and most lanes none.
+            for (uint32_t left = kept; left; left &= left - 1) {
+                const double y = weight_of(at(__builtin_ctz(left)), top, w.inv_t);
+                sum[s] += y >= w.min_p ? y : 0.0;
             }
             if (lists && __any(picked != 0)) {
                 const uint32_t mine = static_cast<uint32_t>(__popc(picked)), upto = wave_scan(mine);
                 uint32_t from = 0;
                 if (lane == 63) from = atomicAdd(a.listed + r, upto);
                 uint32_t to = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(from), 63)) + upto - mine;
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (picked >> e & 1u) {
-                        if (to < kListed) a.list[r * kListed + to] = static_cast<uint64_t>(~key_of(x[e])) << 32 | static_cast<uint32_t>(i + e);
-                        to++;
-                    }
+                for (uint32_t left = picked; left; left &= left - 1, to++) {
+                    const int i = __builtin_ctz(left);
+                    if (to < kListed) a.list[r * kListed + to] = static_cast<uint64_t>(~key_of(at(i))) << 32 | static_cast<uint32_t>(begin + s * kBlockTokens + i);
+                }
             }
         }
-        sum = wave_sum_f64(sum);
-        __syncthreads();
-        if (lane == 0) sh_weight[wave] = sum;
-        __syncthreads();
-        const int block = i0 / kBlockTokens + tid;
-        if (tid < kStepTokens / kBlockTokens && block < a.n_blocks)
-            a.sums[r * a.n_blocks + block] = (sh_weight[4 * tid] + sh_weight[4 * tid + 1]) + (sh_weight[4 * tid + 2] + sh_weight[4 * tid + 3]);
     }
+#pragma unroll
+    for (int s = 0; s < STEPS; s++) {
+        const double x = wave_sum_f64(sum[s]);
+        if (lane == 0) sh_weight[s][wave] = x;
+    }
+    __syncthreads();
+    const int32_t block = group * STEPS + tid;
+    if (tid < STEPS && block < a.n_blocks) a.sums[r * a.n_blocks + block] = (sh_weight[tid][0] + sh_weight[tid][1]) + (sh_weight[tid][2] + sh_weight[tid][3]);
 }
 
-// ------------------------------------------------------------------ 3: the cuts, and the token
+// ------------------------------------------------------------------ 4: the cuts, and the token
 
 // The order of the cuts: ascending.
 __device__ __forceinline__ u64 order_of(uint32_t key, int32_t i) { return static_cast<u64>(~key) << 32 | static_cast<uint32_t>(i); }
@@ -527,8 +602,8 @@ struct PickShared {
     double scan_f[kThreads / 64];
     u64 least, most, cut;
     double before, taken, left;
-    uint32_t before_n, n, at;
-    int32_t block;
+    uint32_t before_n, n;
+    int32_t block, first[kThreads / 64];
 };
 
 // A cut: after `need` tokens (by_count), or where the weights' sum first reaches `target`.
@@ -558,7 +633,9 @@ __device__ u64 find_cut(PickShared& sh, const Row& w, float top, int fixed, cons
             least = least < x ? least : x;
             most = most > x ? most : x;
         });
-        if (least <= most) {
+        least = ~wave_max_u64(~least);
+        most = wave_max_u64(most);
+        if ((tid & 63) == 0 && least <= most) {
             atomicMin(&sh.least, least);
             atomicMax(&sh.most, most);
         }
@@ -570,10 +647,6 @@ __device__ u64 find_cut(PickShared& sh, const Row& w, float top, int fixed, cons
             __syncthreads();
             sh.count[tid] = 0;
             sh.weight[tid] = 0;
-            if (tid == 0) {
-                sh.at = 0xffffffffu;
-                sh.n = 0;
-            }
             __syncthreads();
             each([&](u64 x) {
                 if (x < lo || x > hi) return;
@@ -586,13 +659,9 @@ __device__ u64 find_cut(PickShared& sh, const Row& w, float top, int fixed, cons
             const double s = static_cast<double>(sh.weight[tid]) / units;
             const uint32_t cs = before_n + block_scan(sh.scan, c);
             const double ss = before + block_scan(sh.scan_f, s);
-            if (c) {
-                if (g.by_count ? cs >= g.need : ss >= g.target) atomicMin(&sh.at, static_cast<uint32_t>(tid));
-                atomicMax(&sh.n, static_cast<uint32_t>(tid));
-            }
-            __syncthreads();
-            const uint32_t at = sh.at != 0xffffffffu ? sh.at : sh.n;  // (none reaches it: the last)
-            if (static_cast<uint32_t>(tid) == at) {
+            int at = block_first<false>(sh.first, c && (g.by_count ? cs >= g.need : ss >= g.target));
+            if (at == kThreads) at = block_first<true>(sh.first, c != 0);  // (none reaches it: the last)
+            if (tid == at) {
                 sh.before_n = cs - c;
                 sh.before = ss - s;
             }
@@ -607,10 +676,7 @@ __device__ u64 find_cut(PickShared& sh, const Row& w, float top, int fixed, cons
     }
     // Those, sorted by how many are smaller: four threads to each.
     __syncthreads();
-    if (tid == 0) {
-        sh.n = 0;
-        sh.at = 0xffffffffu;
-    }
+    if (tid == 0) sh.n = 0;
     sh.count[tid] = 0;
     __syncthreads();
     each([&](u64 x) {
@@ -632,10 +698,8 @@ __device__ u64 find_cut(PickShared& sh, const Row& w, float top, int fixed, cons
     __syncthreads();
     const double mine = tid < many ? weight_of(ordered_value(sh.sorted[tid]), top, w.inv_t) : 0.0;
     const double upto = before + block_scan(sh.scan_f, mine);
-    if (tid < many && (tid == many - 1 || (g.by_count ? before_n + static_cast<uint32_t>(tid) + 1 >= g.need : upto >= g.target)))
-        atomicMin(&sh.at, static_cast<uint32_t>(tid));
-    __syncthreads();
-    if (static_cast<uint32_t>(tid) == sh.at) {
+    const int at = block_first<false>(sh.first, tid < many && (tid == many - 1 || (g.by_count ? before_n + static_cast<uint32_t>(tid) + 1 >= g.need : upto >= g.target)));
+    if (tid == at) {
         sh.taken = upto;
         sh.cut = sh.sorted[tid];
     }
@@ -678,11 +742,12 @@ __global__ __launch_bounds__(kThreads) void sample_pick(SampleArgs a) {
                 for (int i = tid; i < n; i += kThreads) one(ordered_value(sh.list[i]), sh.list[i]);
                 if (!crowded) return;
                 for (int32_t i = tid * 8; i < a.vocab; i += kStepTokens) {
-                    float x[8];
-                    load8(row, i, a.vocab, x);
-#pragma unroll 1
-                    for (int e = 0; e < 8; e++)
-                        if (x[e] > -__builtin_inff()) one(x[e], order_of(key_of(x[e]), i + e));
+                    const Eight<T> x = load8(row, i, a.vocab);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float l = to_f32(x.v[e]);
+                        if (l > -__builtin_inff()) one(l, order_of(key_of(l), i + e));
+                    }
                 }
             };
             double total = f.total;
@@ -737,8 +802,6 @@ __global__ __launch_bounds__(kThreads) void sample_pick(SampleArgs a) {
         if (lane == 0) {
             sh.block = block < 0 ? last : block;
             sh.left = block < 0 ? __builtin_inf() : left;
-            sh.at = 0xffffffffu;
-            sh.n = 0;
         }
     }
     __syncthreads();
@@ -755,16 +818,19 @@ __global__ __launch_bounds__(kThreads) void sample_pick(SampleArgs a) {
         sum += y[e];
     }
     double at = block_scan(sh.scan_f, sum) - sum;
+    int32_t mine = -1;  // this thread's first token past u, or its last of any weight
+    bool past = false;
 #pragma unroll
     for (int e = 0; e < PER; e++) {
         at += y[e];
-        if (y[e] > 0.0) {
-            atomicMax(&sh.n, static_cast<uint32_t>(i0 + e));
-            if (at > sh.left) atomicMin(&sh.at, static_cast<uint32_t>(i0 + e));
+        if (y[e] > 0.0 && !past) {
+            mine = i0 + e;
+            past = at > sh.left;
         }
     }
-    __syncthreads();
-    if (tid == 0) a.out[r] = static_cast<int32_t>(sh.at != 0xffffffffu ? sh.at : sh.n);
+    int of = block_first<false>(sh.first, past);
+    if (of == kThreads) of = block_first<true>(sh.first, mine >= 0);
+    if (tid == of) a.out[r] = mine;
 }
 
 template <typename T>
@@ -781,11 +847,22 @@ int launch(neko_hip_ctx* ctx, const char* what, SampleArgs a, int64_t rows) {
         a.min_p = from(all.min_p);
         a.u = from(all.u);
         a.out = from(all.out);
-        hipLaunchKernelGGL((sample_parts<T>), dim3(parts), dim3(kThreads), 0, ctx->stream, a);
+        const dim3 by_row(static_cast<uint32_t>(n));
+        switch (a.part_tokens / kStepTokens) {
+            case 1: hipLaunchKernelGGL((sample_parts<T, 1>), dim3(parts), dim3(kThreads), 0, ctx->stream, a); break;
+            case 2: hipLaunchKernelGGL((sample_parts<T, 2>), dim3(parts), dim3(kThreads), 0, ctx->stream, a); break;
+            default: hipLaunchKernelGGL((sample_parts<T, kMostSteps>), dim3(parts), dim3(kThreads), 0, ctx->stream, a); break;
+        }
         if (int rc = after_launch(ctx, what)) return rc;
-        hipLaunchKernelGGL((sample_sums<T>), dim3(parts), dim3(kThreads), 0, ctx->stream, a);
+        if (a.top_k || a.top_p) {
+            hipLaunchKernelGGL(sample_find, by_row, dim3(kThreads), 0, ctx->stream, a);
+            if (int rc = after_launch(ctx, what)) return rc;
+        }
+        const uint32_t groups = static_cast<uint32_t>(n * a.groups);
+        if (a.groups == a.n_blocks) hipLaunchKernelGGL((sample_sums<T, 1>), dim3(groups), dim3(256), 0, ctx->stream, a);
+        else hipLaunchKernelGGL((sample_sums<T, kMostSteps>), dim3(groups), dim3(256), 0, ctx->stream, a);
         if (int rc = after_launch(ctx, what)) return rc;
-        hipLaunchKernelGGL((sample_pick<T>), dim3(static_cast<uint32_t>(n)), dim3(kThreads), 0, ctx->stream, a);
+        hipLaunchKernelGGL((sample_pick<T>), by_row, dim3(kThreads), 0, ctx->stream, a);
         if (int rc = after_launch(ctx, what)) return rc;
     }
     return NEKO_OK;
@@ -831,9 +908,11 @@ extern "C" int neko_hip_sample(neko_hip_ctx* ctx, const void* logits, int64_t st
     const int64_t steps = (vocab + kStepTokens - 1) / kStepTokens;
     const int64_t held = std::min(rows, kSlabRows);
     const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>(steps, (2LL * ctx->cu_count + held - 1) / held));
-    const int64_t each = std::min<int64_t>(kMostSteps, (steps + wanted - 1) / wanted);
+    const int64_t even = (steps + wanted - 1) / wanted, each = even > 2 ? kMostSteps : even;
     a.parts = static_cast<int32_t>((steps + each - 1) / each);
     a.part_tokens = static_cast<int32_t>(each * kStepTokens);
+    // One block to a workgroup where that leaves CUs free.
+    a.groups = a.n_blocks * held <= 4 * ctx->cu_count ? a.n_blocks : (a.n_blocks + kMostSteps - 1) / kMostSteps;
     // A bin's number of tokens, up to part_tokens, and above it their weights, each below 1.04 units.
     auto bits_of = [](int64_t n) {
         int bits = 0;
