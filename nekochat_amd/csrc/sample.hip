@@ -33,7 +33,8 @@ constexpr int kBins = 1024;  // one to a thread; the last holds whatever is furt
 constexpr double kBinsPerT = 32.0;
 constexpr int kBlockTokens = 2048;               // of a sum: 256 threads of 8
 constexpr int kStepTokens = kThreads * 8;        // four blocks
-constexpr int kMostSteps = 4;                    // of a part: a thread holds its tokens in registers
+constexpr int kMostSteps = 3;                    // of a part: a thread holds its tokens in registers
+constexpr int kMostBlocks = 16;                  // of a workgroup in launch 3
 constexpr int kListed = 4096;                    // tokens in the cuts' bins that are held in LDS
 constexpr int kAtOnce = 20;                      // parts' bins that are on their way at once in launch 2
 constexpr int kRanked = 256;                     // of those, what is sorted by ranks
@@ -73,7 +74,7 @@ struct SampleArgs {
     int32_t vocab;
     int32_t parts, part_tokens;  // of a row; whole steps
     int32_t n_blocks;            // blocks of a row
-    int32_t groups;              // workgroups of a row in launch 3
+    int32_t groups, group_blocks;  // workgroups of a row in launch 3, and their blocks
     int32_t count_bits;          // the low bits of a bin: its tokens; the others: their weights in units of 2^-fixed
     int32_t fixed;
     int32_t narrow;              // fixed-point weights of launch 4, relative to the row's largest: units of 2^-narrow
@@ -500,18 +501,18 @@ __global__ __launch_bounds__(kThreads) void sample_find(SampleArgs a) {
 
 // ------------------------------------------------------------------ 3: kept blocks' sums, and the list
 
-// STEPS blocks to a workgroup of 256 threads.
-template <typename T, int STEPS>
+// Some blocks to a workgroup of 256 threads, the next one's tokens on their way while one's are weighed.
+template <typename T>
 __global__ __launch_bounds__(256) void sample_sums(SampleArgs a) {
     __shared__ double by_sh[64];  // e^(-b / 32) of b = 32 i + j: i's, and j's
-    __shared__ double sh_weight[STEPS][4];
+    __shared__ double sh_weight[kMostBlocks][4];
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
     const int64_t r = blockIdx.x / static_cast<uint32_t>(a.groups);
     const int32_t group = static_cast<int32_t>(blockIdx.x - static_cast<uint32_t>(r) * static_cast<uint32_t>(a.groups));
-    const int32_t begin = group * STEPS * kBlockTokens + tid * 8;
-    Eight<T> held[STEPS];
-#pragma unroll
-    for (int s = 0; s < STEPS; s++) held[s] = load8(static_cast<const T*>(a.logits) + r * a.stride, begin + s * kBlockTokens, a.vocab);
+    const int32_t first_block = group * a.group_blocks, blocks = std::min(a.group_blocks, a.n_blocks - first_block);
+    int32_t i0 = first_block * kBlockTokens + tid * 8;
+    const T* row = static_cast<const T*>(a.logits) + r * a.stride;
+    Eight<T> next = load8(row, i0, a.vocab);
     const Row w = row_of(a, r);
     if (w.greedy) return;
     const uint32_t best = static_cast<uint32_t>(row_best(a, r) >> 32);
@@ -522,34 +523,33 @@ __global__ __launch_bounds__(256) void sample_sums(SampleArgs a) {
     f.lo = kBins;
     if (w.cuts()) f = a.found[r];
     const bool whole = f.lo == kBins, lists = !whole && f.listed <= kListed;
-    double sum[STEPS];
+    const double place = place_of(top, w.inv_t), per = bins_per(w.inv_t), first = rint(place);
     if (whole) {
-        // e^((z - z of the largest) / 32), by e^(-b / 32) of the bin and the polynomial.
-        const double place = place_of(top, w.inv_t), per = bins_per(w.inv_t), first = rint(place);
         if (tid < 64) by_sh[tid] = tid < 32 ? exp(-1.0 * tid) / edge_weight<true>(place - first) : exp((tid - 32) * (-1.0 / kBinsPerT));
         __syncthreads();
-#pragma unroll
-        for (int s = 0; s < STEPS; s++) {
-            sum[s] = 0.0;
+    }
+#pragma unroll 1
+    for (int s = 0; s < blocks; s++, i0 += kBlockTokens) {
+        const Eight<T> x = next;
+        if (s + 1 < blocks) next = load8(row, i0 + kBlockTokens, a.vocab);
+        double sum = 0.0;
+        if (whole) {
+            // e^((z - z of the largest) / 32), by e^(-b / 32) of the bin and the polynomial.
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float l = fmaxf(to_f32(held[s].v[e]), -__builtin_inff());  // (NaN: -inf)
+                const float l = fmaxf(to_f32(x.v[e]), -__builtin_inff());  // (NaN: -inf)
                 const double z = fmin(static_cast<double>(l) * per, 1e300), g = rint(z);
                 const int b = static_cast<int>(fmin(first - g, kBins - 1.0));
                 double y = by_sh[b >> 5] * by_sh[32 + (b & 31)] * edge_weight<true>(z - g);
                 if (b == kBins - 1) y = l > -__builtin_inff() ? weight_of(l, top, w.inv_t) : 0.0;
                 if (l == top) y = 1.0;
-                sum[s] += y >= w.min_p ? y : 0.0;
+                sum += y >= w.min_p ? y : 0.0;
             }
-        }
-    } else {
-#pragma unroll
-        for (int s = 0; s < STEPS; s++) {
-            sum[s] = 0.0;
+        } else {
             uint32_t kept = 0, picked = 0;  // tokens that are surely kept; tokens of the list
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const float l = to_f32(held[s].v[e]);
+                const float l = to_f32(x.v[e]);
                 kept |= l >= f.above_lo ? 1u << e : 0u;
                 picked |= l >= f.above_hi || (l >= f.above_k && !(l >= f.before_k)) ? 1u << e : 0u;
             }
@@ -557,13 +557,13 @@ __global__ __launch_bounds__(256) void sample_sums(SampleArgs a) {
             auto at = [&](int i) {
                 float l = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 8; e++) l = i == e ? to_f32(held[s].v[e]) : l;
+                for (int e = 0; e < 8; e++) l = i == e ? to_f32(x.v[e]) : l;
                 return l;
             };
             // One of each lane's at a time: a wave has few of them, and most lanes none.
             for (uint32_t left = kept; left; left &= left - 1) {
                 const double y = weight_of(at(__builtin_ctz(left)), top, w.inv_t);
-                sum[s] += y >= w.min_p ? y : 0.0;
+                sum += y >= w.min_p ? y : 0.0;
             }
             if (lists && __any(picked != 0)) {
                 const uint32_t mine = static_cast<uint32_t>(__popc(picked)), upto = wave_scan(mine);
@@ -572,19 +572,15 @@ __global__ __launch_bounds__(256) void sample_sums(SampleArgs a) {
                 uint32_t to = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(from), 63)) + upto - mine;
                 for (uint32_t left = picked; left; left &= left - 1, to++) {
                     const int i = __builtin_ctz(left);
-                    if (to < kListed) a.list[r * kListed + to] = static_cast<uint64_t>(~key_of(at(i))) << 32 | static_cast<uint32_t>(begin + s * kBlockTokens + i);
+                    if (to < kListed) a.list[r * kListed + to] = static_cast<uint64_t>(~key_of(at(i))) << 32 | static_cast<uint32_t>(i0 + i);
                 }
             }
         }
-    }
-#pragma unroll
-    for (int s = 0; s < STEPS; s++) {
-        const double x = wave_sum_f64(sum[s]);
-        if (lane == 0) sh_weight[s][wave] = x;
+        sum = wave_sum_f64(sum);
+        if (lane == 0) sh_weight[s][wave] = sum;
     }
     __syncthreads();
-    const int32_t block = group * STEPS + tid;
-    if (tid < STEPS && block < a.n_blocks) a.sums[r * a.n_blocks + block] = (sh_weight[tid][0] + sh_weight[tid][1]) + (sh_weight[tid][2] + sh_weight[tid][3]);
+    if (tid < blocks) a.sums[r * a.n_blocks + first_block + tid] = (sh_weight[tid][0] + sh_weight[tid][1]) + (sh_weight[tid][2] + sh_weight[tid][3]);
 }
 
 // ------------------------------------------------------------------ 4: the cuts, and the token
@@ -859,8 +855,7 @@ int launch(neko_hip_ctx* ctx, const char* what, SampleArgs a, int64_t rows) {
             if (int rc = after_launch(ctx, what)) return rc;
         }
         const uint32_t groups = static_cast<uint32_t>(n * a.groups);
-        if (a.groups == a.n_blocks) hipLaunchKernelGGL((sample_sums<T, 1>), dim3(groups), dim3(256), 0, ctx->stream, a);
-        else hipLaunchKernelGGL((sample_sums<T, kMostSteps>), dim3(groups), dim3(256), 0, ctx->stream, a);
+        hipLaunchKernelGGL((sample_sums<T>), dim3(groups), dim3(256), 0, ctx->stream, a);
         if (int rc = after_launch(ctx, what)) return rc;
         hipLaunchKernelGGL((sample_pick<T>), by_row, dim3(kThreads), 0, ctx->stream, a);
         if (int rc = after_launch(ctx, what)) return rc;
@@ -911,8 +906,9 @@ extern "C" int neko_hip_sample(neko_hip_ctx* ctx, const void* logits, int64_t st
     const int64_t even = (steps + wanted - 1) / wanted, each = even > 2 ? kMostSteps : even;
     a.parts = static_cast<int32_t>((steps + each - 1) / each);
     a.part_tokens = static_cast<int32_t>(each * kStepTokens);
-    // One block to a workgroup where that leaves CUs free.
-    a.groups = a.n_blocks * held <= 4 * ctx->cu_count ? a.n_blocks : (a.n_blocks + kMostSteps - 1) / kMostSteps;
+    // Ten workgroups to a CU, of as many blocks as that takes: twice what is resident, since rows without cuts take longer.
+    a.group_blocks = static_cast<int32_t>(std::clamp<int64_t>((a.n_blocks * held + 10 * ctx->cu_count - 1) / (10 * ctx->cu_count), 1, kMostBlocks));
+    a.groups = (a.n_blocks + a.group_blocks - 1) / a.group_blocks;
     // A bin's number of tokens, up to part_tokens, and above it their weights, each below 1.04 units.
     auto bits_of = [](int64_t n) {
         int bits = 0;
