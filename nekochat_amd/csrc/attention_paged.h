@@ -71,7 +71,10 @@ __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
 
 // The item of workgroup j of a kv head (SPLIT: the j-th tile that has splits, its first one), by every wave for itself:
 // sequences' tiles and splits are summed 64 * K at a time, K of them to a lane. False past the last.
-template <bool SPLIT, int K>
+// TREE: as many splits as are resident at once and no more. A tree's sequence is all tiles of one length, and with a few
+// workgroups past those the launch takes as long as with as many again (16 trees of up to 64 rows over up to 8192 keys: 616
+// of 512 84 us, @@).
+template <bool SPLIT, bool TREE, int K>
 __device__ __forceinline__ bool attn_find_by(const Paged& p, const AttnTiling& t, uint32_t j, AttnItem* it) {
     const int32_t lane = static_cast<int32_t>(threadIdx.x) & 63;
     const int32_t reach = paged_reach(p);
@@ -86,7 +89,7 @@ __device__ __forceinline__ bool attn_find_by(const Paged& p, const AttnTiling& t
         }
     };
     if (K == 1) load(0);
-    const int32_t chunk = attn_plan(t, p, [&](double& work, int64_t& n) {
+    int32_t chunk = attn_plan(t, p, [&](double& work, int64_t& n) {
         work = 0.0;  // (whole numbers below 2^53: exact)
         uint32_t all = 0;
         for (int32_t base = 0; base < p.n_seq; base += 64 * K) {
@@ -101,6 +104,22 @@ __device__ __forceinline__ bool attn_find_by(const Paged& p, const AttnTiling& t
         work = wave_sum_f64(work) * p.n_kv;
         n = static_cast<int64_t>(all) * p.n_kv;
     });
+    if (TREE && K == 1 && chunk < kUnsplit) {
+        // 64 chunks from this one to about twice it, one to a lane (a quotient's rounding may count a split too many or few).
+        const int32_t step = chunk / 64 + 1;
+        const float by = __builtin_amdgcn_rcpf(static_cast<float>(chunk + lane * step));
+        const float n = static_cast<float>(tiles[0]), of = static_cast<float>(units[0]);
+        float blocks = 0.0f, all = 0.0f;
+        for (int32_t s = 0; s < p.n_seq; s++) {
+            const float n1 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, n), s));
+            const float of1 = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, of), s));
+            blocks = __builtin_fmaf(n1, ceilf(of1 * by), blocks);
+            all += n1;
+        }
+        const float room = static_cast<float>(t.target) * __builtin_amdgcn_rcpf(static_cast<float>(p.n_kv)) * 1.0001f;
+        const uint64_t fits = __ballot(blocks <= room);
+        if (__builtin_amdgcn_readfirstlane(all < room)) chunk += (fits ? __builtin_ctzll(fits) : 63) * step;
+    }
     uint32_t past_tiles = 0, past = 0;  // of the sequences before
     for (int32_t base = 0; base < p.n_seq; base += 64 * K) {
         if (K > 1) load(base);
@@ -153,9 +172,9 @@ __device__ __forceinline__ bool attn_find_by(const Paged& p, const AttnTiling& t
     return false;
 }
 // One sequence to a lane where that holds the batch, else eight, whose loads wait for each other no more.
-template <bool SPLIT>
+template <bool SPLIT, bool TREE>
 __device__ __forceinline__ bool attn_find(const Paged& p, const AttnTiling& t, uint32_t j, AttnItem* it) {
-    return p.n_seq <= 64 ? attn_find_by<SPLIT, 1>(p, t, j, it) : attn_find_by<SPLIT, 8>(p, t, j, it);
+    return p.n_seq <= 64 ? attn_find_by<SPLIT, TREE, 1>(p, t, j, it) : attn_find_by<SPLIT, TREE, 8>(p, t, j, it);
 }
 
 // The keys that a tile's rows see, first and last row: row i sees [lo(i), hi(i)).

@@ -85,7 +85,7 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
     __shared__ int32_t item_sh[16];
     if (wave == 0) {
         AttnItem f;
-        const bool found = attn_find<false>(a.p, a.t, item, &f);
+        const bool found = attn_find<false, TREE>(a.p, a.t, item, &f);
         if (found) {
             const SeqRows r = paged_seq(a.p, f.s);
             const TileKeys k = TREE ? tree_tile_keys(a, r, f) : tile_keys(a, r, f);
@@ -496,13 +496,13 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
 
 // Joins the splits of one tile, eight rows of 128 dimensions to a workgroup: DH / 4 lanes to a row, four dimensions
 // each, the partial results of eight splits asked for at once.
-template <typename TQ, int DH>
+template <typename TQ, int DH, bool TREE>
 __global__ __launch_bounds__(256) void attn_paged_merge(PagedAttnArgs a) {
     constexpr int LPR = DH / 4, RPB = 256 / LPR, AHEAD = 8;
     int kvh;
     const uint32_t item = item_of(a, &kvh);
     AttnItem it;
-    if (!attn_find<true>(a.p, a.t, item, &it)) return;
+    if (!attn_find<true, TREE>(a.p, a.t, item, &it)) return;
     const SeqRows r = paged_seq(a.p, it.s);
     const int d = static_cast<int>(threadIdx.x) % LPR * 4;
     const int i = static_cast<int>(blockIdx.y) * RPB + static_cast<int>(threadIdx.x) / LPR;
@@ -611,7 +611,8 @@ int launch_dims(neko_hip_ctx* ctx, const char* what, PagedAttnArgs a, int dtype)
         if (!attn_may_split(x.t, x.p)) return NEKO_OK;
         const int64_t tiles = attn_split_tiles_bound(x.t, x.p.rows, x.p.n_seq, x.p.n_kv) * x.p.n_kv;
         const dim3 grid(static_cast<uint32_t>(tiles), static_cast<uint32_t>((DH << x.t.tile_log2) / 1024));
-        hipLaunchKernelGGL((attn_paged_merge<TQ, DH>), grid, dim3(256), 0, ctx->stream, x);
+        if (x.words > 0) hipLaunchKernelGGL((attn_paged_merge<TQ, DH, true>), grid, dim3(256), 0, ctx->stream, x);
+        else hipLaunchKernelGGL((attn_paged_merge<TQ, DH, false>), grid, dim3(256), 0, ctx->stream, x);
         return after_launch(ctx, what);
     };
     if (many) {

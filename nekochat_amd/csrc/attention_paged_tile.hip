@@ -87,7 +87,7 @@ __global__ __launch_bounds__(256, DH <= 64 && sizeof(TQ) == 2 ? 3 : DH <= 128 ? 
     int kvh;
     const uint32_t item = item_of(a, &kvh);
     AttnItem it;
-    if (!attn_find<false>(a.p, a.t, item, &it)) return;
+    if (!attn_find<false, TREE>(a.p, a.t, item, &it)) return;
     const SeqRows r = paged_seq(a.p, it.s);
     const TileKeys tk = TREE ? tree_tile_keys(a, r, it) : tile_keys(a, r, it);
     const int hd = a.p.hd;
