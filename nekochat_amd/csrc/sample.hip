@@ -35,6 +35,7 @@ constexpr int kBlockTokens = 2048;               // of a sum: 256 threads of 8
 constexpr int kStepTokens = kThreads * 8;        // four blocks
 constexpr int kMostSteps = 3;                    // of a part: a thread holds its tokens in registers
 constexpr int kMostBlocks = 16;                  // of a workgroup in launch 3
+constexpr int kGroupListed = 512;                // tokens of its own that one lists in LDS first
 constexpr int kListed = 4096;                    // tokens in the cuts' bins that are held in LDS
 constexpr int kAtOnce = 20;                      // parts' bins that are on their way at once in launch 2
 constexpr int kRanked = 256;                     // of those, what is sorted by ranks
@@ -49,7 +50,7 @@ struct Part {
     uint32_t unused;
 };
 
-// What launch 2 finds of a row: cuts that fall into bins lo .. hi (top-p) and by_k (top-k: after `need` of its tokens).
+// What launch 2 finds of a row (of one without cuts, `best` alone): cuts that fall into bins lo .. hi (top-p) and by_k (top-k: after `need` of its tokens).
 struct Found {
     int32_t lo, hi, bin_k;
     uint32_t need;
@@ -57,7 +58,8 @@ struct Found {
     // Logits: at least above_lo, in a bin before lo; at least above_hi, up to hi; at least above_k and not before_k, bin_k's
     // (where that is past hi). NaN: none.
     float above_lo, above_hi, above_k, before_k;
-    uint32_t unused;
+    uint32_t few;               // all tokens that may stay are listed, up to kRanked
+    uint64_t best;              // as of launch 1, over the row's parts
     double below_lo, below_k;   // weights' sums of the bins before lo and bin_k
     double total;               // of the row
 };  // (weights relative to the row's largest)
@@ -169,22 +171,21 @@ __device__ __forceinline__ Eight<T> load8(const T* row, int32_t i, int32_t n) {
 }
 
 __device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
-#pragma unroll
-    for (int m = 1; m < 64; m *= 2) {
-        const uint64_t o = static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(v), m));
-        v = v > o ? v : o;
-    }
-    return v;
+    const uint32_t hi = static_cast<uint32_t>(v >> 32), most = wave_max_u32(hi);
+    return static_cast<uint64_t>(most) << 32 | wave_max_u32(hi == most ? static_cast<uint32_t>(v) : 0u);
 }
 
 // The largest logit of a row, from launch 1's parts, by every wave for itself: key << 32 | ~index.
-__device__ __forceinline__ uint64_t row_best(const SampleArgs& a, int64_t r) {
+__device__ __forceinline__ uint64_t best_of_parts(const SampleArgs& a, int64_t r) {
     uint64_t b = 0;
     for (int32_t i = static_cast<int32_t>(threadIdx.x) & 63; i < a.parts; i += 64) {
         const uint64_t o = a.part[r * a.parts + i].best;
         b = b > o ? b : o;
     }
     return wave_max_u64(b);
+}
+__device__ __forceinline__ uint64_t row_best(const SampleArgs& a, int64_t r) {
+    return a.top_k || a.top_p ? a.found[r].best : best_of_parts(a, r);
 }
 
 typedef unsigned long long u64;
@@ -349,8 +350,8 @@ __global__ __launch_bounds__(kThreads, 8) void sample_parts(SampleArgs a) {
 // ------------------------------------------------------------------ 2: the cuts' bins
 
 // Thread t's bin of the row, counted down from the largest's: its tokens and their weights, relative to the row's largest.
-// sh_off, sh_n, sh_by: by part, a round of kThreads parts at a time.
-__device__ __forceinline__ void row_bin(const SampleArgs& a, int64_t r, const Row& w, float top, int* sh_off, uint32_t* sh_n, double* sh_by, uint32_t* count,
+// sh_off, sh_n, sh_by: by part, a round of kThreads parts at a time. held: where there are at most 64, each lane's.
+__device__ __forceinline__ void row_bin(const SampleArgs& a, int64_t r, const Row& w, float top, const Part& held, int* sh_off, uint32_t* sh_n, double* sh_by, uint32_t* count,
                                         double* weight, uint32_t* all, double* total) {
     const int t = static_cast<int>(threadIdx.x);
     const double place = place_of(top, w.inv_t);
@@ -362,12 +363,12 @@ __device__ __forceinline__ void row_bin(const SampleArgs& a, int64_t r, const Ro
     for (int32_t i0 = 0; i0 < a.parts; i0 += kThreads) {
         const int32_t here = std::min(a.parts - i0, kThreads);
         __syncthreads();
-        for (int32_t i = t; i < kThreads + kAtOnce; i += kThreads) {  // (past the last: parts that hold nothing)
+        for (int32_t i = t; i < here + kAtOnce; i += kThreads) {  // (past the last: parts that hold nothing)
             int off = -1;
             double by = 0.0;
             uint32_t many = 0;
             if (i < here) {
-                const Part p = a.part[r * a.parts + i0 + i];
+                const Part p = a.parts <= 64 ? held : a.part[r * a.parts + i0 + i];
                 const uint32_t key = static_cast<uint32_t>(p.best >> 32);
                 if (key > kMinusInf) {
                     const double its = place_of(value_of(key), w.inv_t);
@@ -436,15 +437,20 @@ __global__ __launch_bounds__(kThreads) void sample_find(SampleArgs a) {
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
     const int64_t r = blockIdx.x;
     const Row w = row_of(a, r);
-    if (!w.cuts()) return;
-    const uint32_t best = static_cast<uint32_t>(row_best(a, r) >> 32);
-    if (best <= kMinusInf) return;
-    const float top = value_of(best);
+    Part held = {};
+    if (a.parts <= 64 && lane < a.parts) held = a.part[r * a.parts + lane];
+    const uint64_t best = a.parts <= 64 ? wave_max_u64(held.best) : best_of_parts(a, r);
+    const uint32_t best_key = static_cast<uint32_t>(best >> 32);
+    if (!w.cuts() || best_key <= kMinusInf) {
+        if (tid == 0) a.found[r].best = best;
+        return;
+    }
+    const float top = value_of(best_key);
     const double place = place_of(top, w.inv_t);
     int32_t lo = kBins, hi = -1, bin_k = -1;
     uint32_t n, all;
     double s, total;
-    row_bin(a, r, w, top, off_sh, n_sh, by_sh, &n, &s, &all, &total);
+    row_bin(a, r, w, top, held, off_sh, n_sh, by_sh, &n, &s, &all, &total);
     // (the last bin: what the others leave)
     uint32_t counts = block_scan(sh_count, n);
     double weights = block_scan(sh_weight, s);
@@ -458,6 +464,7 @@ __global__ __launch_bounds__(kThreads) void sample_find(SampleArgs a) {
     auto first_bin = [&](bool is) { return std::min(block_first<false>(first_sh, is), kBins - 1); };
     if (tid == 0) {
         f_sh.listed = 0;
+        f_sh.few = 0;
         f_sh.need = 0;
         f_sh.below_k = 0.0;
     }
@@ -480,11 +487,17 @@ __global__ __launch_bounds__(kThreads) void sample_find(SampleArgs a) {
         lo = hi = bin_k;
     }
     if (lo < kBins) {
-        const uint32_t here = wave_scan((tid >= lo && tid <= hi) || tid == bin_k ? n : 0u);
+        // Where all that may stay is little it is listed whole, and launch 4 needs no sums.
+        const int32_t end = by_k ? bin_k : hi;
+        if (tid == end && counts <= kRanked) f_sh.few = counts;
+        __syncthreads();
+        const bool few = f_sh.few != 0;
+        const uint32_t here = few ? 0u : wave_scan((tid >= lo && tid <= hi) || tid == bin_k ? n : 0u);
         if (lane == 63 && here) atomicAdd(&f_sh.listed, here);
         if (tid == lo) f_sh.below_lo = weights - s;
         if (wave < 4) {
-            const float v = bin_value(wave == 0 ? lo - 1 : wave == 1 ? hi : bin_k > hi ? bin_k - (wave == 3) : -1, place, w.inv_t);
+            const int b = wave == 0 ? lo - 1 : wave == 1 ? hi : bin_k > hi ? bin_k - (wave == 3) : -1;
+            const float v = bin_value(few ? (wave == 1 ? end : -1) : b, place, w.inv_t);
             if (lane == 0) (wave == 0 ? f_sh.above_lo : wave == 1 ? f_sh.above_hi : wave == 2 ? f_sh.above_k : f_sh.before_k) = v;
         }
         __syncthreads();
@@ -495,6 +508,8 @@ __global__ __launch_bounds__(kThreads) void sample_find(SampleArgs a) {
         f.hi = hi;
         f.bin_k = bin_k;
         f.total = total;
+        f.best = best;
+        if (f.few) f.listed = f.few;
         a.found[r] = f;
     }
 }
@@ -506,6 +521,8 @@ template <typename T>
 __global__ __launch_bounds__(256) void sample_sums(SampleArgs a) {
     __shared__ double by_sh[64];  // e^(-b / 32) of b = 32 i + j: i's, and j's
     __shared__ double sh_weight[kMostBlocks][4];
+    __shared__ u64 list_sh[kGroupListed];
+    __shared__ uint32_t n_sh, from_sh;
     const int tid = static_cast<int>(threadIdx.x), lane = tid & 63, wave = tid >> 6;
     const int64_t r = blockIdx.x / static_cast<uint32_t>(a.groups);
     const int32_t group = static_cast<int32_t>(blockIdx.x - static_cast<uint32_t>(r) * static_cast<uint32_t>(a.groups));
@@ -524,6 +541,8 @@ __global__ __launch_bounds__(256) void sample_sums(SampleArgs a) {
     if (w.cuts()) f = a.found[r];
     const bool whole = f.lo == kBins, lists = !whole && f.listed <= kListed;
     const double place = place_of(top, w.inv_t), per = bins_per(w.inv_t), first = rint(place);
+    if (tid == 0) n_sh = 0;
+    if (!whole) __syncthreads();
     if (whole) {
         if (tid < 64) by_sh[tid] = tid < 32 ? exp(-1.0 * tid) / edge_weight<true>(place - first) : exp((tid - 32) * (-1.0 / kBinsPerT));
         __syncthreads();
@@ -568,11 +587,17 @@ __global__ __launch_bounds__(256) void sample_sums(SampleArgs a) {
             if (lists && __any(picked != 0)) {
                 const uint32_t mine = static_cast<uint32_t>(__popc(picked)), upto = wave_scan(mine);
                 uint32_t from = 0;
-                if (lane == 63) from = atomicAdd(a.listed + r, upto);
+                if (lane == 63) from = atomicAdd(&n_sh, upto);
                 uint32_t to = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(from), 63)) + upto - mine;
                 for (uint32_t left = picked; left; left &= left - 1, to++) {
                     const int i = __builtin_ctz(left);
-                    if (to < kListed) a.list[r * kListed + to] = static_cast<uint64_t>(~key_of(at(i))) << 32 | static_cast<uint32_t>(i0 + i);
+                    const u64 x = static_cast<u64>(~key_of(at(i))) << 32 | static_cast<uint32_t>(i0 + i);
+                    if (to < kGroupListed) {
+                        list_sh[to] = x;
+                    } else {
+                        const uint32_t k = atomicAdd(a.listed + r, 1u);
+                        if (k < kListed) a.list[r * kListed + k] = x;
+                    }
                 }
             }
         }
@@ -580,6 +605,14 @@ __global__ __launch_bounds__(256) void sample_sums(SampleArgs a) {
         if (lane == 0) sh_weight[s][wave] = sum;
     }
     __syncthreads();
+    if (lists) {
+        // (one place in the list for all: a wave that asks for its own waits 2 us for it)
+        const uint32_t n = std::min<uint32_t>(n_sh, kGroupListed);
+        if (tid == 0 && n) from_sh = atomicAdd(a.listed + r, n);
+        __syncthreads();
+        for (uint32_t i = tid; i < n; i += 256)
+            if (from_sh + i < kListed) a.list[r * kListed + from_sh + i] = list_sh[i];
+    }
     if (tid < blocks) a.sums[r * a.n_blocks + first_block + tid] = (sh_weight[tid][0] + sh_weight[tid][1]) + (sh_weight[tid][2] + sh_weight[tid][3]);
 }
 
@@ -594,6 +627,7 @@ struct PickShared {
     u64 weight[kBins];
     uint32_t count[kBins];
     u64 few[kRanked], sorted[kRanked];
+    double few_weight[kRanked];
     uint32_t scan[kThreads / 64];
     double scan_f[kThreads / 64];
     u64 least, most, cut;
@@ -608,6 +642,19 @@ struct Goal {
     uint32_t need;
     double target;
 };
+
+// The rank of thread e's number of sh.few (e < n <= kRanked) among the n, all different: four threads to each. sh.count
+// holds it afterwards.
+__device__ __forceinline__ void rank_few(PickShared& sh, int n) {
+    const int tid = static_cast<int>(threadIdx.x), e = tid & (kRanked - 1);
+    if (tid < kRanked) sh.count[tid] = 0;
+    __syncthreads();
+    const u64 x = sh.few[e];
+    uint32_t rank = 0;
+    for (int j = tid / kRanked; j < n; j += kThreads / kRanked) rank += sh.few[j] < x;
+    if (e < n && rank) atomicAdd(&sh.count[e], rank);
+    __syncthreads();
+}
 
 // Of tokens (each(f) calls f(its place in the order) for every one, at most n of them) the last that the goal takes,
 // before_n tokens of the sum `before` coming before them: its place; the sum with it in sh.taken. More than a few are
@@ -670,10 +717,9 @@ __device__ u64 find_cut(PickShared& sh, const Row& w, float top, int fixed, cons
             hi = hi < last ? hi : last;
         }
     }
-    // Those, sorted by how many are smaller: four threads to each.
+    // Those, sorted by how many are smaller.
     __syncthreads();
     if (tid == 0) sh.n = 0;
-    sh.count[tid] = 0;
     __syncthreads();
     each([&](u64 x) {
         if (x < lo || x > hi) return;
@@ -682,14 +728,7 @@ __device__ u64 find_cut(PickShared& sh, const Row& w, float top, int fixed, cons
     });
     __syncthreads();
     const int many = static_cast<int>(std::min<uint32_t>(sh.n, kRanked));
-    {
-        const int e = tid & (kRanked - 1);
-        const u64 x = sh.few[e];
-        uint32_t rank = 0;
-        for (int j = tid / kRanked; j < many; j += kThreads / kRanked) rank += sh.few[j] < x;
-        if (e < many && rank) atomicAdd(&sh.count[e], rank);
-    }
-    __syncthreads();
+    rank_few(sh, many);
     if (tid < many) sh.sorted[sh.count[tid]] = sh.few[tid];
     __syncthreads();
     const double mine = tid < many ? weight_of(ordered_value(sh.sorted[tid]), top, w.inv_t) : 0.0;
@@ -701,6 +740,42 @@ __device__ u64 find_cut(PickShared& sh, const Row& w, float top, int fixed, cons
     }
     __syncthreads();
     return sh.cut;
+}
+
+// The token of a row of which everything that may stay is listed.
+__device__ __forceinline__ void pick_few(const SampleArgs& a, PickShared& sh, int64_t r, const Row& w, float top, const Found& f) {
+    const int tid = static_cast<int>(threadIdx.x);
+    const int n = static_cast<int>(std::min<uint32_t>(f.few, kRanked));
+    if (tid < n) sh.few[tid] = a.list[r * kListed + tid];
+    __syncthreads();
+    rank_few(sh, n);
+    if (tid < n) sh.sorted[sh.count[tid]] = sh.few[tid];
+    __syncthreads();
+    const u64 x = tid < n ? sh.sorted[tid] : 0;
+    const double y = tid < n ? weight_of(ordered_value(x), top, w.inv_t) : 0.0;
+    const double upto = block_scan(sh.scan_f, y);
+    int stay = f.bin_k >= 0 ? std::min(n, w.k) : n;
+    if (tid == stay - 1) sh.taken = upto;
+    __syncthreads();
+    if (w.by_p) stay = std::min(stay, block_first<false>(sh.first, tid < stay && upto >= w.p * (f.bin_k >= 0 ? sh.taken : f.total)) + 1);
+    const bool stays = tid < stay && y >= w.min_p;
+    // The same by index.
+    if (tid < n) sh.few[tid] = stays ? static_cast<uint32_t>(x) : ~u64(0) - static_cast<u64>(tid);
+    __syncthreads();
+    rank_few(sh, n);
+    if (tid < n) {
+        sh.sorted[sh.count[tid]] = static_cast<uint32_t>(x);
+        sh.few_weight[sh.count[tid]] = stays ? y : 0.0;
+    }
+    __syncthreads();
+    const double mine = tid < n ? sh.few_weight[tid] : 0.0, at = block_scan(sh.scan_f, mine);
+    if (tid == n - 1) sh.left = at;
+    __syncthreads();
+    const float u = a.u[r];
+    const double target = (u > 0.0f ? static_cast<double>(fminf(u, 0x1.fffffep-1f)) : 0.0) * sh.left;
+    int of = block_first<false>(sh.first, mine > 0.0 && at > target);
+    if (of == kThreads) of = block_first<true>(sh.first, mine > 0.0);
+    if (tid == of) a.out[r] = static_cast<int32_t>(sh.sorted[tid]);
 }
 
 template <typename T>
@@ -721,6 +796,10 @@ __global__ __launch_bounds__(kThreads) void sample_pick(SampleArgs a) {
     u64 cut = order_of(kMinusInf + 1, 0x7fffffff);  // what stays: tokens up to it
     if (w.cuts()) {
         const Found f = a.found[r];
+        if (f.lo < kBins && f.few > 0) {
+            pick_few(a, sh, r, w, top, f);
+            return;
+        }
         if (f.lo < kBins && f.listed > 0) {
             const double place = place_of(top, w.inv_t);
             // The tokens of the cuts' bins: from the list, or, where there are more than it holds (logits much alike, high
