@@ -73,7 +73,7 @@ __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v) {
 // sequences' tiles and splits are summed 64 * K at a time, K of them to a lane. False past the last.
 // TREE: as many splits as are resident at once and no more. A tree's sequence is all tiles of one length, and with a few
 // workgroups past those the launch takes as long as with as many again (16 trees of up to 64 rows over up to 8192 keys: 616
-// of 512 84 us, @@).
+// of 512 84 us, no more than these 74).
 template <bool SPLIT, bool TREE, int K>
 __device__ __forceinline__ bool attn_find_by(const Paged& p, const AttnTiling& t, uint32_t j, AttnItem* it) {
     const int32_t lane = static_cast<int32_t>(threadIdx.x) & 63;

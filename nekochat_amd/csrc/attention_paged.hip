@@ -18,7 +18,8 @@
 //
 // What bounds it: with many keys the reading of them, two sequences of 65521 tokens (32 / 8 heads of 128, f16) in 51 us,
 // 5.3 TB/s of codes, and 5 for the merge; with fewer, launches and loads that wait for each other (32 ragged ones of up to
-// 4096 tokens 18.1 us, one of 777 11.0).
+// 4096 tokens 18.1 us, one of 777 11.0). Of drafted trees, two of 7
+// tokens (28 rows) over 65500 53 us and 6 for the merge, one of 26 over 777 12.3.
 #include <algorithm>
 #include <atomic>
 
@@ -37,6 +38,18 @@ constexpr int kFewRows = 32;        // flattened rows up to which a sequence is 
 // f32: faster up to 8 and mostly to 30 (1024 rows 45 and 59), level from there to 40, 1.2 times as long at 67.
 template <typename TQ>
 constexpr double kFewPairs = sizeof(TQ) == 2 ? 20e6 : 40e6;
+// Drafted trees: two 16-row tiles to a workgroup where that is work enough, which halves what is loaded and converted, and
+// sequences of more rows before the tiles of 128 are faster. 150 batches of 8 to 256 rows a sequence. f16 and 128
+// dimensions: from 8 million pairs on faster (64 trees of 32 rows over 1500 keys 119 us one by one, 65 by two; 4 of 64 over
+// 30000 189 and 87; 16 of 32 over 6000 68 and 52), and where the tiles one by one are more than are resident (16 of 128 rows
+// over 300 20.4 and 15.6); slower below (one of 32 over 3000 16.7 and 17.2, 16 of 32 over 300 8.8 and 11.3). 64 dimensions
+// have twice the waves: from 20 million (16 of 64 rows over 1500 32.7 and 35.3, 16 of 32 over 6000 60 and 45).
+// The tiles of 128 against two of 16: f16, 64 trees of 64 rows over 1500 keys 133 us and 97, 4 of 96 over 30000 104 and
+// 124; f32, whose conversion of q costs the tiles more, 4 of 96 over 30000 163 and 141, 64 of 128 over 1500 193 and 178.
+template <typename TQ>
+constexpr int kFewTreeRows = sizeof(TQ) == 2 ? 64 : 128;
+template <int DH>
+constexpr double kTwoPairs = DH <= 64 ? 20e6 : 8e6;
 constexpr int kSpareRows = 256;     // flattened rows past one token to a sequence that still make a decoding batch
 
 template <int N>
@@ -52,8 +65,8 @@ struct KvTile {
 };
 
 // Waves per SIMD that the kernel is compiled for.
-template <typename TQ, int DH>
-constexpr int kResident = DH <= 64 ? 4 : DH <= 128 ? 3 : 1;
+template <typename TQ, int DH, int RT = 1>
+constexpr int kResident = DH <= 64 ? (RT == 1 ? 4 : 3) : DH <= 128 ? (RT == 1 ? 3 : 2) : 1;
 
 // Four dimensions, from d on, of a finished row.
 template <typename TQ>
@@ -66,16 +79,17 @@ __device__ __forceinline__ void store_row(const PagedAttnArgs& a, const SeqRows&
     __builtin_memcpy(static_cast<TQ*>(a.out) + static_cast<int64_t>(r.begin + tok) * a.os + static_cast<int64_t>(head) * a.p.hd + d, v, sizeof(v));
 }
 
-// TREE: rows of drafted trees (attention_paged.h).
-template <typename TQ, int DH, int NW, bool MODS, bool TREE>
-__global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kResident<TQ, DH>)) void attn_paged_kernel(PagedAttnArgs a) {
+// TREE: rows of drafted trees (attention_paged.h). RT: 16-row tiles that a workgroup takes at once, each key's codes loaded
+// and converted once for all.
+template <typename TQ, int DH, int NW, bool MODS, bool TREE, int RT>
+__global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH, RT> ? NW / 4 : kResident<TQ, DH, RT>)) void attn_paged_kernel(PagedAttnArgs a) {
     constexpr bool kTwo = sizeof(TQ) == 4;
     constexpr int NU = DH / 64, NE = DH / 16, VW = DH / 64;
     constexpr int kRow = DH + 4;  // floats of a row in LDS
     extern __shared__ __align__(16) float o_sh[];  // [NW][16][kRow]
     __shared__ float m_sh[NW][16], l_sh[NW][16], seen_sh[NW][16];
-    __shared__ half8 q_sh[kTwo ? 2 : 1][2 * NU][64];
-    __shared__ float sc_sh[16];
+    __shared__ half8 q_sh[RT][kTwo ? 2 : 1][2 * NU][64];
+    __shared__ float sc_sh[RT][16];
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6);
     const int c = lane & 15, g4 = lane >> 4;
@@ -111,20 +125,29 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
     const TileKeys tk = {shared_at(7), shared_at(8), shared_at(9), shared_at(10), shared_at(11), shared_at(12)};
     const int hd = a.p.hd;
 
-    // This lane's row (rows past the last repeat it and are not written).
+    // This lane's rows (those past the last repeat it and are not written).
     const int32_t n_rows = r.n * a.t.group;
-    const int32_t row = min((it.tile << 4) + c, n_rows - 1);
-    const int32_t tok = static_cast<int32_t>(fast_div(static_cast<uint32_t>(row), a.by_group));
-    const int head = kvh * a.t.group + (row - tok * a.t.group);
-    const int32_t depth = TREE ? tree_depth(a, r, tok) : tok;
-    const int32_t pos = r.len - r.n + depth;
-    const int32_t hi = TREE ? tk.hi_min : min(pos + 1, min(r.len, paged_reach(a.p))), lo = key_lo(pos, a.t.window);
+    int32_t tok[RT], depth[RT], pos[RT], hi[RT], lo[RT];
+    int head[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        const int32_t row = min(((it.tile * RT + t) << 4) + c, n_rows - 1);
+        tok[t] = static_cast<int32_t>(fast_div(static_cast<uint32_t>(row), a.by_group));
+        head[t] = kvh * a.t.group + (row - tok[t] * a.t.group);
+        depth[t] = TREE ? tree_depth(a, r, tok[t]) : tok[t];
+        pos[t] = r.len - r.n + depth[t];
+        hi[t] = TREE ? tk.hi_min : min(pos[t] + 1, min(r.len, paged_reach(a.p)));
+        lo[t] = key_lo(pos[t], a.t.window);
+    }
 
     // q as the B operands of the first product, the same for all waves, by one of them: in LDS, so that each
     // wave's registers have room for other things (168 of them at three waves per SIMD). f32 rows are brought to
     // [2^14, 2^15) and split; sc_sh then undoes that. A scale's sign goes into q; a scale of 0 weights all alike.
-    if (wave == 1) {
-        const TQ* qr = static_cast<const TQ*>(a.q) + static_cast<int64_t>(r.begin + tok) * a.qs + static_cast<int64_t>(head) * hd;
+    if (wave >= 1 && wave <= RT) {
+        const int t = wave - 1, mine = RT == 1 ? 0 : t;
+        const int32_t my_tok = RT == 1 || t == 0 ? tok[0] : tok[RT - 1];
+        const int my_head = RT == 1 || t == 0 ? head[0] : head[RT - 1];
+        const TQ* qr = static_cast<const TQ*>(a.q) + static_cast<int64_t>(r.begin + my_tok) * a.qs + static_cast<int64_t>(my_head) * hd;
         const float sign = a.scale == 0.0f ? 0.0f : a.scale < 0.0f ? -1.0f : 1.0f;
         TQ x[2 * NU][8];
 #pragma unroll
@@ -143,7 +166,7 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
             mx = swap32_max(swap16_max(mx));
             const int ex = mx > 0.0f && mx < __builtin_inff() ? 15 - __builtin_amdgcn_frexp_expf(mx) : 0;
             const int e1 = ex / 2, e2 = ex - e1;  // two factors of which each is a normal float
-            sc_sh[c] = ldexpf(a.scale == 0.0f ? 1.0f : fabsf(a.scale), -ex);
+            sc_sh[mine][c] = ldexpf(a.scale == 0.0f ? 1.0f : fabsf(a.scale), -ex);
 #pragma unroll
             for (int u = 0; u < 2 * NU; u++) {
                 half8 y, z;
@@ -153,8 +176,8 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
                     y[e] = static_cast<half_t>(v);
                     z[e] = static_cast<half_t>(v - to_f32(y[e]));
                 }
-                q_sh[0][u][lane] = y;
-                q_sh[1][u][lane] = z;
+                q_sh[mine][0][u][lane] = y;
+                q_sh[mine][1][u][lane] = z;
             }
         } else {
 #pragma unroll
@@ -162,11 +185,13 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
                 half8 y;
                 __builtin_memcpy(&y, x[u], sizeof(y));
                 if (sign != 1.0f) y *= static_cast<half_t>(sign);
-                q_sh[0][u][lane] = y;
+                q_sh[mine][0][u][lane] = y;
             }
         }
     }
-    const float slope = MODS && a.slopes ? a.slopes[head] : 0.0f;
+    float slope[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) slope[t] = MODS && a.slopes ? a.slopes[head[t]] : 0.0f;
     const float inv_cap = MODS && a.softcap > 0.0f ? fminf(1.0f / a.softcap, 0x1.fffffep127f) : 0.0f;
 
     // This wave's tiles of 32 keys, from key kw on.
@@ -212,11 +237,17 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
         }
     };
 
-    float4v o[NE] = {};
-    float m = -__builtin_inff(), l = 0.0f;
-    bool seen = false;
+    float4v o[RT][NE] = {};
+    float m[RT], l[RT];
+    bool seen[RT];
+#pragma unroll
+    for (int t = 0; t < RT; t++) {
+        m[t] = -__builtin_inff();
+        l[t] = 0.0f;
+        seen[t] = false;
+    }
     // acc += V^T B of one tile, four dimensions of each lane: x, a word of each key's row.
-    auto product = [&](const uint32_t (&x)[2][4], half8 bh, half8 bl, float4v* acc) __attribute__((always_inline)) {
+    auto product = [&](const uint32_t (&x)[2][4], const half8 (&bh)[RT], const half8 (&bl)[RT], int w) __attribute__((always_inline)) {
         half2v y[4][2][2];  // [dimension][block][key pair]
 #pragma unroll
         for (int b = 0; b < 2; b++) {
@@ -237,8 +268,11 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
         for (int e = 0; e < 4; e++) {
             const half8 A = {y[e][0][0][0], y[e][0][0][1], y[e][0][1][0], y[e][0][1][1],
                              y[e][1][0][0], y[e][1][0][1], y[e][1][1][0], y[e][1][1][1]};
-            acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bl, acc[e], 0, 0, 0);
-            acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bh, acc[e], 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < RT; t++) {
+                o[t][4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bl[t], o[t][4 * w + e], 0, 0, 0);
+                o[t][4 * w + e] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, bh[t], o[t][4 * w + e], 0, 0, 0);
+            }
         }
     };
     auto step = [&](int tile, KvTile<DH>& t, int32_t pages, int kes, int ves) __attribute__((always_inline)) {
@@ -252,7 +286,7 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
             ve2[b] = __builtin_amdgcn_readlane(ves, idx);
             ok[b] = __builtin_amdgcn_readlane(pages, idx) >= 0;
         }
-        float4v s[2] = {};
+        float4v s[RT][2] = {};
 #pragma unroll
         for (int b = 0; b < 2; b++)
 #pragma unroll
@@ -268,10 +302,31 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
                         A[4 * w + 2] = x1[0];
                         A[4 * w + 3] = x1[1];
                     }
-                    if constexpr (kTwo) s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, q_sh[1][2 * u + h][lane], s[b], 0, 0, 0);
-                    s[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, q_sh[0][2 * u + h][lane], s[b], 0, 0, 0);
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) {
+                        if constexpr (kTwo) s[rt][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, q_sh[rt][1][2 * u + h][lane], s[rt][b], 0, 0, 0);
+                        s[rt][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(A, q_sh[rt][0][2 * u + h][lane], s[rt][b], 0, 0, 0);
+                    }
                 }
-        const float sc = kTwo ? sc_sh[c] : a.scale == 0.0f ? 1.0f : fabsf(a.scale);
+        // Keys that some row of the tile does not see.
+        const bool partial = j0 < tk.lo_max || j0 + 32 > tk.hi_min || !ok[0] || !ok[1];
+        if (partial) {
+            // What no row sees may be anything, codes of no token included.
+            const uint32_t many_any = tk.hi_max > tk.lo_min ? static_cast<uint32_t>(tk.hi_max - tk.lo_min) : 0u;
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const bool held = static_cast<uint32_t>(j0 + 16 * b + 4 * g4 + i - tk.lo_min) < (ok[b] ? many_any : 0u);
+#pragma unroll
+                    for (int w = 0; w < VW; w++) t.v[b][i].w[w] = held ? t.v[b][i].w[w] : 0u;
+                }
+        }
+        half8 ph[RT], pl[RT];
+        uint32_t sees[RT];  // (TREE) the tile's keys that the row sees
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+        const float sc = kTwo ? sc_sh[rt][c] : a.scale == 0.0f ? 1.0f : fabsf(a.scale);
         float f[2];  // score -> exponent of 2
 #pragma unroll
         for (int b = 0; b < 2; b++) {
@@ -283,12 +338,12 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
 #pragma unroll
             for (int b = 0; b < 2; b++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) s[b][i] *= f[b];
+                for (int i = 0; i < 4; i++) s[rt][b][i] *= f[b];
             if (a.softcap > 0.0f) {
 #pragma unroll
                 for (int b = 0; b < 2; b++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) s[b][i] = cap_score(s[b][i], a.softcap, inv_cap);
+                    for (int i = 0; i < 4; i++) s[rt][b][i] = cap_score(s[rt][b][i], a.softcap, inv_cap);
             }
             if (a.slopes) {
                 const bool in_tree = TREE && j0 + 32 > tk.hi_min;
@@ -298,61 +353,53 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
                     for (int i = 0; i < 4; i++) {
                         int32_t j = j0 + 16 * b + 4 * g4 + i;
                         if (in_tree) j = tree_key_place(a, r, j);
-                        s[b][i] = __builtin_fmaf(slope, static_cast<float>(j - pos), s[b][i]);
+                        s[rt][b][i] = __builtin_fmaf(slope[rt], static_cast<float>(j - pos[rt]), s[rt][b][i]);
                     }
             }
             f[0] = f[1] = kAttnLog2e;
         }
-        // Keys that some row of the tile does not see.
-        const bool partial = j0 < tk.lo_max || j0 + 32 > tk.hi_min || !ok[0] || !ok[1];
+        sees[rt] = 0;
         bool any_visible = true;
-        uint32_t sees = 0;  // (TREE) the tile's keys that the row sees
         if (partial) {
             any_visible = false;
-            if constexpr (TREE) sees = tree_sees(a, r, tok, depth, lo, hi, j0) & ((ok[0] ? 0xffffu : 0u) | (ok[1] ? 0xffff0000u : 0u));
-            // Visible: lo <= j < hi, as one unsigned comparison; no key of a block without a page. Likewise what any row sees.
-            const uint32_t many = hi > lo ? static_cast<uint32_t>(hi - lo) : 0u;
-            const uint32_t many_any = tk.hi_max > tk.lo_min ? static_cast<uint32_t>(tk.hi_max - tk.lo_min) : 0u;
+            if constexpr (TREE) sees[rt] = tree_sees(a, r, tok[rt], depth[rt], lo[rt], hi[rt], j0) & ((ok[0] ? 0xffffu : 0u) | (ok[1] ? 0xffff0000u : 0u));
+            // Visible: lo <= j < hi, as one unsigned comparison; no key of a block without a page.
+            const uint32_t many = hi[rt] > lo[rt] ? static_cast<uint32_t>(hi[rt] - lo[rt]) : 0u;
 #pragma unroll
             for (int b = 0; b < 2; b++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     const int32_t j = j0 + 16 * b + 4 * g4 + i;
-                    const bool vis = TREE ? (sees >> (16 * b + 4 * g4 + i) & 1u) != 0 : static_cast<uint32_t>(j - lo) < (ok[b] ? many : 0u);
-                    s[b][i] = vis ? s[b][i] : -__builtin_inff();
+                    const bool vis = TREE ? (sees[rt] >> (16 * b + 4 * g4 + i) & 1u) != 0 : static_cast<uint32_t>(j - lo[rt]) < (ok[b] ? many : 0u);
+                    s[rt][b][i] = vis ? s[rt][b][i] : -__builtin_inff();
                     any_visible |= vis;
-                    // What no row sees may be anything, codes of no token included.
-                    const bool held = static_cast<uint32_t>(j - tk.lo_min) < (ok[b] ? many_any : 0u);
-#pragma unroll
-                    for (int w = 0; w < VW; w++) t.v[b][i].w[w] = held ? t.v[b][i].w[w] : 0u;
                 }
         }
-        seen = seen || any_visible;
+        seen[rt] = seen[rt] || any_visible;
         float top = -__builtin_inff();
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            const float mx = fmaxf(fmaxf(s[b][0], s[b][1]), fmaxf(s[b][2], s[b][3]));
+            const float mx = fmaxf(fmaxf(s[rt][b][0], s[rt][b][1]), fmaxf(s[rt][b][2], s[rt][b][3]));
             top = fmaxf(top, __builtin_fmaf(mx, f[b], static_cast<float>(ve2[b])));
         }
         top = ceilf(swap32_max(swap16_max(top)));
-        if (__any(top > m)) {
-            const float mn = fmaxf(m, top);
-            const float corr = __builtin_amdgcn_exp2f(m - (mn == -__builtin_inff() ? 0.0f : mn));
-            m = mn;
-            l *= corr;
+        if (__any(top > m[rt])) {
+            const float mn = fmaxf(m[rt], top);
+            const float corr = __builtin_amdgcn_exp2f(m[rt] - (mn == -__builtin_inff() ? 0.0f : mn));
+            m[rt] = mn;
+            l[rt] *= corr;
 #pragma unroll
             for (int e = 0; e < NE; e++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) o[e][i] *= corr;
+                for (int i = 0; i < 4; i++) o[rt][e][i] *= corr;
         }
-        const float ms = m == -__builtin_inff() ? 0.0f : m;
-        half8 ph, pl;
+        const float ms = m[rt] == -__builtin_inff() ? 0.0f : m[rt];
         float base[2] = {static_cast<float>(ve2[0]) - ms, static_cast<float>(ve2[1]) - ms};
         if (__any(fabsf(ms) >= kFarMax)) {  // exponents in place of scores
 #pragma unroll
             for (int b = 0; b < 2; b++) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) s[b][i] = exponent_of(s[b][i], f[b], static_cast<float>(ve2[b]), ms);
+                for (int i = 0; i < 4; i++) s[rt][b][i] = exponent_of(s[rt][b][i], f[b], static_cast<float>(ve2[b]), ms);
                 f[b] = 1.0f;
                 base[b] = 0.0f;
             }
@@ -362,13 +409,14 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
             float sum = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][i], f[b], base[b]));
+                const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(s[rt][b][i], f[b], base[b]));
                 sum += p;
                 const float y = p * kPScale;
-                ph[4 * b + i] = static_cast<half_t>(y);
-                pl[4 * b + i] = static_cast<half_t>(y - to_f32(ph[4 * b + i]));
+                ph[rt][4 * b + i] = static_cast<half_t>(y);
+                pl[rt][4 * b + i] = static_cast<half_t>(y - to_f32(ph[rt][4 * b + i]));
             }
-            l = __builtin_fmaf(sum, exp2i(-ve2[b]), l);
+            l[rt] = __builtin_fmaf(sum, exp2i(-ve2[b]), l[rt]);
+        }
         }
         // A NaN code times a weight of zero is NaN, so where rows see different keys NaN codes are taken out, noted by
         // key and lane in this wave's part of the LDS that is free until the end, and put into the dimensions of the
@@ -408,18 +456,21 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
             for (int b = 0; b < 2; b++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) x[b][i] = t.v[b][i].w[w];
-            product(x, ph, pl, o + 4 * w);
+            product(x, ph, pl, w);
         }
         if (mend) {
 #pragma unroll 1
             for (int k = 0; k < 32; k++) {
-                if (TREE ? (sees >> k & 1u) == 0 : j0 + k < lo || j0 + k >= hi) continue;  // (a block without a page has no NaN left)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const uint32_t at = nan_at[k * 16 + 4 * g4 + i];
+                for (int rt = 0; rt < RT; rt++) {
+                    if (TREE ? (sees[rt] >> k & 1u) == 0 : j0 + k < lo[rt] || j0 + k >= hi[rt]) continue;  // (a block without a page has no NaN left)
 #pragma unroll
-                    for (int e = 0; e < NE; e++)
-                        o[e][i] = nan_if(o[e][i], at, e);
+                    for (int i = 0; i < 4; i++) {
+                        const uint32_t at = nan_at[k * 16 + 4 * g4 + i];
+#pragma unroll
+                        for (int e = 0; e < NE; e++)
+                            o[rt][e][i] = nan_if(o[rt][e][i], at, e);
+                    }
                 }
             }
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -442,54 +493,59 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH> ? NW / 4 : kRe
         t = next;
     }
 
-    if (TREE && depth < 0) {  // (tiles that all others see whole are not masked for a row that sees nothing)
-        m = -__builtin_inff();
-        l = 0.0f;
-        seen = false;
-    }
-    // The waves' results meet in LDS.
-    l = swap32_sum(swap16_sum(l));
-    const float any_seen = swap32_max(swap16_max(seen ? 1.0f : 0.0f));
-    if (g4 == 0) {
-        m_sh[wave][c] = m;
-        l_sh[wave][c] = l;
-        seen_sh[wave][c] = any_seen;
-    }
-    const int rows_here = min(kTileRows, n_rows - (it.tile << 4));
-    if (c < rows_here) {
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-#pragma unroll
-            for (int e = 0; e < NE; e += 4)
-                *reinterpret_cast<float4v*>(o_sh + (wave * kTileRows + c) * kRow + (4 * g4 + i) * NE + e) =
-                    float4v{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
-    }
-    __syncthreads();
     constexpr int LPR = DH / 4;  // threads to a row, four dimensions each
     const uint32_t block = it.block * static_cast<uint32_t>(a.p.n_kv) + kvh;
-    for (int i = static_cast<int>(threadIdx.x) / LPR; i < rows_here; i += 64 * NW / LPR) {
-        const int d = static_cast<int>(threadIdx.x) % LPR * 4;
-        float mm = -__builtin_inff(), ll = 0.0f, ss = 0.0f;
+    if (it.splits > 1 && block >= a.blocks) return;
 #pragma unroll
-        for (int w = 0; w < NW; w++) mm = fmaxf(mm, m_sh[w][i]);
-        const float ms = mm == -__builtin_inff() ? 0.0f : mm;
-        float4v x = {};
-#pragma unroll 4
-        for (int w = 0; w < NW; w++) {
-            const float f = __builtin_amdgcn_exp2f(m_sh[w][i] - ms);
-            const float4v y = *reinterpret_cast<const float4v*>(o_sh + (w * kTileRows + i) * kRow + d);
-            ll = __builtin_fmaf(l_sh[w][i], f, ll);
-            ss = fmaxf(ss, seen_sh[w][i]);
-#pragma unroll
-            for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf(y[e], f, x[e]);
+    for (int t = 0; t < RT; t++) {
+        if (t > 0) __syncthreads();  // (the LDS of the tile before)
+        if (TREE && depth[t] < 0) {  // (tiles that all others see whole are not masked for a row that sees nothing)
+            m[t] = -__builtin_inff();
+            l[t] = 0.0f;
+            seen[t] = false;
         }
-        if (it.splits > 1) {
-            if (block >= a.blocks) return;
-            const int64_t at = static_cast<int64_t>(block) * kTileRows + i;
-            *reinterpret_cast<float4v*>(a.part + at * DH + d) = x;
-            if (d == 0) *reinterpret_cast<float4v*>(a.ml + at * 4) = float4v{mm, ll, ss, 0.0f};
-        } else if (d < hd) {
-            store_row<TQ>(a, r, kvh, (it.tile << 4) + i, d, x, row_factor(ll, ss > 0.0f));
+        // The waves' results meet in LDS.
+        l[t] = swap32_sum(swap16_sum(l[t]));
+        const float any_seen = swap32_max(swap16_max(seen[t] ? 1.0f : 0.0f));
+        if (g4 == 0) {
+            m_sh[wave][c] = m[t];
+            l_sh[wave][c] = l[t];
+            seen_sh[wave][c] = any_seen;
+        }
+        const int32_t row0 = (it.tile * RT + t) << 4;
+        const int rows_here = min(kTileRows, n_rows - row0);
+        if (c < rows_here) {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+                for (int e = 0; e < NE; e += 4)
+                    *reinterpret_cast<float4v*>(o_sh + (wave * kTileRows + c) * kRow + (4 * g4 + i) * NE + e) =
+                        float4v{o[t][e][i], o[t][e + 1][i], o[t][e + 2][i], o[t][e + 3][i]};
+        }
+        __syncthreads();
+        for (int i = static_cast<int>(threadIdx.x) / LPR; i < rows_here; i += 64 * NW / LPR) {
+            const int d = static_cast<int>(threadIdx.x) % LPR * 4;
+            float mm = -__builtin_inff(), ll = 0.0f, ss = 0.0f;
+#pragma unroll
+            for (int w = 0; w < NW; w++) mm = fmaxf(mm, m_sh[w][i]);
+            const float ms = mm == -__builtin_inff() ? 0.0f : mm;
+            float4v x = {};
+#pragma unroll 4
+            for (int w = 0; w < NW; w++) {
+                const float f = __builtin_amdgcn_exp2f(m_sh[w][i] - ms);
+                const float4v y = *reinterpret_cast<const float4v*>(o_sh + (w * kTileRows + i) * kRow + d);
+                ll = __builtin_fmaf(l_sh[w][i], f, ll);
+                ss = fmaxf(ss, seen_sh[w][i]);
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[e] = __builtin_fmaf(y[e], f, x[e]);
+            }
+            if (it.splits > 1) {
+                const int64_t at = (static_cast<int64_t>(block) * RT + t) * kTileRows + i;
+                *reinterpret_cast<float4v*>(a.part + at * DH + d) = x;
+                if (d == 0) *reinterpret_cast<float4v*>(a.ml + at * 4) = float4v{mm, ll, ss, 0.0f};
+            } else if (d < hd) {
+                store_row<TQ>(a, r, kvh, row0 + i, d, x, row_factor(ll, ss > 0.0f));
+            }
         }
     }
 }
@@ -555,46 +611,51 @@ Grid grid_of(const PagedAttnArgs& a, int dh) {
     return g;
 }
 
-// The tiling of the 16-row kernel with `waves` waves to a workgroup, `resident` workgroups to a CU.
+// The tiling of the 16-row kernel (tile_log2 is set) with `waves` waves to a workgroup, `resident` workgroups to a CU.
 void few_form(const neko_hip_ctx* ctx, PagedAttnArgs& a, int waves, int resident) {
-    a.t.tile_log2 = 4;
     a.t.unit_log2 = 5 + __builtin_ctz(static_cast<unsigned>(waves));
     a.t.least = paged_reach(a.p) <= (kLeast << a.t.unit_log2) ? kLeast : kLeast / 2;
     a.t.target = resident * ctx->cu_count;
     attn_form(a);
 }
 
-template <typename TQ, int DH, int NW, bool MODS, bool TREE>
+template <typename TQ, int DH, int NW, bool MODS, bool TREE, int RT>
 int launch_few(neko_hip_ctx* ctx, const char* what, const PagedAttnArgs& a) {
     static std::atomic<uint64_t> allowed{0};
     constexpr size_t lds = NW * kTileRows * (DH + 4) * sizeof(float);
-    if (lds + 4096 > 64 * 1024)
-        if (int rc = allow_lds(ctx, reinterpret_cast<const void*>(&attn_paged_kernel<TQ, DH, NW, MODS, TREE>), lds, allowed)) return rc;
-    hipLaunchKernelGGL((attn_paged_kernel<TQ, DH, NW, MODS, TREE>), dim3(a.blocks), dim3(64 * NW), lds, ctx->stream, a);
+    if (lds + 4096 + RT * (sizeof(TQ) == 4 ? 2 : 1) * DH * 32 > 64 * 1024)
+        if (int rc = allow_lds(ctx, reinterpret_cast<const void*>(&attn_paged_kernel<TQ, DH, NW, MODS, TREE, RT>), lds, allowed)) return rc;
+    hipLaunchKernelGGL((attn_paged_kernel<TQ, DH, NW, MODS, TREE, RT>), dim3(a.blocks), dim3(64 * NW), lds, ctx->stream, a);
     return after_launch(ctx, what);
 }
 
 template <typename TQ, int DH>
 int launch_dims(neko_hip_ctx* ctx, const char* what, PagedAttnArgs a, int dtype) {
-    // Sequences of up to kFewRows rows on the 16-row kernel, the rest on the tiles. Which a batch has is known on the
+    // Sequences of up to few_rows rows on the 16-row kernel, the rest on the tiles. Which a batch has is known on the
     // device alone, so both are launched, except where there is one sequence, where there are no more rows than a
     // padded decoding batch has, or where all there can be is little: then the 16-row kernel takes whatever there is.
     const int64_t most = static_cast<int64_t>(a.p.rows) * a.t.group;
     const int64_t reach = paged_reach(a.p), per_row = std::max(reach / 2, reach - a.p.rows / (2 * a.p.n_seq));
     const double pairs = static_cast<double>(a.p.rows) * a.n_head * static_cast<double>(a.t.window > 0 ? std::min<int64_t>(per_row, a.t.window) : per_row);
-    const bool many = pairs > kFewPairs<TQ> && (a.p.n_seq == 1 ? most > kFewRows : most > static_cast<int64_t>(a.p.n_seq) * a.t.group + kSpareRows);
+    constexpr bool kTwoFit = sizeof(TQ) == 2 || DH <= 128;  // (f32 of 256 dimensions: 256 bytes of a lane's registers spill)
+    const int few_rows = a.words > 0 && kTwoFit ? kFewTreeRows<TQ> : kFewRows;
+    const int64_t some = a.words > 0 ? static_cast<int64_t>(a.p.n_seq) * few_rows : static_cast<int64_t>(a.p.n_seq) * a.t.group + kSpareRows;
+    const bool many = pairs > kFewPairs<TQ> && most > (a.p.n_seq == 1 ? few_rows : some);
     const bool few = a.p.n_seq > 1 || !many;
     constexpr int kMostWaves = DH <= 128 ? 8 : 4;
     PagedAttnArgs f = a, t = a;
     // Few items: many waves to each, whose results meet in LDS.
-    f.t.tile_log2 = 4;
+    const bool two = kTwoFit && a.words > 0 && most > 16 * static_cast<int64_t>(a.p.n_seq) &&
+                     (pairs > kTwoPairs<DH> || most / 16 * a.p.n_kv > kResident<TQ, 128> * ctx->cu_count);
+    f.t.tile_log2 = two ? 5 : 4;
     const int64_t items = attn_tiles_bound(f.t, a.p.rows, a.p.n_seq) * a.p.n_kv;
-    const bool wide = items <= ctx->cu_count;
-    few_form(ctx, f, wide ? kMostWaves : 4, wide ? kResident<TQ, DH> * 4 / kMostWaves : kResident<TQ, DH>);
+    const bool wide = items <= (two ? ctx->cu_count / 4 : ctx->cu_count);
+    const int resident = two ? kResident<TQ, DH, 2> : kResident<TQ, DH>;
+    few_form(ctx, f, wide ? kMostWaves : 4, wide ? resident * 4 / kMostWaves : resident);
     f.t.min_rows = 1;
-    f.t.max_rows = many ? kFewRows : 0x7fffffff;
+    f.t.max_rows = many ? few_rows : 0x7fffffff;
     attn_paged_tile_form(ctx, t);
-    t.t.min_rows = few ? kFewRows + 1 : 1;
+    t.t.min_rows = few ? few_rows + 1 : 1;
     t.t.max_rows = 0x7fffffff;
     const Grid fg = few ? grid_of(f, DH) : Grid{}, tg = many ? grid_of(t, DH) : Grid{};
     NEKO_REQUIRE(ctx, fg.blocks <= 0x7fffffff && tg.blocks <= 0x7fffffff, "%s: grid too large", what);
@@ -622,13 +683,18 @@ int launch_dims(neko_hip_ctx* ctx, const char* what, PagedAttnArgs a, int dtype)
     }
     if (few) {
         place(f, fg, ws);
-        int rc;
-        auto by_form = [&](auto tree) {
+        int rc = NEKO_OK;
+        auto by_form = [&](auto tree, auto tiles) {
             constexpr bool TREE = decltype(tree)::value;
-            if (wide) return mods ? launch_few<TQ, DH, kMostWaves, true, TREE>(ctx, what, f) : launch_few<TQ, DH, kMostWaves, false, TREE>(ctx, what, f);
-            return mods ? launch_few<TQ, DH, 4, true, TREE>(ctx, what, f) : launch_few<TQ, DH, 4, false, TREE>(ctx, what, f);
+            constexpr int RT = decltype(tiles)::value;
+            if (wide) return mods ? launch_few<TQ, DH, kMostWaves, true, TREE, RT>(ctx, what, f) : launch_few<TQ, DH, kMostWaves, false, TREE, RT>(ctx, what, f);
+            return mods ? launch_few<TQ, DH, 4, true, TREE, RT>(ctx, what, f) : launch_few<TQ, DH, 4, false, TREE, RT>(ctx, what, f);
         };
-        rc = a.words > 0 ? by_form(std::true_type{}) : by_form(std::false_type{});
+        constexpr std::integral_constant<int, 1> one{};
+        if constexpr (kTwoFit) {
+            if (two) rc = by_form(std::true_type{}, std::integral_constant<int, 2>{});
+        }
+        if (!two) rc = a.words > 0 ? by_form(std::true_type{}, one) : by_form(std::false_type{}, one);
         if (rc) return rc;
         if (int rc2 = merge(f)) return rc2;
     }
