@@ -310,18 +310,6 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH, RT> ? NW / 4 :
                 }
         // Keys that some row of the tile does not see.
         const bool partial = j0 < tk.lo_max || j0 + 32 > tk.hi_min || !ok[0] || !ok[1];
-        if (partial) {
-            // What no row sees may be anything, codes of no token included.
-            const uint32_t many_any = tk.hi_max > tk.lo_min ? static_cast<uint32_t>(tk.hi_max - tk.lo_min) : 0u;
-#pragma unroll
-            for (int b = 0; b < 2; b++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const bool held = static_cast<uint32_t>(j0 + 16 * b + 4 * g4 + i - tk.lo_min) < (ok[b] ? many_any : 0u);
-#pragma unroll
-                    for (int w = 0; w < VW; w++) t.v[b][i].w[w] = held ? t.v[b][i].w[w] : 0u;
-                }
-        }
         half8 ph[RT], pl[RT];
         uint32_t sees[RT];  // (TREE) the tile's keys that the row sees
 #pragma unroll
@@ -363,8 +351,9 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH, RT> ? NW / 4 :
         if (partial) {
             any_visible = false;
             if constexpr (TREE) sees[rt] = tree_sees(a, r, tok[rt], depth[rt], lo[rt], hi[rt], j0) & ((ok[0] ? 0xffffu : 0u) | (ok[1] ? 0xffff0000u : 0u));
-            // Visible: lo <= j < hi, as one unsigned comparison; no key of a block without a page.
+            // Visible: lo <= j < hi, as one unsigned comparison; no key of a block without a page. Likewise what any row sees.
             const uint32_t many = hi[rt] > lo[rt] ? static_cast<uint32_t>(hi[rt] - lo[rt]) : 0u;
+            const uint32_t many_any = tk.hi_max > tk.lo_min ? static_cast<uint32_t>(tk.hi_max - tk.lo_min) : 0u;
 #pragma unroll
             for (int b = 0; b < 2; b++)
 #pragma unroll
@@ -373,6 +362,11 @@ __global__ __launch_bounds__(64 * NW, (NW / 4 > kResident<TQ, DH, RT> ? NW / 4 :
                     const bool vis = TREE ? (sees[rt] >> (16 * b + 4 * g4 + i) & 1u) != 0 : static_cast<uint32_t>(j - lo[rt]) < (ok[b] ? many : 0u);
                     s[rt][b][i] = vis ? s[rt][b][i] : -__builtin_inff();
                     any_visible |= vis;
+                    if (rt > 0) continue;
+                    // What no row sees may be anything, codes of no token included.
+                    const bool held = static_cast<uint32_t>(j - tk.lo_min) < (ok[b] ? many_any : 0u);
+#pragma unroll
+                    for (int w = 0; w < VW; w++) t.v[b][i].w[w] = held ? t.v[b][i].w[w] : 0u;
                 }
         }
         seen[rt] = seen[rt] || any_visible;
