@@ -39,7 +39,8 @@ constexpr int kGroupListed = 512;                // tokens of its own that one l
 constexpr int kListed = 4096;                    // tokens in the cuts' bins that are held in LDS
 constexpr int kAtOnce = 20;                      // parts' bins that are on their way at once in launch 2
 constexpr int kRanked = 256;                     // of those, what is sorted by ranks
-constexpr int64_t kSlabRows = 1024;              // of a launch: the workspace holds so many
+constexpr int64_t kSlabRows = 1024;              // of a launch: the workspace holds so many,
+constexpr size_t kSlabBytes = size_t(256) << 20; // or as many as take this
 constexpr uint32_t kMinusInf = 0x007fffffu;      // its key; tokens at or below are left out
 
 // What launch 1 leaves of a part.
@@ -909,10 +910,10 @@ __global__ __launch_bounds__(kThreads) void sample_pick(SampleArgs a) {
 }
 
 template <typename T>
-int launch(neko_hip_ctx* ctx, const char* what, SampleArgs a, int64_t rows) {
+int launch(neko_hip_ctx* ctx, const char* what, SampleArgs a, int64_t rows, int64_t slab) {
     const SampleArgs all = a;
-    for (int64_t r = 0; r < rows; r += kSlabRows) {
-        const int64_t n = std::min(kSlabRows, rows - r);
+    for (int64_t r = 0; r < rows; r += slab) {
+        const int64_t n = std::min(slab, rows - r);
         const uint32_t parts = static_cast<uint32_t>(n * a.parts);
         auto from = [&](auto* p) { return p ? p + r : p; };
         a.logits = static_cast<const T*>(all.logits) + r * all.stride;
@@ -997,9 +998,14 @@ extern "C" int neko_hip_sample(neko_hip_ctx* ctx, const void* logits, int64_t st
     a.count_bits = bits_of(a.part_tokens);
     a.fixed = std::min(44, 63 - 2 * a.count_bits);
     a.narrow = std::min(44, 62 - bits_of(vocab));
-    const size_t parts = static_cast<size_t>(held) * a.parts, hist = a.top_k || a.top_p ? parts * kBins : 0;
-    const size_t bytes[] = {parts * sizeof(Part), static_cast<size_t>(held) * a.n_blocks * 8, static_cast<size_t>(held) * sizeof(Found),
-                            hist * 8, hist ? static_cast<size_t>(held) * kListed * 8 : 0, static_cast<size_t>(held) * 4};
+    const bool hist = a.top_k || a.top_p;
+    const size_t parts = static_cast<size_t>(a.parts);
+    size_t bytes[] = {parts * sizeof(Part), static_cast<size_t>(a.n_blocks) * 8, sizeof(Found), hist ? parts * kBins * 8 : 0, hist ? kListed * size_t(8) : 0,
+                      sizeof(uint32_t)};  // of a row
+    size_t of_row = 0;
+    for (size_t b : bytes) of_row += b;
+    const int64_t slab = std::clamp<int64_t>(static_cast<int64_t>(kSlabBytes / of_row), 1, held);
+    for (size_t& b : bytes) b *= static_cast<size_t>(slab);
     size_t all = 0;
     for (size_t b : bytes) all += b;
     void* ws = nullptr;
@@ -1016,5 +1022,5 @@ extern "C" int neko_hip_sample(neko_hip_ctx* ctx, const void* logits, int64_t st
     a.bins = static_cast<uint64_t*>(at[3]);
     a.list = static_cast<uint64_t*>(at[4]);
     a.listed = static_cast<uint32_t*>(at[5]);
-    return dtype == NEKO_DT_F16 ? launch<half_t>(ctx, what, a, rows) : launch<float>(ctx, what, a, rows);
+    return dtype == NEKO_DT_F16 ? launch<half_t>(ctx, what, a, rows, slab) : launch<float>(ctx, what, a, rows, slab);
 }
