@@ -74,6 +74,46 @@ def test_sample_many_rows(dev):
     _check(dev, x, torch.rand(1500, generator=g), **_settings(1500, 5000, g, "all"))
 
 
+def test_sample_the_largest_vocabulary(dev):
+    """As many tokens as a call takes, in more rows than one set of launches does at once: all rows' logits are alike, so a
+    row's token is that of a call of its own.
+
+    Which token's share of the running sum u falls into is checked to b = V 2^-44 / S + 2^-26 of the sum S (in weights of the
+    largest): listed tokens' weights are rounded to units of 2^-44, by half of one each, and doubles' sums by less than 2^-40
+    of S; the cut of top-p is within 2^-27 of S, by which the running sum moves and what u is compared with too."""
+    _case("sample, vocabulary 2^24, 50 rows")
+    g = torch.Generator().manual_seed(24)
+    vocab, rows = 1 << 24, 50
+    x = (torch.randn((1, vocab), generator=g) * 2).half()
+    u = torch.rand(rows, generator=g)
+    u[49] = u[46] = u[0]
+    dx, l = x.to(dev).expand(rows, vocab).contiguous(), x[0].double().numpy()
+    w = np.exp(l - l.max())
+    order = np.argsort(-l, kind="stable")
+    for kw in ({"top_p": 0.9}, {"top_k": 50, "top_p": 0.95}, {"min_p": 0.01}):
+        make = lambda n: {k: torch.full((n,), v, dtype=torch.int32 if k == "top_k" else torch.float32).to(dev) for k, v in kw.items()}  # noqa: E731
+        got = ops.sample(dx, u.to(dev), **make(rows)).tolist()
+        print(kw, got[:4], flush=True)
+        alone = []
+        for r in range(rows):
+            alone += ops.sample(dx[:1], u[r:r + 1].to(dev), **make(1)).tolist()
+        assert got == alone and got[0] == got[46] == got[49]
+        stays = order[: kw.get("top_k", vocab)]
+        cum = np.cumsum(w[stays])
+        if "top_p" in kw:
+            stays = stays[: int(np.searchsorted(cum, float(np.float32(kw["top_p"])) * cum[-1])) + 1]
+        stays = np.sort(stays[w[stays] >= float(np.float32(kw.get("min_p", 0.0)))])
+        cum = np.cumsum(w[stays])
+        for r, token in enumerate(got):
+            at = int(np.searchsorted(stays, token))
+            near = vocab * 2.0 ** -44 / cum[-1] + 2.0 ** -26
+            before, after = (cum[at - 1] if at else 0.0) / cum[-1], (cum[at] if at < len(cum) else cum[-1]) / cum[-1]
+            if at == len(stays) or stays[at] != token:  # (right at the cut)
+                assert abs(after - before) <= near
+                after = before
+            assert before - near <= float(u[r]) <= after + near, (r, token, before, float(u[r]), after)
+
+
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_sample_settings_that_cut_nothing(dev, dtype):
     """Settings at and past their ends, and not numbers."""

@@ -138,6 +138,17 @@ def test_attention_split_keys(dev, trees, dtype):
     _check(dev, 8, 2, 128, dtype, t, 11, what=str(len(trees)))
 
 
+@pytest.mark.parametrize("hd,dtype,window", [(128, "f16", 0), (64, "f32", 11), (128, "f32", 0), (256, "f16", 0)])
+@pytest.mark.parametrize("seqs,most", [(24, 24), (70, 9)])
+def test_attention_many_trees(dev, seqs, most, hd, dtype, window):
+    """More 16-row tiles than are resident, of more sequences than a wave has lanes too."""
+    _case(f"attention of {seqs} trees, {hd} {dtype} window {window}")
+    rng = np.random.default_rng(seqs)
+    trees = [(T.random_parents(n, 4, rng, 1 if n > 4 and s % 5 == 0 else 0), int(rng.integers(0, 90)))
+             for s, n in enumerate(int(rng.integers(0 if i % 7 == 6 else most - 4, most + 1)) for i in range(seqs))]
+    _check(dev, 32, 8, hd, dtype, T.Trees([t if t[0] else ([], 0) for t in trees], 16, seqs), seqs, what="many", window=window)
+
+
 @pytest.mark.parametrize("wide", [False, True])
 def test_attention_any_mask(dev, wide):
     """Masks that are no tree's: rows that see nothing of it, not themselves, later rows; bits past the sequence's rows;
