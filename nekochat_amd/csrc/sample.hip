@@ -35,6 +35,9 @@ constexpr int kBlockTokens = 2048;               // of a sum: 256 threads of 8
 constexpr int kStepTokens = kThreads * 8;        // four blocks
 constexpr int kMostSteps = 3;                    // of a part: a thread holds its tokens in registers
 constexpr int kMostBlocks = 16;                  // of a workgroup in launch 3
+// Rows' counters a cache line apart: workgroups of all XCDs add to them (launch 3 of 128 rows with a top-k of 50 17 us, on four
+// lines 21).
+constexpr int kLine = 32;
 constexpr int kGroupListed = 512;                // tokens of its own that one lists in LDS first
 constexpr int kListed = 4096;                    // tokens in the cuts' bins that are held in LDS
 constexpr int kAtOnce = 20;                      // parts' bins that are on their way at once in launch 2
@@ -84,7 +87,7 @@ struct SampleArgs {
     Part* part;                  // [rows][parts]
     uint64_t* bins;              // [rows][parts][kBins]
     Found* found;                // [rows]
-    uint32_t* listed;            // [rows] tokens listed so far
+    uint32_t* listed;            // [rows][kLine] tokens listed so far
     uint64_t* list;              // [rows][kListed] ~key << 32 | index: ascending is the order of the cuts
     double* sums;                // [rows][n_blocks]
 };
@@ -287,7 +290,7 @@ __global__ __launch_bounds__(kThreads, 8) void sample_parts(SampleArgs a) {
     }
     if (tid == 0) {
         out->best = static_cast<uint64_t>(key) << 32;
-        if (part == 0) a.listed[r] = 0;
+        if (part == 0) a.listed[r * kLine] = 0;
     }
     if (!w.cuts() || key <= kMinusInf) return;
     const double per = bins_per(w.inv_t), first = rint(place_of(top, w.inv_t)), units = ldexp(1.0, a.fixed + a.count_bits);
@@ -596,7 +599,7 @@ __global__ __launch_bounds__(256) void sample_sums(SampleArgs a) {
                     if (to < kGroupListed) {
                         list_sh[to] = x;
                     } else {
-                        const uint32_t k = atomicAdd(a.listed + r, 1u);
+                        const uint32_t k = atomicAdd(a.listed + r * kLine, 1u);
                         if (k < kListed) a.list[r * kListed + k] = x;
                     }
                 }
@@ -609,7 +612,7 @@ __global__ __launch_bounds__(256) void sample_sums(SampleArgs a) {
     if (lists) {
         // (one place in the list for all: a wave that asks for its own waits 2 us for it)
         const uint32_t n = std::min<uint32_t>(n_sh, kGroupListed);
-        if (tid == 0 && n) from_sh = atomicAdd(a.listed + r, n);
+        if (tid == 0 && n) from_sh = atomicAdd(a.listed + r * kLine, n);
         __syncthreads();
         for (uint32_t i = tid; i < n; i += 256)
             if (from_sh + i < kListed) a.list[r * kListed + from_sh + i] = list_sh[i];
@@ -1001,7 +1004,7 @@ extern "C" int neko_hip_sample(neko_hip_ctx* ctx, const void* logits, int64_t st
     const bool hist = a.top_k || a.top_p;
     const size_t parts = static_cast<size_t>(a.parts);
     size_t bytes[] = {parts * sizeof(Part), static_cast<size_t>(a.n_blocks) * 8, sizeof(Found), hist ? parts * kBins * 8 : 0, hist ? kListed * size_t(8) : 0,
-                      sizeof(uint32_t)};  // of a row
+                      kLine * sizeof(uint32_t)};  // of a row
     size_t of_row = 0;
     for (size_t b : bytes) of_row += b;
     const int64_t slab = std::clamp<int64_t>(static_cast<int64_t>(kSlabBytes / of_row), 1, held);
