@@ -302,8 +302,9 @@ int neko_hip_keep_paged(neko_hip_ctx* ctx, const neko_paged_kv* kv, const neko_p
 
 /* ---------------------------------------------------------------- sampling */
 
-/* A token of each row of logits, from a uniform number of the row's own. No counterpart in the reference. With w_i =
- * exp((l_i - max l) / temperature) over the vocabulary:
+/* A token of each row of logits, from a uniform number of the row's own (the reference samples one row of host logits at
+ * a time, with random numbers of its own: shared/cpp/sampler.cpp). With w_i = exp((l_i - max l) / temperature) over the
+ * vocabulary:
  *   top_k   the top_k largest logits stay, of equal ones the lower index first;
  *   top_p   of those, in that order, the shortest prefix whose sum of w is at least top_p times their sum (at least one);
  *   min_p   of those, the ones with w >= min_p (above 1: 1);
@@ -314,9 +315,12 @@ int neko_hip_keep_paged(neko_hip_ctx* ctx, const neko_paged_kv* kv, const neko_p
  *   u         f32 [rows] in [0, 1) (brought into it otherwise; NaN: 0).
  *   tokens    int32 [rows]; -1 where every logit is -inf or NaN. Such logits are never chosen; where the largest is +inf,
  *             only those that are.
- * Weights and their sums are held in 64 bits: the token is that of an evaluation in 64 bits unless u * sum or a cut lies
- * within about 2^-40 of a border; the same inputs give the same token in every batch. rows up to 2^20, vocab up to 2^24.
- * Partial results go to the context's workspace (see neko_hip_matmul): up to 150 KB for a row, less for each of many. */
+ * Weights and their sums are held in 64 bits, the sums that top_p's cut is found among to 2^-28: the token is that of an
+ * evaluation in 64 bits unless u lies within vocab * 2^-44 of the weights' sum from a border between two tokens, or top_p's
+ * cut within 2^-27 of it. The same call gives the same tokens again; in a batch of another size a row's can differ at such
+ * a border only. rows up to 2^20, vocab up to 2^24. Partial results go to the context's workspace (see neko_hip_matmul):
+ * for a row 8 bytes per 2048 tokens and, with a top_k or top_p, at most 8 KB per 8192 tokens and 33 KB; 256 MB in all
+ * (or one row's), more rows in turn. Its size goes by rows, vocab and which settings are given. */
 int neko_hip_sample(neko_hip_ctx* ctx, const void* logits, int64_t stride, int64_t rows, int64_t vocab,
                     const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, const float* u,
                     int32_t* tokens, int dtype);

@@ -18,8 +18,8 @@
 //
 // What bounds it: with many keys the reading of them, two sequences of 65521 tokens (32 / 8 heads of 128, f16) in 51 us,
 // 5.3 TB/s of codes, and 5 for the merge; with fewer, launches and loads that wait for each other (32 ragged ones of up to
-// 4096 tokens 18.1 us, one of 777 11.0). Of drafted trees, two of 7
-// tokens (28 rows) over 65500 53 us and 6 for the merge, one of 26 over 777 12.3.
+// 4096 tokens 18.1 us, one of 777 11.0). Of drafted trees, two of 7 tokens (28 rows) over 65500 53 us, 5.0 TB/s of codes, and
+// 6 for the merge, one of 26 over 777 12.2.
 #include <algorithm>
 #include <atomic>
 
