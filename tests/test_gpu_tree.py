@@ -149,6 +149,19 @@ def test_attention_many_trees(dev, seqs, most, hd, dtype, window):
     _check(dev, 32, 8, hd, dtype, T.Trees([t if t[0] else ([], 0) for t in trees], 16, seqs), seqs, what="many", window=window)
 
 
+@pytest.mark.parametrize("hd,dtype,wide", [(64, "f16", False), (128, "f32", False), (128, "f16", True)])
+def test_attention_trees_of_most_rows(dev, hd, dtype, wide):
+    """32 words of mask."""
+    _case(f"attention of trees of 1024 rows, {hd} {dtype} wide {wide}")
+    rng = np.random.default_rng(1024)
+    trees = [(T.random_parents(1024, 30, rng), 37), ([-1], 3), (list(range(-1, 998)), 5)]
+    t = T.Trees(trees, 16, 7)
+    if wide:
+        t = T.Trees(trees, 16, 7, slack=_wide(t, 2, 16))
+    assert t.words == 32
+    _check(dev, 2, 1, hd, dtype, t, 9, what="1024 rows")
+
+
 @pytest.mark.parametrize("wide", [False, True])
 def test_attention_any_mask(dev, wide):
     """Masks that are no tree's: rows that see nothing of it, not themselves, later rows; bits past the sequence's rows;
@@ -593,6 +606,37 @@ def _step(m, cache, batch, tokens, depth, mask, parents, u, settings, most):
     path, count, after, new_len = ops.accept_tree(tokens, sampled, parents, start, length, most)
     ops.keep_paged(cache, table, start, length, path, count)
     return q, out, logits, sampled, path, count, after, new_len
+
+
+def test_pages_past_32_bits(dev):
+    """A step over pages whose codes stand past 4 GiB of the cache's start: bit for bit the one over the same pages at its start."""
+    _case("pages past 32 bits")
+    H, KV, hd, page, first = 8, 2, 128, 16, (1 << 32) // 4096 + 3
+    rng = np.random.default_rng(32)
+    t = T.Trees([(T.random_parents(20, 5, rng, 2), 45), (T.random_parents(9, 3, rng), 0), (T.random_parents(40, 6, rng), 130)], page, 3)
+    n = t.batch.n_pages
+    small = _cache_on(P.random_cache(n, KV, page, hd, 4), dev)
+    large = ops.PagedKV.empty(first + n, page, KV, hd, dev)
+    assert large.k_pages[first:].data_ptr() - large.k_pages.data_ptr() > 1 << 32
+    for x, y in zip((large.k_pages, large.v_pages, large.k_scales, large.v_scales), (small.k_pages, small.v_pages, small.k_scales, small.v_scales)):
+        x[first:].view(torch.uint8).copy_(y.view(torch.uint8))
+    g = torch.Generator().manual_seed(5)
+    qkv = torch.randn((t.rows, (H + 2 * KV) * hd), generator=g).half().to(dev)
+    table, start, length, depth = t.tensors(dev)
+    cs = torch.from_numpy(ops.rope_table(1e4, hd, 300)).to(dev)
+    count = torch.tensor([4, 3, 5], dtype=torch.int32, device=dev)
+    path = torch.tensor([[0, 3, 7, 18, -1], [0, 2, 8, -1, -1], [0, 1, 20, 30, 39]], dtype=torch.int32, device=dev)
+    got = []
+    for cache, tab in ((small, table), (large, torch.where(table >= 0, table + first, table))):
+        q = torch.zeros((t.rows, H * hd), dtype=torch.float16, device=dev)
+        ops.qk_norm_rope_tree_paged(qkv, H, cache, tab, start, length, depth, cs, 1e-6, q_out=q)
+        out = ops.attention_tree_paged(q, cache, tab, start, length, depth, t.mask().to(dev), H)
+        ops.keep_paged(cache, tab, start, length, path, count)
+        torch.cuda.synchronize()
+        got.append((q.cpu(), out.cpu(), *(x[-n:].cpu() for x in (cache.k_pages, cache.v_pages, cache.k_scales, cache.v_scales))))
+    assert all(_same(a, b) for a, b in zip(*got))
+    # The pages before them are as an empty cache has them.
+    assert bool((large.k_scales[:first] == 1).all()) and not bool(large.k_pages[:first].view(torch.uint8).any())
 
 
 def test_speculative_steps(dev):
