@@ -23,10 +23,11 @@
 //
 // What bounds it: one row of 151936 f16 logits, 27.5 us, four launches that need each other (6.8, 9.2, 4.7 and 8.1 by
 // themselves, most of each loads and barriers in turn). 128 such rows in f32, their settings mixed, 73 us: 26.9 of launch 1, of
-// which 13 are the reading (6 TB/s, from the last-level cache in part) and the rest LDS atomics, several tokens of a wave in
-// one bin; 9.2 of 2; 24.4 of 3, where rows that keep most of the vocabulary take the weights' exponentials again; 13.9 of 4.
+// which 13 are the reading (6 TB/s, from the last-level cache in part) and the rest some 33 instructions a token, half of them
+// in double (the same without the atomics); 9.2 of 2; 24.4 of 3, where rows that keep most of the vocabulary take the weights' exponentials again; 13.9 of 4.
 // Not kept: launch 3 by the polynomial for rows of many kept tokens too (rows with a top-p of 0.9 32 -> 37 us, of 0.99 46 -> 42);
-// the largest logits of 64 tokens each, so that launch 3 reads no others (no faster, launch 1 1.7 us slower).
+// the largest logits of 64 tokens each, so that launch 3 reads no others (no faster, launch 1 1.7 us slower); the bins' polynomial
+// with its scale in its coefficients (f32 28.0 -> 26.3, but the f16 form's registers spill: without a histogram 11.5 -> 14.7).
 #include <algorithm>
 
 #include "internal.h"
