@@ -285,8 +285,10 @@ int neko_hip_attention_tree_paged(neko_hip_ctx* ctx, const void* q, int64_t q_st
 /* The path that sampled tokens take through each tree: from the root on, to the first child (the lowest row with that
  * parent) that holds the token sampled at the row before, while there is one. tokens, sampled, parents int32 [rows], as
  * in neko_tree_plan (negative samples agree with nothing). Written for each sequence: path int32 [n_seq][max_path], the
- * rows of the path within the tree, then -1; count, its rows (0 where the sequence has none; at most max_path); next, the
- * token sampled at its last row (-1 if none); new_len = kv_len - n + count. The outputs overlap nothing. */
+ * rows of the path within the tree, then -1; count, its rows (at most max_path); next, the token sampled at its last row (-1
+ * if none); new_len = kv_len - n + count. A sequence without rows, or whose first row is padding (its parent is not -1, or
+ * kv_len is below n: then all rows are), has no path: count 0, next -1, new_len the tokens before the tree (0 where kv_len is
+ * below n). The outputs overlap nothing. */
 int neko_hip_accept_tree(neko_hip_ctx* ctx, const int32_t* tokens, const int32_t* sampled, const int32_t* parents, int64_t rows,
                          const int32_t* row_start, const int32_t* kv_len, int64_t n_seq, int32_t* path, int64_t max_path,
                          int32_t* count, int32_t* next, int32_t* new_len);

@@ -1,8 +1,9 @@
 // Drafted trees over the paged 8-bit KV cache: the path that sampled tokens take from a tree's root, and the path's tokens
 // moved together in the pages.
 //
-// Accept. at = the root; while a child of `at` holds the token sampled at `at`, the first such child is the next. A wave to
-// a sequence: parents, tokens and samples of up to 256 rows stay in its registers, so a step is two lane reads and a
+// Accept. at = the root; while a child of `at` holds the token sampled at `at`, the first such child is the next. Where row 0
+// is no root, or the length is short of the rows, all rows are padding: nothing of them was appended, and there is no path. A
+// wave to a sequence: parents, tokens and samples of up to 256 rows stay in its registers, so a step is two lane reads and a
 // ballot for each 64 rows, no load.
 //
 // Keep. The cached value of slot base + path[k] goes to slot base + k, as if the append had made it there: under the
@@ -49,7 +50,8 @@ __global__ __launch_bounds__(64) void accept_kernel(AcceptArgs a) {
     }
     int32_t* path = a.path + static_cast<int64_t>(s) * a.max_path;
     int32_t at = 0, count = 0, last = -1;
-    while (r.n > 0) {
+    const bool root = r.n > 0 && r.len >= r.n && __builtin_amdgcn_readfirstlane(parent[0]) == -1;
+    while (root) {
         if (lane == 0) path[count] = at;
         count++;
         // The token sampled at `at`, and the first child that holds it.

