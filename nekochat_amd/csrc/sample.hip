@@ -91,7 +91,7 @@ struct SampleArgs {
     int32_t groups, group_blocks;  // workgroups of a row in launch 3, and their blocks
     int32_t count_bits;          // the low bits of a bin: its tokens; the others: their weights in units of 2^-fixed
     int32_t fixed;
-    int32_t narrow;              // fixed-point weights of launch 4, relative to the row's largest: units of 2^-narrow
+    int32_t narrow;              // fixed-point weights of a cut's parts, relative to the row's largest: units of 2^-narrow, and of 2^-32 of those
     Part* part;                  // [rows][parts]
     uint64_t* bins;              // [rows][parts][kBins]
     Found* found;                // [rows]
@@ -163,6 +163,13 @@ __device__ __forceinline__ double weight_of(float l, float top, double inv_t) {
 // w * units, rounded, below 2^52: the low bits of its sum with 2^52.
 __device__ __forceinline__ uint64_t fixed_of(double w, double units) {
     return __builtin_bit_cast(uint64_t, __builtin_fma(w, units, 0x1p52)) - __builtin_bit_cast(uint64_t, 0x1p52);
+}
+
+// What that leaves of w * units, half a unit at most either way, in 2^-32 of one (a sum of 2^24 of them below 2^56). units: a
+// power of two, so that both differences are exact.
+__device__ __forceinline__ uint64_t fixed_left(double w, double units) {
+    const double left = __builtin_fma(w, units, -(__builtin_fma(w, units, 0x1p52) - 0x1p52));
+    return __builtin_bit_cast(uint64_t, __builtin_fma(left, 0x1p32, 0x1.8p52)) - __builtin_bit_cast(uint64_t, 0x1.8p52);
 }
 
 // Logits i .. i + 7 of a row, -inf from n on. Rows may stand at any element.
@@ -636,7 +643,7 @@ __device__ __forceinline__ float ordered_value(u64 x) { return value_of(~static_
 
 struct PickShared {
     u64 list[kListed];
-    u64 weight[kBins];
+    u64 weight[kBins], low[kBins];
     uint32_t count[kBins];
     u64 few[kRanked], sorted[kRanked];
     double few_weight[kRanked];
@@ -670,7 +677,9 @@ __device__ __forceinline__ void rank_few(PickShared& sh, int n) {
 
 // Of tokens (each(f) calls f(its place in the order) for every one, at most n of them) the last that the goal takes,
 // before_n tokens of the sum `before` coming before them: its place; the sum with it in sh.taken. More than a few are
-// narrowed first, to one of 1024 equal parts of the order's range and again, by histograms in fixed point.
+// narrowed first, to one of 1024 equal parts of the order's range and again, by histograms in fixed point. There a weight is
+// two whole numbers, the units and what their rounding left in 2^-32 of them: 2^24 equal weights far below the row's largest,
+// which the units alone hold to 2^-38 each, are all off the same way (the sum by 2^-14; of both numbers, 2^-46).
 template <typename Each>
 __device__ u64 find_cut(PickShared& sh, const Row& w, float top, int fixed, const Goal& g, uint32_t n, uint32_t before_n, double before, Each&& each) {
     const int tid = static_cast<int>(threadIdx.x);
@@ -702,16 +711,19 @@ __device__ u64 find_cut(PickShared& sh, const Row& w, float top, int fixed, cons
             __syncthreads();
             sh.count[tid] = 0;
             sh.weight[tid] = 0;
+            sh.low[tid] = 0;
             __syncthreads();
             each([&](u64 x) {
                 if (x < lo || x > hi) return;
                 const int to = static_cast<int>((x - lo) >> shift);
+                const double y = weight_of(ordered_value(x), top, w.inv_t);
                 atomicAdd(&sh.count[to], 1u);
-                atomicAdd(&sh.weight[to], static_cast<u64>(fixed_of(weight_of(ordered_value(x), top, w.inv_t), units)));
+                atomicAdd(&sh.weight[to], static_cast<u64>(fixed_of(y, units)));
+                atomicAdd(&sh.low[to], static_cast<u64>(fixed_left(y, units)));
             });
             __syncthreads();
             const uint32_t c = sh.count[tid];
-            const double s = static_cast<double>(sh.weight[tid]) / units;
+            const double s = (static_cast<double>(sh.weight[tid]) + static_cast<double>(static_cast<int64_t>(sh.low[tid])) * 0x1p-32) / units;
             const uint32_t cs = before_n + block_scan(sh.scan, c);
             const double ss = before + block_scan(sh.scan_f, s);
             int at = block_first<false>(sh.first, c && (g.by_count ? cs >= g.need : ss >= g.target));

@@ -321,3 +321,43 @@ def test_sample_refuses(dev):
         with pytest.raises(NekoError):
             f()
     assert ops.sample(x[:0], u[:0]).shape == (0,)
+
+
+# ------------------------------------------------------------------ the stated accuracy
+
+def _kept_of_ties(vocab, top, p):
+    """One logit of `top` at index 0 over vocab - 1 zeros, temperature 1: how many tokens top-p keeps, and a zero's weight."""
+    w = np.exp(-np.longdouble(top))
+    total = 1 + (vocab - 1) * w
+    return max(1, 1 + int(np.ceil((np.longdouble(np.float32(p)) * total - 1) / w))), w
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("vocab,top,p", [(1 << 20, 20.0, 0.999), (1 << 20, 14.0, 0.8), (1 << 22, 20.0, 0.995), (1 << 24, 20.0, 0.99), (1 << 24, 24.0, 0.9999)])
+def test_sample_ties_far_below_the_largest(dev, vocab, top, p, dtype):
+    """Weights far below the row's largest, alike and many, so that each one's rounding adds up: the cut of top-p is within
+    2^-27 of the weights' sum S of the exact one, and the token's share of the running sum within V 2^-44 / S besides.
+
+    The running sum up to zero i (index i) is 1 + i w. Moving the cut by c moves the kept sum by c, hence what u is compared
+    with; with both bounds the token is within (2^-27 + V 2^-44 / S) S / w of the exact one, and one for the rounding to whole
+    tokens."""
+    _case(f"sample, {vocab} tokens, one of {top} over zeros, top-p {p} {dtype}")
+    x = torch.zeros((1, vocab), dtype=DT[dtype], device=dev)
+    x[0, 0] = top
+    us = [1 - 2.0 ** -24, 0.9999, 0.99, 0.97, 0.5]
+    n, w = _kept_of_ties(vocab, top, p)
+    assert 2 < n < vocab - 1
+    total, kept = 1 + (vocab - 1) * w, 1 + (n - 1) * w
+    rows = x.expand(len(us), vocab)[: len(us)].contiguous()
+    for k in (0, vocab - 7):
+        kw = {"top_p": torch.full((len(us),), p, device=dev)}
+        if k:
+            kw["top_k"] = torch.full((len(us),), k, dtype=torch.int32, device=dev)
+            n, _ = _kept_of_ties(k, top, p)
+            total, kept = 1 + (k - 1) * w, 1 + (n - 1) * w
+        got = ops.sample(rows, torch.tensor(us, device=dev), **kw).tolist()
+        off = float((2.0 ** -27 * total + vocab * np.longdouble(2.0) ** -44) / w) + 1
+        for u, token in zip(us, got):
+            want = max(0, int(np.floor((np.longdouble(np.float32(u)) * kept - 1) / w)) + 1)
+            print(f"k {k} u {u:.8f}: {token}, exactly {want}, bound {off:.1f}", flush=True)
+            assert abs(token - want) <= off and 0 <= token < n + off
