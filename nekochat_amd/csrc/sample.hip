@@ -559,11 +559,11 @@ __global__ __launch_bounds__(256) void sample_sums(SampleArgs a) {
     f.lo = kBins;
     if (w.cuts()) f = a.found[r];
     const bool whole = f.lo == kBins, lists = !whole && f.listed <= kListed;
-    const double place = place_of(top, w.inv_t), per = bins_per(w.inv_t), first = rint(place);
+    const double per = bins_per(w.inv_t);
     if (tid == 0) n_sh = 0;
     if (!whole) __syncthreads();
     if (whole) {
-        if (tid < 64) by_sh[tid] = tid < 32 ? exp(-1.0 * tid) / edge_weight<true>(place - first) : exp((tid - 32) * (-1.0 / kBinsPerT));
+        if (tid < 64) by_sh[tid] = tid < 32 ? exp(-1.0 * tid) : exp((tid - 32) * (-1.0 / kBinsPerT));
         __syncthreads();
     }
 #pragma unroll 1
@@ -572,12 +572,13 @@ __global__ __launch_bounds__(256) void sample_sums(SampleArgs a) {
         if (s + 1 < blocks) next = load8(row, i0 + kBlockTokens, a.vocab);
         double sum = 0.0;
         if (whole) {
-            // e^((z - z of the largest) / 32), by e^(-b / 32) of the bin and the polynomial.
+            // e^(z / 32), by e^(-b / 32) of whole steps b down from the largest and the polynomial. (z from the difference,
+            // which is exact: a difference of places is off by their own rounding, 2^-33 of the weight for logits of 10^6.)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const float l = fmaxf(to_f32(x.v[e]), -__builtin_inff());  // (NaN: -inf)
-                const double z = fmin(static_cast<double>(l) * per, 1e300), g = rint(z);
-                const int b = static_cast<int>(fmin(first - g, kBins - 1.0));
+                const double z = (static_cast<double>(l) - static_cast<double>(top)) * per, g = rint(z);
+                const int b = static_cast<int>(fmin(-g, kBins - 1.0));
                 double y = by_sh[b >> 5] * by_sh[32 + (b & 31)] * edge_weight<true>(z - g);
                 if (b == kBins - 1) y = l > -__builtin_inff() ? weight_of(l, top, w.inv_t) : 0.0;
                 if (l == top) y = 1.0;

@@ -361,3 +361,30 @@ def test_sample_ties_far_below_the_largest(dev, vocab, top, p, dtype):
             want = max(0, int(np.floor((np.longdouble(np.float32(u)) * kept - 1) / w)) + 1)
             print(f"k {k} u {u:.8f}: {token}, exactly {want}, bound {off:.1f}", flush=True)
             assert abs(token - want) <= off and 0 <= token < n + off
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 20, -(2.0 ** 20), 2.0 ** 14])
+def test_sample_logits_far_from_zero(dev, scale):
+    """Logits whose size is large against their differences: weights go by the differences, so a u that is V 2^-44 or more
+    from a border is on its own side of it. u is the number of f32 next to a border, in rows where that is V 2^-44 to 2^-34
+    from it."""
+    _case(f"sample, logits about {scale}")
+    rng = np.random.default_rng(13)
+    vocab, rows = 16, 60000
+    step = abs(scale) * 2.0 ** -23
+    l = scale + np.floor(rng.random((rows, vocab)) * 4 / step) * step
+    t = (rng.random(rows) * 1.4 + 0.3).astype(np.float32) * np.float32(1.0 if abs(scale) > 2.0 ** 15 else 0.01)
+    l = (scale + (l - scale) * (1.0 if abs(scale) > 2.0 ** 15 else 2.0 ** -6)).astype(np.float32)
+    x = l.astype(np.longdouble)
+    cum = np.cumsum(np.exp((x - x.max(1, keepdims=True)) / t.astype(np.longdouble)[:, None]), 1)
+    cum /= cum[:, -1:]
+    border = cum[np.arange(rows), rng.integers(0, vocab - 1, rows)]
+    u = border.astype(np.float32)
+    away = np.abs(u.astype(np.longdouble) - border)
+    take = (away > vocab * 2.0 ** -44) & (away < 2.0 ** -34) & (u < 1)
+    l, t, u, cum = l[take], t[take], u[take], cum[take]
+    assert len(l) > 20
+    want = (cum <= u.astype(np.longdouble)[:, None]).sum(1)
+    got = ops.sample(torch.from_numpy(l).to(dev), torch.from_numpy(u).to(dev), temperature=torch.from_numpy(t).to(dev)).cpu().numpy()
+    print(f"{int((got != want).sum())} of {len(l)} on the wrong side", flush=True)
+    assert np.array_equal(got, want)
