@@ -156,6 +156,9 @@ __device__ __forceinline__ uint64_t bin_weight(double f, double units, uint32_t 
     const uint64_t y = __builtin_bit_cast(uint64_t, __builtin_fma(edge_weight<false>(f), units, 0x1p52));
     return (y & 0xffffffff00000000ull) | (static_cast<uint32_t>(y) & ~count_mask);
 }
+// A weight of launch 3 without cuts -- two tables' values, the polynomial and their products, from the same exponent -- and
+// weight_of differ by less than five units of 2^-52, so where they may fall on either side of a number this tells.
+constexpr double kNear = 0x1p-48;
 __device__ __forceinline__ double weight_of(float l, float top, double inv_t) {
     const double w = exp((static_cast<double>(l) - static_cast<double>(top)) * inv_t);
     return l == top ? 1.0 : w == w ? w : 0.0;  // (no number: an infinite distance at an infinite temperature)
@@ -572,6 +575,7 @@ __global__ __launch_bounds__(256) void sample_sums(SampleArgs a) {
         if (s + 1 < blocks) next = load8(row, i0 + kBlockTokens, a.vocab);
         double sum = 0.0;
         if (whole) {
+            bool near = false;
             // e^(z / 32), by e^(-b / 32) of whole steps b down from the largest and the polynomial. (z from the difference,
             // which is exact: a difference of places is off by their own rounding, 2^-33 of the weight for logits of 10^6.)
 #pragma unroll
@@ -582,7 +586,20 @@ __global__ __launch_bounds__(256) void sample_sums(SampleArgs a) {
                 double y = by_sh[b >> 5] * by_sh[32 + (b & 31)] * edge_weight<true>(z - g);
                 if (b == kBins - 1) y = l > -__builtin_inff() ? weight_of(l, top, w.inv_t) : 0.0;
                 if (l == top) y = 1.0;
+                near |= fabs(y - w.min_p) < w.min_p * kNear;
                 sum += y >= w.min_p ? y : 0.0;
+            }
+            // Launch 4 takes exponentials: next to min_p they decide here too, or it finds a block whose only token it drops.
+            if (__any(near)) {
+                sum = 0.0;
+#pragma unroll 1
+                for (int e = 0; e < 8; e++) {
+                    float l = -__builtin_inff();
+#pragma unroll
+                    for (int i = 0; i < 8; i++) l = i == e ? fmaxf(to_f32(x.v[i]), l) : l;
+                    const double y = weight_of(l, top, w.inv_t);
+                    sum += y >= w.min_p ? y : 0.0;
+                }
             }
         } else {
             uint32_t kept = 0, picked = 0;  // tokens that are surely kept; tokens of the list
@@ -905,7 +922,8 @@ __global__ __launch_bounds__(kThreads) void sample_pick(SampleArgs a) {
         }
     }
     __syncthreads();
-    // Two tokens to a thread.
+    // Two tokens to a thread. (Some thread has one: a block of a sum above 0 holds a token of that weight, by the same
+    // exponential and comparisons in launch 3.)
     constexpr int PER = kBlockTokens / kThreads;
     const int32_t i0 = sh.block * kBlockTokens + tid * PER;
     double y[PER], sum = 0.0;

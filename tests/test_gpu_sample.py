@@ -388,3 +388,70 @@ def test_sample_logits_far_from_zero(dev, scale):
     got = ops.sample(torch.from_numpy(l).to(dev), torch.from_numpy(u).to(dev), temperature=torch.from_numpy(t).to(dev)).cpu().numpy()
     print(f"{int((got != want).sum())} of {len(l)} on the wrong side", flush=True)
     assert np.array_equal(got, want)
+
+
+# (temperature, logit, min_p), f32: e^x is within 1.1 * 2^-53 of min_p, relative, for x = logit * (1 / temperature) in double, whose
+# two roundings move the weight by 2 |x| 2^-53 from the exact one; |x| < 10.
+NEXT_TO_MIN_P = """
+0x1.016486p+0 -0x1.b05ba4p+0 0x1.7dc912p-3; 0x1.035c18p+0 -0x1.52dc34p+1 0x1.2c47a2p-4;
+0x1.052658p+0 -0x1.7b8588p-3 0x1.aaf31p-1; 0x1.0885a4p+0 -0x1.d5764p-6 0x1.f1ff3cp-1;
+0x1.09015p+0 -0x1.2aaaep+1 0x1.adf856p-4; 0x1.099ec8p+0 -0x1.9785p-4 0x1.d12f74p-1;
+0x1.0b7eep-1 -0x1.1cd438p+1 0x1.cf21ep-7; 0x1.13721ep+0 -0x1.3a274p-1 0x1.217906p-1;
+0x1.1d49cap-1 -0x1.a35572p+0 0x1.b13284p-5; 0x1.224188p-1 -0x1.53f88ap+1 0x1.2e80aep-7;
+0x1.2449ecp-1 -0x1.db5c6cp-2 0x1.c617c2p-2; 0x1.24635ap+0 -0x1.174b68p+1 0x1.2f22d4p-3;
+0x1.2b79bcp+0 -0x1.13571cp-2 0x1.96dc84p-1; 0x1.2ee9eap+0 -0x1.f3cce8p+0 0x1.8953dep-3;
+0x1.30546ap+0 -0x1.c1c278p+0 0x1.d3324p-3; 0x1.3511d8p+0 -0x1.e559f8p+0 0x1.a9ec12p-3;
+0x1.39997cp-2 -0x1.525d06p+1 0x1.7609f2p-13; 0x1.3b01dp-1 -0x1.f7ecc8p-2 0x1.cc2d0cp-2;
+0x1.3ea258p+0 -0x1.1e49dcp+0 0x1.a0f538p-2; 0x1.4613ap-1 -0x1.26318p-3 0x1.989d02p-1;
+0x1.49473p-1 -0x1.c49f46p-1 0x1.03039ap-2; 0x1.51876p-1 -0x1.f62d0cp+0 0x1.a1eda2p-5;
+0x1.540ab2p-1 -0x1.22f8f4p+1 0x1.0b3c28p-5; 0x1.54da58p-1 -0x1.dbdf3ap+0 0x1.f60918p-5;
+0x1.55ecfcp-1 -0x1.6db14p-1 0x1.5f69dap-2; 0x1.5bbdbp+0 -0x1.6bd52p+1 0x1.f9552ep-4;
+0x1.671792p-1 -0x1.c469c4p+0 0x1.49a428p-4; 0x1.6bff12p+0 -0x1.c39caap-1 0x1.13549ep-1;
+0x1.6ddbaep+0 -0x1.787ad2p+1 0x1.05881p-3; 0x1.73c9d8p+0 -0x1.4c3044p+1 0x1.56f85p-3;
+0x1.881daep+0 -0x1.66b916p+1 0x1.48a1fap-3; 0x1.8f856ap-2 -0x1.9191a4p+0 0x1.25fe64p-6;
+0x1.967af2p+0 -0x1.90a1cp-1 0x1.38c92ap-1; 0x1.96f7a6p+0 -0x1.b3c7p+0 0x1.5ef674p-2;
+0x1.98b76p+0 -0x1.8fc798p-1 0x1.39f516p-1; 0x1.9de7acp-2 -0x1.fb091p+0 0x1.e802bep-8;
+0x1.ad0318p+0 -0x1.e9601ep+0 0x1.4743b4p-2; 0x1.b1e97ep+0 -0x1.43890cp+0 0x1.e5d318p-2;
+0x1.b1f75p+0 -0x1.49883p+0 0x1.df33b4p-2; 0x1.c2c88ep-2 -0x1.aebffp-1 0x1.2eee28p-3;
+0x1.d0715ep-1 -0x1.f8a67ap-1 0x1.5977d8p-2; 0x1.db724ap-2 -0x1.49f5bcp+0 0x1.fe419p-5;
+0x1.dc5d3ap-1 -0x1.7fe036p+1 0x1.4634fep-5; 0x1.dcb15ep-1 -0x1.f5e4bcp+0 0x1.f2b71p-4;
+0x1.debcep-1 -0x1.4f1e76p+0 0x1.f90676p-3; 0x1.ef5f9cp-1 -0x1.bc8c16p-1 0x1.a16978p-2;
+0x1.f96f04p-2 -0x1.28b588p+0 0x1.875a84p-4;
+"""
+
+
+def test_sample_min_p_next_to_a_weight(dev):
+    """Weights within (1.1 + 2 * 10) 2^-53 < 2^-48 of min_p, each in a block of its own behind the largest's: whichever side they fall to, a token is
+    chosen, and one that may stay. u asks for the last token that stays."""
+    _case("sample, min_p next to a weight")
+    rows = [[float.fromhex(v) for v in r.split()] for r in NEXT_TO_MIN_P.replace("\n", " ").split(";") if r.strip()]
+    n, vocab = len(rows), 5000
+    x = torch.full((n, vocab), -float("inf"))
+    x[:, 0] = 0.0
+    t, x[:, 4099], m = (torch.tensor([r[i] for r in rows]) for i in range(3))
+    exact = np.exp(x[:, 4099].numpy().astype(np.longdouble) / t.numpy().astype(np.longdouble))
+    assert float(np.abs(exact / m.numpy().astype(np.longdouble) - 1).max()) <= 2.0 ** -48
+    out = torch.full((n,), -7, dtype=torch.int32, device=dev)
+    ops.sample(x.to(dev), torch.full((n,), 0.99, device=dev), temperature=t.to(dev), min_p=m.to(dev), out=out)
+    got = out.tolist()
+    print(got, flush=True)
+    assert set(got) <= {0, 4099}
+
+
+def test_sample_min_p_of_one(dev):
+    """min_p = 1 where weights are 1 or the number below it, each in a block of its own: a token is chosen, one whose weight is
+    1 but for the rounding of its exponential (2^-52)."""
+    _case("sample, min_p of 1, weights next to 1")
+    g = torch.Generator().manual_seed(12)
+    vocab, rows = 30 * 2048, 64
+    for temperature, scale in ((1e15, 8.0), (1e16, 8.0), (3e16, 8.0), (1e17, 8.0), (1e18, 8.0), (1.0, 1e-16), (0.7, 3e-16)):
+        x = torch.full((rows, vocab), -float("inf"))
+        x[:, 700::2048] = torch.rand((rows, 30), generator=g) * scale
+        u = torch.rand(rows, generator=g)
+        out = torch.full((rows,), -7, dtype=torch.int32, device=dev)
+        ops.sample(x.to(dev), u.to(dev), temperature=torch.full((rows,), temperature, device=dev), min_p=torch.ones(rows, device=dev), out=out)
+        got = out.cpu().long()
+        assert bool(((got >= 0) & (got < vocab)).all()), (temperature, got.tolist())
+        l = x.numpy().astype(np.longdouble)
+        chosen = np.exp((l[np.arange(rows), got.numpy()] - l.max(1)) / np.longdouble(np.float32(temperature)))
+        assert float((1 - chosen).max()) <= 2.0 ** -52, temperature
