@@ -41,7 +41,10 @@ constexpr int kBins = 1024;  // one to a thread; the last holds whatever is furt
 constexpr double kBinsPerT = 32.0;
 constexpr int kBlockTokens = 2048;               // of a sum: 256 threads of 8
 constexpr int kStepTokens = kThreads * 8;        // four blocks
-constexpr int kMostSteps = 3;                    // of a part: a thread holds its tokens in registers
+// Of a part: a thread holds its tokens in registers. Three of f16 spill beside their conversions (128 rows of 151936 with a
+// top-k of 50 70.6 us, of two steps 56.3; with none of the cuts 45.8 and 41.9).
+template <typename T>
+constexpr int kMostSteps = sizeof(T) == 2 ? 2 : 3;
 constexpr int kMostBlocks = 16;                  // of a workgroup in launch 3
 // Rows' counters a cache line apart: workgroups of all XCDs add to them (launch 3 of 128 rows with a top-k of 50 17 us, on four
 // lines 21).
@@ -138,7 +141,12 @@ __device__ __forceinline__ float value_of(uint32_t k) {
 __device__ __forceinline__ double bins_per(double inv_t) { return fmax(kBinsPerT * inv_t, 1e-300); }
 __device__ __forceinline__ double place_of(float l, double inv_t) { return fmin(static_cast<double>(l) * bins_per(inv_t), 1e300); }
 __device__ __forceinline__ int bin_at(double place, double top) { return static_cast<int>(fmax(fmin(rint(top) - rint(place), kBins - 1.0), 0.0)); }
-// e^(f / 32) for -1/2 <= f <= 1/2: the series, cut off by (1/64)^5 / 5! = 8e-12 or (LONG) (1/64)^7 / 7! = 5e-17.
+// From this place on other logits than the largest are at least 2^21 bins away, and only those equal to it weigh anything.
+constexpr double kFarPlace = 0x1p45;
+// What a logit lies past the middle of its bin, that of place g: the product's exact value counts (a rounded one is off by 2^-53
+// of the place, 2^-26 of the weight for a logit of 2^27 temperatures).
+__device__ __forceinline__ double past_middle(float l, double per, double g) { return __builtin_fma(static_cast<double>(l), per, -g); }
+// e^(f / 32) for -1/2 <= f <= 1/2, and a little more: the series, cut off by (1/64)^5 / 5! = 8e-12 or (LONG) (1/64)^7 / 7! = 5e-17.
 template <bool LONG>
 __device__ __forceinline__ double edge_weight(double f) {
     const double x = f * (1.0 / 32.0);
@@ -315,33 +323,44 @@ __global__ __launch_bounds__(kThreads, 8) void sample_parts(SampleArgs a) {
     const uint32_t mask = (1u << a.count_bits) - 1;
     double further = 0.0;  // what the last bin's tokens weigh
     uint32_t n = 0;        // and how many there are
+    if (fabs(first) >= kFarPlace) {  // (infinities too)
 #pragma unroll
-    for (int s = 0; s < STEPS; s++) {
-        u64 y[8];
-        int b[8];
-        bool far = false;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float l = to_f32(x[s].v[e]);
-            const double z = fmin(static_cast<double>(fmaxf(l, -__builtin_inff())) * per, 1e300), g = rint(z);  // (NaN: -inf)
-            b[e] = static_cast<int>(fmin(first - g, kBins - 1.0));
-            y[e] = bin_weight(z - g, units, mask) | 1u;
-            far |= b[e] == kBins - 1 && l > -__builtin_inff();
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            if (b[e] < kBins - 1) atomicAdd(&bins[b[e]], y[e]);
-        if (__any(far)) {
+        for (int s = 0; s < STEPS; s++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const float l = to_f32(x[s].v[e]);
-                if (b[e] == kBins - 1 && l > -__builtin_inff()) {
-                    n++;
-                    further += exp((fmin(static_cast<double>(l) * per, 1e300) - first) * (1.0 / kBinsPerT));
+                if (l == top) atomicAdd(&bins[0], static_cast<u64>(bin_weight(0.0, units, mask) | 1u));
+                else if (l > -__builtin_inff()) n++;
+            }
+    } else {
+#pragma unroll
+        for (int s = 0; s < STEPS; s++) {
+            u64 y[8];
+            int b[8];
+            bool far = false;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float l = fmaxf(to_f32(x[s].v[e]), -__builtin_inff());  // (NaN: -inf)
+                const double g = rint(static_cast<double>(l) * per);
+                b[e] = static_cast<int>(fmin(first - g, kBins - 1.0));
+                y[e] = bin_weight(past_middle(l, per, g), units, mask) | 1u;
+                far |= b[e] == kBins - 1 && l > -__builtin_inff();
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (b[e] < kBins - 1) atomicAdd(&bins[b[e]], y[e]);
+            if (__any(far)) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float l = to_f32(x[s].v[e]);
+                    if (b[e] == kBins - 1 && l > -__builtin_inff()) {
+                        n++;
+                        further += exp((static_cast<double>(l) * per - first) * (1.0 / kBinsPerT));
+                    }
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
-        __builtin_amdgcn_sched_barrier(0);
     }
     __syncthreads();
     // (without the high bits of each 2^52)
@@ -376,9 +395,10 @@ __global__ __launch_bounds__(kThreads, 8) void sample_parts(SampleArgs a) {
 __device__ __forceinline__ void row_bin(const SampleArgs& a, int64_t r, const Row& w, float top, const Part& held, int* sh_off, uint32_t* sh_n, double* sh_by, uint32_t* count,
                                         double* weight, uint32_t* all, double* total) {
     const int t = static_cast<int>(threadIdx.x);
-    const double place = place_of(top, w.inv_t);
+    const double place = place_of(top, w.inv_t), first = rint(place);
     // (in units of the largest's own fixed-point weight)
-    const double unit = static_cast<double>((bin_weight(place - rint(place), ldexp(1.0, a.fixed + a.count_bits), (1u << a.count_bits) - 1) - kHigh) >> a.count_bits);
+    const double rest = fabs(first) < kFarPlace ? past_middle(top, bins_per(w.inv_t), first) : 0.0;
+    const double unit = static_cast<double>((bin_weight(rest, ldexp(1.0, a.fixed + a.count_bits), (1u << a.count_bits) - 1) - kHigh) >> a.count_bits);
     uint32_t n = 0, n_all = 0;
     double s = 0.0, s_all = 0.0, edge = 0.0;
     const uint64_t* bins = a.bins + r * a.parts * kBins;
@@ -966,10 +986,12 @@ int launch(neko_hip_ctx* ctx, const char* what, SampleArgs a, int64_t rows, int6
         a.u = from(all.u);
         a.out = from(all.out);
         const dim3 by_row(static_cast<uint32_t>(n));
+        auto parts_of = [&](auto steps) { hipLaunchKernelGGL((sample_parts<T, decltype(steps)::value>), dim3(parts), dim3(kThreads), 0, ctx->stream, a); };
         switch (a.part_tokens / kStepTokens) {
-            case 1: hipLaunchKernelGGL((sample_parts<T, 1>), dim3(parts), dim3(kThreads), 0, ctx->stream, a); break;
-            case 2: hipLaunchKernelGGL((sample_parts<T, 2>), dim3(parts), dim3(kThreads), 0, ctx->stream, a); break;
-            default: hipLaunchKernelGGL((sample_parts<T, kMostSteps>), dim3(parts), dim3(kThreads), 0, ctx->stream, a); break;
+            case 1: parts_of(std::integral_constant<int, 1>{}); break;
+            case 2: parts_of(std::integral_constant<int, 2>{}); break;
+            default:
+                if constexpr (kMostSteps<T> > 2) parts_of(std::integral_constant<int, kMostSteps<T>>{});
         }
         if (int rc = after_launch(ctx, what)) return rc;
         if (a.top_k || a.top_p) {
@@ -1025,7 +1047,7 @@ extern "C" int neko_hip_sample(neko_hip_ctx* ctx, const void* logits, int64_t st
     const int64_t steps = (vocab + kStepTokens - 1) / kStepTokens;
     const int64_t held = std::min(rows, kSlabRows);
     const int64_t wanted = std::max<int64_t>(1, std::min<int64_t>(steps, (2LL * ctx->cu_count + held - 1) / held));
-    const int64_t even = (steps + wanted - 1) / wanted, each = even > 2 ? kMostSteps : even;
+    const int64_t even = (steps + wanted - 1) / wanted, each = std::min<int64_t>(even, dtype == NEKO_DT_F16 ? kMostSteps<half_t> : kMostSteps<float>);
     a.parts = static_cast<int32_t>((steps + each - 1) / each);
     a.part_tokens = static_cast<int32_t>(each * kStepTokens);
     // Ten workgroups to a CU, of as many blocks as that takes: twice what is resident, since rows without cuts take longer.
@@ -1041,7 +1063,8 @@ extern "C" int neko_hip_sample(neko_hip_ctx* ctx, const void* logits, int64_t st
     a.fixed = std::min(44, 63 - 2 * a.count_bits);
     a.narrow = std::min(44, 62 - bits_of(vocab));
     const bool hist = a.top_k || a.top_p;
-    const size_t parts = static_cast<size_t>(a.parts);
+    // (of either type: what a call of one has made room for holds the other)
+    const size_t parts = static_cast<size_t>((steps + std::min<int64_t>(even, kMostSteps<half_t>) - 1) / std::min<int64_t>(even, kMostSteps<half_t>));
     size_t bytes[] = {parts * sizeof(Part), static_cast<size_t>(a.n_blocks) * 8, sizeof(Found), hist ? parts * kBins * 8 : 0, hist ? kListed * size_t(8) : 0,
                       kLine * sizeof(uint32_t)};  // of a row
     size_t of_row = 0;

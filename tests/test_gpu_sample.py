@@ -455,3 +455,77 @@ def test_sample_min_p_of_one(dev):
         l = x.numpy().astype(np.longdouble)
         chosen = np.exp((l[np.arange(rows), got.numpy()] - l.max(1)) / np.longdouble(np.float32(temperature)))
         assert float((1 - chosen).max()) <= 2.0 ** -52, temperature
+
+
+def test_sample_top_p_of_logits_far_from_zero(dev):
+    """Small temperatures, logits 2^27 times as large: one of 1000 and 30000 of the next f32 below it, 8 to 9 temperatures away.
+    The cut of top-p is where the weights by the difference put it, when those are more than 2^-27 of the sum from a border:
+    u = 1 - 2^-24 asks for the last token that stays, whose weight is e^-9 / 5 or e^-8 / 11 > 2^-24 of the kept ones'."""
+    _case("sample, top-p of logits far from zero")
+    rng = np.random.default_rng(14)
+    rows, ties = 2000, 30000
+    low = np.nextafter(np.float32(1000.0), np.float32(0.0))
+    t = (float(np.float32(1000.0) - low) / (8 + rng.random(rows))).astype(np.float32)
+    w = np.exp((np.longdouble(low) - 1000) / t.astype(np.longdouble))
+    j = rng.integers(1, ties, rows)  # ties kept up to the border
+    border = (1 + j * w) / (1 + ties * w)
+    p = border.astype(np.float32)
+    off = p.astype(np.longdouble) - border
+    take = (np.abs(off) > 1.25 * 2.0 ** -27) & (np.abs(off) < 2.0 ** -25)
+    t, j, p, off = t[take], j[take], p[take], off[take]
+    n = len(t)
+    assert n > 500
+    x = torch.full((n, ties + 1), float(low), device=dev)
+    x[:, 0] = 1000.0
+    want = j + (off > 0)
+    got = ops.sample(x, torch.full((n,), 1 - 2.0 ** -24, device=dev), temperature=torch.from_numpy(t).to(dev), top_p=torch.from_numpy(p).to(dev)).cpu().numpy()
+    print(f"{int((got != want).sum())} of {n} cut elsewhere", flush=True)
+    assert np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("vocab", [7, 300, 6000, 30000])
+def test_sample_largest_logits_far_from_all_others(dev, vocab):
+    """Logits so large against the temperature that only those equal to the largest weigh anything, in several parts of the
+    row: whole numbers of tokens, cuts and borders met exactly."""
+    _case(f"sample, ties far from all others, vocabulary {vocab}")
+    x = torch.full((6, vocab), -1.0)
+    x[:, ::2] = torch.tensor([1e30, 1e30, -1.0, 65504.0, 3e38, 1e-3])[:, None]
+    x[2, 1::2] = -3e38
+    t = torch.tensor([0.5, 1e3, 1e-30, 1e-20, 1e-30, 1e-25])
+    u = torch.tensor([0.0, 0.25, 0.5, 0.75, 0.875, 0.9375])
+    half = (vocab + 1) // 2
+    k = torch.tensor([1, 2, half, half + 1, vocab - 1, 0], dtype=torch.int32)
+    p = torch.tensor([0.5, 0.25, 0.125, 0.75, 0.0625, 0.875])
+    _check(dev, x, u, exact_ties=True, temperature=t, top_p=p)
+    _check(dev, x, u, exact_ties=True, temperature=t, top_k=k)
+    _check(dev, x, u, exact_ties=True, temperature=t, top_k=k, top_p=p, min_p=torch.full((6,), 0.5))
+
+
+def test_sample_captured_in_the_workspace_of_the_other_type(dev):
+    """The workspace goes by rows, vocabulary and settings, not by the type: a call of one type has made room for the other's."""
+    _case("sample, captured after a call of the other type")
+    for first, then in ((torch.float32, torch.float16), (torch.float16, torch.float32)):
+        x = (torch.randn((130, 151936), generator=torch.Generator().manual_seed(15)) * 2).to(dev)
+        u, p = torch.rand(130, generator=torch.Generator().manual_seed(16)).to(dev), torch.full((130,), 0.9, device=dev)
+        out = torch.empty(130, dtype=torch.int32, device=dev)
+        a, b = x.to(first), x.to(then)
+        del x
+
+        def work():  # (a thread's context and workspace are its own)
+            stream = torch.cuda.Stream(dev)
+            with torch.cuda.stream(stream):
+                ops.sample(a, u, top_p=p)
+            stream.synchronize()
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+                ops.sample(b, u, top_p=p, out=out)
+            graph.replay()
+            torch.cuda.synchronize()
+            got.append((out.clone(), ops.sample(b, u, top_p=p)))
+
+        got = []
+        t = threading.Thread(target=work)
+        t.start()
+        t.join()
+        torch.cuda.synchronize()
+        assert len(got) == 1 and torch.equal(*got[0])
