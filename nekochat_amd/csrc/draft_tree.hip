@@ -12,8 +12,8 @@
 // order. Paths increase, so a token's source lies behind every slot that is written before it is read, and a page's
 // scale changes only after all tokens that come from it.
 //
-// What bounds both: the launch and loads that need each other. Accept: one tree of 26 rows 4.0 us, 256 of up to 64 4.1.
-// Keep, 8 kv heads of 128: one tree of 26 3.9 us, 64 of up to 61 (2.6 MB) 5.1.
+// What bounds both: the launch and loads that need each other. Accept: one tree of 26 rows 3.9 us, 256 of up to 64 4.0.
+// Keep, 8 kv heads of 128: one tree of 26 3.8 us, 64 of up to 61 (2.6 MB) 5.1.
 #include <algorithm>
 
 #include "internal.h"

@@ -21,13 +21,16 @@
 //   4 one workgroup to a row: the cuts within the list, its kept tokens' weights added to their blocks' sums, and the block
 //     and in it the token that u falls on
 //
-// What bounds it: one row of 151936 f16 logits, 27.5 us, four launches that need each other (6.8, 9.2, 4.7 and 8.1 by
-// themselves, most of each loads and barriers in turn). 128 such rows in f32, their settings mixed, 73 us: 26.9 of launch 1, of
+// What bounds it: one row of 151936 f16 logits, 27 us, four launches that need each other (6.6, 9.1, 4.7 and 8.4 by
+// themselves, most of each loads and barriers in turn). 128 such rows in f32, their settings mixed, 73 us: 26.5 of launch 1, of
 // which 13 are the reading (6 TB/s, from the last-level cache in part) and the rest some 33 instructions a token, half of them
-// in double (the same without the atomics); 9.2 of 2; 24.4 of 3, where rows that keep most of the vocabulary take the weights' exponentials again; 13.9 of 4.
+// in double (the same without the atomics); 9.3 of 2; 24 of 3, where rows that keep most of the vocabulary take the weights'
+// exponentials again; 13.9 of 4. In f16 73 too (26.2, 9.4, 25.5 and 14.2): half the reading, the same arithmetic. Where a cut's
+// bin holds more than 4096 tokens one workgroup reads the row again, some five times for a cut: 8 rows of 262144 logits of a
+// spread of 0.2 at a temperature of 1.5, top-p 0.5, 413 us (44 with a spread of 1.2), one of 2^24 49 ms.
 // Not kept: launch 3 by the polynomial for rows of many kept tokens too (rows with a top-p of 0.9 32 -> 37 us, of 0.99 46 -> 42);
 // the largest logits of 64 tokens each, so that launch 3 reads no others (no faster, launch 1 1.7 us slower); the bins' polynomial
-// with its scale in its coefficients (f32 28.0 -> 26.3, but the f16 form's registers spill: without a histogram 11.5 -> 14.7).
+// with its scale in its coefficients (f32 28.0 -> 26.3, but f16 parts, of three steps then, spilled more: without a histogram 11.5 -> 14.7).
 #include <algorithm>
 
 #include "internal.h"
@@ -51,7 +54,9 @@ constexpr int kMostBlocks = 16;                  // of a workgroup in launch 3
 constexpr int kLine = 32;
 constexpr int kGroupListed = 512;                // tokens of its own that one lists in LDS first
 constexpr int kListed = 4096;                    // tokens in the cuts' bins that are held in LDS
-constexpr int kAtOnce = 20;                      // parts' bins that are on their way at once in launch 2
+// Parts' bins that are on their way at once in launch 2: a round holds those of one row of 160 thousand tokens, of which each part
+// is one step; more take rounds.
+constexpr int kAtOnce = 20;
 constexpr int kRanked = 256;                     // of those, what is sorted by ranks
 constexpr int64_t kSlabRows = 1024;              // of a launch: the workspace holds so many,
 constexpr size_t kSlabBytes = size_t(256) << 20; // or as many as take this
