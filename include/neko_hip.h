@@ -317,12 +317,13 @@ int neko_hip_keep_paged(neko_hip_ctx* ctx, const neko_paged_kv* kv, const neko_p
  *   u         f32 [rows] in [0, 1) (brought into it otherwise; NaN: 0).
  *   tokens    int32 [rows]; -1 where every logit is -inf or NaN. Such logits are never chosen; where the largest is +inf,
  *             only those that are.
- * Weights and their sums are held in 64 bits, the sums that top_p's cut is found among to 2^-28: the token is that of an
- * evaluation in 64 bits unless u lies within vocab * 2^-44 of the weights' sum from a border between two tokens, top_p's cut
- * within 2^-27 of it, or min_p within 2^-45 of a weight, relative. The same call gives the same tokens again; in a batch of another size a row's can differ at such
- * a border only. rows up to 2^20, vocab up to 2^24. Partial results go to the context's workspace (see neko_hip_matmul):
- * for a row 8 bytes per 2048 tokens and, with a top_k or top_p, at most 8 KB per 8192 tokens and 33 KB; 256 MB in all
- * (or one row's), more rows in turn. Its size goes by rows, vocab and which settings are given. */
+ * Weights and their sums are held in 64 bits, the sums that top_p's cut is found among to 2^-28: the token is that of
+ * an evaluation in 64 bits unless u lies within vocab * 2^-44 of the weights' sum from a border between two tokens,
+ * top_p's cut within 2^-27 of it, or min_p within 2^-45 of a weight, relative. The same call gives the same tokens
+ * again; in a batch of another size a row's can differ at such a border only. rows up to 2^20, vocab up to 2^24.
+ * Partial results go to the context's workspace (see neko_hip_matmul): for a row 8 bytes per 2048 tokens and, with a
+ * top_k or top_p, at most 8 KB per 8192 tokens and 33 KB; 256 MB in all (or one row's), more rows in turn. Its size
+ * goes by rows, vocab and which settings are given. */
 int neko_hip_sample(neko_hip_ctx* ctx, const void* logits, int64_t stride, int64_t rows, int64_t vocab,
                     const float* temperature, const int32_t* top_k, const float* top_p, const float* min_p, const float* u,
                     int32_t* tokens, int dtype);

@@ -634,7 +634,8 @@ int launch_dims(neko_hip_ctx* ctx, const char* what, PagedAttnArgs a, int dtype)
     const int64_t most = static_cast<int64_t>(a.p.rows) * a.t.group;
     const int64_t reach = paged_reach(a.p), per_row = std::max(reach / 2, reach - a.p.rows / (2 * a.p.n_seq));
     const double pairs = static_cast<double>(a.p.rows) * a.n_head * static_cast<double>(a.t.window > 0 ? std::min<int64_t>(per_row, a.t.window) : per_row);
-    constexpr bool kTwoFit = sizeof(TQ) == 2 || DH <= 128;  // (f32 of 256 dimensions: 256 bytes of a lane's registers spill; f16 of 256 with a cap or bias 36, f32 of 128 with one 8)
+    // (f32 of 256 dimensions: 256 bytes of a lane's registers spill; f16 of 256 with a cap or bias 36, f32 of 128 with one 8)
+    constexpr bool kTwoFit = sizeof(TQ) == 2 || DH <= 128;
     const int few_rows = a.words > 0 && kTwoFit ? kFewTreeRows<TQ> : kFewRows;
     const int64_t some = a.words > 0 ? static_cast<int64_t>(a.p.n_seq) * few_rows : static_cast<int64_t>(a.p.n_seq) * a.t.group + kSpareRows;
     const bool many = pairs > kFewPairs<TQ> && most > (a.p.n_seq == 1 ? few_rows : some);
